@@ -211,6 +211,105 @@ WELVET_API welvet_status welvet_b200_volume_cell_outputs(welvet_b200_volume* v, 
                                                          int32_t* post_width);
 WELVET_API void welvet_b200_volume_release(welvet_b200_volume* v);
 
+/* ---------------------------------------------------------------- paged key-value cache
+ *
+ * No counterpart in the reference, whose MHA layer rebuilds its keys and values inside every
+ * forward (src/layers/mha/mha.cpp:123-183). The caller owns all memory: two pools of pages, a page
+ * table, lengths. The handle keeps their description, the workspaces of the calls (allocated by
+ * create, none later) and an error word. Calls run asynchronously on `stream`, can be captured in
+ * a CUDA graph, and must not overlap another call on the same handle. The current device when the
+ * library was first used owns every pointer. */
+
+typedef struct welvet_b200_kv_desc {
+  int32_t dtype;         /* pages: 1 Float32, 2 Float16, 3 BFloat16, 4 FP8E4M3 (OCP, saturating) */
+  int32_t num_heads;     /* query heads, a multiple of num_kv_heads */
+  int32_t num_kv_heads;
+  int32_t head_dim;      /* 1..256 */
+  int32_t page_size;     /* slots of a page */
+  int32_t num_pages;     /* pages of a pool */
+  int32_t num_seqs;
+  int32_t pages_per_seq; /* a sequence has max_slots = pages_per_seq * page_size slots */
+  void* k_pages;         /* element (page, slot, head, d) at page*s[0] + slot*s[1] + head*s[2] + d */
+  void* v_pages;
+  int64_t k_strides[3];  /* in elements */
+  int64_t v_strides[3];
+  float k_scale;         /* a stored unit stands for this much (1 unless FP8) */
+  float v_scale;
+  const int32_t* page_table; /* [num_seqs][pages_per_seq], rows table_stride apart */
+  int64_t table_stride;
+  int32_t* lens;         /* [num_seqs] slots in use */
+  int32_t* seen;         /* [num_seqs] tokens seen, >= lens once slots were evicted; NULL: lens */
+  float* weights;        /* [num_seqs][num_kv_heads][max_slots] accumulated attention weight, or NULL */
+  int32_t* positions;    /* same shape: the token position a slot holds (needs seen), or NULL: the
+                            slot index. Eviction needs weights, positions and seen */
+} welvet_b200_kv_desc;
+
+typedef struct welvet_b200_kv welvet_b200_kv;
+WELVET_API welvet_status welvet_b200_kv_create(const welvet_b200_kv_desc* desc, welvet_b200_kv** out);
+
+/* New tokens into the cache: k, v [rows][num_kv_heads * head_dim] float32, rows k_ld / v_ld apart.
+ * Rows cu_tokens[s] .. cu_tokens[s+1]-1 (device, [num_seqs + 1]) go to sequence s; NULL: one row per
+ * sequence (rows = num_seqs). Row i of a sequence takes slot start[s] + i and position
+ * start_seen[s] + i; afterwards lens = start + n and seen = start_seen + n (start, start_seen NULL:
+ * lens and seen themselves, advanced in place). theta > 0 rotates k, and q [rows][num_heads *
+ * head_dim] into q_out (may be q), as the MHA cell does (pairs d, d + head_dim/2); values are stored
+ * as they are. A slot past max_slots or a page id outside the pool is skipped and recorded. */
+WELVET_API welvet_status welvet_b200_kv_append(welvet_b200_kv* kv, int32_t rows, const float* k, int64_t k_ld,
+                                               const float* v, int64_t v_ld, const float* q, int64_t q_ld,
+                                               float* q_out, int64_t q_out_ld, const int32_t* cu_tokens, double theta,
+                                               const int32_t* start, const int32_t* start_seen, void* stream);
+
+/* Attention of one new token per sequence: q, out [num_seqs][num_heads * head_dim] float32, rows
+ * q_ld / out_ld apart; softmax over the sequence's slots of scale * q.k (scale <= 0: head_dim^-0.5).
+ * window > 0 keeps positions above (query position - window), the query's position being seen - 1;
+ * alibi adds the MHA cell's linear biases. A sequence with no slot allowed gets zeros. accumulate:
+ * weights[slot] = weights_in[slot] (NULL: weights) + the slot's attention weights summed over the
+ * query heads of its key-value head, for slots below lens. */
+WELVET_API welvet_status welvet_b200_kv_attend(welvet_b200_kv* kv, const float* q, int64_t q_ld, float* out,
+                                               int64_t out_ld, float scale, int32_t window, int32_t alibi,
+                                               int32_t accumulate, const float* weights_in, void* stream);
+
+/* Cuts every sequence with more than `budget` slots to `keep` (per key-value head): positions
+ * < sinks and >= seen - recent stay, then the largest accumulated weights (ties: the lower slot;
+ * NaN counts as -infinity). Slots >= keep that stay move, in ascending order, into the slots < keep that go,
+ * with their weights and positions; lens becomes keep. lens_in / weights_in / positions_in (NULL:
+ * the cache's own) are read instead of the records that are written. Pages that evicted sequences
+ * share with others must be copied first. sinks + recent <= keep <= budget. */
+WELVET_API welvet_status welvet_b200_kv_evict(welvet_b200_kv* kv, int32_t keep, int32_t budget, int32_t sinks,
+                                              int32_t recent, const int32_t* lens_in, const float* weights_in,
+                                              const int32_t* positions_in, void* stream);
+
+/* Synchronizes `stream`; status 1 (cleared by the report) if an earlier call met a page id outside
+ * the pool or a length outside the sequence's slots: those rows were skipped. */
+WELVET_API welvet_status welvet_b200_kv_check_error(welvet_b200_kv* kv, void* stream);
+WELVET_API void welvet_b200_kv_release(welvet_b200_kv* kv);
+
+/* ---------------------------------------------------------------- 4-bit Dense with group scales
+ *
+ * No counterpart in the reference (one scale per tensor). y = act(sum over groups of scale *
+ * (codes . x) + bias): codes Int4 (14, two's complement), Uint4 (15, minus the group's zero point)
+ * or FP4 (16, E2M1); `group` consecutive inputs share a scale, 32 or a multiple of 64 (the last group
+ * may be shorter); scales Float16 (2) or BFloat16 (3). codes [out][(in + 1) / 2] bytes, low nibble =
+ * even input; scales and zeros [out][ceil(in / group)]. */
+
+/* Round-to-nearest quantisation of W_dev [out][in] float32 into those arrays (device). */
+WELVET_API welvet_status welvet_b200_group_quantize(int32_t in, int32_t out, int32_t group, int32_t code,
+                                                    int32_t scale_dtype, const float* W_dev, uint8_t* codes_dev,
+                                                    void* scales_dev, uint8_t* zeros_dev, void* stream);
+
+typedef struct welvet_b200_gdense welvet_b200_gdense;
+/* Copies the arrays (device or host per weights_on_device; zeros with Uint4 only) into the layout
+ * the kernels read. bias: host, rows o < bias_len, as in welvet_dense_mount. Synchronous. */
+WELVET_API welvet_status welvet_b200_gdense_mount(int32_t in, int32_t out, int32_t group, int32_t code,
+                                                  int32_t scale_dtype, int32_t act, const uint8_t* codes,
+                                                  const void* scales, const uint8_t* zeros, int32_t weights_on_device,
+                                                  const double* bias, size_t bias_len, welvet_b200_gdense** g_out);
+/* x_dev [rows][in] (rows x_ld apart) -> pre_dev (may be NULL), post_dev [rows][out], asynchronous on
+ * `stream`. Made for 1..8 rows; more rows run in passes of 8 over the weights. */
+WELVET_API welvet_status welvet_b200_gdense_execute_device(welvet_b200_gdense* g, int32_t rows, const float* x_dev,
+                                                           int64_t x_ld, float* pre_dev, float* post_dev, void* stream);
+WELVET_API void welvet_b200_gdense_release(welvet_b200_gdense* g);
+
 /* ---------------------------------------------------------------- multi-GPU (one box)
  *
  * No counterpart in the reference, which runs every kernel on device 0

@@ -1,0 +1,284 @@
+"""The 4-bit Dense layer with group scales against 64-bit sums of its definition, and its quantiser
+against the rounding rule in numpy."""
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+FP4 = np.array([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0, -0.0, -0.5, -1.0, -1.5, -2.0, -3.0, -4.0, -6.0])
+
+
+@pytest.fixture(scope="module")
+def D(wb):
+    import welvet.cuda_b200.decode as decode
+    return decode
+
+
+def make(rng, rows, cols, group, code, scale_dtype="f16"):
+    import torch
+    groups = -(-cols // group)
+    c = rng.integers(0, 16, (rows, 2 * ((cols + 1) // 2)), dtype=np.uint8)
+    codes = (c[:, 0::2] | (c[:, 1::2] << 4)).astype(np.uint8)
+    s = torch.from_numpy(rng.uniform(0.002, 0.02, (rows, groups)).astype(np.float32)).to(
+        torch.float16 if scale_dtype == "f16" else torch.bfloat16)
+    zeros = rng.integers(0, 16, (rows, groups), dtype=np.uint8) if code == "uint4" else None
+    c = c[:, :cols].astype(np.int64)
+    which = np.arange(cols) // group
+    if code == "fp4":
+        w = FP4[c]
+    elif code == "int4":
+        w = np.where(c > 7, c - 16, c).astype(np.float64)
+    else:
+        w = c - zeros[:, which].astype(np.float64)
+    return codes, s, zeros, w * s.double().numpy()[:, which]
+
+
+def mount(D, codes, s, zeros, cols, group, code, **kw):
+    import torch
+    z = None if zeros is None else torch.from_numpy(zeros).cuda()
+    return D.GroupDense.from_codes(torch.from_numpy(codes).cuda(), s.cuda(), cols, group, D.CODES[code], zeros=z, **kw)
+
+
+def check(y, x, W, what=""):
+    """|y - y64| <= 2^-18 * sum |W x| + 2 ulp, the tensor GEMV's bound."""
+    x = x.astype(np.float64)
+    y64 = x @ W.T
+    bound = 2.0 ** -18 * (np.abs(x) @ np.abs(W).T) + 2 * np.spacing(np.abs(y64).astype(np.float32)).astype(np.float64)
+    err = np.abs(y.astype(np.float64) - y64)
+    assert np.all(err <= bound), (what, float(np.max(err - bound)))
+
+
+SHAPES = [(1, 1), (1, 33), (16, 64), (17, 31), (64, 96), (100, 130), (257, 1000), (1024, 4096), (40, 16385), (4099, 515),
+          (8192, 64), (300, 2048)]
+
+
+@pytest.mark.parametrize("code", ["int4", "uint4", "fp4"])
+@pytest.mark.parametrize("group", [32, 64, 128, 192, 4096])
+@pytest.mark.parametrize("shape", range(len(SHAPES)))
+def test_forward(D, code, group, shape):
+    import torch
+    rows, cols = SHAPES[shape]
+    rng = np.random.default_rng(shape * 10 + group)
+    codes, s, zeros, W = make(rng, rows, cols, group, code, "f16" if shape % 2 else "bf16")
+    g = mount(D, codes, s, zeros, cols, group, code)
+    for n in (1, 2, 3, 4, 5, 8) if shape < 6 else (1, 1 + shape % 8):
+        x = rng.standard_normal((n, cols)).astype(np.float32)
+        y = torch.full((n, rows), float("nan"), device="cuda")
+        g.forward(torch.from_numpy(x).cuda(), y)
+        check(y.cpu().numpy(), x, W, (rows, cols, n))
+
+
+@pytest.mark.parametrize("n", [9, 16, 17, 40])
+def test_more_rows(D, n):
+    import torch
+    rng = np.random.default_rng(n)
+    codes, s, zeros, W = make(rng, 130, 700, 64, "uint4")
+    g = mount(D, codes, s, zeros, 700, 64, "uint4")
+    x = rng.standard_normal((n, 700)).astype(np.float32)
+    y = torch.empty((n, 130), device="cuda")
+    g.forward(torch.from_numpy(x).cuda(), y)
+    check(y.cpu().numpy(), x, W)
+
+
+@pytest.mark.parametrize("act", ["linear", "relu", "silu", "gelu", "tanh", "sigmoid", "leaky_relu", "relu2"])
+@pytest.mark.parametrize("bias_len", [0, 7, 100])
+def test_bias_and_activation(D, oracle, act, bias_len):
+    """The Dense layer's epilogue: bias for rows o < bias_len, activation in 64 bits, both rounded."""
+    import torch
+    rng = np.random.default_rng(bias_len)
+    codes, s, zeros, W = make(rng, 100, 256, 32, "fp4")
+    bias = rng.standard_normal(bias_len) if bias_len else None
+    g = mount(D, codes, s, zeros, 256, 32, "fp4", act=D.ACTS[act], bias=bias)
+    x = rng.standard_normal((3, 256)).astype(np.float32)
+    pre, y = torch.empty((3, 100), device="cuda"), torch.empty((3, 100), device="cuda")
+    g.forward(torch.from_numpy(x).cuda(), y, pre)
+    full = np.zeros(100)
+    full[: bias_len] = 0 if bias is None else bias
+    y64 = x.astype(np.float64) @ W.T + full
+    got = pre.cpu().numpy().astype(np.float64)
+    bound = 2.0 ** -18 * (np.abs(x) @ np.abs(W).T) + 4 * np.spacing(np.abs(y64).astype(np.float32))
+    assert np.all(np.abs(got - y64) <= bound)
+    f = {"linear": lambda v: v, "relu": lambda v: np.maximum(v, 0), "silu": lambda v: v / (1 + np.exp(-v)),
+         "gelu": lambda v: 0.5 * v * (1 + np.tanh(0.7978845608028654 * (v + 0.044715 * v ** 3))), "tanh": np.tanh,
+         "sigmoid": lambda v: 1 / (1 + np.exp(-v)), "leaky_relu": lambda v: np.where(v < 0, 0.01 * v, v),
+         "relu2": lambda v: np.where(v < 0, 0, v * v)}[act]
+    # post is the activation of the unrounded pre: the derivative carries its rounding (2 |v| + 1 bounds all)
+    np.testing.assert_allclose(y.cpu().numpy(), f(got), rtol=4e-7, atol=1e-7 * (1 + 2 * np.abs(got).max()) * np.abs(got).max())
+
+
+def test_strided_rows_streams_graph(D):
+    import torch
+    rng = np.random.default_rng(12)
+    codes, s, zeros, W = make(rng, 512, 1030, 128, "int4")
+    g = mount(D, codes, s, zeros, 1030, 128, "int4")
+    wide = rng.standard_normal((4, 3001)).astype(np.float32)
+    gw = torch.from_numpy(wide).cuda()
+    for at in (0, 1, 1971):  # rows that start off 16-byte boundaries
+        y = torch.empty((4, 512), device="cuda")
+        g.forward(gw[:, at: at + 1030], y)
+        check(y.cpu().numpy(), wide[:, at: at + 1030], W)
+    x = torch.from_numpy(np.ascontiguousarray(wide[:, :1030])).cuda()
+    y = torch.empty((4, 512), device="cuda")
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        g.forward(x, y)
+    side.synchronize()
+    check(y.cpu().numpy(), wide[:, :1030], W)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        g.forward(x, y)
+    new = rng.standard_normal((4, 1030)).astype(np.float32)
+    x.copy_(torch.from_numpy(new))
+    graph.replay()
+    check(y.cpu().numpy(), new, W)
+
+
+def test_chain_reads_what_the_layer_before_wrote(D):
+    """Three layers back to back, many times: each reads the output of the one before it."""
+    import torch
+    rng = np.random.default_rng(13)
+    parts = [make(rng, 768, 768, 64, c) for c in ("int4", "uint4", "fp4")]
+    layers = [mount(D, *p[:3], 768, 64, c) for p, c in zip(parts, ("int4", "uint4", "fp4"))]
+    x = torch.from_numpy(rng.standard_normal((2, 768)).astype(np.float32)).cuda()
+    first = None
+    for _ in range(50):
+        bufs = [torch.empty((2, 768), device="cuda") for _ in range(3)]
+        src = x
+        for g, dst in zip(layers, bufs):
+            g.forward(src, dst)
+            src = dst
+        torch.cuda.synchronize()
+        got = [b.cpu().numpy() for b in bufs]
+        if first is None:
+            first = got
+            src = x.cpu().numpy()
+            for b, p in zip(got, parts):
+                check(b, src, p[3])
+                src = b
+        for a, b in zip(first, got):
+            np.testing.assert_array_equal(a, b)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-6, 1e6, 1e30])
+def test_range_of_x(D, scale):
+    """Tokens of very different magnitude share a call; large and small values share a token."""
+    import torch
+    rng = np.random.default_rng(14)
+    codes, s, zeros, W = make(rng, 200, 2000, 64, "fp4")
+    g = mount(D, codes, s, zeros, 2000, 64, "fp4")
+    x = rng.standard_normal((3, 2000)).astype(np.float32)
+    x[0] *= np.float32(scale)
+    x[1, ::7] *= np.float32(1e-4)
+    x[2] = 0
+    y = torch.empty((3, 200), device="cuda")
+    g.forward(torch.from_numpy(x).cuda(), y)
+    check(y.cpu().numpy(), x, W)
+    assert not y[2].any()
+
+
+@pytest.mark.parametrize("code", ["int4", "uint4", "fp4"])
+def test_non_finite_x_stays_in_its_token(D, code):
+    import torch
+    rng = np.random.default_rng(15)
+    codes, s, zeros, W = make(rng, 200, 500, 64, code)
+    g = mount(D, codes, s, zeros, 500, 64, code)
+    x = rng.standard_normal((4, 500)).astype(np.float32)
+    x[1, 77], x[2, 3] = np.nan, np.inf
+    y = torch.empty((4, 200), device="cuda")
+    g.forward(torch.from_numpy(x).cuda(), y)
+    got = y.cpu().numpy()
+    check(got[[0, 3]], x[[0, 3]], W)
+    assert np.all(np.isnan(got[1])) and not np.any(np.isfinite(got[2]) & (W[:, 3] != 0))
+
+
+def test_host_arrays(D, wb):
+    """The C entry with host pointers gives the device mount's bits."""
+    import ctypes
+
+    import torch
+    rng = np.random.default_rng(16)
+    codes, s, zeros, W = make(rng, 70, 300, 32, "uint4")
+    a = mount(D, codes, s, zeros, 300, 32, "uint4")
+    h = ctypes.c_void_p()
+    sb = s.view(torch.int16).numpy()
+    wb.check(wb.lib().welvet_b200_gdense_mount(300, 70, 32, 15, 2, -1, codes.ctypes.data, sb.ctypes.data, zeros.ctypes.data, 0,
+                                               None, 0, ctypes.byref(h)))
+    b = D.GroupDense(h, 300, 70)
+    x = torch.randn((2, 300), device="cuda")
+    ya, yb = torch.empty((2, 70), device="cuda"), torch.empty((2, 70), device="cuda")
+    a.forward(x, ya)
+    b.forward(x, yb)
+    assert torch.equal(ya, yb)
+
+
+@pytest.mark.parametrize("code", ["int4", "uint4", "fp4"])
+@pytest.mark.parametrize("scale_dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,cols,group", [(5, 64, 32), (33, 130, 64), (64, 1001, 128), (3, 31, 64)])
+def test_quantize(D, code, scale_dtype, rows, cols, group):
+    import torch
+    rng = np.random.default_rng(cols)
+    dt = torch.float16 if scale_dtype == "f16" else torch.bfloat16
+    W = (rng.standard_normal((rows, cols)) * 0.05).astype(np.float32)
+    W[0, : min(cols, group)] = 0
+    codes, s, zeros = D.group_quantize(torch.from_numpy(W).cuda(), group, D.CODES[code], dt)
+    c = codes.cpu().numpy()
+    c = np.stack([c & 15, c >> 4], -1).reshape(rows, -1)
+    assert not c[:, cols:].any()
+    got = s.float().cpu().numpy()
+    for g in range(-(-cols // group)):
+        w = W[:, g * group: (g + 1) * group]
+        q = c[:, g * group: min(cols, (g + 1) * group)].astype(np.int64)
+        lo, hi = np.minimum(w.min(1), 0), np.maximum(w.max(1), 0)
+        amax = np.maximum(-lo, hi)
+        want = amax / np.float32(6) if code == "fp4" else amax / np.float32(7) if code == "int4" else (hi - lo) / np.float32(15)
+        want = torch.from_numpy(want).to(dt).float().numpy()
+        np.testing.assert_array_equal(got[:, g], want)
+        step = np.where(want > 0, want, 1)[:, None].astype(np.float32)
+        v = np.where(want[:, None] > 0, w / step, 0).astype(np.float32)
+        if code == "int4":
+            expect = np.clip(np.rint(v), -8, 7).astype(np.int64) & 15
+        elif code == "uint4":
+            z = np.where(want > 0, np.clip(np.rint(-lo / step[:, 0]), 0, 15), 0).astype(np.float32)
+            np.testing.assert_array_equal(zeros.cpu().numpy()[:, g], z.astype(np.uint8))
+            expect = np.clip(np.rint(v) + z[:, None], 0, 15).astype(np.int64)
+        else:
+            expect = np.argmin(np.abs(np.clip(v, -6, 6)[..., None] - FP4.astype(np.float32)), -1)  # ties: the lower code
+        np.testing.assert_array_equal(q, expect)
+
+
+@pytest.mark.parametrize("code", ["int4", "uint4", "fp4"])
+def test_quantized_layer_is_near_the_layer(D, code):
+    """W ~ N(0, 0.02), which one scale per tensor in FP4 turns into zeros: the relative error of y is the
+    step's, about a tenth."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(0)
+    W = torch.randn((1024, 2048), generator=g, device="cuda") * 0.02
+    x = torch.randn((2, 2048), generator=g, device="cuda")
+    y = torch.empty((2, 1024), device="cuda")
+    D.GroupDense.quantize(W, 64, D.CODES[code]).forward(x, y)
+    want = x.double() @ W.double().T
+    assert float((y - want).norm() / want.norm()) < 0.15
+
+
+def test_refusals(D, wb):
+    import torch
+    codes, s = torch.zeros((4, 32), dtype=torch.uint8, device="cuda"), torch.zeros((4, 1), dtype=torch.float16, device="cuda")
+    z = torch.zeros((4, 1), dtype=torch.uint8, device="cuda")
+    for kw, code in ((dict(code=D.UINT4), 1), (dict(code=D.INT4, zeros=z), 1), (dict(code=9), 2), (dict(code=D.FP4, act=9), 1)):
+        with pytest.raises(wb.WelvetError) as e:
+            c = kw.pop("code")
+            D.GroupDense.from_codes(codes, s, 64, 64, c, **kw)
+        assert e.value.code == code
+    for group in (48, 16, 0, -64):
+        with pytest.raises((wb.WelvetError, ValueError)):
+            D.GroupDense.from_codes(codes, s, 64, group, D.FP4)
+    for args in ((codes[:, :31], s), (codes.int(), s), (codes.cpu(), s), (codes, s.float()), (codes, s[:3])):
+        with pytest.raises(ValueError):
+            D.GroupDense.from_codes(*args, 64, 64, D.FP4)
+    g = D.GroupDense.from_codes(codes, s, 64, 64, D.FP4)
+    x, y = torch.zeros((2, 64), device="cuda"), torch.zeros((2, 4), device="cuda")
+    for a in ((x[:, :32], y), (x.half(), y), (x, y[:1]), (x, y.t()), (x.cpu(), y)):
+        with pytest.raises(ValueError):
+            g.forward(*a)
+    g.forward(x[:0], y[:0])  # no rows: nothing to do

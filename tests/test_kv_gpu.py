@@ -1,0 +1,584 @@
+"""The paged key-value cache (append, decode attention, eviction) against 64-bit statements of its
+definitions, at the sizes, layouts and masks where such code goes wrong."""
+import math
+
+import numpy as np
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+DT = ("f32", "f16", "bf16", "f8")
+EPS = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def D(wb):
+    import welvet.cuda_b200.decode as decode
+    return decode
+
+
+def types():
+    import torch
+    return {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16, "f8": torch.float8_e4m3fn}
+
+
+def make_cache(rng, dtype, n, per, page, kv, dim, layout="slots", fill="randn", spare=3):
+    """Pools (filled with NaN where `fill` is nan), a table whose pages lie in random order."""
+    import torch
+    pages = n * per + spare
+    shape = (pages, page, kv, dim) if layout == "slots" else (pages, kv, page, dim)
+    pools = []
+    for _ in range(2):
+        x = torch.from_numpy(rng.standard_normal(shape).astype(np.float32)).cuda()
+        if fill == "nan":
+            x.fill_(float("nan"))
+        x = x.to(types()[dtype])
+        pools.append(x if layout == "slots" else x.transpose(1, 2))
+    table = torch.from_numpy(rng.permutation(pages)[: n * per].reshape(n, per).astype(np.int32)).cuda()
+    return pools[0], pools[1], table
+
+
+def i32(a):
+    import torch
+    return torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).cuda()
+
+
+def rows_of(pool, table, b, n, h):
+    """float64 [n, dim] of a sequence's first n slots of one key-value head."""
+    page = pool.shape[1]
+    j = np.arange(n)
+    t = table.cpu().numpy()[b]
+    x = pool.float().cpu().numpy()
+    return x[t[j // page], j % page, h].astype(np.float64)
+
+
+def attend64(q, kp, vp, table, lens, scale, window=0, alibi=False, positions=None, seen=None, ks=1.0, vs=1.0):
+    """(out, weights per query head, bound on the error of out) in 64 bits. The bound: a score's fp32
+    sum of dim products and the roundings of its scale move it by dz, a weight by the factor 2 dz
+    (its own and the normaliser's), and the running sums of n weights add their roundings."""
+    n, H, dim = q.shape
+    kv = kp.shape[2]
+    q = q.double().cpu().numpy()
+    out, bound = np.zeros(q.shape), np.zeros(q.shape)
+    ws = [np.zeros((H, max(0, int(x)))) for x in lens]
+    for b in range(n):
+        L = int(lens[b])
+        for h in range(H):
+            g = h // (H // kv)
+            k, v = rows_of(kp, table, b, L, g) * ks, rows_of(vp, table, b, L, g) * vs
+            pos = np.arange(L) if positions is None else positions[b, g, :L]
+            last = L - 1 if positions is None else seen[b] - 1
+            ok = np.ones(L, bool) if not window else pos > last - window
+            if not ok.any():
+                continue
+            k, v, pos = k[ok], v[ok], pos[ok]
+            z = (k @ q[b, h]) * scale
+            if alibi:
+                z = z - 2.0 ** (-8.0 * (h + 1) / H) * (last - pos)
+            w = np.exp(z - z.max())
+            w /= w.sum()
+            out[b, h] = w @ v
+            ws[b][h, ok] = w
+            dz = np.max((dim + 8) * EPS * scale * (np.abs(k) @ np.abs(q[b, h])) + 4 * EPS * (np.abs(z) * 1.5 + np.abs(z.max())))
+            bound[b, h] = (2 * dz + (16 + len(z) / 8) * EPS) * (w @ np.abs(v)) + EPS * np.abs(out[b, h])
+    return out, ws, bound
+
+
+CASES = [
+    # heads, kv, dim, page, lens
+    (1, 1, 64, 16, [1]),
+    (4, 4, 128, 16, [0, 1, 15, 16, 17]),
+    (8, 2, 128, 16, [200, 0, 333, 64]),
+    (6, 2, 64, 32, [5, 700, 31, 32, 33]),
+    (5, 1, 80, 24, [95, 257, 1]),
+    (12, 4, 96, 7, [50, 7, 8, 129]),
+    (16, 1, 256, 64, [1025, 3]),
+    (24, 1, 128, 16, [300, 40]),
+    (2, 2, 40, 16, [77]),
+    (3, 3, 33, 5, [61, 5, 4]),
+    (2, 1, 8, 1, [9, 130]),
+    (2, 1, 4, 16, [33]),
+    (32, 8, 128, 16, [2049, 511, 4100]),
+]
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("case", range(len(CASES)))
+def test_attend(D, dtype, case):
+    import torch
+    H, kv, dim, page, lens = CASES[case]
+    rng = np.random.default_rng(100 * case + DT.index(dtype))
+    n, per = len(lens), max(1, -(-max(lens) // page)) + 1
+    kp, vp, table = make_cache(rng, dtype, n, per, page, kv, dim, layout="slots" if case % 2 else "heads")
+    ks, vs = (0.5, 2.0) if dtype == "f8" else (1.0, 1.0)
+    q = torch.from_numpy((rng.standard_normal((n, H, dim)) * 1.5).astype(np.float32)).cuda()
+    out = torch.full((n, H, dim), float("nan"), device="cuda")
+    c = D.PagedKV(kp, vp, table, i32(lens), num_heads=H, k_scale=ks, v_scale=vs)
+    c.attend(q, out)
+    c.check_error()
+    want, _, bound = attend64(q, kp, vp, table, lens, 1.0 / math.sqrt(dim), ks=ks, vs=vs)
+    err = np.abs(out.cpu().numpy() - want)
+    assert np.all(err <= bound), float(np.max(err - bound))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("window,alibi", [(1, False), (16, False), (100, True), (10 ** 6, True)])
+def test_attend_window_alibi(D, dtype, window, alibi):
+    """Keys outside the window hold NaN and infinity, so does every slot past the length."""
+    import torch
+    rng = np.random.default_rng(window + DT.index(dtype))
+    H, kv, dim, page, lens = 6, 2, 64, 16, [1, 40, 16, 177, 0, 1000]
+    n, per = len(lens), 70
+    kp, vp, table = make_cache(rng, dtype, n, per, page, kv, dim)
+    t = table.cpu().numpy()
+    bad = float("nan") if dtype == "f8" else None
+    for b, L in enumerate(lens):
+        for j in list(range(0, max(0, L - window))) + list(range(L, per * page)):
+            value = bad if bad is not None else (float("nan"), float("inf"), -float("inf"))[j % 3]
+            if j < 200 or j >= L:
+                kp.view(torch.uint8 if dtype == "f8" else kp.dtype)[int(t[b, j // page]), j % page] = 0x7f if dtype == "f8" else value
+                vp.view(torch.uint8 if dtype == "f8" else vp.dtype)[int(t[b, j // page]), j % page] = 0x7f if dtype == "f8" else value
+    q = torch.from_numpy(rng.standard_normal((n, H, dim)).astype(np.float32)).cuda()
+    out = torch.empty((n, H, dim), device="cuda")
+    c = D.PagedKV(kp, vp, table, i32(lens), num_heads=H)
+    c.attend(q, out, scale=0.3, window=window, alibi=alibi)
+    c.check_error()
+    scale = float(np.float32(0.3))
+    want, _, bound = attend64(q, kp, vp, table, lens, scale, window, alibi)
+    err = np.abs(out.cpu().numpy() - want)
+    assert np.all(err <= bound), float(np.max(err - bound))
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_attend_accumulates_weights(D, dtype):
+    import torch
+    rng = np.random.default_rng(7 + DT.index(dtype))
+    H, kv, dim, page, lens = 12, 4, 64, 16, [1, 40, 0, 177, 1500]
+    n, per = len(lens), 100
+    kp, vp, table = make_cache(rng, dtype, n, per, page, kv, dim)
+    q = torch.from_numpy(rng.standard_normal((n, H, dim)).astype(np.float32)).cuda()
+    out = torch.empty((n, H, dim), device="cuda")
+    w0 = torch.rand((n, kv, per * page), device="cuda")
+    w = torch.full_like(w0, -7.0)
+    c = D.PagedKV(kp, vp, table, i32(lens), num_heads=H, weights=w)
+    c.attend(q, out, accumulate=True, weights_in=w0)
+    want, ws, bound = attend64(q, kp, vp, table, lens, 1.0 / math.sqrt(dim))
+    assert np.all(np.abs(out.cpu().numpy() - want) <= bound)
+    got, old = w.cpu().numpy(), w0.cpu().numpy()
+    for b, L in enumerate(lens):
+        assert np.all(got[b, :, L:] == -7.0)
+        sums = ws[b].reshape(kv, H // kv, L).sum(1)
+        # a weight is off by its share of the bound above: at most dz ~ 2^-13 here, far above fp32's
+        np.testing.assert_allclose(got[b, :, :L] - old[b, :, :L], sums, rtol=2e-4, atol=4 * EPS)
+    # in place, and the sum over slots is the number of heads of a group
+    w.copy_(w0)
+    c.attend(q, out, accumulate=True)
+    np.testing.assert_array_equal(w.cpu().numpy()[3, :, :177], got[3, :, :177])
+    total = (w - w0).double().sum(-1).cpu().numpy()
+    np.testing.assert_allclose(total[[0, 1, 3, 4]], H // kv, rtol=1e-4)
+
+
+def test_attend_window_goes_by_positions(D):
+    """Once slots were evicted a slot's index is not its position."""
+    import torch
+    rng = np.random.default_rng(3)
+    H, kv, dim, page, n, per = 4, 2, 64, 16, 3, 6
+    lens = [90, 33, 64]
+    seen = [400, 33, 5000]
+    kp, vp, table = make_cache(rng, "bf16", n, per, page, kv, dim)
+    positions = np.zeros((n, kv, per * page), np.int32)
+    for b in range(n):
+        for h in range(kv):
+            positions[b, h, : lens[b]] = rng.permutation(seen[b])[: lens[b]]
+    q = torch.from_numpy(rng.standard_normal((n, H, dim)).astype(np.float32)).cuda()
+    out = torch.empty((n, H, dim), device="cuda")
+    c = D.PagedKV(kp, vp, table, i32(lens), num_heads=H, seen=i32(seen), positions=i32(positions))
+    for window, alibi in ((200, False), (50, True), (0, True), (1, False)):
+        c.attend(q, out, window=window, alibi=alibi)
+        want, _, bound = attend64(q, kp, vp, table, lens, 0.125, window, alibi, positions, seen)
+        assert np.all(np.abs(out.cpu().numpy() - want) <= bound)
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_attend_large_and_equal_scores(D, dtype):
+    """Scores in the hundreds (a weight of one), and keys that are all the same (weights 1 / n)."""
+    import torch
+    rng = np.random.default_rng(11)
+    H, kv, dim, page, lens = 4, 1, 64, 16, [500, 129]
+    kp, vp, table = make_cache(rng, dtype, 2, 40, page, kv, dim)
+    q = torch.from_numpy((rng.standard_normal((2, H, dim)) * 100).astype(np.float32)).cuda()
+    out = torch.empty((2, H, dim), device="cuda")
+    c = D.PagedKV(kp, vp, table, i32(lens), num_heads=H)
+    c.attend(q, out)
+    want, _, bound = attend64(q, kp, vp, table, lens, 0.125)
+    assert np.all(np.abs(out.cpu().numpy() - want) <= bound)
+    kp.zero_() if dtype != "f8" else kp.view(torch.uint8).zero_()
+    c.attend(q, out)
+    want, _, bound = attend64(q, kp, vp, table, lens, 0.125)
+    assert np.all(np.abs(out.cpu().numpy() - want) <= bound)
+
+
+def test_attend_strided_rows_other_stream_and_graph(D):
+    """q and out as parts of wider rows, a call on a side stream, and a captured call replayed after the
+    cache has grown."""
+    import torch
+    rng = np.random.default_rng(5)
+    H, kv, dim, page, n, per = 8, 2, 128, 16, 3, 20
+    kp, vp, table = make_cache(rng, "bf16", n, per, page, kv, dim)
+    lens = i32([10, 200, 33])
+    wide = torch.from_numpy(rng.standard_normal((n, (H + 2 * kv) * dim)).astype(np.float32)).cuda()
+    outw = torch.zeros((n, 2 * H * dim), device="cuda")
+    c = D.PagedKV(kp, vp, table, lens, num_heads=H)
+    q = wide[:, : H * dim]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        c.attend(q, outw[:, H * dim:])
+    side.synchronize()
+    for new in ([10, 200, 33], [11, 320, 0]):
+        if new[0] == 11:
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                c.attend(q, outw[:, H * dim:])
+            lens.copy_(i32(new))
+            g.replay()
+            torch.cuda.synchronize()
+        want, _, bound = attend64(q.reshape(n, H, dim), kp, vp, table, new, dim ** -0.5)
+        got = outw[:, H * dim:].reshape(n, H, dim).cpu().numpy()
+        assert np.all(np.abs(got - want) <= bound)
+        assert not outw[:, : H * dim].any()
+
+
+def test_attend_same_bits_each_time(D):
+    import torch
+    rng = np.random.default_rng(6)
+    lens = list(rng.integers(1, 3000, 9))
+    kp, vp, table = make_cache(rng, "bf16", 9, 200, 16, 2, 128)
+    q = torch.from_numpy(rng.standard_normal((9, 16, 128)).astype(np.float32)).cuda()
+    w = torch.zeros((9, 2, 3200), device="cuda")
+    c = D.PagedKV(kp, vp, table, i32(lens), num_heads=16, weights=w)
+    got = []
+    for _ in range(5):
+        out = torch.empty((9, 16, 128), device="cuda")
+        w.zero_()
+        c.attend(q, out, accumulate=True)
+        got.append((out.cpu().numpy(), w.cpu().numpy().copy()))
+    for o, x in got[1:]:
+        np.testing.assert_array_equal(o, got[0][0])
+        np.testing.assert_array_equal(x, got[0][1])
+
+
+def test_attend_long_offsets(D):
+    """A pool whose offsets pass 2^31 elements: the last pages are the ones in use."""
+    import torch
+    page, kv, dim = 64, 8, 128
+    pages = (2 ** 31 + 2 ** 24) // (page * kv * dim)
+    kp = torch.empty((pages, page, kv, dim), dtype=torch.float8_e4m3fn, device="cuda")
+    vp = torch.empty_like(kp)
+    rng = np.random.default_rng(8)
+    used = [pages - 1, pages - 3, pages - 2, 0]
+    for p in used:
+        for t in (kp, vp):
+            t[p] = torch.from_numpy(rng.standard_normal((page, kv, dim)).astype(np.float32)).cuda().to(torch.float8_e4m3fn)
+    table = i32([used])
+    q = torch.from_numpy(rng.standard_normal((1, 16, dim)).astype(np.float32)).cuda()
+    out = torch.empty((1, 16, dim), device="cuda")
+    D.PagedKV(kp, vp, table, i32([250]), num_heads=16).attend(q, out)
+    small = [t[torch.tensor(used, device="cuda")] if False else torch.stack([t[p] for p in used]) for t in (kp, vp)]
+    want, _, bound = attend64(q, small[0], small[1], i32([[0, 1, 2, 3]]), [250], dim ** -0.5)
+    assert np.all(np.abs(out.cpu().numpy() - want) <= bound)
+
+
+# ---------------------------------------------------------------- append
+
+
+def stored64(x, dtype, scale):
+    """x / scale in 64 bits, and half a step of the type there."""
+    y = x / scale
+    if dtype == "f8":
+        y = np.clip(y, -448, 448)
+        return y, np.maximum(np.abs(y) * 2.0 ** -4, 2.0 ** -10)
+    if dtype == "f16":
+        return y, np.maximum(np.abs(y) * 2.0 ** -11, 2.0 ** -25)
+    return y, np.abs(y) * (2.0 ** -8 if dtype == "bf16" else 2.0 ** -23)
+
+
+def rotate64(x, pos, theta):
+    d = x.shape[-1]
+    half = d // 2
+    y = x.copy()
+    if theta > 0:
+        a = pos[:, None] * theta ** (-2.0 * np.arange(half) / d)
+        c, s = np.cos(a)[:, None], np.sin(a)[:, None]
+        y[..., :half] = x[..., :half] * c - x[..., half: 2 * half] * s
+        y[..., half: 2 * half] = x[..., :half] * s + x[..., half: 2 * half] * c
+    return y
+
+
+def rotation_bound(x, theta):
+    """The angle is held to 1.6 * 2^-24 (32-bit half turns), sine and cosine to an ulp, and two products
+    and a sum round: 6 * 2^-24 of the pair."""
+    half = x.shape[-1] // 2
+    m = np.abs(x)
+    b = np.zeros_like(m)
+    if theta > 0:
+        b[..., : half] = b[..., half: 2 * half] = 6 * EPS * (m[..., :half] + m[..., half: 2 * half])
+    return b
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("kv,H,dim,page,theta,new,start", [
+    (2, 4, 128, 16, 10000.0, [3, 0, 17, 1], [0, 5, 31, 100]),
+    (1, 1, 64, 1, 500000.0, [9], [0]),
+    (3, 3, 33, 7, 10000.0, [2, 20], [6, 0]),
+    (4, 8, 80, 24, 0.0, [1, 1, 1], [23, 24, 25]),
+    (2, 2, 2, 16, 10000.0, [40], [3]),
+    (8, 32, 256, 64, 10000.0, [5, 0, 0], [1, 2, 3]),
+])
+def test_append(D, dtype, kv, H, dim, page, theta, new, start):
+    import torch
+    rng = np.random.default_rng(dim + len(new))
+    n = len(new)
+    total, per = sum(new), max(1, -(-max(a + b for a, b in zip(new, start)) // page))
+    kp, vp, table = make_cache(rng, dtype, n, per, page, kv, dim, layout="heads" if dim == 80 else "slots")
+    before = [t.float().cpu().numpy().copy() for t in (kp, vp)]
+    cu = np.concatenate([[0], np.cumsum(new)])
+    seen = [s + 1000000 * i for i, s in enumerate(start)]
+    k, v = (rng.standard_normal((total, kv, dim)).astype(np.float32) * 3 for _ in range(2))
+    q = rng.standard_normal((total, H, dim)).astype(np.float32)
+    if dtype == "f8":
+        v[0, 0, 0] = 1e6
+    gk, gv, gq = (torch.from_numpy(t).cuda() for t in (k, v, q))
+    positions = i32(np.full((n, kv, per * page), -5))
+    weights = torch.full((n, kv, per * page), 2.0, device="cuda")
+    lens, gseen = i32([0] * n), i32([0] * n)
+    ks, vs = (0.25, 0.125) if dtype == "f8" else (1.0, 1.0)
+    c = D.PagedKV(kp, vp, table, lens, num_heads=H, seen=gseen, weights=weights, positions=positions, k_scale=ks, v_scale=vs)
+    q_out = torch.empty_like(gq)
+    c.append(gk, gv, q=gq, q_out=q_out, cu_tokens=i32(cu), theta=theta, start=i32(start), start_seen=i32(seen))
+    c.check_error()
+    assert lens.tolist() == [a + b for a, b in zip(start, new)] and gseen.tolist() == [a + b for a, b in zip(seen, new)]
+    pos = np.concatenate([np.arange(s, s + m) for s, m in zip(seen, new)]).astype(np.float64)
+    wk, wq = rotate64(k.astype(np.float64), pos, theta), rotate64(q.astype(np.float64), pos, theta)
+    assert np.all(np.abs(q_out.cpu().numpy() - wq) <= rotation_bound(q, theta) + EPS * np.abs(wq))
+    t = table.cpu().numpy()
+    for pool, want, scale, bound, old in ((kp, wk, ks, rotation_bound(k, theta), before[0]),
+                                          (vp, v.astype(np.float64), vs, 0.0, before[1])):
+        got = pool.float().cpu().numpy()
+        exp, tol = old.copy(), np.zeros_like(old)
+        st, half = stored64(want, dtype, scale)
+        for b in range(n):
+            for i in range(new[b]):
+                j = start[b] + i
+                exp[t[b, j // page], j % page] = st[cu[b] + i]
+                tol[t[b, j // page], j % page] = (half + bound / scale * (1 + 2.0 ** -4))[cu[b] + i]
+        assert np.all(np.abs(got - exp) <= tol)
+    p, w = positions.cpu().numpy(), weights.cpu().numpy()
+    for b in range(n):
+        here = slice(start[b], start[b] + new[b])
+        assert np.all(p[b, :, here] == np.arange(seen[b], seen[b] + new[b])) and np.all(w[b, :, here] == 0)
+        p[b, :, here], w[b, :, here] = -5, 2.0
+    assert np.all(p == -5) and np.all(w == 2.0)
+
+
+def test_append_in_place_from_fused_rows(D):
+    """One token a sequence from rows that hold q, k and v side by side, q rotated in place, lengths
+    advanced by the call; two calls follow one another."""
+    import torch
+    rng = np.random.default_rng(2)
+    n, H, kv, dim, page, per = 5, 4, 2, 64, 16, 4
+    kp, vp, table = make_cache(rng, "f32", n, per, page, kv, dim)
+    lens = i32([0, 15, 16, 40, 62])
+    c = D.PagedKV(kp, vp, table, lens, num_heads=H)
+    start = np.array([0, 15, 16, 40, 62])
+    for step in range(2):
+        rows = rng.standard_normal((n, (H + 2 * kv) * dim)).astype(np.float32)
+        g = torch.from_numpy(rows).cuda()
+        q, k, v = g[:, : H * dim], g[:, H * dim: (H + kv) * dim], g[:, (H + kv) * dim:]
+        c.append(k, v, q=q, q_out=q, theta=10000.0)
+        assert lens.tolist() == list(start + step + 1)
+        want = rotate64(rows[:, : H * dim].reshape(n, H, dim).astype(np.float64), (start + step).astype(np.float64), 10000.0)
+        np.testing.assert_allclose(q.reshape(n, H, dim).cpu().numpy(), want, atol=3e-6)
+        for b in range(n):
+            j = int(start[b]) + step
+            page_id = int(table[b, j // page])
+            assert torch.equal(vp[page_id, j % page], v[b].reshape(kv, dim))
+    c.check_error()
+
+
+def test_append_past_the_end_and_bad_pages_are_reported(D, wb):
+    import torch
+    rng = np.random.default_rng(9)
+    n, kv, dim, page, per = 3, 2, 64, 16, 2
+    kp, vp, table = make_cache(rng, "bf16", n, per, page, kv, dim, fill="nan")
+    k = torch.ones((n, kv, dim), device="cuda")
+    lens = i32([32, 31, -4])
+    c = D.PagedKV(kp, vp, table, lens, num_heads=2)
+    c.append(k, k)
+    with pytest.raises(wb.WelvetError) as e:
+        c.check_error()
+    assert e.value.code == 1 and "slots" in str(e.value)
+    c.check_error()  # cleared
+    assert lens.tolist()[:2] == [32, 32]
+    written = torch.isfinite(kp.float()).all(-1).sum().item()
+    assert written == kv  # one row of the sequence that had room
+    for bad in (-1, 10 ** 6, 2 ** 31 - 1):
+        broken = table.clone()
+        broken[1, 0] = bad
+        lens = i32([3, 3, 3])
+        c = D.PagedKV(kp, vp, broken, lens, num_heads=2)
+        c.append(k, k)
+        with pytest.raises(wb.WelvetError) as e:
+            c.check_error()
+        assert "page" in str(e.value)
+        q, out = torch.ones((n, 2, dim), device="cuda"), torch.empty((n, 2, dim), device="cuda")
+        kp.zero_(), vp.fill_(1.0)
+        c.attend(q, out)
+        with pytest.raises(wb.WelvetError):
+            c.check_error()
+        assert torch.all(out[0] == 1.0) and torch.all(out[1] == 0.0)  # its slots are as if masked
+    # entries past the length are never looked at
+    broken = table.clone()
+    broken[:, 1] = -1
+    c = D.PagedKV(kp, vp, broken, i32([16, 15, 1]), num_heads=2)
+    c.attend(q, out)
+    c.check_error()
+
+
+# ---------------------------------------------------------------- eviction
+
+
+def evict_reference(kp, vp, table, lens, seen, weights, positions, keep, budget, sinks, recent):
+    k, v, w, p = kp.copy(), vp.copy(), weights.copy(), positions.copy()
+    page, out = kp.shape[1], list(lens)
+    for b, n in enumerate(lens):
+        if n <= budget:
+            continue
+        out[b] = keep
+        for h in range(w.shape[1]):
+            rank = sorted(range(n), key=lambda j: (not (positions[b, h, j] < sinks or positions[b, h, j] >= seen[b] - recent),
+                                                   math.inf if math.isnan(weights[b, h, j]) else -float(weights[b, h, j]), j))
+            stays = set(rank[:keep])
+            fill = [j for j in range(keep) if j not in stays]
+            take = [j for j in range(keep, n) if j in stays]
+            assert len(fill) == len(take)
+            for to, frm in zip(fill, take):
+                a, c = (table[b, to // page], to % page, h), (table[b, frm // page], frm % page, h)
+                k[a], v[a] = kp[c], vp[c]
+                w[b, h, to], p[b, h, to] = weights[b, h, frm], positions[b, h, frm]
+    return k, v, w, p, out
+
+
+@pytest.mark.parametrize("dtype,kv,dim,page,lens,keep,budget,sinks,recent,kind", [
+    ("bf16", 2, 64, 16, [100, 33, 64, 65, 0], 32, 32, 4, 8, "random"),
+    ("f32", 1, 8, 4, [7, 3, 2], 1, 1, 0, 0, "random"),
+    ("f8", 3, 32, 16, [500, 499], 250, 499, 2, 100, "random"),
+    ("f16", 2, 33, 5, [41, 80], 40, 40, 0, 3, "ties"),
+    ("bf16", 1, 128, 16, [3000, 2048, 1025], 1024, 1024, 4, 200, "zeros"),
+    ("f32", 2, 20, 16, [50, 90], 30, 40, 1, 1, "special"),
+    ("f8", 2, 64, 64, [9000, 5000], 4999, 5000, 16, 512, "random"),
+    ("bf16", 2, 64, 16, [70], 60, 60, 20, 40, "random"),
+    ("bf16", 2, 64, 16, [70], 69, 69, 0, 0, "negative"),
+])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict(D, dtype, kv, dim, page, lens, keep, budget, sinks, recent, kind, in_place):
+    import torch
+    rng = np.random.default_rng(keep + dim)
+    n, per = len(lens), -(-max(lens) // page) + 1
+    S = per * page
+    kp, vp, table = make_cache(rng, dtype, n, per, page, kv, dim, layout="heads" if dim == 64 else "slots")
+    w = rng.lognormal(-4, 3, (n, kv, S)).astype(np.float32)
+    if kind == "ties":
+        w = rng.integers(0, 3, (n, kv, S)).astype(np.float32)
+    elif kind == "zeros":
+        w[rng.random(w.shape) < 0.8] = 0.0
+        w[rng.random(w.shape) < 0.2] = -0.0
+    elif kind == "special":
+        w[rng.random(w.shape) < 0.3] = np.nan
+        w[rng.random(w.shape) < 0.1] = np.inf
+        w[rng.random(w.shape) < 0.1] = -np.inf
+    elif kind == "negative":
+        w = -w
+    seen = np.array([2 * x + 3 for x in lens], np.int32)
+    pos = np.zeros((n, kv, S), np.int32)
+    for b in range(n):
+        for h in range(kv):
+            pos[b, h, : lens[b]] = rng.permutation(max(1, seen[b]))[: lens[b]]
+    bits = {"f32": torch.int32, "f16": torch.int16, "bf16": torch.int16, "f8": torch.uint8}[dtype]
+    view = lambda t: (t.transpose(1, 2).view(bits).transpose(1, 2) if dim == 64 else t.view(bits))  # noqa: E731
+    k0, v0 = view(kp).cpu().numpy().copy(), view(vp).cpu().numpy().copy()
+    gl, gw, gp = i32(lens), torch.from_numpy(w).cuda(), i32(pos)
+    if in_place:
+        lens_o, w_o, p_o = gl, gw, gp
+        args = {}
+    else:
+        lens_o, w_o, p_o = i32([0] * n), torch.full_like(gw, -1.0), torch.full_like(gp, -1)
+        args = dict(lens_in=gl, weights_in=gw, positions_in=gp)
+    c = D.PagedKV(kp, vp, table, lens_o, num_heads=kv, seen=i32(seen), weights=w_o, positions=p_o)
+    c.evict(keep, budget=budget, sinks=sinks, recent=recent, **args)
+    c.check_error()
+    k, v, ww, pp, out = evict_reference(k0, v0, table.cpu().numpy(), lens, seen, w, pos, keep, budget, sinks, recent)
+    assert lens_o.tolist() == out
+    np.testing.assert_array_equal(view(kp).cpu().numpy(), k)
+    np.testing.assert_array_equal(view(vp).cpu().numpy(), v)
+    gotw, gotp = w_o.cpu().numpy().view(np.int32), p_o.cpu().numpy()
+    for b in range(n):
+        np.testing.assert_array_equal(gotw[b, :, : out[b]], ww.view(np.int32)[b, :, : out[b]])
+        np.testing.assert_array_equal(gotp[b, :, : out[b]], pp[b, :, : out[b]])
+        if not in_place:
+            assert np.all(w_o.cpu().numpy()[b, :, out[b]:] == -1.0) and np.all(gotp[b, :, out[b]:] == -1)
+
+
+def test_cache_refusals(D, wb):
+    """What the host can see is refused before any launch (status 1 or 2, or a ValueError)."""
+    import torch
+    rng = np.random.default_rng(1)
+    kp, vp, table = make_cache(rng, "bf16", 2, 4, 16, 2, 64)
+    lens = i32([3, 3])
+    for bad in (dict(num_heads=3), dict(num_heads=0), dict(num_heads=4, k_scale=0.0), dict(num_heads=4, v_scale=float("nan")),
+                dict(num_heads=4, positions=i32(np.zeros((2, 2, 64))))):
+        with pytest.raises(wb.WelvetError) as e:
+            D.PagedKV(kp, vp, table, lens, **bad)
+        assert e.value.code == 1
+    with pytest.raises(wb.WelvetError) as e:
+        big = torch.zeros((2, 4, 1, 264), device="cuda")
+        D.PagedKV(big, big.clone(), table, lens, num_heads=1)
+    assert e.value.code == 2
+    for args in ((kp, vp.float(), table, lens), (kp.to(torch.float64), vp.to(torch.float64), table, lens),
+                 (kp, vp, table.long(), lens), (kp, vp, table, lens.long()), (kp, vp, table, i32([1])),
+                 (kp.cpu(), vp.cpu(), table, lens), (kp[..., ::2], vp[..., ::2], table, lens)):
+        with pytest.raises(ValueError):
+            D.PagedKV(*args, num_heads=4)
+    c = D.PagedKV(kp, vp, table, lens, num_heads=4)
+    q, out, k = torch.zeros((2, 4, 64), device="cuda"), torch.zeros((2, 4, 64), device="cuda"), torch.zeros((2, 2, 64), device="cuda")
+    for f in (lambda: c.attend(q, out, accumulate=True), lambda: c.attend(q, out, window=-1),
+              lambda: c.attend(q, out, scale=float("inf")), lambda: c.evict(3), lambda: c.append(k[:1], k[:1]),
+              lambda: c.append(k, k, theta=float("nan")), lambda: c.append(k, k, start_seen=lens)):
+        with pytest.raises(wb.WelvetError) as e:
+            f()
+        assert e.value.code == 1
+    for f in (lambda: c.attend(q[:1], out), lambda: c.attend(q.double(), out), lambda: c.attend(q[:, :, :32], out),
+              lambda: c.append(k, k[:1]), lambda: c.append(k, k, q=q), lambda: c.attend(q.cpu(), out),
+              lambda: c.append(k, k, cu_tokens=i32([0, 2]))):
+        with pytest.raises(ValueError):
+            f()
+    w = torch.zeros((2, 2, 64), device="cuda")
+    c = D.PagedKV(kp, vp, table, lens, num_heads=4, seen=i32([3, 3]), weights=w, positions=i32(np.zeros((2, 2, 64))))
+    for a in (dict(keep=0), dict(keep=4, budget=3), dict(keep=4, sinks=3, recent=2), dict(keep=4, sinks=-1)):
+        with pytest.raises(wb.WelvetError) as e:
+            c.evict(**a)
+        assert e.value.code == 1
+    c.check_error()
+
+
+def test_append_nothing(D):
+    """No new token at all: lengths are carried over, nothing is written."""
+    import torch
+    rng = np.random.default_rng(4)
+    kp, vp, table = make_cache(rng, "bf16", 2, 4, 16, 2, 64)
+    old = kp.clone()
+    lens = i32([0, 0])
+    c = D.PagedKV(kp, vp, table, lens, num_heads=4)
+    k = torch.zeros((0, 2, 64), device="cuda")
+    c.append(k, k, cu_tokens=i32([0, 0, 0]), start=i32([5, 9]))
+    assert lens.tolist() == [5, 9] and torch.equal(kp, old)

@@ -1,0 +1,55 @@
+// kvcache.cuh -- conversions of the key-value cache's storage types, and small helpers.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include <cstdint>
+#include <type_traits>
+
+namespace wb {
+
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__nv_fp8_e4m3 x) { return static_cast<float>(x); }
+
+// Round to nearest even; E4M3 saturates at +-448 (NaN stays NaN). E4M3 pages hold the OCP format
+// with its subnormals, unlike the weight codec, which follows the reference's flush to zero.
+template <typename T>
+__device__ __forceinline__ T to_stored(float x) {
+  if constexpr (std::is_same_v<T, float>) return x;
+  else if constexpr (std::is_same_v<T, __half>) return __float2half_rn(x);
+  else if constexpr (std::is_same_v<T, __nv_bfloat16>) return __float2bfloat16_rn(x);
+  else return __nv_fp8_e4m3(x);
+}
+
+// Four values x * s to consecutive elements (aligned to four elements).
+template <typename T>
+__device__ __forceinline__ void store4(T* dst, const float (&x)[4], float s) {
+  if constexpr (std::is_same_v<T, float>) {
+    *reinterpret_cast<float4*>(dst) = make_float4(x[0] * s, x[1] * s, x[2] * s, x[3] * s);
+  } else if constexpr (sizeof(T) == 2) {
+    union { T t[4]; uint2 u; } o;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o.t[i] = to_stored<T>(x[i] * s);
+    *reinterpret_cast<uint2*>(dst) = o.u;
+  } else {
+    const __nv_fp8x4_e4m3 o(make_float4(x[0] * s, x[1] * s, x[2] * s, x[3] * s));
+    *reinterpret_cast<__nv_fp8x4_e4m3*>(dst) = o;
+  }
+}
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+// The MHA cell's slope of head h (src/cuda/kernels.cu:520-528): 2^(-8 (h + 1) / heads).
+__device__ __forceinline__ float alibi_slope(int h, int heads) {
+  return exp2f(-8.0f * static_cast<float>(h + 1) / static_cast<float>(heads));
+}
+
+} // namespace wb
