@@ -582,3 +582,54 @@ def test_append_nothing(D):
     k = torch.zeros((0, 2, 64), device="cuda")
     c.append(k, k, cu_tokens=i32([0, 0, 0]), start=i32([5, 9]))
     assert lens.tolist() == [5, 9] and torch.equal(kp, old)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("dim", [16, 48, 56, 112, 120, 192, 248])
+def test_attend_dims_between_the_tiles(D, dtype, dim):
+    """Head widths that fill a row of shared memory only in part."""
+    import torch
+    rng = np.random.default_rng(dim)
+    H, kv, page, lens = 4, 2, 16, [70, 16, 129]
+    kp, vp, table = make_cache(rng, dtype, 3, 9, page, kv, dim)
+    q = torch.from_numpy(rng.standard_normal((3, H, dim)).astype(np.float32)).cuda()
+    out = torch.empty((3, H, dim), device="cuda")
+    D.PagedKV(kp, vp, table, i32(lens), num_heads=H).attend(q, out)
+    want, _, bound = attend64(q, kp, vp, table, lens, 1.0 / math.sqrt(dim))
+    assert np.all(np.abs(out.cpu().numpy() - want) <= bound)
+
+
+@pytest.mark.parametrize("dim", [64, 33])
+def test_attend_accumulates_within_the_window(D, dim):
+    import torch
+    rng = np.random.default_rng(21)
+    H, kv, page, lens, window = 4, 2, 16, [1000, 30], 100
+    kp, vp, table = make_cache(rng, "bf16", 2, 64, page, kv, dim)
+    q = torch.from_numpy(rng.standard_normal((2, H, dim)).astype(np.float32)).cuda()
+    out = torch.empty((2, H, dim), device="cuda")
+    w = torch.full((2, kv, 1024), 0.5, device="cuda")
+    c = D.PagedKV(kp, vp, table, i32(lens), num_heads=H, weights=w)
+    c.attend(q, out)  # leaves scores of all slots behind
+    c.attend(q, out, accumulate=True, window=window)
+    _, ws, _ = attend64(q, kp, vp, table, lens, 1.0 / math.sqrt(dim), window)
+    got = w.cpu().numpy()
+    for b, L in enumerate(lens):
+        np.testing.assert_allclose(got[b, :, :L] - 0.5, ws[b].reshape(kv, 2, L).sum(1), rtol=2e-4, atol=4 * EPS)
+        assert np.all(got[b, :, L:] == 0.5) and np.all(got[b, :, : max(0, L - window)] == 0.5)
+
+
+def test_attend_many_sequences(D):
+    """More sequences than a block has threads, most of them empty or a token long."""
+    import torch
+    rng = np.random.default_rng(22)
+    n, H, kv, dim, page = 700, 2, 1, 64, 16
+    lens = [int(x) for x in rng.choice([0, 1, 2, 17, 64, 65, 300], n)]
+    kp, vp, table = make_cache(rng, "f16", n, 19, page, kv, dim)
+    q = torch.from_numpy(rng.standard_normal((n, H, dim)).astype(np.float32)).cuda()
+    out = torch.full((n, H, dim), float("nan"), device="cuda")
+    c = D.PagedKV(kp, vp, table, i32(lens), num_heads=H)
+    for _ in range(3):
+        c.attend(q, out)
+    pages = [t.float().cpu() for t in (kp, vp)]
+    want, _, bound = attend64(q, pages[0], pages[1], table, lens, 0.125)
+    assert np.all(np.abs(out.cpu().numpy() - want) <= bound)

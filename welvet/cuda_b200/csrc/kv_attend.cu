@@ -1,0 +1,877 @@
+// kv_attend.cu -- attention of one new token per sequence over a paged key-value cache (sm_100a).
+//
+// z_j = scale q.k_j - slope (p_q - p_j), w = softmax(z), o = sum_j w_j v_j, in one pass over the
+// keys with a running maximum and sum; all scores are held in units of log2, so that a weight is
+// one exp2. HBM bound: a key and a value row are read once for all the query heads that share
+// them, 2 sizeof(T) head_dim bytes against 4 head_dim flops per query head.
+#include "kvcache.cuh"
+#include "kvcache.hpp"
+#include "pipeline.cuh"
+
+#include <algorithm>
+#include <cmath>
+
+namespace wb {
+namespace {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct AttendParams {
+  KvAttendArgs a;
+  KvView c;
+  int splits;      // simple form
+  float* part;     // partial results: o, m, l
+  float* scores;   // with accumulate: [num_seqs][num_heads][max_slots], units of log2
+  float* lse;      // [num_seqs][num_heads]
+  // tiled form
+  int group;       // query heads per key-value head
+  int units;       // num_kv * head groups of 8: work units of a sequence
+  int head_groups;
+  int page_shift;  // log2(page_size), or -1
+  int* counters;   // [num_seqs][units], zero between calls
+};
+
+// ---------------------------------------------------------------- one query head a block
+
+constexpr int kSimpleWarps = 4;
+constexpr int kSimpleDims = 8;  // dims a lane holds: head_dim <= 256
+
+// The form for layouts that 16-byte copies cannot serve (rows off 16-byte boundaries, a head_dim
+// that is no multiple of 8 elements). A block takes one split of one (sequence, query head); a warp
+// a key at a time, lanes over the head's dims, one pass with the running maximum and sum. Keys
+// shared by the heads of a group are read again for each head.
+template <typename T>
+__global__ void __launch_bounds__(32 * kSimpleWarps) k_attend_simple(const __grid_constant__ AttendParams p) {
+  __shared__ float s_m[kSimpleWarps], s_l[kSimpleWarps];
+  __shared__ float s_o[kSimpleWarps][32 * kSimpleDims];
+  const KvView& c = p.c;
+  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int D = c.head_dim, kv = h / (c.num_heads / c.num_kv);
+  int len = c.lens[b];
+  if (len < 0 || len > c.max_slots) {
+    if (threadIdx.x == 0) atomicCAS(c.err, 0, kKvErrSlot);
+    len = len < 0 ? 0 : c.max_slots;
+  }
+  const int64_t per = (len + p.splits - 1) / p.splits;
+  const int j0 = static_cast<int>(per * split < len ? per * split : len);
+  const int j1 = static_cast<int>(per * (split + 1) < len ? per * (split + 1) : len);
+  const int q_pos = c.positions ? c.seen[b] - 1 : len - 1;
+  const int64_t rec = (static_cast<int64_t>(b) * c.num_kv + kv) * c.max_slots;
+  const float slope = p.a.alibi ? alibi_slope(h, c.num_heads) * kLog2e : 0.0f;
+  float q[kSimpleDims], o[kSimpleDims];
+#pragma unroll
+  for (int i = 0; i < kSimpleDims; ++i) {
+    const int d = lane + 32 * i;
+    q[i] = d < D ? p.a.q[b * p.a.q_ld + static_cast<int64_t>(h) * D + d] * (p.a.scale * c.k_scale * kLog2e) : 0.0f;
+    o[i] = 0.0f;
+  }
+  float m = -INFINITY, l = 0.0f;
+  for (int j = j0 + w; j < j1; j += kSimpleWarps) {
+    const int pos = c.positions ? c.positions[rec + j] : j;
+    const int page = c.table[b * c.table_stride + j / c.page_size];
+    bool ok = page >= 0 && page < c.num_pages;
+    if (!ok && lane == 0) atomicCAS(c.err, 0, kKvErrPage);
+    if (p.a.window > 0 && pos <= q_pos - p.a.window) ok = false;
+    float z = -INFINITY;
+    if (ok) {
+      const T* kr = reinterpret_cast<const T*>(c.k.base) + page * c.k.page + (j % c.page_size) * c.k.slot + kv * c.k.head;
+      float dot = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kSimpleDims; ++i) {
+        const int d = lane + 32 * i;
+        if (d < D) dot += q[i] * to_float(kr[d]);
+      }
+      z = warp_sum(dot) - slope * static_cast<float>(q_pos - pos);
+      const T* vr = reinterpret_cast<const T*>(c.v.base) + page * c.v.page + (j % c.page_size) * c.v.slot + kv * c.v.head;
+      const float m_new = fmaxf(m, z);
+      const float ref = m_new == -INFINITY ? 0.0f : m_new;
+      const float e = exp2f(z - ref), corr = exp2f(m - ref);
+      l = l * corr + e;
+#pragma unroll
+      for (int i = 0; i < kSimpleDims; ++i) {
+        const int d = lane + 32 * i;
+        if (d < D) o[i] = o[i] * corr + e * to_float(vr[d]);
+      }
+      m = m_new;
+    }
+    if (p.a.accumulate && lane == 0)
+      p.scores[(static_cast<int64_t>(b) * c.num_heads + h) * c.max_slots + j] = ok ? z : -INFINITY;
+  }
+  if (lane == 0) {
+    s_m[w] = m;
+    s_l[w] = l;
+  }
+#pragma unroll
+  for (int i = 0; i < kSimpleDims; ++i) s_o[w][lane + 32 * i] = o[i];
+  __syncthreads();
+  float mm = s_m[0];
+#pragma unroll
+  for (int i = 1; i < kSimpleWarps; ++i) mm = fmaxf(mm, s_m[i]);
+  const float ref = mm == -INFINITY ? 0.0f : mm;
+  float* dst = p.part + ((static_cast<int64_t>(b) * c.num_heads + h) * p.splits + split) * (D + 2);
+  for (int d = threadIdx.x; d < D; d += 32 * kSimpleWarps) {
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSimpleWarps; ++i) v += s_o[i][d] * exp2f(s_m[i] - ref);
+    dst[d] = v;
+  }
+  if (threadIdx.x == 0) {
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSimpleWarps; ++i) v += s_l[i] * exp2f(s_m[i] - ref);
+    dst[D] = mm;
+    dst[D + 1] = v;
+  }
+}
+
+// Joins the splits of one (sequence, query head) in split order. A row that nothing is allowed
+// in has l = 0 and m = -inf from every split: its output is zero.
+__global__ void k_attend_join(const __grid_constant__ AttendParams p) {
+  const KvView& c = p.c;
+  const int h = blockIdx.x, b = blockIdx.y, D = c.head_dim;
+  const float* src = p.part + (static_cast<int64_t>(b) * c.num_heads + h) * p.splits * (D + 2);
+  float m = -INFINITY;
+  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, src[s * (D + 2) + D]);
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float l = 0.0f;
+  for (int s = 0; s < p.splits; ++s) l += src[s * (D + 2) + D + 1] * exp2f(src[s * (D + 2) + D] - ref);
+  const float inv = l == 0.0f ? 0.0f : c.v_scale / l;
+  for (int d = threadIdx.x; d < D; d += blockDim.x) {
+    float v = 0.0f;
+    for (int s = 0; s < p.splits; ++s) v += src[s * (D + 2) + d] * exp2f(src[s * (D + 2) + D] - ref);
+    p.a.out[b * p.a.out_ld + static_cast<int64_t>(h) * D + d] = v * inv;
+  }
+  if (threadIdx.x == 0 && p.a.accumulate) p.lse[static_cast<int64_t>(b) * c.num_heads + h] = l == 0.0f ? INFINITY : ref + log2f(l);
+}
+
+// weights[j] = weights_in[j] + sum over the group's heads of 2^(score - lse), heads in order.
+__global__ void k_attend_weights(const __grid_constant__ AttendParams p) {
+  const KvView& c = p.c;
+  const int kv = blockIdx.y, b = blockIdx.z, group = c.num_heads / c.num_kv;
+  int len = c.lens[b];
+  len = len < 0 ? 0 : (len > c.max_slots ? c.max_slots : len);
+  const int lo = p.a.window > 0 && !c.positions ? len - p.a.window : 0;  // slots below have no score
+  const int64_t rec = (static_cast<int64_t>(b) * c.num_kv + kv) * c.max_slots;
+  const int64_t row = static_cast<int64_t>(b) * c.num_heads + kv * group;
+  for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < len; j += gridDim.x * blockDim.x) {
+    float s = p.a.weights_in[rec + j];
+    for (int i = 0; i < group && j >= lo; ++i) s += exp2f(p.scores[(row + i) * c.max_slots + j] - p.lse[row + i]);
+    c.weights[rec + j] = s;
+  }
+}
+
+// ---------------------------------------------------------------- tiled form
+//
+// Eight query heads of one key-value head are the rows of a warp's m16n8 MMAs, twice: rows 0-7
+// carry the leading part of each head's query (or weights), rows 8-15 the rest of it, so that one
+// MMA with the key rows as its B operand gives both partial products and their sum is two
+// registers of the same thread. Parts by type of the pages:
+//   f16, E4M3 (exact in f16)  two f16 parts, 22 bits, of the query scaled by a power of two and of
+//                             the weights scaled by 2^15 (f16's subnormals then lie below 2^-39)
+//   bf16                      three bf16 parts, 24 bits: the third in a second MMA
+//   f32                       two tf32 parts of both operands, 22 bits
+// The register-path MMA is used, not tcgen05: with 8 query rows an M = 128 tile would be 94 %
+// padding, and at HBM speed the warp MMAs of a 16-key tile take about a third of its time.
+//
+// Work is cut into tiles of 16 keys per warp; the grid's blocks take equal runs of all tiles of
+// all (sequence, key-value head) units, so that ragged lengths balance. A unit that lies within
+// one block is finished there; otherwise each block leaves its partial (o, m, l) and the last one
+// to arrive joins them in block order, which keeps the result independent of timing.
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+// 16 bytes, or zeros where `bytes` is 0.
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kN>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(kN) : "memory"); }
+
+__device__ __forceinline__ void mma(__half, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma(__nv_bfloat16, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma(float, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// x = part 0 + part 1 in tf32 (22 bits); the MMA reads the upper 19 bits of part 1.
+__device__ __forceinline__ void tf32_parts(float x, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  lo = __float_as_uint(x - __uint_as_float(hi));
+}
+
+// Two values as packed parts of the MMA type.
+__device__ __forceinline__ void parts2(float x, float y, uint32_t (&part)[2]) {  // f16
+  const __half2 h = __floats2half2_rn(x, y);
+  const float2 f = __half22float2(h);
+  const __half2 l = __floats2half2_rn(x - f.x, y - f.y);
+  part[0] = *reinterpret_cast<const uint32_t*>(&h);
+  part[1] = *reinterpret_cast<const uint32_t*>(&l);
+}
+__device__ __forceinline__ void parts3(float x, float y, uint32_t (&part)[3]) {  // bf16
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x, y);
+    const float2 f = __bfloat1622float2(h);
+    x -= f.x;
+    y -= f.y;
+    part[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+
+__device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+
+template <typename T, int DP>
+struct Tiled {
+  static constexpr bool kF32 = std::is_same_v<T, float>;
+  static constexpr bool kBF16 = std::is_same_v<T, __nv_bfloat16>;
+  static constexpr bool kFP8 = std::is_same_v<T, __nv_fp8_e4m3>;
+  using M = std::conditional_t<kFP8, __half, T>;  // MMA operand type
+  static constexpr int kRow = DP * static_cast<int>(sizeof(T));  // bytes of a row in shared memory (at most, unpadded)
+  static constexpr int kWarps = kRow <= 512 ? 4 : 2;
+  static constexpr int kStages = kRow <= 128 ? 4 : 3;
+  static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kKeys = 16 * kWarps;  // keys of a block tile
+  static constexpr int kSets = kBF16 ? 2 : 1;
+  static constexpr int kSteps = kF32 ? DP / 8 : DP / 16;  // MMA steps over a head's dims
+  static constexpr float kBias = kF32 || kBF16 ? 0.0f : 15.0f;  // log2 of the weights' scale
+  static constexpr int kRowMax = kRow == 64 ? 80 : kRow;  // the longest pitch of a row
+  static constexpr int kRing = kStages * kWarps * 2 * 16 * kRowMax;
+  static constexpr int kSmemQ = kSets * kSteps * 512, kSmemO = 8 * DP * 4;
+  static constexpr int kSmem = kRing + kSmemQ + kSmemO;
+};
+
+// A position in the list of all tiles: sequence b, unit u, tile of the unit's nt.
+struct Cursor {
+  int b, u, tile, nt, len, lo, first;
+};
+
+__device__ __forceinline__ void cursor_seq(const AttendParams& p, int keys, Cursor& c) {
+  int len = p.c.lens[c.b];
+  len = len < 0 ? 0 : (len > p.c.max_slots ? p.c.max_slots : len);
+  c.len = len;
+  c.lo = p.a.window > 0 && !p.c.positions && len > p.a.window ? len - p.a.window : 0;
+  c.first = c.lo / keys;
+  c.nt = len > 0 ? (len + keys - 1) / keys - c.first : 1;  // an empty sequence still has its zeros to write
+}
+
+__device__ __forceinline__ void cursor_next(const AttendParams& p, int keys, Cursor& c) {
+  if (++c.tile < c.nt) return;
+  c.tile = 0;
+  if (++c.u < p.units) return;
+  c.u = 0;
+  if (++c.b < p.c.num_seqs) cursor_seq(p, keys, c);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const __grid_constant__ AttendParams p) {
+  using G = Tiled<T, DP>;
+  using M = typename G::M;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ long long s_sum[G::kWarps];
+  __shared__ long long s_off;
+  __shared__ int s_b, s_last;
+  __shared__ float s_m[G::kWarps][8], s_l[G::kWarps][8], s_mult[8];
+  __shared__ uint32_t s_ok[G::kWarps][G::kStages];
+  const KvView& c = p.c;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int D = c.head_dim;
+  const int row_bytes = D * static_cast<int>(sizeof(T)), chunks = row_bytes / 16;
+  // Rows of a multiple of 128 bytes (and rows whose pitch would not fit) are stored with their
+  // 16-byte chunks xored by the key; others with a pitch of an odd number of chunks. Both keep
+  // ldmatrix free of bank conflicts.
+  const int pad_chunks = (chunks + 1) & ~1;  // the MMAs read whole steps of 32 bytes
+  const bool swz = (row_bytes & 127) == 0 || 16 * (pad_chunks + 1) > G::kRowMax;
+  const int pitch = swz ? (row_bytes + 127) & ~127 : 16 * (pad_chunks + 1);
+  uint8_t* const ring = smem + w * (G::kStages * 32 * pitch);
+  const uint32_t ring_addr = pipe::smem_u32(ring);
+  uint4* const sq = reinterpret_cast<uint4*>(smem + G::kRing);
+  float* const so = reinterpret_cast<float*>(smem + G::kRing + G::kSmemQ);
+
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (pad_chunks != chunks) {  // columns that no copy writes
+    for (int i = lane; i < G::kStages * 32; i += 32)
+      *reinterpret_cast<uint4*>(ring + i * pitch + ((swz ? chunks ^ (i & 7) : chunks) << 4)) = make_uint4(0, 0, 0, 0);
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // this block's run of tiles
+  long long mine = 0;
+  for (int b = tid; b < c.num_seqs; b += G::kThreads) {
+    Cursor s;
+    s.b = b;
+    cursor_seq(p, G::kKeys, s);
+    if (blockIdx.x == 0 && (c.lens[b] < 0 || c.lens[b] > c.max_slots)) atomicCAS(c.err, 0, kKvErrSlot);
+    mine += s.nt;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+  if (lane == 0) s_sum[w] = mine;
+  __syncthreads();
+  long long total = 0;
+#pragma unroll
+  for (int i = 0; i < G::kWarps; ++i) total += s_sum[i];
+  total *= p.units;
+  const long long n_cta = total < gridDim.x ? total : gridDim.x;  // no block's run is empty
+  auto run_start = [&](long long i) { return i * total / n_cta; };
+  const long long t0 = run_start(blockIdx.x), t1 = run_start(blockIdx.x + 1);
+  if (blockIdx.x >= n_cta) return;
+  for (long long base = 0, acc = 0;; base += G::kThreads) {  // the sequence that t0 lies in
+    const int b = static_cast<int>(base) + tid;
+    Cursor s;
+    s.b = b;
+    s.nt = 0;
+    if (b < c.num_seqs) cursor_seq(p, G::kKeys, s);
+    const long long n = static_cast<long long>(s.nt) * p.units;
+    long long x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) s_sum[w] = x;
+    __syncthreads();
+    long long before = acc, all = 0;
+#pragma unroll
+    for (int i = 0; i < G::kWarps; ++i) {
+      if (i < w) before += s_sum[i];
+      all += s_sum[i];
+    }
+    if (before + x - n <= t0 && t0 < before + x) {
+      s_b = b;
+      s_off = t0 - (before + x - n);
+    }
+    acc += all;
+    if (t0 < acc) break;
+  }
+  __syncthreads();
+  Cursor cur;
+  cur.b = s_b;
+  cursor_seq(p, G::kKeys, cur);
+  cur.u = static_cast<int>(s_off / cur.nt);
+  cur.tile = static_cast<int>(s_off - static_cast<long long>(cur.u) * cur.nt);
+  Cursor nxt = cur;
+  long long issued = t0;
+
+  // Copies the warp's 16 keys and values of the tile at `nxt`; rows that the mask leaves out are
+  // zeros (their contents, even NaN, must not reach the sums).
+  auto issue = [&](int stage) {
+    if (issued < t1) {
+      const int kv = nxt.u / p.head_groups;
+      const int j = (nxt.first + nxt.tile) * G::kKeys + 16 * w + (lane & 15);
+      bool ok = j >= nxt.lo && j < nxt.len;
+      int64_t koff = 0, voff = 0;
+      if (ok) {
+        const int slot_page = p.page_shift >= 0 ? j >> p.page_shift : j / c.page_size;
+        const int page = c.table[nxt.b * c.table_stride + slot_page];
+        const int in = j - slot_page * c.page_size;
+        if (p.a.window > 0 && c.positions) {
+          const int64_t rec = (static_cast<int64_t>(nxt.b) * c.num_kv + kv) * c.max_slots + j;
+          ok = c.positions[rec] > c.seen[nxt.b] - 1 - p.a.window;
+        }
+        if (page < 0 || page >= c.num_pages) {
+          atomicCAS(c.err, 0, kKvErrPage);
+          ok = false;
+        }
+        if (ok) {
+          koff = (page * c.k.page + in * c.k.slot + kv * c.k.head) * static_cast<int64_t>(sizeof(T));
+          voff = (page * c.v.page + in * c.v.slot + kv * c.v.head) * static_cast<int64_t>(sizeof(T));
+        }
+      }
+      const uint32_t okm = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+      if (lane == 0) s_ok[w][stage] = okm;
+      const uint32_t dst = ring_addr + stage * 32 * pitch;
+      // eight lanes a row, four rows at a time
+#pragma unroll
+      for (int r0 = 0; r0 < 16; r0 += 4) {
+        const int r = r0 + (lane >> 3);
+        const int64_t ko = __shfl_sync(0xffffffffu, koff, r), vo = __shfl_sync(0xffffffffu, voff, r);
+        const int n = (okm >> r) & 1 ? 16 : 0;
+        for (int ch = lane & 7; ch < chunks; ch += 8) {
+          const uint32_t at = r * pitch + ((swz ? ch ^ (r & 7) : ch) << 4);
+          cp16(dst + at, c.k.base + ko + 16 * ch, n);
+          cp16(dst + 16 * pitch + at, c.v.base + vo + 16 * ch, n);
+        }
+      }
+      ++issued;
+      cursor_next(p, G::kKeys, nxt);
+    }
+    cp_commit();
+  };
+#pragma unroll
+  for (int s = 0; s < G::kStages - 1; ++s) issue(s);
+
+  float o[DP / 8][4];
+  float m = -INFINITY, l = 0.0f, mult = 0.0f, slope = 0.0f;
+  int stage = 0, q_pos = 0;
+  bool fresh = true;  // the unit's query is not in shared memory yet
+  long long unit_start = 0;
+
+  for (long long tile = t0; tile < t1; ++tile) {
+    const int kv = cur.u / p.head_groups, h0 = (cur.u - kv * p.head_groups) * 8;
+    const int heads = p.group - h0 < 8 ? p.group - h0 : 8;  // of this unit
+    const int head = kv * p.group + h0;                      // the first of them
+    if (fresh) {
+      fresh = false;
+      unit_start = tile - cur.tile;
+      q_pos = c.positions ? c.seen[cur.b] - 1 : cur.len - 1;
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+      m = -INFINITY;
+      l = 0.0f;
+      const float* q = p.a.q + cur.b * p.a.q_ld + static_cast<int64_t>(head) * D;
+      const float base = p.a.scale * c.k_scale * kLog2e;
+      if constexpr (G::kF32 || G::kBF16) {
+        if (tid < 8) s_mult[tid] = base;
+      } else {
+        // a power of two that brings the head's largest |q| to [2^13, 2^14)
+        constexpr int kPer = G::kThreads / 8;
+        const int h = tid / kPer;
+        float mx = 0.0f;
+        if (h < heads)
+          for (int d = tid % kPer; d < D; d += kPer) mx = fmaxf(mx, fabsf(q[h * D + d]));
+#pragma unroll
+        for (int x = kPer / 2; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+        int e = 0;
+        if (mx > 0.0f && mx < INFINITY) e = min(126, max(-126, 13 - ilogbf(mx)));
+        if (tid % kPer == 0) {
+          s_mult[h] = ldexpf(1.0f, e);
+        }
+      }
+      __syncthreads();
+      for (int i = tid; i < G::kSteps * 32; i += G::kThreads) {
+        const int step = i >> 5, gg = (i & 31) >> 2, tt = i & 3;
+        auto value = [&](int d) { return gg < heads && d < D ? q[gg * D + d] : 0.0f; };
+        if constexpr (G::kF32) {
+          uint32_t a[4];
+          tf32_parts(value(8 * step + tt), a[0], a[1]);
+          tf32_parts(value(8 * step + 4 + tt), a[2], a[3]);
+          sq[i] = make_uint4(a[0], a[1], a[2], a[3]);
+        } else {
+          const int d0 = 16 * step + (G::kFP8 ? 4 * tt : 2 * tt), d1 = d0 + (G::kFP8 ? 2 : 8);
+          if constexpr (G::kBF16) {
+            uint32_t x[3], y[3];
+            parts3(value(d0), value(d0 + 1), x);
+            parts3(value(d1), value(d1 + 1), y);
+            sq[i] = make_uint4(x[0], x[1], y[0], y[1]);
+            sq[G::kSteps * 32 + i] = make_uint4(x[2], 0u, y[2], 0u);
+          } else {
+            const float f = s_mult[gg];
+            uint32_t x[2], y[2];
+            parts2(value(d0) * f, value(d0 + 1) * f, x);
+            parts2(value(d1) * f, value(d1 + 1) * f, y);
+            sq[i] = make_uint4(x[0], x[1], y[0], y[1]);
+          }
+        }
+      }
+      mult = G::kF32 || G::kBF16 ? base : base / s_mult[g];
+      slope = p.a.alibi ? alibi_slope(head + g, c.num_heads) * kLog2e : 0.0f;
+      __syncthreads();
+    }
+
+    cp_wait<G::kStages - 2>();
+    __syncwarp();
+    const uint32_t kbase = ring_addr + stage * 32 * pitch, vbase = kbase + 16 * pitch;
+    const uint32_t okm = s_ok[w][stage];
+    const int j0 = (cur.first + cur.tile) * G::kKeys + 16 * w;
+
+    // scores of keys j0 + 8 n + 2 t + e for head g
+    float s[2][4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+    if constexpr (G::kF32) {
+#pragma unroll
+      for (int st = 0; st < G::kSteps; st += 2) {
+        if (8 * st < D) {
+          uint32_t a0[4], a1[4];
+          *reinterpret_cast<uint4*>(a0) = sq[st * 32 + lane];
+          *reinterpret_cast<uint4*>(a1) = sq[(st + 1) * 32 + lane];
+#pragma unroll
+          for (int n = 0; n < 2; ++n) {
+            // four chunks (16 dims) of eight keys
+            const int r = 8 * n + (lane & 7), ch = 2 * st + (lane >> 3);
+            uint32_t k[4], hi[4], lo[4];
+            ldsm4(k, kbase + r * pitch + ((swz ? ch ^ (r & 7) : ch) << 4));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) tf32_parts(__uint_as_float(k[e]), hi[e], lo[e]);
+            mma(M(), s[n], a0, hi[0], hi[1]);
+            mma(M(), s[n], a0, lo[0], lo[1]);
+            if (8 * st + 8 < D) {
+              mma(M(), s[n], a1, hi[2], hi[3]);
+              mma(M(), s[n], a1, lo[2], lo[3]);
+            }
+          }
+        }
+      }
+    } else if constexpr (G::kFP8) {
+#pragma unroll
+      for (int st = 0; st < G::kSteps; st += 2) {
+        if (16 * st < D) {
+          const int r = 8 * ((lane >> 3) & 1) + (lane & 7), ch = st + (lane >> 4);
+          uint32_t k[4];
+          ldsm4(k, kbase + r * pitch + ((swz ? ch ^ (r & 7) : ch) << 4));
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            uint32_t a[4];
+            *reinterpret_cast<uint4*>(a) = sq[(st + x) * 32 + lane];
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              uint32_t b0, b1;
+              e4m3_pairs(k[2 * x + n], b0, b1);
+              mma(M(), s[n], a, b0, b1);
+            }
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int st = 0; st < G::kSteps; ++st) {
+        if (16 * st < D) {
+          const int r = 8 * (lane >> 4) + (lane & 7), ch = 2 * st + ((lane >> 3) & 1);
+          uint32_t k[4];
+          ldsm4(k, kbase + r * pitch + ((swz ? ch ^ (r & 7) : ch) << 4));
+#pragma unroll
+          for (int x = 0; x < G::kSets; ++x) {
+            uint32_t a[4];
+            *reinterpret_cast<uint4*>(a) = sq[(x * G::kSteps + st) * 32 + lane];
+            mma(M(), s[0], a, k[0], k[1]);
+            mma(M(), s[1], a, k[2], k[3]);
+          }
+        }
+      }
+    }
+    float z[2][2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        z[n][e] = (s[n][e] + s[n][e + 2]) * mult;
+        const int i = 8 * n + 2 * t + e;
+        if (p.a.alibi && ((okm >> i) & 1)) {
+          const int pos = c.positions ? c.positions[(static_cast<int64_t>(cur.b) * c.num_kv + kv) * c.max_slots + j0 + i] : j0 + i;
+          z[n][e] -= slope * static_cast<float>(q_pos - pos);
+        }
+        if (!((okm >> i) & 1)) z[n][e] = -INFINITY;
+      }
+    if (p.a.accumulate && g < heads) {
+      float* sc = p.scores + (static_cast<int64_t>(cur.b) * c.num_heads + head + g) * c.max_slots + j0;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (j0 + 8 * n + 2 * t + e < cur.len) sc[8 * n + 2 * t + e] = z[n][e];
+    }
+    float mx = fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[1][0], z[1][1]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    if (__any_sync(0xffffffffu, mx > m)) {
+      const float m_new = fmaxf(m, mx);
+      const float corr = m == -INFINITY ? 0.0f : exp2f(m - m_new);
+      l *= corr;
+#pragma unroll
+      for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][e] *= corr;
+      m = m_new;
+    }
+    const float ref = (m == -INFINITY ? 0.0f : m) - G::kBias;
+    float pw[2][2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        pw[n][e] = exp2f(z[n][e] - ref);
+        l += pw[n][e];
+      }
+
+    // o += weights . values
+    if constexpr (G::kF32) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        uint32_t a[4];  // k index t is key 2 t, t + 4 is key 2 t + 1
+        tf32_parts(pw[n][0], a[0], a[1]);
+        tf32_parts(pw[n][1], a[2], a[3]);
+        const int r0 = 8 * n + 2 * t, r1 = r0 + 1;
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) {
+          if (8 * i < D) {
+            const int ch = 2 * i + (g >> 2);
+            const float v0 = __uint_as_float(lds32(vbase + r0 * pitch + ((swz ? ch ^ (r0 & 7) : ch) << 4) + 4 * (g & 3)));
+            const float v1 = __uint_as_float(lds32(vbase + r1 * pitch + ((swz ? ch ^ (r1 & 7) : ch) << 4) + 4 * (g & 3)));
+            uint32_t h0, l0, h1, l1;
+            tf32_parts(v0, h0, l0);
+            tf32_parts(v1, h1, l1);
+            mma(M(), o[i], a, h0, h1);
+            mma(M(), o[i], a, l0, l1);
+          }
+        }
+      }
+    } else {
+      uint32_t a[G::kSets][4];
+      if constexpr (G::kBF16) {
+        uint32_t x[3], y[3];
+        parts3(pw[0][0], pw[0][1], x);
+        parts3(pw[1][0], pw[1][1], y);
+        a[0][0] = x[0]; a[0][1] = x[1]; a[0][2] = y[0]; a[0][3] = y[1];
+        a[1][0] = x[2]; a[1][1] = 0u; a[1][2] = y[2]; a[1][3] = 0u;
+      } else {
+        uint32_t x[2], y[2];
+        parts2(pw[0][0], pw[0][1], x);
+        parts2(pw[1][0], pw[1][1], y);
+        a[0][0] = x[0]; a[0][1] = x[1]; a[0][2] = y[0]; a[0][3] = y[1];
+      }
+      const int r = 8 * ((lane >> 3) & 1) + (lane & 7);
+#pragma unroll
+      for (int i = 0; i < DP / 8; i += G::kFP8 ? 4 : 2) {
+        if (8 * i < D) {
+          const int ch = (G::kFP8 ? i / 2 : i) + (lane >> 4);
+          uint32_t v[4];
+          ldsm4t(v, vbase + r * pitch + ((swz ? ch ^ (r & 7) : ch) << 4));
+          if constexpr (G::kFP8) {
+            // a register holds dims 2 g, 2 g + 1 of keys 2 t, 2 t + 1: regroup the bytes by dim
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              uint32_t e0, o0, e1, o1;
+              e4m3_pairs(__byte_perm(v[2 * x], 0, 0x3120), e0, o0);
+              e4m3_pairs(__byte_perm(v[2 * x + 1], 0, 0x3120), e1, o1);
+              mma(M(), o[i + 2 * x], a[0], e0, e1);
+              mma(M(), o[i + 2 * x + 1], a[0], o0, o1);
+            }
+          } else {
+#pragma unroll
+            for (int x = 0; x < G::kSets; ++x) {
+              mma(M(), o[i], a[x], v[0], v[1]);
+              mma(M(), o[i + 1], a[x], v[2], v[3]);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();  // the stage is read; its slot can be filled again
+    issue(stage + G::kStages - 1 >= G::kStages ? stage - 1 : stage + G::kStages - 1);
+    stage = stage + 1 == G::kStages ? 0 : stage + 1;
+
+    const bool unit_ends = cur.tile + 1 == cur.nt;
+    if (unit_ends || tile + 1 == t1) {
+      // join the warps: each adds its sums in turn
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if (t == 0) {
+        s_m[w][g] = m;
+        s_l[w][g] = l;
+      }
+      __syncthreads();
+      float mm = s_m[0][g], ll = 0.0f;
+#pragma unroll
+      for (int i = 1; i < G::kWarps; ++i) mm = fmaxf(mm, s_m[i][g]);
+      const float r = mm == -INFINITY ? 0.0f : mm;
+#pragma unroll
+      for (int i = 0; i < G::kWarps; ++i) ll += s_l[i][g] * exp2f(s_m[i][g] - r);
+      const float f = exp2f(m - r);
+      for (int x = 0; x < G::kWarps; ++x) {
+        if (x == w) {
+#pragma unroll
+          for (int i = 0; i < DP / 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int d = G::kFP8 ? 16 * (i >> 1) + 4 * t + 2 * e + (i & 1) : 8 * i + 2 * t + e;
+              float v = (o[i][e] + o[i][e + 2]) * f;
+              if (w > 0) v += so[g * DP + d];
+              so[g * DP + d] = v;
+            }
+        }
+        __syncthreads();
+      }
+      const int seg = cur.b * p.units + cur.u;
+      float* out = p.a.out + cur.b * p.a.out_ld + static_cast<int64_t>(head) * D;
+      float* lse = p.lse + static_cast<int64_t>(cur.b) * c.num_heads + head;
+      if (t == 0 && w == 0) s_mult[g] = ll;  // reuse: the unit's sum and maximum
+      if (t == 0 && w == 0) s_m[0][g] = mm;
+      __syncthreads();
+      if (unit_ends && unit_start >= t0) {
+        for (int i = tid; i < heads * D; i += G::kThreads) {
+          const int h = i / D, d = i - h * D;
+          out[i] = s_mult[h] == 0.0f ? 0.0f : so[h * DP + d] * (c.v_scale / s_mult[h]);
+        }
+        if (p.a.accumulate && tid < heads)
+          lse[tid] = s_mult[tid] == 0.0f ? INFINITY : (s_m[0][tid] == -INFINITY ? 0.0f : s_m[0][tid]) - G::kBias + log2f(s_mult[tid]);
+      } else {
+        // a block leaves at most two partial units: one that began before its run, one that goes on after it
+        const int stride = D + 2;
+        float* dst = p.part + (2ll * blockIdx.x + (unit_start >= t0 ? 1 : 0)) * 8 * stride;
+        for (int i = tid; i < heads * D; i += G::kThreads) {
+          const int h = i / D, d = i - h * D;
+          dst[h * stride + d] = so[h * DP + d];
+        }
+        if (tid < heads) {
+          dst[tid * stride + D] = s_m[0][tid];
+          dst[tid * stride + D + 1] = s_mult[tid];
+        }
+        const long long c0 = ((unit_start + 1) * n_cta - 1) / total, c1 = ((unit_start + cur.nt) * n_cta - 1) / total;
+        __syncthreads();
+        if (tid == 0) {
+          __threadfence();
+          s_last = atomicAdd(p.counters + seg, 1) == static_cast<int>(c1 - c0);
+        }
+        __syncthreads();
+        if (s_last) {
+          __threadfence();
+          if (tid == 0) p.counters[seg] = 0;
+          auto part_of = [&](long long i) {
+            return p.part + (2 * i + (unit_start >= run_start(i) ? 1 : 0)) * 8 * stride;
+          };
+          for (int i = tid; i < heads * D; i += G::kThreads) {
+            const int h = i / D, d = i - h * D;
+            float mj = -INFINITY, lj = 0.0f, v = 0.0f;
+            for (long long x = c0; x <= c1; ++x) mj = fmaxf(mj, __ldcg(part_of(x) + h * stride + D));
+            const float rj = mj == -INFINITY ? 0.0f : mj;
+            for (long long x = c0; x <= c1; ++x) {
+              const float* src = part_of(x) + h * stride;
+              const float fj = exp2f(__ldcg(src + D) - rj);
+              v += __ldcg(src + d) * fj;
+              lj += __ldcg(src + D + 1) * fj;
+            }
+            out[i] = lj == 0.0f ? 0.0f : v * (c.v_scale / lj);
+            if (p.a.accumulate && d == 0) lse[h] = lj == 0.0f ? INFINITY : rj - G::kBias + log2f(lj);
+          }
+        }
+      }
+      __syncthreads();  // before the next unit's query replaces what was read here
+      fresh = true;
+    }
+    cursor_next(p, G::kKeys, cur);
+  }
+  cp_wait<0>();
+}
+
+int simple_splits(const KvView& v) {
+  const int64_t rows = static_cast<int64_t>(v.num_seqs) * v.num_heads;
+  int64_t s = (148 * 16 + rows - 1) / rows;
+  s = std::min<int64_t>(s, (v.max_slots + 127) / 128);
+  s = std::min<int64_t>(s, 64);
+  return s < 1 ? 1 : static_cast<int>(s);
+}
+
+// The tiled form copies rows in 16-byte pieces.
+bool tiled(const KvView& v, KvType type) {
+  const int size = kv_size(type);
+  return v.head_dim % 8 == 0 && v.head_dim * size % 16 == 0 && pool_aligned(v.k, size, 16) && pool_aligned(v.v, size, 16);
+}
+
+template <typename F>
+Status by_shape(const KvView& v, KvType type, F&& f) {
+  return by_type(type, [&](auto* t) {
+    using T = std::remove_pointer_t<decltype(t)>;
+    if (v.head_dim <= 64) return f(Tiled<T, 64>{}, k_attend_tiled<T, 64>);
+    if (v.head_dim <= 128) return f(Tiled<T, 128>{}, k_attend_tiled<T, 128>);
+    return f(Tiled<T, 256>{}, k_attend_tiled<T, 256>);
+  });
+}
+
+int head_groups(const KvView& v) { return (v.num_heads / v.num_kv + 7) / 8; }
+
+} // namespace
+
+Status attend_plan(KvCache* c) {
+  const KvView& v = c->view;
+  const size_t rows = static_cast<size_t>(v.num_seqs) * v.num_heads;
+  c->attend_tiled = tiled(v, c->type);
+  if (!c->attend_tiled) {
+    c->part_bytes = rows * simple_splits(v) * (v.head_dim + 2) * 4;
+    return Status::Ok();
+  }
+  return by_shape(v, c->type, [&](auto g, auto* kernel) {
+    using G = decltype(g);
+    WB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G::kSmem));
+    int per_sm = 0, sms = 0;
+    WB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, G::kThreads, G::kSmem));
+    WB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c->device));
+    if (per_sm < 1) return Status::Internal("kv attend: the kernel does not fit");
+    const int64_t units = static_cast<int64_t>(v.num_kv) * head_groups(v);
+    const int64_t most = v.num_seqs * units * ((v.max_slots + G::kKeys - 1) / G::kKeys);
+    c->attend_blocks = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(per_sm) * sms, most));
+    c->part_bytes = static_cast<size_t>(c->attend_blocks) * 2 * 8 * (v.head_dim + 2) * 4;
+    c->counter_bytes = static_cast<size_t>(v.num_seqs) * units * 4;
+    return Status::Ok();
+  });
+}
+
+Status kv_attend(KvCache* c, const KvAttendArgs& a, cudaStream_t st) {
+  WB_CUDA(cudaSetDevice(c->device));
+  AttendParams p;
+  p.a = a;
+  p.c = c->view;
+  const KvView& v = c->view;
+  if (!(p.a.scale > 0.0f)) p.a.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(v.head_dim)));
+  if (!p.a.weights_in) p.a.weights_in = v.weights;
+  p.part = c->part;
+  p.scores = c->scores;
+  p.lse = c->lse;
+  p.group = v.num_heads / v.num_kv;
+  p.head_groups = head_groups(v);
+  p.units = v.num_kv * p.head_groups;
+  p.page_shift = (v.page_size & (v.page_size - 1)) == 0 ? 31 - __builtin_clz(v.page_size) : -1;
+  p.counters = c->counters;
+  const unsigned B = v.num_seqs, H = v.num_heads;
+  if (c->attend_tiled) {
+    WB_TRY(by_shape(v, c->type, [&](auto g, auto* kernel) {
+      using G = decltype(g);
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      at[0].val.programmaticStreamSerializationAllowed = 1;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3(c->attend_blocks);
+      cfg.blockDim = dim3(G::kThreads);
+      cfg.dynamicSmemBytes = G::kSmem;
+      cfg.stream = st;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p), "kv attend launch");
+    }));
+  } else {
+    p.splits = simple_splits(v);
+    WB_TRY(by_type(c->type, [&](auto* t) {
+      using T = std::remove_pointer_t<decltype(t)>;
+      k_attend_simple<T><<<dim3(p.splits, H, B), 32 * kSimpleWarps, 0, st>>>(p);
+      return cuda_status(cudaGetLastError(), "kv attend launch");
+    }));
+    k_attend_join<<<dim3(H, B), 128, 0, st>>>(p);
+  }
+  if (a.accumulate) {
+    const unsigned blocks = (v.max_slots + 255) / 256;
+    k_attend_weights<<<dim3(blocks < 64 ? blocks : 64, v.num_kv, B), 256, 0, st>>>(p);
+  }
+  return cuda_status(cudaGetLastError(), "kv attend launch");
+}
+
+} // namespace wb

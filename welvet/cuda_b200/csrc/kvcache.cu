@@ -1,4 +1,4 @@
-// kvcache.cu -- append, decode attention and eviction over a paged key-value cache (sm_100a).
+// kvcache.cu -- append and eviction over a paged key-value cache, and its handle (sm_100a).
 #include "kvcache.hpp"
 #include "kvcache.cuh"
 
@@ -148,143 +148,6 @@ __global__ void __launch_bounds__(kAppendThreads) k_append(const __grid_constant
     const int64_t len = static_cast<int64_t>(p.a.start[s]) + n, tot = static_cast<int64_t>(p.a.start_seen[s]) + n;
     c.lens[s] = static_cast<int32_t>(len < c.max_slots ? len : c.max_slots);
     if (c.seen != c.lens) c.seen[s] = static_cast<int32_t>(tot);
-  }
-}
-
-// ---------------------------------------------------------------- attention, one query head a block
-
-struct AttendParams {
-  KvAttendArgs a;
-  KvView c;
-  int splits;
-  float* part;    // [num_seqs][num_heads][splits][head_dim + 2]: o, m, l
-  float* scores;  // with accumulate
-  float* lse;
-};
-
-constexpr int kSimpleWarps = 4;
-constexpr int kSimpleDims = 8;  // dims a lane holds: head_dim <= 256
-
-// A block takes one split of one (sequence, query head); a warp a key at a time, lanes over the
-// head's dims, one pass with the running maximum and sum. Keys shared by the heads of a group are
-// read again for each head.
-template <typename T>
-__global__ void __launch_bounds__(32 * kSimpleWarps) k_attend_simple(const __grid_constant__ AttendParams p) {
-  __shared__ float s_m[kSimpleWarps], s_l[kSimpleWarps];
-  __shared__ float s_o[kSimpleWarps][32 * kSimpleDims];
-  const KvView& c = p.c;
-  const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int D = c.head_dim, kv = h / (c.num_heads / c.num_kv);
-  int len = c.lens[b];
-  if (len < 0 || len > c.max_slots) {
-    if (threadIdx.x == 0) atomicCAS(c.err, 0, kKvErrSlot);
-    len = len < 0 ? 0 : c.max_slots;
-  }
-  const int64_t per = (len + p.splits - 1) / p.splits;
-  const int j0 = static_cast<int>(per * split < len ? per * split : len);
-  const int j1 = static_cast<int>(per * (split + 1) < len ? per * (split + 1) : len);
-  const int q_pos = c.positions ? c.seen[b] - 1 : len - 1;
-  const int64_t rec = (static_cast<int64_t>(b) * c.num_kv + kv) * c.max_slots;
-  const float slope = p.a.alibi ? alibi_slope(h, c.num_heads) : 0.0f;
-  float q[kSimpleDims], o[kSimpleDims];
-#pragma unroll
-  for (int i = 0; i < kSimpleDims; ++i) {
-    const int d = lane + 32 * i;
-    q[i] = d < D ? p.a.q[b * p.a.q_ld + static_cast<int64_t>(h) * D + d] * (p.a.scale * c.k_scale) : 0.0f;
-    o[i] = 0.0f;
-  }
-  float m = -INFINITY, l = 0.0f;
-  for (int j = j0 + w; j < j1; j += kSimpleWarps) {
-    const int pos = c.positions ? c.positions[rec + j] : j;
-    const int page = c.table[b * c.table_stride + j / c.page_size];
-    bool ok = page >= 0 && page < c.num_pages;
-    if (!ok && lane == 0) atomicCAS(c.err, 0, kKvErrPage);
-    if (p.a.window > 0 && pos <= q_pos - p.a.window) ok = false;
-    float z = -INFINITY;
-    if (ok) {
-      const T* kr = reinterpret_cast<const T*>(c.k.base) + page * c.k.page + (j % c.page_size) * c.k.slot + kv * c.k.head;
-      float dot = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kSimpleDims; ++i) {
-        const int d = lane + 32 * i;
-        if (d < D) dot += q[i] * to_float(kr[d]);
-      }
-      z = warp_sum(dot) - slope * static_cast<float>(q_pos - pos);
-      const T* vr = reinterpret_cast<const T*>(c.v.base) + page * c.v.page + (j % c.page_size) * c.v.slot + kv * c.v.head;
-      const float m_new = fmaxf(m, z);
-      const float ref = m_new == -INFINITY ? 0.0f : m_new;
-      const float e = expf(z - ref), corr = expf(m - ref);
-      l = l * corr + e;
-#pragma unroll
-      for (int i = 0; i < kSimpleDims; ++i) {
-        const int d = lane + 32 * i;
-        if (d < D) o[i] = o[i] * corr + e * to_float(vr[d]);
-      }
-      m = m_new;
-    }
-    if (p.a.accumulate && lane == 0)
-      p.scores[(static_cast<int64_t>(b) * c.num_heads + h) * c.max_slots + j] = ok ? z : -INFINITY;
-  }
-  if (lane == 0) {
-    s_m[w] = m;
-    s_l[w] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < kSimpleDims; ++i) s_o[w][lane + 32 * i] = o[i];
-  __syncthreads();
-  float mm = s_m[0];
-#pragma unroll
-  for (int i = 1; i < kSimpleWarps; ++i) mm = fmaxf(mm, s_m[i]);
-  const float ref = mm == -INFINITY ? 0.0f : mm;
-  float* dst = p.part + ((static_cast<int64_t>(b) * c.num_heads + h) * p.splits + split) * (D + 2);
-  for (int d = threadIdx.x; d < D; d += 32 * kSimpleWarps) {
-    float v = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kSimpleWarps; ++i) v += s_o[i][d] * expf(s_m[i] - ref);
-    dst[d] = v;
-  }
-  if (threadIdx.x == 0) {
-    float v = 0.0f;
-#pragma unroll
-    for (int i = 0; i < kSimpleWarps; ++i) v += s_l[i] * expf(s_m[i] - ref);
-    dst[D] = mm;
-    dst[D + 1] = v;
-  }
-}
-
-// Joins the splits of one (sequence, query head) in split order. A row that nothing is allowed
-// in has l = 0 and m = -inf from every split: its output is zero.
-__global__ void k_attend_join(const __grid_constant__ AttendParams p) {
-  const KvView& c = p.c;
-  const int h = blockIdx.x, b = blockIdx.y, D = c.head_dim;
-  const float* src = p.part + (static_cast<int64_t>(b) * c.num_heads + h) * p.splits * (D + 2);
-  float m = -INFINITY;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, src[s * (D + 2) + D]);
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float l = 0.0f;
-  for (int s = 0; s < p.splits; ++s) l += src[s * (D + 2) + D + 1] * expf(src[s * (D + 2) + D] - ref);
-  const float inv = l == 0.0f ? 0.0f : c.v_scale / l;
-  for (int d = threadIdx.x; d < D; d += blockDim.x) {
-    float v = 0.0f;
-    for (int s = 0; s < p.splits; ++s) v += src[s * (D + 2) + d] * expf(src[s * (D + 2) + D] - ref);
-    p.a.out[b * p.a.out_ld + static_cast<int64_t>(h) * D + d] = v * inv;
-  }
-  if (threadIdx.x == 0 && p.a.accumulate) p.lse[static_cast<int64_t>(b) * c.num_heads + h] = l == 0.0f ? INFINITY : ref + logf(l);
-}
-
-// weights[j] = weights_in[j] + sum over the group's heads of exp(score - lse), heads in order.
-__global__ void k_attend_weights(const __grid_constant__ AttendParams p) {
-  const KvView& c = p.c;
-  const int kv = blockIdx.y, b = blockIdx.z, group = c.num_heads / c.num_kv;
-  int len = c.lens[b];
-  len = len < 0 ? 0 : (len > c.max_slots ? c.max_slots : len);
-  const int64_t rec = (static_cast<int64_t>(b) * c.num_kv + kv) * c.max_slots;
-  const int64_t row = static_cast<int64_t>(b) * c.num_heads + kv * group;
-  for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < len; j += gridDim.x * blockDim.x) {
-    float s = p.a.weights_in[rec + j];
-    for (int i = 0; i < group; ++i) s += expf(p.scores[(row + i) * c.max_slots + j] - p.lse[row + i]);
-    c.weights[rec + j] = s;
   }
 }
 
@@ -470,32 +333,7 @@ __global__ void __launch_bounds__(256) k_evict_move(const __grid_constant__ Evic
   }
 }
 
-template <typename F>
-Status by_type(KvType t, F&& f) {
-  switch (t) {
-  case KvType::F32: return f(static_cast<float*>(nullptr));
-  case KvType::F16: return f(static_cast<__half*>(nullptr));
-  case KvType::BF16: return f(static_cast<__nv_bfloat16*>(nullptr));
-  case KvType::E4M3: return f(static_cast<__nv_fp8_e4m3*>(nullptr));
-  }
-  return Status::Internal("kv: type");
-}
-
-bool pool_aligned(const KvPool& p, int size, int bytes) {
-  return reinterpret_cast<uintptr_t>(p.base) % bytes == 0 && p.page * size % bytes == 0 && p.slot * size % bytes == 0 &&
-         p.head * size % bytes == 0;
-}
-
 bool f32_aligned(const float* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0; }
-
-int attend_splits(const KvView& v) {
-  const int64_t rows = static_cast<int64_t>(v.num_seqs) * v.num_heads;
-  int64_t s = (148 * 16 + rows - 1) / rows;
-  const int64_t most = (v.max_slots + 127) / 128;
-  if (s > most) s = most;
-  if (s > 64) s = 64;
-  return s < 1 ? 1 : static_cast<int>(s);
-}
 
 } // namespace
 
@@ -515,13 +353,15 @@ static Status kv_alloc(KvCache* c) {
     bytes += (n + 255) / 256 * 256;
     return at;
   };
-  const size_t err = take(4), ticket = take(4);
-  const size_t part = take(rows * attend_splits(v) * (v.head_dim + 2) * 4);
+  WB_TRY(attend_plan(c));
+  const size_t err = take(4), ticket = take(4), counters = take(c->counter_bytes);
+  const size_t part = take(c->part_bytes);  // from here on nothing needs to start as zero
   const size_t scores = take(v.weights ? rows * v.max_slots * 4 : 0), lse = take(v.weights ? rows * 4 : 0);
   const size_t moves = take(v.positions ? heads * 2 * (v.max_slots / 2) * 4 : 0), n_moves = take(v.positions ? heads * 4 : 0);
   WB_CUDA(cudaMalloc(&c->work, bytes));
   c->err = reinterpret_cast<int*>(c->work + err);
   c->ticket = reinterpret_cast<int*>(c->work + ticket);
+  c->counters = reinterpret_cast<int*>(c->work + counters);
   c->part = reinterpret_cast<float*>(c->work + part);
   c->scores = reinterpret_cast<float*>(c->work + scores);
   c->lse = reinterpret_cast<float*>(c->work + lse);
@@ -575,31 +415,6 @@ Status kv_append(KvCache* c, const KvAppendArgs& a, cudaStream_t st) {
     else k_append<T, false><<<blocks, kAppendThreads, 0, st>>>(p);
     return cuda_status(cudaGetLastError(), "kv append launch");
   });
-}
-
-Status kv_attend(KvCache* c, const KvAttendArgs& a, cudaStream_t st) {
-  WB_CUDA(cudaSetDevice(c->device));
-  AttendParams p;
-  p.a = a;
-  p.c = c->view;
-  if (!(p.a.scale > 0.0f)) p.a.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(p.c.head_dim)));
-  if (!p.a.weights_in) p.a.weights_in = p.c.weights;
-  p.splits = attend_splits(p.c);
-  p.part = c->part;
-  p.scores = c->scores;
-  p.lse = c->lse;
-  const unsigned B = p.c.num_seqs, H = p.c.num_heads;
-  WB_TRY(by_type(c->type, [&](auto* t) {
-    using T = std::remove_pointer_t<decltype(t)>;
-    k_attend_simple<T><<<dim3(p.splits, H, B), 32 * kSimpleWarps, 0, st>>>(p);
-    return cuda_status(cudaGetLastError(), "kv attend launch");
-  }));
-  k_attend_join<<<dim3(H, B), 128, 0, st>>>(p);
-  if (a.accumulate) {
-    const unsigned blocks = (p.c.max_slots + 255) / 256;
-    k_attend_weights<<<dim3(blocks < 64 ? blocks : 64, p.c.num_kv, B), 256, 0, st>>>(p);
-  }
-  return cuda_status(cudaGetLastError(), "kv attend join launch");
 }
 
 Status kv_evict(KvCache* c, const KvEvictArgs& a, cudaStream_t st) {

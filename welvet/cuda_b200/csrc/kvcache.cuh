@@ -5,6 +5,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include "kvcache.hpp"
+
 #include <cstdint>
 #include <type_traits>
 
@@ -50,6 +52,18 @@ __device__ __forceinline__ float warp_sum(float v) {
 // The MHA cell's slope of head h (src/cuda/kernels.cu:520-528): 2^(-8 (h + 1) / heads).
 __device__ __forceinline__ float alibi_slope(int h, int heads) {
   return exp2f(-8.0f * static_cast<float>(h + 1) / static_cast<float>(heads));
+}
+
+// f(T*) with the C++ type of the pages.
+template <typename F>
+Status by_type(KvType t, F&& f) {
+  switch (t) {
+  case KvType::F32: return f(static_cast<float*>(nullptr));
+  case KvType::F16: return f(static_cast<__half*>(nullptr));
+  case KvType::BF16: return f(static_cast<__nv_bfloat16*>(nullptr));
+  case KvType::E4M3: return f(static_cast<__nv_fp8_e4m3*>(nullptr));
+  }
+  return Status::Internal("kv: type");
 }
 
 } // namespace wb

@@ -53,7 +53,12 @@ struct KvCache {
   uint8_t* work = nullptr;       // the one allocation behind what follows
   int* err = nullptr;
   int* ticket = nullptr;         // block counter of append (zero between calls)
-  float* part = nullptr;         // attend's partial results
+  // attend (kv_attend.cu)
+  bool attend_tiled = false;
+  int attend_blocks = 0;         // blocks of the tiled form
+  size_t part_bytes = 0, counter_bytes = 0;
+  float* part = nullptr;         // partial results
+  int* counters = nullptr;       // blocks done per (sequence, unit), zero between calls
   float* scores = nullptr;       // [num_seqs][num_heads][max_slots]; with weights only
   float* lse = nullptr;          // [num_seqs][num_heads]
   int32_t* moves = nullptr;      // evict: [num_seqs][num_kv][2][max_slots / 2] slots to fill, slots to take
@@ -62,6 +67,9 @@ struct KvCache {
 };
 
 Status kv_create(int device, KvType type, const KvView& view, KvCache** out);
+
+// Picks the form of attend and sizes its workspaces (kv_create).
+Status attend_plan(KvCache* c);
 
 struct KvAppendArgs {
   int rows = 0;
@@ -99,5 +107,10 @@ Status kv_evict(KvCache* c, const KvEvictArgs& a, cudaStream_t st);
 
 // Synchronizes the stream; reports and clears the error word.
 Status kv_check_error(KvCache* c, cudaStream_t st);
+
+inline bool pool_aligned(const KvPool& p, int size, int bytes) {
+  return reinterpret_cast<uintptr_t>(p.base) % bytes == 0 && p.page * size % bytes == 0 && p.slot * size % bytes == 0 &&
+         p.head * size % bytes == 0;
+}
 
 } // namespace wb
