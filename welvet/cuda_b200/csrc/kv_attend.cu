@@ -246,7 +246,8 @@ __device__ __forceinline__ void e4m3_pairs(uint32_t w, uint32_t& lo, uint32_t& h
       "cvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
 }
 
-template <typename T, int DP>
+// kFull: head_dim is DP itself, and everything that goes by it is a constant.
+template <typename T, int DP, bool kFull>
 struct Tiled {
   static constexpr bool kF32 = std::is_same_v<T, float>;
   static constexpr bool kBF16 = std::is_same_v<T, __nv_bfloat16>;
@@ -257,6 +258,8 @@ struct Tiled {
   static constexpr int kStages = kRow <= 128 ? 4 : 3;
   static constexpr int kThreads = 32 * kWarps;
   static constexpr int kKeys = 16 * kWarps;  // keys of a block tile
+  static constexpr int kLanes = kRow < 128 ? kRow / 16 : 8;  // lanes that copy a row
+  static constexpr bool kSwz = kRow % 128 == 0;              // with kFull: chunks xored by the key
   static constexpr int kSets = kBF16 ? 2 : 1;
   static constexpr int kSteps = kF32 ? DP / 8 : DP / 16;  // MMA steps over a head's dims
   static constexpr float kBias = kF32 || kBF16 ? 0.0f : 15.0f;  // log2 of the weights' scale
@@ -266,9 +269,15 @@ struct Tiled {
   static constexpr int kSmem = kRing + kSmemQ + kSmemO;
 };
 
-// A position in the list of all tiles: sequence b, unit u, tile of the unit's nt.
+// Beginning and finishing a unit costs a block about as much as kOver tiles: the list that the
+// blocks divide has kOver places before each unit's tiles, so that runs of short units (one tile
+// each) get fewer of them.
+constexpr int kOver = 4;
+
+// A tile's place in that list: `at`, of sequence b, unit u, tile of the unit's nt.
 struct Cursor {
-  int b, u, tile, nt, len, lo, first;
+  int b, u, kv, hg, tile, nt, len, lo, first;
+  long long at;
 };
 
 __device__ __forceinline__ void cursor_seq(const AttendParams& p, int keys, Cursor& c) {
@@ -281,16 +290,27 @@ __device__ __forceinline__ void cursor_seq(const AttendParams& p, int keys, Curs
 }
 
 __device__ __forceinline__ void cursor_next(const AttendParams& p, int keys, Cursor& c) {
+  ++c.at;
   if (++c.tile < c.nt) return;
   c.tile = 0;
-  if (++c.u < p.units) return;
-  c.u = 0;
+  c.at += kOver;
+  ++c.u;
+  if (++c.hg < p.head_groups) return;
+  c.hg = 0;
+  if (++c.kv < p.c.num_kv) return;
+  c.kv = c.u = 0;
   if (++c.b < p.c.num_seqs) cursor_seq(p, keys, c);
 }
 
-template <typename T, int DP>
-__global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const __grid_constant__ AttendParams p) {
-  using G = Tiled<T, DP>;
+__device__ __forceinline__ float exp2_fast(float x) {  // ex2.approx: 2 ulp, 2^-inf = 0
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <typename T, int DP, bool kFull>
+__global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads) k_attend_tiled(const __grid_constant__ AttendParams p) {
+  using G = Tiled<T, DP, kFull>;
   using M = typename G::M;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long s_sum[G::kWarps];
@@ -300,14 +320,19 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
   __shared__ uint32_t s_ok[G::kWarps][G::kStages];
   const KvView& c = p.c;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int D = c.head_dim;
+  const int D = kFull ? DP : c.head_dim;
   const int row_bytes = D * static_cast<int>(sizeof(T)), chunks = row_bytes / 16;
   // Rows of a multiple of 128 bytes (and rows whose pitch would not fit) are stored with their
   // 16-byte chunks xored by the key; others with a pitch of an odd number of chunks. Both keep
   // ldmatrix free of bank conflicts.
   const int pad_chunks = (chunks + 1) & ~1;  // the MMAs read whole steps of 32 bytes
-  const bool swz = (row_bytes & 127) == 0 || 16 * (pad_chunks + 1) > G::kRowMax;
+  const bool swz = kFull ? G::kSwz : (row_bytes & 127) == 0 || 16 * (pad_chunks + 1) > G::kRowMax;
   const int pitch = swz ? (row_bytes + 127) & ~127 : 16 * (pad_chunks + 1);
+  // offset of chunk ch + x of row r, x a constant of a loop whose bits ch leaves clear
+  auto chunk_at = [&](int r, int ch, int x) -> uint32_t {
+    if constexpr (kFull && G::kSwz) return (r * pitch + ((ch ^ (r & 7)) << 4) ^ ((x & 7) << 4)) + (x >> 3) * 128;
+    else return r * pitch + ((swz ? (ch + x) ^ (r & 7) : ch + x) << 4);
+  };
   uint8_t* const ring = smem + w * (G::kStages * 32 * pitch);
   const uint32_t ring_addr = pipe::smem_u32(ring);
   uint4* const sq = reinterpret_cast<uint4*>(smem + G::kRing);
@@ -327,7 +352,7 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
     s.b = b;
     cursor_seq(p, G::kKeys, s);
     if (blockIdx.x == 0 && (c.lens[b] < 0 || c.lens[b] > c.max_slots)) atomicCAS(c.err, 0, kKvErrSlot);
-    mine += s.nt;
+    mine += s.nt + kOver;
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
@@ -337,7 +362,11 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
 #pragma unroll
   for (int i = 0; i < G::kWarps; ++i) total += s_sum[i];
   total *= p.units;
-  const long long n_cta = total < gridDim.x ? total : gridDim.x;  // no block's run is empty
+  // A unit cut into P runs costs its last block about P / 14 tiles of joining: runs are at least
+  // as long as balances that, and never empty.
+  const float tiles = static_cast<float>(total) / static_cast<float>(static_cast<long long>(c.num_seqs) * p.units);
+  const int shortest = max(1, static_cast<int>(sqrtf(tiles * (1.0f / 14.0f))));
+  const long long n_cta = max(1ll, min(static_cast<long long>(gridDim.x), total / shortest));
   auto run_start = [&](long long i) { return i * total / n_cta; };
   const long long t0 = run_start(blockIdx.x), t1 = run_start(blockIdx.x + 1);
   if (blockIdx.x >= n_cta) return;
@@ -347,7 +376,7 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
     s.b = b;
     s.nt = 0;
     if (b < c.num_seqs) cursor_seq(p, G::kKeys, s);
-    const long long n = static_cast<long long>(s.nt) * p.units;
+    const long long n = b < c.num_seqs ? static_cast<long long>(s.nt + kOver) * p.units : 0;
     long long x = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -374,52 +403,96 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
   Cursor cur;
   cur.b = s_b;
   cursor_seq(p, G::kKeys, cur);
-  cur.u = static_cast<int>(s_off / cur.nt);
-  cur.tile = static_cast<int>(s_off - static_cast<long long>(cur.u) * cur.nt);
+  cur.u = static_cast<int>(s_off / (cur.nt + kOver));
+  cur.tile = static_cast<int>(s_off - static_cast<long long>(cur.u) * (cur.nt + kOver)) - kOver;
+  cur.kv = cur.u / p.head_groups;
+  cur.hg = cur.u - cur.kv * p.head_groups;
+  cur.at = t0;
+  if (cur.tile < 0) {
+    cur.at -= cur.tile;
+    cur.tile = 0;
+  }
   Cursor nxt = cur;
-  long long issued = t0;
 
   // Copies the warp's 16 keys and values of the tile at `nxt`; rows that the mask leaves out are
   // zeros (their contents, even NaN, must not reach the sums).
+  const bool one_page = c.page_size % 16 == 0 && !(p.a.window > 0 && c.positions);
   auto issue = [&](int stage) {
-    if (issued < t1) {
-      const int kv = nxt.u / p.head_groups;
-      const int j = (nxt.first + nxt.tile) * G::kKeys + 16 * w + (lane & 15);
-      bool ok = j >= nxt.lo && j < nxt.len;
-      int64_t koff = 0, voff = 0;
-      if (ok) {
-        const int slot_page = p.page_shift >= 0 ? j >> p.page_shift : j / c.page_size;
-        const int page = c.table[nxt.b * c.table_stride + slot_page];
-        const int in = j - slot_page * c.page_size;
-        if (p.a.window > 0 && c.positions) {
-          const int64_t rec = (static_cast<int64_t>(nxt.b) * c.num_kv + kv) * c.max_slots + j;
-          ok = c.positions[rec] > c.seen[nxt.b] - 1 - p.a.window;
-        }
-        if (page < 0 || page >= c.num_pages) {
-          atomicCAS(c.err, 0, kKvErrPage);
-          ok = false;
-        }
-        if (ok) {
-          koff = (page * c.k.page + in * c.k.slot + kv * c.k.head) * static_cast<int64_t>(sizeof(T));
-          voff = (page * c.v.page + in * c.v.slot + kv * c.v.head) * static_cast<int64_t>(sizeof(T));
-        }
-      }
-      const uint32_t okm = __ballot_sync(0xffffffffu, ok) & 0xffffu;
-      if (lane == 0) s_ok[w][stage] = okm;
+    if (nxt.at < t1) {
+      const int kv = nxt.kv, j0 = (nxt.first + nxt.tile) * G::kKeys + 16 * w;
       const uint32_t dst = ring_addr + stage * 32 * pitch;
-      // eight lanes a row, four rows at a time
+      constexpr int kRows = 32 / G::kLanes;  // rows copied at a time
+      const int lr = lane / G::kLanes, lc = lane % G::kLanes;
+      uint32_t okm;
+      if (one_page) {
+        // the 16 slots lie in one page, and their rows a stride apart
+        const int from = min(max(nxt.lo - j0, 0), 16), to = min(max(nxt.len - j0, 0), 16);
+        okm = ((1u << to) - 1u) & ~((1u << from) - 1u);
+        int page = 0, in = 0;
+        if (okm != 0) {
+          const int slot_page = p.page_shift >= 0 ? j0 >> p.page_shift : j0 / c.page_size;
+          page = c.table[nxt.b * c.table_stride + slot_page];
+          in = j0 - slot_page * c.page_size;
+          if (page < 0 || page >= c.num_pages) {
+            if (lane == 0) atomicCAS(c.err, 0, kKvErrPage);
+            page = in = 0;
+            okm = 0;
+          }
+        }
+        const uint8_t* ks = c.k.base + (page * c.k.page + (in + lr) * c.k.slot + kv * c.k.head) * static_cast<int64_t>(sizeof(T)) + 16 * lc;
+        const uint8_t* vs = c.v.base + (page * c.v.page + (in + lr) * c.v.slot + kv * c.v.head) * static_cast<int64_t>(sizeof(T)) + 16 * lc;
+        const int64_t kstep = c.k.slot * (kRows * static_cast<int64_t>(sizeof(T))), vstep = c.v.slot * (kRows * static_cast<int64_t>(sizeof(T)));
 #pragma unroll
-      for (int r0 = 0; r0 < 16; r0 += 4) {
-        const int r = r0 + (lane >> 3);
-        const int64_t ko = __shfl_sync(0xffffffffu, koff, r), vo = __shfl_sync(0xffffffffu, voff, r);
-        const int n = (okm >> r) & 1 ? 16 : 0;
-        for (int ch = lane & 7; ch < chunks; ch += 8) {
-          const uint32_t at = r * pitch + ((swz ? ch ^ (r & 7) : ch) << 4);
-          cp16(dst + at, c.k.base + ko + 16 * ch, n);
-          cp16(dst + 16 * pitch + at, c.v.base + vo + 16 * ch, n);
+        for (int r0 = 0; r0 < 16; r0 += kRows) {
+          const int n = (okm >> (r0 + lr)) & 1 ? 16 : 0;
+#pragma unroll
+          for (int x = 0; x < G::kRow / 16; x += G::kLanes) {
+            if (kFull || x + lc < chunks) {
+              uint32_t at;
+              if constexpr (kFull && G::kSwz) at = (r0 + lr) * pitch + (((lc ^ lr) ^ (r0 & 7)) << 4) + 16 * x;
+              else at = (r0 + lr) * pitch + ((swz ? (x + lc) ^ ((r0 + lr) & 7) : x + lc) << 4);
+              cp16(dst + at, ks + 16 * x, n);
+              cp16(dst + 16 * pitch + at, vs + 16 * x, n);
+            }
+          }
+          ks += kstep;
+          vs += vstep;
+        }
+      } else {
+        const int j = j0 + (lane & 15);
+        bool ok = j >= nxt.lo && j < nxt.len;
+        int64_t koff = 0, voff = 0;
+        if (ok) {
+          const int slot_page = p.page_shift >= 0 ? j >> p.page_shift : j / c.page_size;
+          const int page = c.table[nxt.b * c.table_stride + slot_page];
+          const int in = j - slot_page * c.page_size;
+          if (p.a.window > 0 && c.positions) {
+            const int64_t rec = (static_cast<int64_t>(nxt.b) * c.num_kv + kv) * c.max_slots + j;
+            ok = c.positions[rec] > c.seen[nxt.b] - 1 - p.a.window;
+          }
+          if (page < 0 || page >= c.num_pages) {
+            atomicCAS(c.err, 0, kKvErrPage);
+            ok = false;
+          }
+          if (ok) {
+            koff = (page * c.k.page + in * c.k.slot + kv * c.k.head) * static_cast<int64_t>(sizeof(T));
+            voff = (page * c.v.page + in * c.v.slot + kv * c.v.head) * static_cast<int64_t>(sizeof(T));
+          }
+        }
+        okm = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+#pragma unroll
+        for (int r0 = 0; r0 < 16; r0 += kRows) {
+          const int r = r0 + lr;
+          const int64_t ko = __shfl_sync(0xffffffffu, koff, r), vo = __shfl_sync(0xffffffffu, voff, r);
+          const int n = (okm >> r) & 1 ? 16 : 0;
+          for (int ch = lc; ch < chunks; ch += G::kLanes) {
+            const uint32_t at = r * pitch + ((swz ? ch ^ (r & 7) : ch) << 4);
+            cp16(dst + at, c.k.base + ko + 16 * ch, n);
+            cp16(dst + 16 * pitch + at, c.v.base + vo + 16 * ch, n);
+          }
         }
       }
-      ++issued;
+      if (lane == 0) s_ok[w][stage] = okm;
       cursor_next(p, G::kKeys, nxt);
     }
     cp_commit();
@@ -433,13 +506,13 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
   bool fresh = true;  // the unit's query is not in shared memory yet
   long long unit_start = 0;
 
-  for (long long tile = t0; tile < t1; ++tile) {
-    const int kv = cur.u / p.head_groups, h0 = (cur.u - kv * p.head_groups) * 8;
+  while (cur.at < t1) {
+    const int kv = cur.kv, h0 = 8 * cur.hg;
     const int heads = p.group - h0 < 8 ? p.group - h0 : 8;  // of this unit
     const int head = kv * p.group + h0;                      // the first of them
     if (fresh) {
       fresh = false;
-      unit_start = tile - cur.tile;
+      unit_start = cur.at - cur.tile;  // place of the unit's first tile
       q_pos = c.positions ? c.seen[cur.b] - 1 : cur.len - 1;
 #pragma unroll
       for (int i = 0; i < DP / 8; ++i)
@@ -519,9 +592,8 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
 #pragma unroll
           for (int n = 0; n < 2; ++n) {
             // four chunks (16 dims) of eight keys
-            const int r = 8 * n + (lane & 7), ch = 2 * st + (lane >> 3);
             uint32_t k[4], hi[4], lo[4];
-            ldsm4(k, kbase + r * pitch + ((swz ? ch ^ (r & 7) : ch) << 4));
+            ldsm4(k, kbase + chunk_at(8 * n + (lane & 7), lane >> 3, 2 * st));
 #pragma unroll
             for (int e = 0; e < 4; ++e) tf32_parts(__uint_as_float(k[e]), hi[e], lo[e]);
             mma(M(), s[n], a0, hi[0], hi[1]);
@@ -537,9 +609,8 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
 #pragma unroll
       for (int st = 0; st < G::kSteps; st += 2) {
         if (16 * st < D) {
-          const int r = 8 * ((lane >> 3) & 1) + (lane & 7), ch = st + (lane >> 4);
           uint32_t k[4];
-          ldsm4(k, kbase + r * pitch + ((swz ? ch ^ (r & 7) : ch) << 4));
+          ldsm4(k, kbase + chunk_at(8 * ((lane >> 3) & 1) + (lane & 7), lane >> 4, st));
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             uint32_t a[4];
@@ -557,9 +628,8 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
 #pragma unroll
       for (int st = 0; st < G::kSteps; ++st) {
         if (16 * st < D) {
-          const int r = 8 * (lane >> 4) + (lane & 7), ch = 2 * st + ((lane >> 3) & 1);
           uint32_t k[4];
-          ldsm4(k, kbase + r * pitch + ((swz ? ch ^ (r & 7) : ch) << 4));
+          ldsm4(k, kbase + chunk_at(8 * (lane >> 4) + (lane & 7), (lane >> 3) & 1, 2 * st));
 #pragma unroll
           for (int x = 0; x < G::kSets; ++x) {
             uint32_t a[4];
@@ -574,15 +644,24 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        z[n][e] = (s[n][e] + s[n][e + 2]) * mult;
-        const int i = 8 * n + 2 * t + e;
-        if (p.a.alibi && ((okm >> i) & 1)) {
-          const int pos = c.positions ? c.positions[(static_cast<int64_t>(cur.b) * c.num_kv + kv) * c.max_slots + j0 + i] : j0 + i;
-          z[n][e] -= slope * static_cast<float>(q_pos - pos);
+      for (int e = 0; e < 2; ++e) z[n][e] = (s[n][e] + s[n][e + 2]) * mult;
+    if (p.a.alibi) {
+      const int32_t* pos = c.positions ? c.positions + (static_cast<int64_t>(cur.b) * c.num_kv + kv) * c.max_slots : nullptr;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int i = 8 * n + 2 * t + e;
+          if ((okm >> i) & 1) z[n][e] -= slope * static_cast<float>(q_pos - (pos ? pos[j0 + i] : j0 + i));
         }
-        if (!((okm >> i) & 1)) z[n][e] = -INFINITY;
-      }
+    }
+    if (okm != 0xffffu) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (!((okm >> (8 * n + 2 * t + e)) & 1)) z[n][e] = -INFINITY;
+    }
     if (p.a.accumulate && g < heads) {
       float* sc = p.scores + (static_cast<int64_t>(cur.b) * c.num_heads + head + g) * c.max_slots + j0;
 #pragma unroll
@@ -596,7 +675,7 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     if (__any_sync(0xffffffffu, mx > m)) {
       const float m_new = fmaxf(m, mx);
-      const float corr = m == -INFINITY ? 0.0f : exp2f(m - m_new);
+      const float corr = m == -INFINITY ? 0.0f : exp2_fast(m - m_new);
       l *= corr;
 #pragma unroll
       for (int i = 0; i < DP / 8; ++i)
@@ -610,7 +689,7 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        pw[n][e] = exp2f(z[n][e] - ref);
+        pw[n][e] = exp2_fast(z[n][e] - ref);
         l += pw[n][e];
       }
 
@@ -625,9 +704,8 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
 #pragma unroll
         for (int i = 0; i < DP / 8; ++i) {
           if (8 * i < D) {
-            const int ch = 2 * i + (g >> 2);
-            const float v0 = __uint_as_float(lds32(vbase + r0 * pitch + ((swz ? ch ^ (r0 & 7) : ch) << 4) + 4 * (g & 3)));
-            const float v1 = __uint_as_float(lds32(vbase + r1 * pitch + ((swz ? ch ^ (r1 & 7) : ch) << 4) + 4 * (g & 3)));
+            const float v0 = __uint_as_float(lds32(vbase + chunk_at(r0, g >> 2, 2 * i) + 4 * (g & 3)));
+            const float v1 = __uint_as_float(lds32(vbase + chunk_at(r1, g >> 2, 2 * i) + 4 * (g & 3)));
             uint32_t h0, l0, h1, l1;
             tf32_parts(v0, h0, l0);
             tf32_parts(v1, h1, l1);
@@ -654,9 +732,8 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
 #pragma unroll
       for (int i = 0; i < DP / 8; i += G::kFP8 ? 4 : 2) {
         if (8 * i < D) {
-          const int ch = (G::kFP8 ? i / 2 : i) + (lane >> 4);
           uint32_t v[4];
-          ldsm4t(v, vbase + r * pitch + ((swz ? ch ^ (r & 7) : ch) << 4));
+          ldsm4t(v, vbase + chunk_at(r, lane >> 4, G::kFP8 ? i / 2 : i));
           if constexpr (G::kFP8) {
             // a register holds dims 2 g, 2 g + 1 of keys 2 t, 2 t + 1: regroup the bytes by dim
 #pragma unroll
@@ -682,7 +759,7 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
     stage = stage + 1 == G::kStages ? 0 : stage + 1;
 
     const bool unit_ends = cur.tile + 1 == cur.nt;
-    if (unit_ends || tile + 1 == t1) {
+    if (unit_ends || cur.at + 1 == t1) {
       // join the warps: each adds its sums in turn
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
@@ -747,22 +824,57 @@ __global__ void __launch_bounds__(Tiled<T, DP>::kThreads) k_attend_tiled(const _
         if (s_last) {
           __threadfence();
           if (tid == 0) p.counters[seg] = 0;
-          auto part_of = [&](long long i) {
-            return p.part + (2 * i + (unit_start >= run_start(i) ? 1 : 0)) * 8 * stride;
-          };
-          for (int i = tid; i < heads * D; i += G::kThreads) {
-            const int h = i / D, d = i - h * D;
-            float mj = -INFINITY, lj = 0.0f, v = 0.0f;
-            for (long long x = c0; x <= c1; ++x) mj = fmaxf(mj, __ldcg(part_of(x) + h * stride + D));
-            const float rj = mj == -INFINITY ? 0.0f : mj;
-            for (long long x = c0; x <= c1; ++x) {
-              const float* src = part_of(x) + h * stride;
-              const float fj = exp2f(__ldcg(src + D) - rj);
-              v += __ldcg(src + d) * fj;
-              lj += __ldcg(src + D + 1) * fj;
+          const int parts = static_cast<int>(c1 - c0) + 1;
+          // the first block began the unit (its second partial), the others went on with it
+          auto part_of = [&](int i) { return p.part + (2 * (c0 + i) + (i == 0)) * 8 * stride; };
+          // the parts' maxima and sums: kPer threads a head
+          constexpr int kPer = G::kThreads / 8;
+          const int hq = tid / kPer;
+          float mj = -INFINITY, lj = 0.0f;
+          if (hq < heads)
+            for (int x = tid % kPer; x < parts; x += kPer) mj = fmaxf(mj, __ldcg(part_of(x) + hq * stride + D));
+#pragma unroll
+          for (int x = kPer / 2; x > 0; x >>= 1) mj = fmaxf(mj, __shfl_xor_sync(0xffffffffu, mj, x));
+          const float rj = mj == -INFINITY ? 0.0f : mj;
+          constexpr int kElems = 8 * DP / G::kThreads;
+          float v[kElems];
+#pragma unroll
+          for (int e = 0; e < kElems; ++e) v[e] = 0.0f;
+          for (int x0 = 0; x0 < parts; x0 += kPer) {  // a batch of parts: their factors, then their rows
+            const int x = x0 + tid % kPer;
+            float f = 0.0f;
+            if (hq < heads && x < parts) {
+              const float* src = part_of(x) + hq * stride + D;
+              f = exp2f(__ldcg(src) - rj);
+              lj += __ldcg(src + 1) * f;
             }
-            out[i] = lj == 0.0f ? 0.0f : v * (c.v_scale / lj);
-            if (p.a.accumulate && d == 0) lse[h] = lj == 0.0f ? INFINITY : rj - G::kBias + log2f(lj);
+            __syncthreads();
+            so[hq * kPer + tid % kPer] = f;
+            __syncthreads();
+            const int n = min(kPer, parts - x0);
+#pragma unroll
+            for (int e = 0; e < kElems; ++e) {
+              const int i = tid + e * G::kThreads;
+              if (i < heads * D) {
+                const int h = i / D, d = i - h * D;
+                const int64_t at = h * stride + d;
+#pragma unroll 8
+                for (int y = 0; y < n; ++y) v[e] += __ldcg(part_of(x0 + y) + at) * so[h * kPer + y];
+              }
+            }
+          }
+#pragma unroll
+          for (int x = kPer / 2; x > 0; x >>= 1) lj += __shfl_xor_sync(0xffffffffu, lj, x);
+          __syncthreads();
+          if (tid % kPer == 0 && hq < heads) {
+            s_mult[hq] = lj;
+            if (p.a.accumulate) lse[hq] = lj == 0.0f ? INFINITY : rj - G::kBias + log2f(lj);
+          }
+          __syncthreads();
+#pragma unroll
+          for (int e = 0; e < kElems; ++e) {
+            const int i = tid + e * G::kThreads;
+            if (i < heads * D) out[i] = s_mult[i / D] == 0.0f ? 0.0f : v[e] * (c.v_scale / s_mult[i / D]);
           }
         }
       }
@@ -792,9 +904,12 @@ template <typename F>
 Status by_shape(const KvView& v, KvType type, F&& f) {
   return by_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
-    if (v.head_dim <= 64) return f(Tiled<T, 64>{}, k_attend_tiled<T, 64>);
-    if (v.head_dim <= 128) return f(Tiled<T, 128>{}, k_attend_tiled<T, 128>);
-    return f(Tiled<T, 256>{}, k_attend_tiled<T, 256>);
+    if (v.head_dim == 64) return f(Tiled<T, 64, true>{}, k_attend_tiled<T, 64, true>);
+    if (v.head_dim == 128) return f(Tiled<T, 128, true>{}, k_attend_tiled<T, 128, true>);
+    if (v.head_dim == 256) return f(Tiled<T, 256, true>{}, k_attend_tiled<T, 256, true>);
+    if (v.head_dim < 64) return f(Tiled<T, 64, false>{}, k_attend_tiled<T, 64, false>);
+    if (v.head_dim < 128) return f(Tiled<T, 128, false>{}, k_attend_tiled<T, 128, false>);
+    return f(Tiled<T, 256, false>{}, k_attend_tiled<T, 256, false>);
   });
 }
 
