@@ -28,7 +28,7 @@ struct AttendParams {
   int units;       // num_kv * head groups of 8: work units of a sequence
   int head_groups;
   int page_shift;  // log2(page_size), or -1
-  int* counters;   // [num_seqs][units], zero between calls
+  int2* spans;     // [num_seqs][units]: first block and number of blocks of a unit
 };
 
 // ---------------------------------------------------------------- one query head a block
@@ -176,8 +176,9 @@ __global__ void k_attend_weights(const __grid_constant__ AttendParams p) {
 //
 // Work is cut into tiles of 16 keys per warp; the grid's blocks take equal runs of all tiles of
 // all (sequence, key-value head) units, so that ragged lengths balance. A unit that lies within
-// one block is finished there; otherwise each block leaves its partial (o, m, l) and the last one
-// to arrive joins them in block order, which keeps the result independent of timing.
+// one block is finished there; otherwise each block leaves its partial (o, m, l) and a second
+// kernel joins them in block order. (Joined by the last block to arrive, behind a counter, one
+// sequence of 131072 slots took 53 us, the registers of that code among it.)
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -256,7 +257,9 @@ struct Tiled {
   static constexpr int kRow = DP * static_cast<int>(sizeof(T));  // bytes of a row in shared memory (at most, unpadded)
   static constexpr int kWarps = kRow <= 512 ? 4 : 2;
   static constexpr int kStages = kRow <= 128 ? 4 : 3;
+  static constexpr int kDP = DP;
   static constexpr int kThreads = 32 * kWarps;
+  static constexpr int kBlocks = kRow <= 128 ? 3 : (kRow <= 256 && DP <= 128 ? 2 : 1);  // of an SM: what registers allow
   static constexpr int kKeys = 16 * kWarps;  // keys of a block tile
   static constexpr int kLanes = kRow < 128 ? kRow / 16 : 8;  // lanes that copy a row
   static constexpr bool kSwz = kRow % 128 == 0;              // with kFull: chunks xored by the key
@@ -309,13 +312,13 @@ __device__ __forceinline__ float exp2_fast(float x) {  // ex2.approx: 2 ulp, 2^-
 }
 
 template <typename T, int DP, bool kFull>
-__global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads) k_attend_tiled(const __grid_constant__ AttendParams p) {
+__global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kFull>::kBlocks) k_attend_tiled(const __grid_constant__ AttendParams p) {
   using G = Tiled<T, DP, kFull>;
   using M = typename G::M;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long s_sum[G::kWarps];
+  __shared__ long long s_sum[G::kWarps], s_rest[G::kWarps];
   __shared__ long long s_off;
-  __shared__ int s_b, s_last;
+  __shared__ int s_b;
   __shared__ float s_m[G::kWarps][8], s_l[G::kWarps][8], s_mult[8];
   __shared__ uint32_t s_ok[G::kWarps][G::kStages];
   const KvView& c = p.c;
@@ -345,59 +348,70 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads) k_attend_tiled(
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  // this block's run of tiles
-  long long mine = 0;
-  for (int b = tid; b < c.num_seqs; b += G::kThreads) {
+  // This block's run of the list: all units' places, then the sequence that the run begins in.
+  // With no more sequences than threads both come from one reading of the lengths.
+  auto places = [&](int b) -> long long {
+    if (b >= c.num_seqs) return 0;
     Cursor s;
     s.b = b;
     cursor_seq(p, G::kKeys, s);
-    if (blockIdx.x == 0 && (c.lens[b] < 0 || c.lens[b] > c.max_slots)) atomicCAS(c.err, 0, kKvErrSlot);
-    mine += s.nt + kOver;
+    return static_cast<long long>(s.nt + kOver) * p.units;
+  };
+  long long mine = places(tid), scan = mine, rest = 0;
+  for (int b = tid + G::kThreads; b < c.num_seqs; b += G::kThreads) rest += places(b);
+  if (blockIdx.x == 0)
+    for (int b = tid; b < c.num_seqs; b += G::kThreads)
+      if (c.lens[b] < 0 || c.lens[b] > c.max_slots) atomicCAS(c.err, 0, kKvErrSlot);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, scan, o);
+    if (lane >= o) scan += y;
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
-  if (lane == 0) s_sum[w] = mine;
+  for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
+  if (lane == 31) s_sum[w] = scan;
+  if (lane == 0) s_rest[w] = rest;
   __syncthreads();
-  long long total = 0;
+  long long before = 0, chunk = 0, total = 0;
 #pragma unroll
-  for (int i = 0; i < G::kWarps; ++i) total += s_sum[i];
-  total *= p.units;
-  // A unit cut into P runs costs its last block about P / 14 tiles of joining: runs are at least
+  for (int i = 0; i < G::kWarps; ++i) {
+    if (i < w) before += s_sum[i];
+    chunk += s_sum[i];
+    total += s_rest[i];
+  }
+  total += chunk;
+  // A unit cut into P runs costs about P / 14 tiles of joining: runs are at least
   // as long as balances that, and never empty.
   const float tiles = static_cast<float>(total) / static_cast<float>(static_cast<long long>(c.num_seqs) * p.units);
   const int shortest = max(1, static_cast<int>(sqrtf(tiles * (1.0f / 14.0f))));
   const long long n_cta = max(1ll, min(static_cast<long long>(gridDim.x), total / shortest));
   auto run_start = [&](long long i) { return i * total / n_cta; };
-  const long long t0 = run_start(blockIdx.x), t1 = run_start(blockIdx.x + 1);
   if (blockIdx.x >= n_cta) return;
-  for (long long base = 0, acc = 0;; base += G::kThreads) {  // the sequence that t0 lies in
-    const int b = static_cast<int>(base) + tid;
-    Cursor s;
-    s.b = b;
-    s.nt = 0;
-    if (b < c.num_seqs) cursor_seq(p, G::kKeys, s);
-    const long long n = b < c.num_seqs ? static_cast<long long>(s.nt + kOver) * p.units : 0;
-    long long x = n;
+  const long long t0 = run_start(blockIdx.x), t1 = run_start(blockIdx.x + 1);
+  for (long long base = 0, acc = 0;;) {
+    const long long end = acc + before + scan;  // of this thread's sequence
+    if (end - mine <= t0 && t0 < end) {
+      s_b = static_cast<int>(base) + tid;
+      s_off = t0 - (end - mine);
+    }
+    acc += chunk;
+    if (t0 < acc) break;
+    base += G::kThreads;
+    mine = scan = places(static_cast<int>(base) + tid);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
+      const long long y = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += y;
     }
     __syncthreads();
-    if (lane == 31) s_sum[w] = x;
+    if (lane == 31) s_sum[w] = scan;
     __syncthreads();
-    long long before = acc, all = 0;
+    before = chunk = 0;
 #pragma unroll
     for (int i = 0; i < G::kWarps; ++i) {
       if (i < w) before += s_sum[i];
-      all += s_sum[i];
+      chunk += s_sum[i];
     }
-    if (before + x - n <= t0 && t0 < before + x) {
-      s_b = b;
-      s_off = t0 - (before + x - n);
-    }
-    acc += all;
-    if (t0 < acc) break;
   }
   __syncthreads();
   Cursor cur;
@@ -804,7 +818,7 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads) k_attend_tiled(
           lse[tid] = s_mult[tid] == 0.0f ? INFINITY : (s_m[0][tid] == -INFINITY ? 0.0f : s_m[0][tid]) - G::kBias + log2f(s_mult[tid]);
       } else {
         // a block leaves at most two partial units: one that began before its run, one that goes on after it
-        const int stride = D + 2;
+        const int stride = D + 4;  // 16-byte rows
         float* dst = p.part + (2ll * blockIdx.x + (unit_start >= t0 ? 1 : 0)) * 8 * stride;
         for (int i = tid; i < heads * D; i += G::kThreads) {
           const int h = i / D, d = i - h * D;
@@ -814,69 +828,10 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads) k_attend_tiled(
           dst[tid * stride + D] = s_m[0][tid];
           dst[tid * stride + D + 1] = s_mult[tid];
         }
-        const long long c0 = ((unit_start + 1) * n_cta - 1) / total, c1 = ((unit_start + cur.nt) * n_cta - 1) / total;
-        __syncthreads();
-        if (tid == 0) {
-          __threadfence();
-          s_last = atomicAdd(p.counters + seg, 1) == static_cast<int>(c1 - c0);
-        }
-        __syncthreads();
-        if (s_last) {
-          __threadfence();
-          if (tid == 0) p.counters[seg] = 0;
-          const int parts = static_cast<int>(c1 - c0) + 1;
-          // the first block began the unit (its second partial), the others went on with it
-          auto part_of = [&](int i) { return p.part + (2 * (c0 + i) + (i == 0)) * 8 * stride; };
-          // the parts' maxima and sums: kPer threads a head
-          constexpr int kPer = G::kThreads / 8;
-          const int hq = tid / kPer;
-          float mj = -INFINITY, lj = 0.0f;
-          if (hq < heads)
-            for (int x = tid % kPer; x < parts; x += kPer) mj = fmaxf(mj, __ldcg(part_of(x) + hq * stride + D));
-#pragma unroll
-          for (int x = kPer / 2; x > 0; x >>= 1) mj = fmaxf(mj, __shfl_xor_sync(0xffffffffu, mj, x));
-          const float rj = mj == -INFINITY ? 0.0f : mj;
-          constexpr int kElems = 8 * DP / G::kThreads;
-          float v[kElems];
-#pragma unroll
-          for (int e = 0; e < kElems; ++e) v[e] = 0.0f;
-          for (int x0 = 0; x0 < parts; x0 += kPer) {  // a batch of parts: their factors, then their rows
-            const int x = x0 + tid % kPer;
-            float f = 0.0f;
-            if (hq < heads && x < parts) {
-              const float* src = part_of(x) + hq * stride + D;
-              f = exp2f(__ldcg(src) - rj);
-              lj += __ldcg(src + 1) * f;
-            }
-            __syncthreads();
-            so[hq * kPer + tid % kPer] = f;
-            __syncthreads();
-            const int n = min(kPer, parts - x0);
-#pragma unroll
-            for (int e = 0; e < kElems; ++e) {
-              const int i = tid + e * G::kThreads;
-              if (i < heads * D) {
-                const int h = i / D, d = i - h * D;
-                const int64_t at = h * stride + d;
-#pragma unroll 8
-                for (int y = 0; y < n; ++y) v[e] += __ldcg(part_of(x0 + y) + at) * so[h * kPer + y];
-              }
-            }
-          }
-#pragma unroll
-          for (int x = kPer / 2; x > 0; x >>= 1) lj += __shfl_xor_sync(0xffffffffu, lj, x);
-          __syncthreads();
-          if (tid % kPer == 0 && hq < heads) {
-            s_mult[hq] = lj;
-            if (p.a.accumulate) lse[hq] = lj == 0.0f ? INFINITY : rj - G::kBias + log2f(lj);
-          }
-          __syncthreads();
-#pragma unroll
-          for (int e = 0; e < kElems; ++e) {
-            const int i = tid + e * G::kThreads;
-            if (i < heads * D) out[i] = s_mult[i / D] == 0.0f ? 0.0f : v[e] * (c.v_scale / s_mult[i / D]);
-          }
-        }
+      }
+      if (unit_start >= t0 && tid == 0) {  // the block that began the unit says where its parts are
+        const long long c1 = ((unit_start + cur.nt) * n_cta - 1) / total;
+        p.spans[seg] = make_int2(static_cast<int>(blockIdx.x), static_cast<int>(c1 - blockIdx.x) + 1);
       }
       __syncthreads();  // before the next unit's query replaces what was read here
       fresh = true;
@@ -884,6 +839,76 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads) k_attend_tiled(
     cursor_next(p, G::kKeys, cur);
   }
   cp_wait<0>();
+}
+
+// Joins the parts of one (unit, head) in order: the unit's first block left its second slot, the
+// others their first. Four warps take the parts in turn, sums are added in warp order.
+template <int kBias>
+__global__ void __launch_bounds__(128) k_attend_join_parts(const __grid_constant__ AttendParams p) {
+  __shared__ float s_o[4][256];
+  __shared__ float s_m[4], s_l[4];
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const KvView& c = p.c;
+  const int h = blockIdx.x, b = blockIdx.y, D = c.head_dim, stride = D + 4;
+  const int kv = h / p.group, hg = (h - kv * p.group) >> 3, row = (h - kv * p.group) & 7;
+  const int2 span = p.spans[static_cast<int64_t>(b) * p.units + kv * p.head_groups + hg];
+  if (span.y <= 1) return;
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const float* first = p.part + (static_cast<int64_t>(span.x) * 2 * 8 + row) * stride;
+  auto part_of = [&](int i) { return first + static_cast<int64_t>(2 * i + (i == 0)) * 8 * stride; };
+  float m = -INFINITY;
+  for (int i = threadIdx.x; i < span.y; i += 128) m = fmaxf(m, __ldcg(part_of(i) + D));
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+  if (lane == 0) s_m[w] = m;
+  __syncthreads();
+  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  const float ref = m == -INFINITY ? 0.0f : m;
+  float4 v[2] = {};
+  float l = 0.0f;
+  constexpr int kBatch = 8;
+  for (int i0 = w; i0 < span.y; i0 += 4 * kBatch) {
+    float4 r[kBatch][2];
+    float f[kBatch], ls[kBatch];
+#pragma unroll
+    for (int x = 0; x < kBatch; ++x) {
+      const int i = i0 + 4 * x;
+      f[x] = ls[x] = 0.0f;
+      r[x][0] = r[x][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (i < span.y) {
+        const float* src = part_of(i);
+        f[x] = __ldcg(src + D);
+        ls[x] = __ldcg(src + D + 1);
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          if (4 * lane + 128 * e < D) r[x][e] = __ldcg(reinterpret_cast<const float4*>(src + 4 * lane + 128 * e));
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < kBatch; ++x) {
+      if (i0 + 4 * x >= span.y) break;
+      const float fx = exp2_fast(f[x] - ref);
+      l += ls[x] * fx;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        v[e].x += r[x][e].x * fx;
+        v[e].y += r[x][e].y * fx;
+        v[e].z += r[x][e].z * fx;
+        v[e].w += r[x][e].w * fx;
+      }
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (4 * lane + 128 * e < D) *reinterpret_cast<float4*>(&s_o[w][4 * lane + 128 * e]) = v[e];
+  if (lane == 0) s_l[w] = l;
+  __syncthreads();
+  l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+  const float f = l == 0.0f ? 0.0f : c.v_scale / l;
+  float* out = p.a.out + b * p.a.out_ld + static_cast<int64_t>(h) * D;
+  for (int d = threadIdx.x; d < D; d += 128) out[d] = l == 0.0f ? 0.0f : (s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d]) * f;
+  if (threadIdx.x == 0 && p.a.accumulate) p.lse[static_cast<int64_t>(b) * c.num_heads + h] = l == 0.0f ? INFINITY : ref - kBias + log2f(l);
 }
 
 int simple_splits(const KvView& v) {
@@ -913,6 +938,22 @@ Status by_shape(const KvView& v, KvType type, F&& f) {
   });
 }
 
+// A launch that may start while the kernel before it still runs (it waits for its results itself).
+template <typename K, typename P>
+Status launch_after(K* kernel, dim3 grid, int threads, int smem, cudaStream_t st, const P& p) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p), "kv launch");
+}
+
 int head_groups(const KvView& v) { return (v.num_heads / v.num_kv + 7) / 8; }
 
 } // namespace
@@ -935,8 +976,8 @@ Status attend_plan(KvCache* c) {
     const int64_t units = static_cast<int64_t>(v.num_kv) * head_groups(v);
     const int64_t most = v.num_seqs * units * ((v.max_slots + G::kKeys - 1) / G::kKeys);
     c->attend_blocks = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(per_sm) * sms, most));
-    c->part_bytes = static_cast<size_t>(c->attend_blocks) * 2 * 8 * (v.head_dim + 2) * 4;
-    c->counter_bytes = static_cast<size_t>(v.num_seqs) * units * 4;
+    c->part_bytes = static_cast<size_t>(c->attend_blocks) * 2 * 8 * (v.head_dim + 4) * 4;
+    c->span_bytes = static_cast<size_t>(v.num_seqs) * units * 8;
     return Status::Ok();
   });
 }
@@ -956,22 +997,15 @@ Status kv_attend(KvCache* c, const KvAttendArgs& a, cudaStream_t st) {
   p.head_groups = head_groups(v);
   p.units = v.num_kv * p.head_groups;
   p.page_shift = (v.page_size & (v.page_size - 1)) == 0 ? 31 - __builtin_clz(v.page_size) : -1;
-  p.counters = c->counters;
+  p.spans = reinterpret_cast<int2*>(c->spans);
   const unsigned B = v.num_seqs, H = v.num_heads;
   if (c->attend_tiled) {
     WB_TRY(by_shape(v, c->type, [&](auto g, auto* kernel) {
       using G = decltype(g);
-      cudaLaunchAttribute at[1];
-      at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-      at[0].val.programmaticStreamSerializationAllowed = 1;
-      cudaLaunchConfig_t cfg{};
-      cfg.gridDim = dim3(c->attend_blocks);
-      cfg.blockDim = dim3(G::kThreads);
-      cfg.dynamicSmemBytes = G::kSmem;
-      cfg.stream = st;
-      cfg.attrs = at;
-      cfg.numAttrs = 1;
-      return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p), "kv attend launch");
+      WB_TRY(launch_after(kernel, dim3(c->attend_blocks), G::kThreads, G::kSmem, st, p));
+      // a unit of one tile is never cut
+      if (v.max_slots <= G::kKeys) return Status::Ok();
+      return launch_after(k_attend_join_parts<static_cast<int>(G::kBias)>, dim3(H, B), 128, 0, st, p);
     }));
   } else {
     p.splits = simple_splits(v);

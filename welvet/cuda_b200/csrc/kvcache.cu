@@ -354,14 +354,15 @@ static Status kv_alloc(KvCache* c) {
     return at;
   };
   WB_TRY(attend_plan(c));
-  const size_t err = take(4), ticket = take(4), counters = take(c->counter_bytes);
+  const size_t err = take(4), ticket = take(4);
   const size_t part = take(c->part_bytes);  // from here on nothing needs to start as zero
+  const size_t spans = take(c->span_bytes);
   const size_t scores = take(v.weights ? rows * v.max_slots * 4 : 0), lse = take(v.weights ? rows * 4 : 0);
   const size_t moves = take(v.positions ? heads * 2 * (v.max_slots / 2) * 4 : 0), n_moves = take(v.positions ? heads * 4 : 0);
   WB_CUDA(cudaMalloc(&c->work, bytes));
   c->err = reinterpret_cast<int*>(c->work + err);
   c->ticket = reinterpret_cast<int*>(c->work + ticket);
-  c->counters = reinterpret_cast<int*>(c->work + counters);
+  c->spans = c->work + spans;
   c->part = reinterpret_cast<float*>(c->work + part);
   c->scores = reinterpret_cast<float*>(c->work + scores);
   c->lse = reinterpret_cast<float*>(c->work + lse);

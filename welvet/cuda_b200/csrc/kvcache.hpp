@@ -56,9 +56,9 @@ struct KvCache {
   // attend (kv_attend.cu)
   bool attend_tiled = false;
   int attend_blocks = 0;         // blocks of the tiled form
-  size_t part_bytes = 0, counter_bytes = 0;
+  size_t part_bytes = 0, span_bytes = 0;
   float* part = nullptr;         // partial results
-  int* counters = nullptr;       // blocks done per (sequence, unit), zero between calls
+  void* spans = nullptr;         // where each unit's parts are
   float* scores = nullptr;       // [num_seqs][num_heads][max_slots]; with weights only
   float* lse = nullptr;          // [num_seqs][num_heads]
   int32_t* moves = nullptr;      // evict: [num_seqs][num_kv][2][max_slots / 2] slots to fill, slots to take
