@@ -2,9 +2,12 @@
 #include "gdense.hpp"
 
 #include "codec.cuh"
+#include "pipeline.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <algorithm>
 
 namespace wb {
 namespace {
@@ -13,17 +16,125 @@ __device__ __forceinline__ float scale_value(uint16_t bits, int type) {
   return type == kScaleF16 ? __half2float(__ushort_as_half(bits)) : __bfloat162float(__ushort_as_bfloat16(bits));
 }
 
-struct GArgs {
+// ---------------------------------------------------------------- layout
+//
+// The weights are cut into row groups of 16 outputs and chunks of 256 inputs; a record holds one
+// row group's chunk: for each unit of 64 inputs 512 bytes of codes (lane l's 16 bytes are its A
+// fragments of the unit's four m16n8k16 MMAs), then 256 / sg sets of 16 scales and, for Uint4, of
+// 16 zero points, sg being the largest of 32, 64, 128, 256 that divides the group. Records of a row
+// group follow one another, so a warp's piece of work is one contiguous copy. The inputs' order
+// within a unit is the MMAs' own: input 32 (j / 2) + 8 t + 4 (j % 2) + 2 r + e is element e of
+// register r of block j in lane t, so that 8 consecutive inputs of x are a lane's B fragments of two
+// blocks, which span 32 inputs.
+constexpr int kChunk = 256, kUnit = 64;
+
+struct Layout {
+  int row_groups, chunks, units;  // units of 64 inputs in all
+  int sg, shift, sets;            // inputs of a scale set and its logarithm, sets of a record
+  int tail;                       // bytes of a record's scales and zero points
+  int64_t group_bytes;            // records of a row group
+};
+
+Layout layout_of(int rows, int cols, int group, int code) {
+  Layout l;
+  l.row_groups = (rows + 15) / 16;
+  l.units = (cols + kUnit - 1) / kUnit;
+  l.chunks = (cols + kChunk - 1) / kChunk;
+  l.sg = group % 256 == 0 ? 256 : (group % 128 == 0 ? 128 : (group % 64 == 0 ? 64 : 32));
+  l.shift = l.sg == 256 ? 8 : (l.sg == 128 ? 7 : (l.sg == 64 ? 6 : 5));
+  l.sets = kChunk / l.sg;
+  l.tail = l.sets * (code == kCodeUint4 ? 48 : 32);
+  l.group_bytes = static_cast<int64_t>(l.units) * 512 + static_cast<int64_t>(l.chunks) * l.tail;
+  return l;
+}
+
+struct BuildArgs {
   const uint8_t* codes;
   const uint16_t* scales;
   const uint8_t* zeros;
+  int rows, cols, group, groups, code;
+  Layout l;
+  uint8_t* out;
+};
+
+// One block per record.
+__global__ void __launch_bounds__(128) k_group_build(const __grid_constant__ BuildArgs a) {
+  const int chunk = blockIdx.x % a.l.chunks, rg = blockIdx.x / a.l.chunks;
+  const int units = min(kChunk / kUnit, a.l.units - chunk * (kChunk / kUnit));
+  uint8_t* rec = a.out + rg * a.l.group_bytes + static_cast<int64_t>(chunk) * (2048 + a.l.tail);
+  const int64_t row_bytes = (a.cols + 1) / 2;
+  for (int i = threadIdx.x; i < units * 128; i += blockDim.x) {  // 32-bit words of codes
+    const int unit = i >> 7, lane = (i >> 2) & 31, j = i & 3, g = lane >> 2, t = lane & 3;
+    uint32_t word = 0;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {  // A register r: row g + 8 (r & 1), inputs + 2 (r >> 1)
+      const int o = rg * 16 + g + 8 * (r & 1);
+      const int k = chunk * kChunk + unit * kUnit + 32 * (j >> 1) + 8 * t + 4 * (j & 1) + 2 * (r >> 1);
+      uint32_t two = 0;
+      if (o < a.rows && k < a.cols) {
+        two = a.codes[o * row_bytes + k / 2];
+        if (k + 1 >= a.cols) two &= 15u;
+        // Int4 is kept with its sign bit flipped: the code is the value plus 8
+        if (a.code == kCodeInt4) two ^= k + 1 >= a.cols ? 0x08u : 0x88u;
+      }
+      if (a.code == kCodeFp4) word |= two << (8 * r);
+      else word |= (two & 15u) << (4 * r) | (two >> 4) << (4 * r + 16);
+    }
+    *reinterpret_cast<uint32_t*>(rec + unit * 512 + lane * 16 + j * 4) = word;
+  }
+  uint16_t* sc = reinterpret_cast<uint16_t*>(rec + units * 512);
+  uint8_t* zp = rec + units * 512 + a.l.sets * 32;
+  for (int i = threadIdx.x; i < a.l.sets * 16; i += blockDim.x) {  // [set][g][2]: rows g, g + 8
+    const int set = i >> 4, g = (i >> 1) & 7, o = rg * 16 + g + 8 * (i & 1);
+    const int k = chunk * kChunk + set * a.l.sg;
+    const bool ok = o < a.rows && k < a.cols;
+    const int64_t at = static_cast<int64_t>(o) * a.groups + k / a.group;
+    sc[i] = ok ? a.scales[at] : 0;
+    if (a.code == kCodeUint4) zp[i] = ok ? a.zeros[at] : 0;
+  }
+}
+
+// ---------------------------------------------------------------- matrix-vector product
+//
+// HBM bound: in * out / 2 bytes of codes and 2 (Uint4: 3) bytes per group of scales are read once,
+// for 2 in out flops per token. A warp copies records into its own ring of shared memory (one bulk
+// copy each, issued by one lane) and multiplies them on the register path of the tensor cores:
+// codes become exact f16 A fragments, x is two f16 parts (22 bits) after scaling each token's
+// chunk by a power of two, part p of token b in column 2 b + p, so that a thread's pair of
+// accumulators is one token. Products are exact; a scale set's sum (fp32, at most 256 products)
+// is multiplied by its scale and added to the row's fp32 sum.
+// tcgen05 needs N >= 8 and M = 128 rows of dequantised weights in shared or tensor memory; at 1..8
+// tokens the conversion is the work, and the register path takes its result without a store.
+//
+// The blocks take equal runs of all records (row set by row set, chunk by chunk), the warps of a
+// block every kWarps-th record of its run; a row set's sums are added over the warps in shared
+// memory. Row sets that a run's ends cut are joined through global memory by the last block to
+// come, in block order. The weight copies start before the previous kernel's end is waited for.
+constexpr int kMaxTokens = 8;
+constexpr int kGWarps = 8;
+constexpr int kGThreads = 32 * kGWarps;
+constexpr int kRecord = 2048 + 8 * 48;  // the longest record
+constexpr int kGStages = 6;             // records in a warp's ring
+constexpr int kXBytes = 90 * 1024;      // shared memory for x
+
+struct GArgs {
+  const uint8_t* w;
+  Layout l;
   const double* bias;
-  int rows, cols, group, groups, scale_type, act, bias_len;
+  int rows, cols, act, bias_len, scale_type;
   const float* x;
   int64_t x_ld;
   float* pre;
   float* post;
-  int n;
+  int n;             // tokens, 1..8
+  int slabs;         // parts of the inputs whose x fits shared memory, each with its own blocks
+  int slab_chunks;   // chunks of a slab (the last one may have fewer)
+  int slab_blocks;   // blocks of a slab
+  int row_sets;
+  float* part;       // [slabs * slab_blocks][2][rows of a set][8]
+  int* tickets;      // [slabs][row_sets], zero between calls
+  float* slab_sum;   // [slabs][n][rows], with more than one slab
+  int* err;
 };
 
 __device__ __forceinline__ void g_write(const GArgs& a, int o, int b, float y) {
@@ -34,45 +145,296 @@ __device__ __forceinline__ void g_write(const GArgs& a, int o, int b, float y) {
   a.post[at] = static_cast<float>(activate(a.act, v));
 }
 
-constexpr int kMaxTokens = 8;
+__device__ __forceinline__ void g_mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
 
-// A warp per output row: lanes over bytes of the row, the group's scale on every product, fp32 sums.
+// A fragment of one block: E2M1 bytes through the converter; integer codes n as the f16 1024 + n
+// (or 1024 + 16 n, where the nibble stands four bits higher), minus 1024 + zero (or times 1/16,
+// minus 64 + zero), both exact.
 template <int kCode>
-__global__ void __launch_bounds__(256) k_group_gemv_simple(const __grid_constant__ GArgs a) {
-  const int o = blockIdx.x * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
-  if (o >= a.rows) return;
-  float acc[kMaxTokens];
+__device__ __forceinline__ void g_decode(uint32_t w, __half2 z0, __half2 z1, uint32_t (&a)[4]) {
+  if constexpr (kCode == kCodeFp4) {
+    asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+        "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+        : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(w));
+  } else {
+    const uint32_t v = w >> 8;
+    const __half2 sixteenth = __float2half2_rn(0.0625f);
+    auto h = [](uint32_t x) { return *reinterpret_cast<__half2*>(&x); };
+    const __half2 r0 = __hsub2(h((w & 0x000f000fu) | 0x64006400u), z0);
+    const __half2 r1 = __hfma2(h((w & 0x00f000f0u) | 0x64006400u), sixteenth, z1);
+    const __half2 r2 = __hsub2(h((v & 0x000f000fu) | 0x64006400u), z0);
+    const __half2 r3 = __hfma2(h((v & 0x00f000f0u) | 0x64006400u), sixteenth, z1);
+    a[0] = *reinterpret_cast<const uint32_t*>(&r0);
+    a[1] = *reinterpret_cast<const uint32_t*>(&r1);
+    a[2] = *reinterpret_cast<const uint32_t*>(&r2);
+    a[3] = *reinterpret_cast<const uint32_t*>(&r3);
+  }
+}
+
+// kNT n8 tiles of tokens (1: up to 4 tokens, 2: up to 8), kMT row groups a warp (a row set). kSub:
+// sums are scaled every 32 inputs (scale sets of 32) or every unit of 64 (longer ones).
+template <int kCode, int kNT, int kMT, int kSub>
+__global__ void __launch_bounds__(kGThreads) k_group_gemv(const __grid_constant__ GArgs a) {
+  constexpr int kStages = kGStages / kMT;
+  constexpr int kRows = 16 * kMT;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t bars[kGWarps][kStages];
+  __shared__ float s_red[2][kGWarps][kRows][kMaxTokens];
+  __shared__ int s_last;
+  const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
+  uint8_t* const ring = smem + w * (kGStages * kRecord);
+  uint8_t* const sx = smem + kGWarps * kGStages * kRecord;  // x parts: [2 n columns][slab inputs] f16
+  const int slab = blockIdx.x / a.slab_blocks, rank = blockIdx.x - slab * a.slab_blocks;
+  const int c_first = slab * a.slab_chunks, chunks = min(a.slab_chunks, a.l.chunks - c_first);
+  const int pitch = a.slab_chunks * (kChunk * 2) + 64;  // bytes of a column; two columns fill the banks
+  float* const sxs = reinterpret_cast<float*>(sx + 2 * a.n * pitch);  // [token][chunk] 2^-e
+
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (lane == 0) {
 #pragma unroll
-  for (int b = 0; b < kMaxTokens; ++b) acc[b] = 0.0f;
-  const int bytes = (a.cols + 1) / 2;
-  const uint8_t* row = a.codes + static_cast<int64_t>(o) * bytes;
-  for (int i = lane; i < bytes; i += 32) {
-    const uint32_t two = row[i];
-    const int64_t at = static_cast<int64_t>(o) * a.groups + 2 * i / a.group;
-    const float s = scale_value(a.scales[at], a.scale_type);
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int k = 2 * i + e;
-      if (k >= a.cols) break;
-      const uint32_t c = e ? two >> 4 : two & 15u;
-      float w;
-      if (kCode == kCodeFp4) w = dec_fp4_ref(c);
-      else if (kCode == kCodeInt4) w = static_cast<float>(static_cast<int>(c ^ 8u) - 8);
-      else w = static_cast<float>(static_cast<int>(c) - static_cast<int>(a.zeros[at]));
-      w *= s;
-#pragma unroll
-      for (int b = 0; b < kMaxTokens; ++b)
-        if (b < a.n) acc[b] += w * a.x[b * a.x_ld + k];
+    for (int s = 0; s < kStages; ++s) pipe::mbar_init(&bars[w][s], 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+
+  const int64_t total = static_cast<int64_t>(a.row_sets) * chunks;
+  auto run_start = [&](int64_t i) { return i * total / a.slab_blocks; };
+  const int64_t r0 = run_start(rank), r1 = run_start(rank + 1);
+  // the warp's records: r0 + w, + kGWarps, ...
+  int set = static_cast<int>((r0 + w) / chunks), ch = static_cast<int>((r0 + w) - static_cast<int64_t>(set) * chunks);
+  int64_t issued = r0 + w;
+  auto issue = [&](int stage) {
+    if (issued < r1) {
+      if (lane == 0) {
+        const int chunk = c_first + ch;
+        const int bytes = 512 * min(kChunk / kUnit, a.l.units - chunk * (kChunk / kUnit)) + a.l.tail;
+        const int groups = min(kMT, a.l.row_groups - set * kMT);
+        pipe::mbar_expect_tx(&bars[w][stage], bytes * groups);
+        for (int m = 0; m < groups; ++m) {
+          const uint8_t* src = a.w + (set * kMT + m) * a.l.group_bytes + static_cast<int64_t>(chunk) * (2048 + a.l.tail);
+          uint64_t policy;
+          asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+          pipe::bulk_load_hint(ring + (stage * kMT + m) * kRecord, src, bytes, &bars[w][stage], policy);
+        }
+      }
+      issued += kGWarps;
+      ch += kGWarps;
+      while (ch >= chunks) {
+        ch -= chunks;
+        ++set;
+      }
     }
-  }
+  };
 #pragma unroll
-  for (int b = 0; b < kMaxTokens; ++b) {
-    if (b >= a.n) break;
-    float v = acc[b];
+  for (int s = 0; s < kStages; ++s) issue(s);
+
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // x: a warp takes a token's chunk at a time, eight inputs a lane
+  const bool vec = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.x_ld & 3) == 0;
+  for (int i = w; i < a.n * chunks; i += kGWarps) {
+    const int b = i / chunks, c = i - b * chunks;
+    const int k0 = (c_first + c) * kChunk + 8 * lane;
+    const float* src = a.x + b * a.x_ld + k0;
+    float v[8];
+    if (vec && k0 + 8 <= a.cols) {
+      *reinterpret_cast<float4*>(v) = ld_dep4(src);
+      *reinterpret_cast<float4*>(v + 4) = ld_dep4(src + 4);
+    } else {
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
-    if (lane == 0) g_write(a, o, b, v);
+      for (int e = 0; e < 8; ++e) v[e] = k0 + e < a.cols ? ld_dep(src + e) : 0.0f;
+    }
+    float mx = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, isfinite(v[e]) ? fabsf(v[e]) : 0.0f);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    // the chunk's largest finite |x| goes to [2^14, 2^15)
+    const int ex = mx > 0.0f ? min(126, 14 - ilogbf(mx)) : 0;
+    const float f = ldexpf(1.0f, ex);
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float p = v[2 * e] * f, q = v[2 * e + 1] * f;
+      const __half2 h = __floats2half2_rn(p, q);
+      const float2 r = __half22float2(h);
+      // infinities and NaN stay in the first part
+      const __half2 l = __floats2half2_rn(isfinite(p) ? p - r.x : 0.0f, isfinite(q) ? q - r.y : 0.0f);
+      hi[e] = *reinterpret_cast<const uint32_t*>(&h);
+      lo[e] = *reinterpret_cast<const uint32_t*>(&l);
+    }
+    uint8_t* dst = sx + 2 * b * pitch + (c * kChunk + 8 * lane) * 2;
+    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(dst + pitch) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+    if (lane == 0) sxs[b * a.slab_chunks + c] = ldexpf(1.0f, -ex);
   }
+  __syncthreads();
+
+  const uint8_t* xcol[kNT];
+#pragma unroll
+  for (int nt = 0; nt < kNT; ++nt) xcol[nt] = 8 * nt + g < 2 * a.n ? sx + (8 * nt + g) * pitch + 16 * t : nullptr;
+  float acc[kMT][kNT][4];
+#pragma unroll
+  for (int m = 0; m < kMT; ++m)
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) acc[m][nt][e] = 0.0f;
+
+  int stage = 0;
+  uint32_t phase = 0;
+  int buf = 0;
+  int64_t next = r0 + w;  // the warp's next record
+  int64_t rs = r0 / chunks;
+  for (int64_t seg = r0; seg < r1; ++rs) {  // row sets of the run
+    const int64_t set_end = (rs + 1) * chunks, end = set_end < r1 ? set_end : r1;
+    const bool whole = seg == rs * chunks && end == set_end;
+    for (; next < end; next += kGWarps) {
+      const int c = static_cast<int>(next - rs * chunks), chunk = c_first + c;
+      const int units = min(kChunk / kUnit, a.l.units - chunk * (kChunk / kUnit));
+      pipe::warp_wait(&bars[w][stage], phase, a.err, 40);
+      const uint8_t* rec = ring + stage * kMT * kRecord;
+      float xs[kNT];  // of the thread's tokens
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) xs[nt] = 4 * nt + t < a.n ? sxs[(4 * nt + t) * a.slab_chunks + c] : 0.0f;
+      float part[kMT][kNT][4];
+#pragma unroll
+      for (int u = 0; u < kChunk / kUnit; ++u) {
+        if (u >= units) break;
+        uint4 xb[kNT][2];
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+          xb[nt][0] = xb[nt][1] = make_uint4(0, 0, 0, 0);
+          if (xcol[nt]) {
+            const uint4* src = reinterpret_cast<const uint4*>(xcol[nt] + c * (kChunk * 2) + u * (kUnit * 2));
+            xb[nt][0] = src[0];
+            xb[nt][1] = src[4];
+          }
+        }
+#pragma unroll
+        for (int m = 0; m < kMT; ++m) {
+          const uint8_t* mr = rec + m * kRecord;
+          const uint4 codes = *reinterpret_cast<const uint4*>(mr + u * 512 + lane * 16);
+#pragma unroll
+          for (int hf = 0; hf < 2; ++hf) {  // halves of the unit: sets of 32 inputs end with each
+            const int sidx = (u * kUnit + 32 * hf) >> a.l.shift;
+            __half2 z0 = __float2half2_rn(1032.0f), z1 = __float2half2_rn(-72.0f);
+            if constexpr (kCode == kCodeUint4) {
+              const uint32_t z = *reinterpret_cast<const uint16_t*>(mr + units * 512 + a.l.sets * 32 + sidx * 16 + 2 * g);
+              z0 = __half2half2(__ushort_as_half(static_cast<unsigned short>(0x6400u | (z & 0xffu))));
+              z1 = __half2half2(__ushort2half_rn(static_cast<unsigned short>(64u + (z >> 8))));
+              z1 = __hneg2(z1);
+            }
+            if (kSub == 32 || hf == 0) {
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) part[m][nt][e] = 0.0f;
+            }
+#pragma unroll
+            for (int jj = 0; jj < 2; ++jj) {
+              const int j = 2 * hf + jj;
+              const uint32_t word = j == 0 ? codes.x : (j == 1 ? codes.y : (j == 2 ? codes.z : codes.w));
+              uint32_t fr[4];
+              g_decode<kCode>(word, z0, z1, fr);
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt) {
+                const uint4 x = xb[nt][j >> 1];
+                g_mma(part[m][nt], fr, j & 1 ? x.z : x.x, j & 1 ? x.w : x.y);
+              }
+            }
+            if (kSub == 32 || hf == 1) {
+              const uint32_t s2 = *reinterpret_cast<const uint32_t*>(mr + units * 512 + sidx * 32 + 4 * g);
+              const float s0 = scale_value(static_cast<uint16_t>(s2), a.scale_type), s1 = scale_value(static_cast<uint16_t>(s2 >> 16), a.scale_type);
+#pragma unroll
+              for (int nt = 0; nt < kNT; ++nt) {
+                acc[m][nt][0] += part[m][nt][0] * (s0 * xs[nt]);
+                acc[m][nt][1] += part[m][nt][1] * (s0 * xs[nt]);
+                acc[m][nt][2] += part[m][nt][2] * (s1 * xs[nt]);
+                acc[m][nt][3] += part[m][nt][3] * (s1 * xs[nt]);
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+      issue(stage);
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1u;
+      }
+    }
+    // the row set's sums over the warps
+#pragma unroll
+    for (int m = 0; m < kMT; ++m)
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+        s_red[buf][w][16 * m + g][4 * nt + t] = acc[m][nt][0] + acc[m][nt][1];
+        s_red[buf][w][16 * m + g + 8][4 * nt + t] = acc[m][nt][2] + acc[m][nt][3];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[m][nt][e] = 0.0f;
+      }
+    __syncthreads();
+    const int outs = kRows * a.n;
+    auto sum_of = [&](int i) {
+      const int b = i / kRows, r = i - b * kRows;
+      float v = 0.0f;
+#pragma unroll
+      for (int x = 0; x < kGWarps; ++x) v += s_red[buf][x][r][b];
+      return v;
+    };
+    auto write = [&](int i, float v) {
+      const int b = i / kRows, o = static_cast<int>(rs) * kRows + i - b * kRows;
+      if (o >= a.rows) return;
+      if (a.slabs == 1) g_write(a, o, b, v);
+      else a.slab_sum[(static_cast<int64_t>(slab) * a.n + b) * a.rows + o] = v;
+    };
+    if (whole) {
+      for (int i = tid; i < outs; i += kGThreads) write(i, sum_of(i));
+    } else {
+      // cut by the run's ends: the first slot is of the row set that began before the run
+      float* mine = a.part + (2ll * blockIdx.x + (seg == rs * chunks ? 1 : 0)) * (kRows * kMaxTokens);
+      for (int i = tid; i < outs; i += kGThreads) mine[i] = sum_of(i);
+      const int64_t b0 = ((rs * chunks + 1) * a.slab_blocks - 1) / total, b1 = (set_end * a.slab_blocks - 1) / total;
+      int* ticket = a.tickets + static_cast<int64_t>(slab) * a.row_sets + rs;
+      __syncthreads();
+      if (tid == 0) {
+        __threadfence();
+        s_last = atomicAdd(ticket, 1) == static_cast<int>(b1 - b0);
+      }
+      __syncthreads();
+      if (s_last) {
+        __threadfence();
+        if (tid == 0) *ticket = 0;
+        const float* first = a.part + 2ll * (static_cast<int64_t>(slab) * a.slab_blocks + b0) * (kRows * kMaxTokens);
+        for (int i = tid; i < outs; i += kGThreads) {
+          float v = __ldcg(first + kRows * kMaxTokens + i);
+          for (int64_t x = 1; x <= b1 - b0; ++x) v += __ldcg(first + 2 * x * (kRows * kMaxTokens) + i);
+          write(i, v);
+        }
+      }
+    }
+    buf ^= 1;
+    seg = end;
+  }
+}
+
+// y from the slabs' sums, in slab order.
+__global__ void __launch_bounds__(256) k_group_slabs(const __grid_constant__ GArgs a) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int o = blockIdx.x * 256 + threadIdx.x, b = blockIdx.y;
+  if (o >= a.rows) return;
+  float v = 0.0f;
+  for (int s = 0; s < a.slabs; ++s) v += __ldcg(a.slab_sum + (static_cast<int64_t>(s) * a.n + b) * a.rows + o);
+  g_write(a, o, b, v);
 }
 
 // One warp per (row, group): the group's range gives its scale, rounded to the scale's type before
@@ -130,29 +492,135 @@ __global__ void __launch_bounds__(256)
 
 GroupDense::~GroupDense() {
   cudaSetDevice(device);
-  for (void* p : {static_cast<void*>(codes), static_cast<void*>(scales), static_cast<void*>(zeros), static_cast<void*>(bias)})
+  for (void* p : {static_cast<void*>(w), static_cast<void*>(bias), static_cast<void*>(work)})
     if (p) cudaFree(p);
 }
 
-static Status gdense_fill(GroupDense* g, const GroupDenseSrc& src) {
-  WB_CUDA(cudaSetDevice(g->device));
-  const size_t n_codes = static_cast<size_t>(g->rows) * ((g->cols + 1) / 2), n_groups = static_cast<size_t>(g->rows) * g->groups;
-  const cudaMemcpyKind kind = src.on_device ? cudaMemcpyDeviceToDevice : cudaMemcpyHostToDevice;
-  WB_CUDA(cudaMalloc(&g->codes, n_codes));
-  WB_CUDA(cudaMemcpy(g->codes, src.codes, n_codes, kind));
-  WB_CUDA(cudaMalloc(&g->scales, n_groups * 2));
-  WB_CUDA(cudaMemcpy(g->scales, src.scales, n_groups * 2, kind));
-  if (g->code == kCodeUint4) {
-    WB_CUDA(cudaMalloc(&g->zeros, n_groups));
-    WB_CUDA(cudaMemcpy(g->zeros, src.zeros, n_groups, kind));
+namespace {
+
+// Row groups a warp takes together: two share the reads of x, worth it from three tokens on, if the
+// row sets still outnumber the SMs.
+int row_groups_of(int rows, int n) { return n >= 3 && (rows + 31) / 32 >= 2 * 148 ? 2 : 1; }
+
+struct GPlan {
+  int mt, slabs, slab_chunks, slab_blocks, row_sets, smem;
+};
+
+GPlan plan_of(const GroupDense& g, int n) {
+  const Layout l = layout_of(g.rows, g.cols, g.group, g.code);
+  GPlan p;
+  p.mt = row_groups_of(g.rows, n);
+  p.row_sets = (l.row_groups + p.mt - 1) / p.mt;
+  const int fit = (kXBytes - 2 * n * 64) / (n * (2 * kChunk * 2 + 4));  // chunks of x in shared memory
+  p.slabs = (l.chunks + fit - 1) / fit;
+  p.slab_chunks = (l.chunks + p.slabs - 1) / p.slabs;
+  p.slabs = (l.chunks + p.slab_chunks - 1) / p.slab_chunks;
+  p.smem = kGWarps * kGStages * kRecord + 2 * n * (p.slab_chunks * kChunk * 2 + 64) + n * p.slab_chunks * 4;
+  // every warp of a block has a record or more
+  const int64_t last = l.chunks - (p.slabs - 1) * p.slab_chunks;
+  const int64_t most = std::max<int64_t>(1, p.row_sets * last / kGWarps);
+  p.slab_blocks = static_cast<int>(std::min<int64_t>(std::max(1, g.sms / p.slabs), most));
+  return p;
+}
+
+using GKernel = void (*)(GArgs);
+
+template <int kCode, int kSub>
+GKernel kernel_of(int n, int mt) {
+  if (n > 4) return mt == 2 ? k_group_gemv<kCode, 2, 2, kSub> : k_group_gemv<kCode, 2, 1, kSub>;
+  return mt == 2 ? k_group_gemv<kCode, 1, 2, kSub> : k_group_gemv<kCode, 1, 1, kSub>;
+}
+
+template <int kSub>
+GKernel kernel_of(int code, int n, int mt) {
+  if (code == kCodeFp4) return kernel_of<kCodeFp4, kSub>(n, mt);
+  return code == kCodeInt4 ? kernel_of<kCodeInt4, kSub>(n, mt) : kernel_of<kCodeUint4, kSub>(n, mt);
+}
+
+GKernel kernel_of(const GroupDense& g, int n, int mt) {
+  return g.group % 64 == 0 ? kernel_of<64>(g.code, n, mt) : kernel_of<32>(g.code, n, mt);
+}
+
+template <typename K>
+Status g_launch(K* kernel, dim3 grid, int threads, int smem, cudaStream_t st, const GArgs& a) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, a), "group gemv launch");
+}
+
+// Device copies of a mount's host arrays, freed when the mount is done.
+struct Staged {
+  void* p = nullptr;
+  ~Staged() { if (p) cudaFree(p); }
+  Status put(const void* src, size_t n) {
+    WB_CUDA(cudaMalloc(&p, n));
+    return cuda_status(cudaMemcpy(p, src, n, cudaMemcpyHostToDevice), "group dense h2d");
   }
-  g->bias_len = static_cast<int>(src.bias_len < static_cast<size_t>(g->rows) ? src.bias_len : g->rows);
+};
+
+Status gdense_fill(GroupDense* g, const GroupDenseSrc& src) {
+  WB_CUDA(cudaSetDevice(g->device));
+  WB_CUDA(cudaDeviceGetAttribute(&g->sms, cudaDevAttrMultiProcessorCount, g->device));
+  const size_t n_codes = static_cast<size_t>(g->rows) * ((g->cols + 1) / 2), n_groups = static_cast<size_t>(g->rows) * g->groups;
+  BuildArgs b;
+  b.codes = src.codes;
+  b.scales = static_cast<const uint16_t*>(src.scales);
+  b.zeros = src.zeros;
+  Staged codes, scales, zeros;
+  if (!src.on_device) {
+    WB_TRY(codes.put(src.codes, n_codes));
+    WB_TRY(scales.put(src.scales, n_groups * 2));
+    b.codes = static_cast<const uint8_t*>(codes.p);
+    b.scales = static_cast<const uint16_t*>(scales.p);
+    if (src.zeros) {
+      WB_TRY(zeros.put(src.zeros, n_groups));
+      b.zeros = static_cast<const uint8_t*>(zeros.p);
+    }
+  }
+  b.rows = g->rows;
+  b.cols = g->cols;
+  b.group = g->group;
+  b.groups = g->groups;
+  b.code = g->code;
+  b.l = layout_of(g->rows, g->cols, g->group, g->code);
+  WB_CUDA(cudaMalloc(&g->w, b.l.group_bytes * b.l.row_groups));
+  b.out = g->w;
+  k_group_build<<<static_cast<unsigned>(static_cast<int64_t>(b.l.row_groups) * b.l.chunks), 128>>>(b);
+  WB_CUDA(cudaGetLastError());
+  g->bias_len = static_cast<int>(std::min<size_t>(src.bias_len, g->rows));
   if (g->bias_len > 0) {
     WB_CUDA(cudaMalloc(&g->bias, static_cast<size_t>(g->bias_len) * 8));
     WB_CUDA(cudaMemcpy(g->bias, src.bias, static_cast<size_t>(g->bias_len) * 8, cudaMemcpyHostToDevice));
   }
+  // workspaces for every number of tokens
+  size_t part = 0, tickets = 0, slabs = 0;
+  for (int n = 1; n <= kMaxTokens; ++n) {
+    const GPlan p = plan_of(*g, n);
+    part = std::max<size_t>(part, static_cast<size_t>(p.slabs) * p.slab_blocks * 2 * 16 * p.mt * kMaxTokens * 4);
+    tickets = std::max<size_t>(tickets, static_cast<size_t>(p.slabs) * p.row_sets * 4);
+    if (p.slabs > 1) slabs = std::max<size_t>(slabs, static_cast<size_t>(p.slabs) * n * g->rows * 4);
+    WB_CUDA(cudaFuncSetAttribute(kernel_of(*g, n, p.mt), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 kGWarps * kGStages * kRecord + kXBytes + 1024));
+  }
+  auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+  WB_CUDA(cudaMalloc(&g->work, 256 + up(tickets) + up(part) + up(slabs)));
+  g->err = reinterpret_cast<int*>(g->work);
+  g->tickets = reinterpret_cast<int*>(g->work + 256);
+  g->part = reinterpret_cast<float*>(g->work + 256 + up(tickets));
+  g->slab_sum = reinterpret_cast<float*>(g->work + 256 + up(tickets) + up(part));
+  WB_CUDA(cudaMemset(g->work, 0, 256 + up(tickets)));
   return cuda_status(cudaDeviceSynchronize(), "group dense mount");
 }
+
+} // namespace
 
 Status gdense_mount(int device, int rows, int cols, int group, int code, int scale_type, int act, const GroupDenseSrc& src,
                     GroupDense** out) {
@@ -177,30 +645,44 @@ Status gdense_mount(int device, int rows, int cols, int group, int code, int sca
 Status gdense_forward(GroupDense* g, int n, const float* x, int64_t x_ld, float* pre, float* post, cudaStream_t st) {
   WB_CUDA(cudaSetDevice(g->device));
   GArgs a;
-  a.codes = g->codes;
-  a.scales = g->scales;
-  a.zeros = g->zeros;
+  a.w = g->w;
+  a.l = layout_of(g->rows, g->cols, g->group, g->code);
   a.bias = g->bias;
   a.rows = g->rows;
   a.cols = g->cols;
-  a.group = g->group;
-  a.groups = g->groups;
-  a.scale_type = g->scale_type;
   a.act = g->act;
   a.bias_len = g->bias_len;
+  a.scale_type = g->scale_type;
   a.x_ld = x_ld;
+  a.part = g->part;
+  a.tickets = g->tickets;
+  a.slab_sum = g->slab_sum;
+  a.err = g->err;
   for (int b = 0; b < n; b += kMaxTokens) {
-    a.n = n - b < kMaxTokens ? n - b : kMaxTokens;
+    a.n = std::min(n - b, kMaxTokens);
     a.x = x + b * x_ld;
     a.pre = pre ? pre + static_cast<int64_t>(b) * g->rows : nullptr;
     a.post = post + static_cast<int64_t>(b) * g->rows;
-    const int blocks = (g->rows + 7) / 8;
-    if (g->code == kCodeFp4) k_group_gemv_simple<kCodeFp4><<<blocks, 256, 0, st>>>(a);
-    else if (g->code == kCodeInt4) k_group_gemv_simple<kCodeInt4><<<blocks, 256, 0, st>>>(a);
-    else k_group_gemv_simple<kCodeUint4><<<blocks, 256, 0, st>>>(a);
-    WB_TRY(cuda_status(cudaGetLastError(), "group gemv launch"));
+    const GPlan p = plan_of(*g, a.n);
+    a.slabs = p.slabs;
+    a.slab_chunks = p.slab_chunks;
+    a.slab_blocks = p.slab_blocks;
+    a.row_sets = p.row_sets;
+    WB_TRY(g_launch(kernel_of(*g, a.n, p.mt), dim3(p.slabs * p.slab_blocks), kGThreads, p.smem, st, a));
+    if (p.slabs > 1) WB_TRY(g_launch(k_group_slabs, dim3((g->rows + 255) / 256, a.n), 256, 0, st, a));
   }
   return Status::Ok();
+}
+
+Status gdense_check_error(GroupDense* g, cudaStream_t st) {
+  WB_CUDA(cudaSetDevice(g->device));
+  int e = 0;
+  WB_CUDA(cudaMemcpyAsync(&e, g->err, 4, cudaMemcpyDeviceToHost, st));
+  WB_CUDA(cudaStreamSynchronize(st));
+  if (e == 0) return Status::Ok();
+  WB_CUDA(cudaMemsetAsync(g->err, 0, 4, st));
+  WB_CUDA(cudaStreamSynchronize(st));
+  return Status::Internal("group dense: pipeline wait timed out (stage code " + std::to_string(e) + ")");
 }
 
 Status group_quantize(int rows, int cols, int group, int code, int scale_type, const float* W, uint8_t* codes, void* scales,

@@ -47,6 +47,7 @@ _sig("welvet_b200_group_quantize", _ST, c_int32, c_int32, c_int32, c_int32, c_in
 _sig("welvet_b200_gdense_mount", _ST, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
      c_int32, c_void_p, c_size_t, POINTER(c_void_p))
 _sig("welvet_b200_gdense_execute_device", _ST, c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p)
+_sig("welvet_b200_gdense_check_error", _ST, c_void_p, c_void_p)
 _sig("welvet_b200_gdense_release", None, c_void_p)
 
 _append, _attend, _evict, _gemv = (_L.welvet_b200_kv_append, _L.welvet_b200_kv_attend, _L.welvet_b200_kv_evict,
@@ -54,9 +55,13 @@ _append, _attend, _evict, _gemv = (_L.welvet_b200_kv_append, _L.welvet_b200_kv_a
 _F32, _I32 = torch.float32, torch.int32
 
 
-def _stream(stream) -> int:
+# The current stream's handle without the Stream object around it (3 us a call).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+
+
+def _stream(stream, t=None) -> int:
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream
+        return _raw_stream(torch.cuda.current_device() if t is None else t.get_device())
     return getattr(stream, "cuda_stream", stream)
 
 
@@ -154,7 +159,7 @@ class PagedKV:
             _, op, o_ld = _rows(q_out, self._qw, "q_out", rows)
         n = self.num_seqs
         st = _append(self._h, rows, kp, k_ld, vp, v_ld, qp, q_ld, op, o_ld, _ints(cu_tokens, n + 1, "cu_tokens"), theta,
-                     _ints(start, n, "start"), _ints(start_seen, n, "start_seen"), _stream(stream))
+                     _ints(start, n, "start"), _ints(start_seen, n, "start_seen"), _stream(stream, k))
         if st.code != OK:
             _fail(st)
 
@@ -164,7 +169,7 @@ class PagedKV:
         _, qp, q_ld = _rows(q, self._qw, "q", self.num_seqs)
         _, op, o_ld = _rows(out, self._qw, "out", self.num_seqs)
         st = _attend(self._h, qp, q_ld, op, o_ld, scale, window, 1 if alibi else 0, 1 if accumulate else 0,
-                     None if weights_in is None else self._weights(weights_in, "weights_in"), _stream(stream))
+                     None if weights_in is None else self._weights(weights_in, "weights_in"), _stream(stream, q))
         if st.code != OK:
             _fail(st)
 
@@ -174,13 +179,13 @@ class PagedKV:
         st = _evict(self._h, keep, keep if budget is None else budget, sinks, recent,
                     _ints(lens_in, self.num_seqs, "lens_in"),
                     None if weights_in is None else self._weights(weights_in, "weights_in"),
-                    None if positions_in is None else self._positions(positions_in, "positions_in"), _stream(stream))
+                    None if positions_in is None else self._positions(positions_in, "positions_in"), _stream(stream, self.lens))
         if st.code != OK:
             _fail(st)
 
     def check_error(self, stream=None) -> None:
         """Synchronizes and raises (code 1) if an earlier call met a bad page id or length."""
-        check(_L.welvet_b200_kv_check_error(self._h, _stream(stream)))
+        check(_L.welvet_b200_kv_check_error(self._h, _stream(stream, self.lens)))
 
     def release(self) -> None:
         if self._h:
@@ -206,7 +211,7 @@ def group_quantize(W, group: int, code: int, scale_dtype=torch.bfloat16, stream=
     scales = torch.empty((out, groups), dtype=scale_dtype, device=W.device)
     zeros = torch.empty((out, groups), dtype=torch.uint8, device=W.device) if code == UINT4 else None
     check(_L.welvet_b200_group_quantize(in_, out, group, code, _SCALES[scale_dtype], W.data_ptr(), codes.data_ptr(),
-                                        scales.data_ptr(), None if zeros is None else zeros.data_ptr(), _stream(stream)))
+                                        scales.data_ptr(), None if zeros is None else zeros.data_ptr(), _stream(stream, W)))
     return codes, scales, zeros
 
 
@@ -249,9 +254,13 @@ class GroupDense:
         for t, what in ((y, "y"), (pre, "pre")):
             if t is not None and (t.dtype is not _F32 or not t.is_cuda or not t.is_contiguous() or t.shape != (rows, self.out)):
                 raise ValueError(f"{what}: expected a contiguous float32 CUDA tensor ({rows}, {self.out})")
-        st = _gemv(self._h, rows, xp, x_ld, None if pre is None else pre.data_ptr(), y.data_ptr(), _stream(stream))
+        st = _gemv(self._h, rows, xp, x_ld, None if pre is None else pre.data_ptr(), y.data_ptr(), _stream(stream, x))
         if st.code != OK:
             _fail(st)
+
+    def check_error(self, stream=None) -> None:
+        """Synchronizes and raises (code 4) if a weight copy of an earlier call timed out."""
+        check(_L.welvet_b200_gdense_check_error(self._h, _stream(stream)))
 
     def release(self) -> None:
         if self._h:
