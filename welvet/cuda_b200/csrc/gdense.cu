@@ -8,6 +8,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <type_traits>
 
 namespace wb {
 namespace {
@@ -151,6 +152,13 @@ __device__ __forceinline__ void g_mma(float (&d)[4], const uint32_t (&a)[4], uin
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same from zero.
+__device__ __forceinline__ void g_mma0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 // A fragment of one block: E2M1 bytes through the converter; integer codes n as the f16 1024 + n
 // (or 1024 + 16 n, where the nibble stands four bits higher), minus 1024 + zero (or times 1/16,
 // minus 64 + zero), both exact.
@@ -180,14 +188,16 @@ __device__ __forceinline__ void g_decode(uint32_t w, __half2 z0, __half2 z1, uin
 }
 
 // kNT n8 tiles of tokens (1: up to 4 tokens, 2: up to 8), kMT row groups a warp (a row set). kSub:
-// sums are scaled every 32 inputs (scale sets of 32) or every unit of 64 (longer ones).
-template <int kCode, int kNT, int kMT, int kSub>
-__global__ void __launch_bounds__(kGThreads) k_group_gemv(const __grid_constant__ GArgs a) {
+// sums are scaled every 32 inputs (scale sets of 32) or every unit of 64 (longer ones). kScale: the
+// scales' type.
+template <int kCode, int kNT, int kMT, int kSub, int kScale>
+__global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_constant__ GArgs a) {
   constexpr int kStages = kGStages / kMT;
   constexpr int kRows = 16 * kMT;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kGWarps][kStages];
   __shared__ float s_red[2][kGWarps][kRows][kMaxTokens];
+  __shared__ __align__(16) uint8_t s_zero[kChunk * 2];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
   uint8_t* const ring = smem + w * (kGStages * kRecord);
@@ -198,6 +208,7 @@ __global__ void __launch_bounds__(kGThreads) k_group_gemv(const __grid_constant_
   float* const sxs = reinterpret_cast<float*>(sx + 2 * a.n * pitch);  // [token][chunk] 2^-e
 
   asm volatile("griddepcontrol.launch_dependents;");
+  if (tid < kChunk / 8) *reinterpret_cast<uint4*>(s_zero + 16 * tid) = make_uint4(0, 0, 0, 0);
   if (lane == 0) {
 #pragma unroll
     for (int s = 0; s < kStages; ++s) pipe::mbar_init(&bars[w][s], 1);
@@ -277,9 +288,15 @@ __global__ void __launch_bounds__(kGThreads) k_group_gemv(const __grid_constant_
   }
   __syncthreads();
 
+  // columns without a token read zeros
   const uint8_t* xcol[kNT];
+  int xstep[kNT];
 #pragma unroll
-  for (int nt = 0; nt < kNT; ++nt) xcol[nt] = 8 * nt + g < 2 * a.n ? sx + (8 * nt + g) * pitch + 16 * t : nullptr;
+  for (int nt = 0; nt < kNT; ++nt) {
+    const bool on = 8 * nt + g < 2 * a.n;
+    xcol[nt] = on ? sx + (8 * nt + g) * pitch + 16 * t : s_zero + 16 * t;
+    xstep[nt] = on ? kChunk * 2 : 0;
+  }
   float acc[kMT][kNT][4];
 #pragma unroll
   for (int m = 0; m < kMT; ++m)
@@ -301,68 +318,83 @@ __global__ void __launch_bounds__(kGThreads) k_group_gemv(const __grid_constant_
       const int units = min(kChunk / kUnit, a.l.units - chunk * (kChunk / kUnit));
       pipe::warp_wait(&bars[w][stage], phase, a.err, 40);
       const uint8_t* rec = ring + stage * kMT * kRecord;
-      float xs[kNT];  // of the thread's tokens
+      const uint8_t* xp[kNT];
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) xs[nt] = 4 * nt + t < a.n ? sxs[(4 * nt + t) * a.slab_chunks + c] : 0.0f;
-      float part[kMT][kNT][4];
+      for (int nt = 0; nt < kNT; ++nt) xp[nt] = xcol[nt] + c * xstep[nt];
+      float sum[kMT][kNT][4];  // the record's, in units of the thread's token's 2^-e
 #pragma unroll
-      for (int u = 0; u < kChunk / kUnit; ++u) {
-        if (u >= units) break;
-        uint4 xb[kNT][2];
+      for (int m = 0; m < kMT; ++m)
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt) {
-          xb[nt][0] = xb[nt][1] = make_uint4(0, 0, 0, 0);
-          if (xcol[nt]) {
-            const uint4* src = reinterpret_cast<const uint4*>(xcol[nt] + c * (kChunk * 2) + u * (kUnit * 2));
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sum[m][nt][e] = 0.0f;
+      // `full`: all four units are there, and nothing stands between their instructions
+      auto record = [&](auto full) {
+        constexpr bool kFull = decltype(full)::value;
+        const int tail_at = kFull ? 2048 : units * 512;
+#pragma unroll
+        for (int u = 0; u < kChunk / kUnit; ++u) {
+          float part[kMT][kNT][4];
+          if (!kFull && u >= units) break;
+          uint4 xb[kNT][2];
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt) {
+            const uint4* src = reinterpret_cast<const uint4*>(xp[nt] + u * (kUnit * 2));
             xb[nt][0] = src[0];
             xb[nt][1] = src[4];
           }
-        }
 #pragma unroll
-        for (int m = 0; m < kMT; ++m) {
-          const uint8_t* mr = rec + m * kRecord;
-          const uint4 codes = *reinterpret_cast<const uint4*>(mr + u * 512 + lane * 16);
+          for (int m = 0; m < kMT; ++m) {
+            const uint8_t* mr = rec + m * kRecord;
+            const uint4 codes = *reinterpret_cast<const uint4*>(mr + u * 512 + lane * 16);
 #pragma unroll
-          for (int hf = 0; hf < 2; ++hf) {  // halves of the unit: sets of 32 inputs end with each
-            const int sidx = (u * kUnit + 32 * hf) >> a.l.shift;
-            __half2 z0 = __float2half2_rn(1032.0f), z1 = __float2half2_rn(-72.0f);
-            if constexpr (kCode == kCodeUint4) {
-              const uint32_t z = *reinterpret_cast<const uint16_t*>(mr + units * 512 + a.l.sets * 32 + sidx * 16 + 2 * g);
-              z0 = __half2half2(__ushort_as_half(static_cast<unsigned short>(0x6400u | (z & 0xffu))));
-              z1 = __half2half2(__ushort2half_rn(static_cast<unsigned short>(64u + (z >> 8))));
-              z1 = __hneg2(z1);
-            }
-            if (kSub == 32 || hf == 0) {
-#pragma unroll
-              for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) part[m][nt][e] = 0.0f;
-            }
-#pragma unroll
-            for (int jj = 0; jj < 2; ++jj) {
-              const int j = 2 * hf + jj;
-              const uint32_t word = j == 0 ? codes.x : (j == 1 ? codes.y : (j == 2 ? codes.z : codes.w));
-              uint32_t fr[4];
-              g_decode<kCode>(word, z0, z1, fr);
-#pragma unroll
-              for (int nt = 0; nt < kNT; ++nt) {
-                const uint4 x = xb[nt][j >> 1];
-                g_mma(part[m][nt], fr, j & 1 ? x.z : x.x, j & 1 ? x.w : x.y);
+            for (int hf = 0; hf < 2; ++hf) {  // halves of the unit: sets of 32 inputs end with each
+              const int sidx = (u * kUnit + 32 * hf) >> a.l.shift;
+              __half2 z0 = __float2half2_rn(1032.0f), z1 = __float2half2_rn(-72.0f);
+              if constexpr (kCode == kCodeUint4) {
+                const uint32_t z = *reinterpret_cast<const uint16_t*>(mr + tail_at + a.l.sets * 32 + sidx * 16 + 2 * g);
+                z0 = __half2half2(__ushort_as_half(static_cast<unsigned short>(0x6400u | (z & 0xffu))));
+                z1 = __half2half2(__ushort2half_rn(static_cast<unsigned short>(64u + (z >> 8))));
+                z1 = __hneg2(z1);
               }
-            }
-            if (kSub == 32 || hf == 1) {
-              const uint32_t s2 = *reinterpret_cast<const uint32_t*>(mr + units * 512 + sidx * 32 + 4 * g);
-              const float s0 = scale_value(static_cast<uint16_t>(s2), a.scale_type), s1 = scale_value(static_cast<uint16_t>(s2 >> 16), a.scale_type);
 #pragma unroll
-              for (int nt = 0; nt < kNT; ++nt) {
-                acc[m][nt][0] += part[m][nt][0] * (s0 * xs[nt]);
-                acc[m][nt][1] += part[m][nt][1] * (s0 * xs[nt]);
-                acc[m][nt][2] += part[m][nt][2] * (s1 * xs[nt]);
-                acc[m][nt][3] += part[m][nt][3] * (s1 * xs[nt]);
+              for (int jj = 0; jj < 2; ++jj) {
+                const int j = 2 * hf + jj;
+                const uint32_t word = j == 0 ? codes.x : (j == 1 ? codes.y : (j == 2 ? codes.z : codes.w));
+                uint32_t fr[4];
+                g_decode<kCode>(word, z0, z1, fr);
+#pragma unroll
+                for (int nt = 0; nt < kNT; ++nt) {
+                  const uint4 x = xb[nt][j >> 1];
+                  const uint32_t b0 = j & 1 ? x.z : x.x, b1 = j & 1 ? x.w : x.y;
+                  if (jj == 0 && (kSub == 32 || hf == 0)) g_mma0(part[m][nt], fr, b0, b1);
+                  else g_mma(part[m][nt], fr, b0, b1);
+                }
+              }
+              if (kSub == 32 || hf == 1) {
+                const uint32_t s2 = *reinterpret_cast<const uint32_t*>(mr + tail_at + sidx * 32 + 4 * g);
+                const float s0 = scale_value(static_cast<uint16_t>(s2), kScale), s1 = scale_value(static_cast<uint16_t>(s2 >> 16), kScale);
+#pragma unroll
+                for (int nt = 0; nt < kNT; ++nt) {
+                  sum[m][nt][0] += part[m][nt][0] * s0;
+                  sum[m][nt][1] += part[m][nt][1] * s0;
+                  sum[m][nt][2] += part[m][nt][2] * s1;
+                  sum[m][nt][3] += part[m][nt][3] * s1;
+                }
               }
             }
           }
         }
+      };
+      if (units == kChunk / kUnit) record(std::true_type{});
+      else record(std::false_type{});
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+        const float xs = 4 * nt + t < a.n ? sxs[(4 * nt + t) * a.slab_chunks + c] : 0.0f;
+#pragma unroll
+        for (int m = 0; m < kMT; ++m)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[m][nt][e] += sum[m][nt][e] * xs;
       }
       __syncwarp();
       issue(stage);
@@ -498,9 +530,11 @@ GroupDense::~GroupDense() {
 
 namespace {
 
-// Row groups a warp takes together: two share the reads of x, worth it from three tokens on, if the
-// row sets still outnumber the SMs.
-int row_groups_of(int rows, int n) { return n >= 3 && (rows + 31) / 32 >= 2 * 148 ? 2 : 1; }
+// Row groups a warp takes together: two share the reads of x and a record's bookkeeping, unless the
+// layer has too few records for every warp.
+int row_groups_of(const Layout& l, int sms) {
+  return static_cast<int64_t>(l.row_groups / 2) * l.chunks >= static_cast<int64_t>(sms) * kGWarps ? 2 : 1;
+}
 
 struct GPlan {
   int mt, slabs, slab_chunks, slab_blocks, row_sets, smem;
@@ -509,7 +543,7 @@ struct GPlan {
 GPlan plan_of(const GroupDense& g, int n) {
   const Layout l = layout_of(g.rows, g.cols, g.group, g.code);
   GPlan p;
-  p.mt = row_groups_of(g.rows, n);
+  p.mt = row_groups_of(l, g.sms);
   p.row_sets = (l.row_groups + p.mt - 1) / p.mt;
   const int fit = (kXBytes - 2 * n * 64) / (n * (2 * kChunk * 2 + 4));  // chunks of x in shared memory
   p.slabs = (l.chunks + fit - 1) / fit;
@@ -525,20 +559,21 @@ GPlan plan_of(const GroupDense& g, int n) {
 
 using GKernel = void (*)(GArgs);
 
-template <int kCode, int kSub>
+template <int kCode, int kSub, int kScale>
 GKernel kernel_of(int n, int mt) {
-  if (n > 4) return mt == 2 ? k_group_gemv<kCode, 2, 2, kSub> : k_group_gemv<kCode, 2, 1, kSub>;
-  return mt == 2 ? k_group_gemv<kCode, 1, 2, kSub> : k_group_gemv<kCode, 1, 1, kSub>;
+  if (n > 4) return mt == 2 ? k_group_gemv<kCode, 2, 2, kSub, kScale> : k_group_gemv<kCode, 2, 1, kSub, kScale>;
+  return mt == 2 ? k_group_gemv<kCode, 1, 2, kSub, kScale> : k_group_gemv<kCode, 1, 1, kSub, kScale>;
 }
 
-template <int kSub>
+template <int kSub, int kScale>
 GKernel kernel_of(int code, int n, int mt) {
-  if (code == kCodeFp4) return kernel_of<kCodeFp4, kSub>(n, mt);
-  return code == kCodeInt4 ? kernel_of<kCodeInt4, kSub>(n, mt) : kernel_of<kCodeUint4, kSub>(n, mt);
+  if (code == kCodeFp4) return kernel_of<kCodeFp4, kSub, kScale>(n, mt);
+  return code == kCodeInt4 ? kernel_of<kCodeInt4, kSub, kScale>(n, mt) : kernel_of<kCodeUint4, kSub, kScale>(n, mt);
 }
 
 GKernel kernel_of(const GroupDense& g, int n, int mt) {
-  return g.group % 64 == 0 ? kernel_of<64>(g.code, n, mt) : kernel_of<32>(g.code, n, mt);
+  if (g.scale_type == kScaleF16) return g.group % 64 == 0 ? kernel_of<64, kScaleF16>(g.code, n, mt) : kernel_of<32, kScaleF16>(g.code, n, mt);
+  return g.group % 64 == 0 ? kernel_of<64, kScaleBF16>(g.code, n, mt) : kernel_of<32, kScaleBF16>(g.code, n, mt);
 }
 
 template <typename K>
