@@ -21,9 +21,9 @@ __device__ __forceinline__ float scale_value(uint16_t bits, int type) {
 //
 // The weights are cut into row groups of 16 outputs and chunks of 256 inputs; a record holds one
 // row group's chunk: for each unit of 64 inputs 512 bytes of codes (lane l's 16 bytes are its A
-// fragments of the unit's four m16n8k16 MMAs), then 256 / sg sets of 16 scales and, for Uint4, of
-// 16 zero points, sg being the largest of 32, 64, 128, 256 that divides the group. Records of a row
-// group follow one another, so a warp's piece of work is one contiguous copy. The inputs' order
+// fragments of the unit's four m16n8k16 MMAs), then 16 scales and, for Uint4, 16 zero points
+// per set of sg inputs ([8 rows][set][row, row + 8]), sg being the largest of 32, 64, 128, 256 that
+// divides the group. Records of a row group follow one another, so a warp's piece of work is one contiguous copy. The inputs' order
 // within a unit is the MMAs' own: input 32 (j / 2) + 8 t + 4 (j % 2) + 2 r + e is element e of
 // register r of block j in lane t, so that 8 consecutive inputs of x are a lane's B fragments of two
 // blocks, which span 32 inputs.
@@ -85,8 +85,8 @@ __global__ void __launch_bounds__(128) k_group_build(const __grid_constant__ Bui
   }
   uint16_t* sc = reinterpret_cast<uint16_t*>(rec + units * 512);
   uint8_t* zp = rec + units * 512 + a.l.sets * 32;
-  for (int i = threadIdx.x; i < a.l.sets * 16; i += blockDim.x) {  // [set][g][2]: rows g, g + 8
-    const int set = i >> 4, g = (i >> 1) & 7, o = rg * 16 + g + 8 * (i & 1);
+  for (int i = threadIdx.x; i < a.l.sets * 16; i += blockDim.x) {  // [g][set][2]: rows g, g + 8
+    const int g = i / (2 * a.l.sets), set = (i >> 1) % a.l.sets, o = rg * 16 + g + 8 * (i & 1);
     const int k = chunk * kChunk + set * a.l.sg;
     const bool ok = o < a.rows && k < a.cols;
     const int64_t at = static_cast<int64_t>(o) * a.groups + k / a.group;
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
   constexpr int kRows = 16 * kMT;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kGWarps][kStages];
-  __shared__ float s_red[2][kGWarps][kRows][kMaxTokens];
+  __shared__ float s_red[2][kGWarps][kRows][4 * kNT];
   __shared__ __align__(16) uint8_t s_zero[kChunk * 2];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -222,25 +222,30 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
   // the warp's records: r0 + w, + kGWarps, ...
   int set = static_cast<int>((r0 + w) / chunks), ch = static_cast<int>((r0 + w) - static_cast<int64_t>(set) * chunks);
   int64_t issued = r0 + w;
+  const int rec_bytes = 2048 + a.l.tail, last_bytes = 512 * (a.l.units - (a.l.chunks - 1) * (kChunk / kUnit)) + a.l.tail;
+  const int to_last = a.l.chunks - 1 - c_first;
+  const uint8_t* src = a.w + static_cast<int64_t>(set) * kMT * a.l.group_bytes + static_cast<int64_t>(c_first + ch) * rec_bytes;
+  uint64_t policy;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
   auto issue = [&](int stage) {
     if (issued < r1) {
       if (lane == 0) {
-        const int chunk = c_first + ch;
-        const int bytes = 512 * min(kChunk / kUnit, a.l.units - chunk * (kChunk / kUnit)) + a.l.tail;
-        const int groups = min(kMT, a.l.row_groups - set * kMT);
-        pipe::mbar_expect_tx(&bars[w][stage], bytes * groups);
-        for (int m = 0; m < groups; ++m) {
-          const uint8_t* src = a.w + (set * kMT + m) * a.l.group_bytes + static_cast<int64_t>(chunk) * (2048 + a.l.tail);
-          uint64_t policy;
-          asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-          pipe::bulk_load_hint(ring + (stage * kMT + m) * kRecord, src, bytes, &bars[w][stage], policy);
-        }
+        const int bytes = ch == to_last ? last_bytes : rec_bytes;
+        const int groups = kMT == 1 ? 1 : min(kMT, a.l.row_groups - set * kMT);
+        uint64_t* bar = &bars[w][stage];
+        pipe::mbar_expect_tx(bar, bytes * groups);
+        pipe::bulk_load_hint(ring + stage * kMT * kRecord, src, bytes, bar, policy);
+        if (kMT > 1 && groups > 1) pipe::bulk_load_hint(ring + (stage * kMT + 1) * kRecord, src + a.l.group_bytes, bytes, bar, policy);
       }
       issued += kGWarps;
       ch += kGWarps;
-      while (ch >= chunks) {
-        ch -= chunks;
-        ++set;
+      src += kGWarps * rec_bytes;
+      if (ch >= chunks) {
+        do {
+          ch -= chunks;
+          ++set;
+        } while (ch >= chunks);
+        src = a.w + static_cast<int64_t>(set) * kMT * a.l.group_bytes + static_cast<int64_t>(c_first + ch) * rec_bytes;
       }
     }
   };
@@ -250,41 +255,51 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // x: a warp takes a token's chunk at a time, eight inputs a lane
   const bool vec = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.x_ld & 3) == 0;
-  for (int i = w; i < a.n * chunks; i += kGWarps) {
-    const int b = i / chunks, c = i - b * chunks;
-    const int k0 = (c_first + c) * kChunk + 8 * lane;
-    const float* src = a.x + b * a.x_ld + k0;
-    float v[8];
-    if (vec && k0 + 8 <= a.cols) {
-      *reinterpret_cast<float4*>(v) = ld_dep4(src);
-      *reinterpret_cast<float4*>(v + 4) = ld_dep4(src + 4);
-    } else {
+  constexpr int kFly = 4;  // chunks whose loads are in flight together
+  for (int i0 = w; i0 < a.n * chunks; i0 += kFly * kGWarps) {
+    float v[kFly][8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = k0 + e < a.cols ? ld_dep(src + e) : 0.0f;
+    for (int y = 0; y < kFly; ++y) {
+      const int i = i0 + y * kGWarps, b = i / chunks, c = i - b * chunks;
+      const int k0 = (c_first + c) * kChunk + 8 * lane;
+      const float* src = a.x + b * a.x_ld + k0;
+      const bool on = i < a.n * chunks;
+      if (vec && on && k0 + 8 <= a.cols) {
+        *reinterpret_cast<float4*>(v[y]) = ld_dep4(src);
+        *reinterpret_cast<float4*>(v[y] + 4) = ld_dep4(src + 4);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[y][e] = on && k0 + e < a.cols ? ld_dep(src + e) : 0.0f;
+      }
     }
-    float mx = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) mx = fmaxf(mx, isfinite(v[e]) ? fabsf(v[e]) : 0.0f);
+    for (int y = 0; y < kFly; ++y) {
+      const int i = i0 + y * kGWarps, b = i / chunks, c = i - b * chunks;
+      if (i >= a.n * chunks) break;
+      float mx = 0.0f;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    // the chunk's largest finite |x| goes to [2^14, 2^15)
-    const int ex = mx > 0.0f ? min(126, 14 - ilogbf(mx)) : 0;
-    const float f = ldexpf(1.0f, ex);
-    uint32_t hi[4], lo[4];
+      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, isfinite(v[y][e]) ? fabsf(v[y][e]) : 0.0f);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float p = v[2 * e] * f, q = v[2 * e + 1] * f;
-      const __half2 h = __floats2half2_rn(p, q);
-      const float2 r = __half22float2(h);
-      // infinities and NaN stay in the first part
-      const __half2 l = __floats2half2_rn(isfinite(p) ? p - r.x : 0.0f, isfinite(q) ? q - r.y : 0.0f);
-      hi[e] = *reinterpret_cast<const uint32_t*>(&h);
-      lo[e] = *reinterpret_cast<const uint32_t*>(&l);
+      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      // the chunk's largest finite |x| goes to [2^14, 2^15)
+      const int ex = mx > 0.0f ? min(126, 14 - ilogbf(mx)) : 0;
+      const float f = ldexpf(1.0f, ex);
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = v[y][2 * e] * f, q = v[y][2 * e + 1] * f;
+        const __half2 h = __floats2half2_rn(p, q);
+        const float2 r = __half22float2(h);
+        // infinities and NaN stay in the first part
+        const __half2 l = __floats2half2_rn(isfinite(p) ? p - r.x : 0.0f, isfinite(q) ? q - r.y : 0.0f);
+        hi[e] = *reinterpret_cast<const uint32_t*>(&h);
+        lo[e] = *reinterpret_cast<const uint32_t*>(&l);
+      }
+      uint8_t* dst = sx + 2 * b * pitch + (c * kChunk + 8 * lane) * 2;
+      *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+      *reinterpret_cast<uint4*>(dst + pitch) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      if (lane == 0) sxs[b * a.slab_chunks + c] = ldexpf(1.0f, -ex);
     }
-    uint8_t* dst = sx + 2 * b * pitch + (c * kChunk + 8 * lane) * 2;
-    *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-    *reinterpret_cast<uint4*>(dst + pitch) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-    if (lane == 0) sxs[b * a.slab_chunks + c] = ldexpf(1.0f, -ex);
   }
   __syncthreads();
 
@@ -316,7 +331,8 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
     for (; next < end; next += kGWarps) {
       const int c = static_cast<int>(next - rs * chunks), chunk = c_first + c;
       const int units = min(kChunk / kUnit, a.l.units - chunk * (kChunk / kUnit));
-      pipe::warp_wait(&bars[w][stage], phase, a.err, 40);
+      pipe::mbar_wait(&bars[w][stage], phase, a.err, 40);
+      __syncwarp();
       const uint8_t* rec = ring + stage * kMT * kRecord;
       const uint8_t* xp[kNT];
 #pragma unroll
@@ -332,6 +348,18 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
       auto record = [&](auto full) {
         constexpr bool kFull = decltype(full)::value;
         const int tail_at = kFull ? 2048 : units * 512;
+        // sets of 32: the lane's eight scales and zero points of two rows at once
+        uint4 sc[kMT][2], zp[kMT];
+        if constexpr (kSub == 32) {
+#pragma unroll
+          for (int m = 0; m < kMT; ++m) {
+            const uint8_t* tl = rec + m * kRecord + tail_at;
+            sc[m][0] = *reinterpret_cast<const uint4*>(tl + 32 * g);
+            sc[m][1] = *reinterpret_cast<const uint4*>(tl + 32 * g + 16);
+            if constexpr (kCode == kCodeUint4) zp[m] = *reinterpret_cast<const uint4*>(tl + 256 + 16 * g);
+          }
+        }
+        auto word_of = [](const uint4& q, int i) { return i == 0 ? q.x : (i == 1 ? q.y : (i == 2 ? q.z : q.w)); };
 #pragma unroll
         for (int u = 0; u < kChunk / kUnit; ++u) {
           float part[kMT][kNT][4];
@@ -349,10 +377,12 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
             const uint4 codes = *reinterpret_cast<const uint4*>(mr + u * 512 + lane * 16);
 #pragma unroll
             for (int hf = 0; hf < 2; ++hf) {  // halves of the unit: sets of 32 inputs end with each
-              const int sidx = (u * kUnit + 32 * hf) >> a.l.shift;
+              const int sidx = kSub == 32 ? 2 * u + hf : (u * kUnit) >> a.l.shift;
               __half2 z0 = __float2half2_rn(1032.0f), z1 = __float2half2_rn(-72.0f);
               if constexpr (kCode == kCodeUint4) {
-                const uint32_t z = *reinterpret_cast<const uint16_t*>(mr + tail_at + a.l.sets * 32 + sidx * 16 + 2 * g);
+                uint32_t z;
+                if constexpr (kSub == 32) z = word_of(zp[m], u) >> (16 * hf) & 0xffffu;
+                else z = *reinterpret_cast<const uint16_t*>(mr + tail_at + a.l.sets * 32 + 2 * (g * a.l.sets + sidx));
                 z0 = __half2half2(__ushort_as_half(static_cast<unsigned short>(0x6400u | (z & 0xffu))));
                 z1 = __half2half2(__ushort2half_rn(static_cast<unsigned short>(64u + (z >> 8))));
                 z1 = __hneg2(z1);
@@ -372,7 +402,9 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
                 }
               }
               if (kSub == 32 || hf == 1) {
-                const uint32_t s2 = *reinterpret_cast<const uint32_t*>(mr + tail_at + sidx * 32 + 4 * g);
+                uint32_t s2;
+                if constexpr (kSub == 32) s2 = word_of(sc[m][u >> 1], 2 * (u & 1) + hf);
+                else s2 = *reinterpret_cast<const uint32_t*>(mr + tail_at + 4 * (g * a.l.sets + sidx));
                 const float s0 = scale_value(static_cast<uint16_t>(s2), kScale), s1 = scale_value(static_cast<uint16_t>(s2 >> 16), kScale);
 #pragma unroll
                 for (int nt = 0; nt < kNT; ++nt) {
