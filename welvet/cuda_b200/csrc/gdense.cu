@@ -107,10 +107,12 @@ __global__ void __launch_bounds__(128) k_group_build(const __grid_constant__ Bui
 // tcgen05 needs N >= 8 and M = 128 rows of dequantised weights in shared or tensor memory; at 1..8
 // tokens the conversion is the work, and the register path takes its result without a store.
 //
-// The blocks take equal runs of all records (row set by row set, chunk by chunk), the warps of a
-// block every kWarps-th record of its run; a row set's sums are added over the warps in shared
-// memory. Row sets that a run's ends cut are joined through global memory by the last block to
-// come, in block order. The weight copies start before the previous kernel's end is waited for.
+// The records (row set by row set, chunk by chunk) are cut into equal runs. Layers that give every
+// warp a row set or more make the runs the warps', which then never wait for one another; smaller
+// ones make them the blocks', whose warps take every eighth record and add their sums in shared
+// memory. Row sets that a run's ends cut are joined through global memory by the last run to come,
+// in run order; small layers avoid that with runs of whole row sets. The weight copies start before
+// the previous kernel's end is waited for.
 constexpr int kMaxTokens = 8;
 constexpr int kGWarps = 8;
 constexpr int kGThreads = 32 * kGWarps;
@@ -132,7 +134,9 @@ struct GArgs {
   int slab_chunks;   // chunks of a slab (the last one may have fewer)
   int slab_blocks;   // blocks of a slab
   int row_sets;
-  float* part;       // [slabs * slab_blocks][2][rows of a set][8]
+  int solo;          // runs are the warps', not the blocks'
+  int aligned;       // (blocks') runs are whole row sets
+  float* part;       // [runs][2][rows of a set][8]
   int* tickets;      // [slabs][row_sets], zero between calls
   float* slab_sum;   // [slabs][n][rows], with more than one slab
   int* err;
@@ -216,12 +220,15 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
   }
   __syncwarp();
 
+  // this block's or this warp's run of records, and the warp's share of it: every step-th from `first`
   const int64_t total = static_cast<int64_t>(a.row_sets) * chunks;
-  auto run_start = [&](int64_t i) { return i * total / a.slab_blocks; };
-  const int64_t r0 = run_start(rank), r1 = run_start(rank + 1);
-  // the warp's records: r0 + w, + kGWarps, ...
-  int set = static_cast<int>((r0 + w) / chunks), ch = static_cast<int>((r0 + w) - static_cast<int64_t>(set) * chunks);
-  int64_t issued = r0 + w;
+  const int64_t runs = a.solo ? a.slab_blocks * kGWarps : a.slab_blocks, run = a.solo ? rank * kGWarps + w : rank;
+  auto run_start = [&](int64_t i) { return a.aligned ? i * a.row_sets / runs * chunks : i * total / runs; };
+  const int64_t r0 = run_start(run), r1 = run_start(run + 1);
+  const int step = a.solo ? 1 : kGWarps;
+  const int64_t first_rec = a.solo ? r0 : r0 + w;
+  int set = static_cast<int>(first_rec / chunks), ch = static_cast<int>(first_rec - static_cast<int64_t>(set) * chunks);
+  int64_t issued = first_rec;
   const int rec_bytes = 2048 + a.l.tail, last_bytes = 512 * (a.l.units - (a.l.chunks - 1) * (kChunk / kUnit)) + a.l.tail;
   const int to_last = a.l.chunks - 1 - c_first;
   const uint8_t* src = a.w + static_cast<int64_t>(set) * kMT * a.l.group_bytes + static_cast<int64_t>(c_first + ch) * rec_bytes;
@@ -237,9 +244,9 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
         pipe::bulk_load_hint(ring + stage * kMT * kRecord, src, bytes, bar, policy);
         if (kMT > 1 && groups > 1) pipe::bulk_load_hint(ring + (stage * kMT + 1) * kRecord, src + a.l.group_bytes, bytes, bar, policy);
       }
-      issued += kGWarps;
-      ch += kGWarps;
-      src += kGWarps * rec_bytes;
+      issued += step;
+      ch += step;
+      src += step * rec_bytes;
       if (ch >= chunks) {
         do {
           ch -= chunks;
@@ -255,7 +262,7 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // x: a warp takes a token's chunk at a time, eight inputs a lane
   const bool vec = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.x_ld & 3) == 0;
-  constexpr int kFly = 4;  // chunks whose loads are in flight together
+  constexpr int kFly = 8;  // chunks whose loads are in flight together
   for (int i0 = w; i0 < a.n * chunks; i0 += kFly * kGWarps) {
     float v[kFly][8];
 #pragma unroll
@@ -323,12 +330,12 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
   int stage = 0;
   uint32_t phase = 0;
   int buf = 0;
-  int64_t next = r0 + w;  // the warp's next record
+  int64_t next = first_rec;  // the warp's next record
   int64_t rs = r0 / chunks;
   for (int64_t seg = r0; seg < r1; ++rs) {  // row sets of the run
     const int64_t set_end = (rs + 1) * chunks, end = set_end < r1 ? set_end : r1;
     const bool whole = seg == rs * chunks && end == set_end;
-    for (; next < end; next += kGWarps) {
+    for (; next < end; next += step) {
       const int c = static_cast<int>(next - rs * chunks), chunk = c_first + c;
       const int units = min(kChunk / kUnit, a.l.units - chunk * (kChunk / kUnit));
       pipe::mbar_wait(&bars[w][stage], phase, a.err, 40);
@@ -435,56 +442,97 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
         phase ^= 1u;
       }
     }
-    // the row set's sums over the warps
-#pragma unroll
-    for (int m = 0; m < kMT; ++m)
-#pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
-        s_red[buf][w][16 * m + g][4 * nt + t] = acc[m][nt][0] + acc[m][nt][1];
-        s_red[buf][w][16 * m + g + 8][4 * nt + t] = acc[m][nt][2] + acc[m][nt][3];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[m][nt][e] = 0.0f;
-      }
-    __syncthreads();
-    const int outs = kRows * a.n;
-    auto sum_of = [&](int i) {
-      const int b = i / kRows, r = i - b * kRows;
-      float v = 0.0f;
-#pragma unroll
-      for (int x = 0; x < kGWarps; ++x) v += s_red[buf][x][r][b];
-      return v;
-    };
-    auto write = [&](int i, float v) {
-      const int b = i / kRows, o = static_cast<int>(rs) * kRows + i - b * kRows;
+    const int64_t slot = 2 * (static_cast<int64_t>(slab) * runs + run);  // of `part`
+    const int64_t run0 = whole ? 0 : ((rs * chunks + 1) * runs - 1) / total, run1 = whole ? 0 : (set_end * runs - 1) / total;
+    int* const ticket = a.tickets + static_cast<int64_t>(slab) * a.row_sets + rs;
+    auto write = [&](int r, int b, float v) {
+      const int o = static_cast<int>(rs) * kRows + r;
       if (o >= a.rows) return;
       if (a.slabs == 1) g_write(a, o, b, v);
       else a.slab_sum[(static_cast<int64_t>(slab) * a.n + b) * a.rows + o] = v;
     };
-    if (whole) {
-      for (int i = tid; i < outs; i += kGThreads) write(i, sum_of(i));
-    } else {
-      // cut by the run's ends: the first slot is of the row set that began before the run
-      float* mine = a.part + (2ll * blockIdx.x + (seg == rs * chunks ? 1 : 0)) * (kRows * kMaxTokens);
-      for (int i = tid; i < outs; i += kGThreads) mine[i] = sum_of(i);
-      const int64_t b0 = ((rs * chunks + 1) * a.slab_blocks - 1) / total, b1 = (set_end * a.slab_blocks - 1) / total;
-      int* ticket = a.tickets + static_cast<int64_t>(slab) * a.row_sets + rs;
-      __syncthreads();
-      if (tid == 0) {
-        __threadfence();
-        s_last = atomicAdd(ticket, 1) == static_cast<int>(b1 - b0);
+    // The runs that cut a row set leave their sums in order of the runs; the last one to come adds
+    // them: the first run's lie in its second slot, the others' in their first.
+    float* const mine = a.part + (slot + (seg == rs * chunks ? 1 : 0)) * (kRows * kMaxTokens);
+    const float* const cut = a.part + 2 * (static_cast<int64_t>(slab) * runs + run0) * (kRows * kMaxTokens);
+    auto joined = [&](int i) {
+      float v = __ldcg(cut + kRows * kMaxTokens + i);
+      for (int64_t x = 1; x <= run1 - run0; ++x) v += __ldcg(cut + 2 * x * (kRows * kMaxTokens) + i);
+      return v;
+    };
+    if (a.solo) {
+      bool last = true;
+      if (!whole) {
+#pragma unroll
+        for (int m = 0; m < kMT; ++m)
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              mine[(16 * m + g + 8 * e) * kMaxTokens + 4 * nt + t] = acc[m][nt][2 * e] + acc[m][nt][2 * e + 1];
+        __syncwarp();
+        int before = 0;
+        if (lane == 0) {
+          __threadfence();
+          before = atomicAdd(ticket, 1);
+        }
+        last = __shfl_sync(0xffffffffu, before, 0) == static_cast<int>(run1 - run0);
+        if (last) {
+          __threadfence();
+          if (lane == 0) *ticket = 0;
+        }
       }
+      if (last) {
+#pragma unroll
+        for (int m = 0; m < kMT; ++m)
+#pragma unroll
+          for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int r = 16 * m + g + 8 * e, b = 4 * nt + t;
+              if (b < a.n) write(r, b, whole ? acc[m][nt][2 * e] + acc[m][nt][2 * e + 1] : joined(r * kMaxTokens + b));
+            }
+      }
+    } else {
+      // the row set's sums over the warps
+#pragma unroll
+      for (int m = 0; m < kMT; ++m)
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            s_red[buf][w][16 * m + g + 8 * e][4 * nt + t] = acc[m][nt][2 * e] + acc[m][nt][2 * e + 1];
       __syncthreads();
-      if (s_last) {
-        __threadfence();
-        if (tid == 0) *ticket = 0;
-        const float* first = a.part + 2ll * (static_cast<int64_t>(slab) * a.slab_blocks + b0) * (kRows * kMaxTokens);
-        for (int i = tid; i < outs; i += kGThreads) {
-          float v = __ldcg(first + kRows * kMaxTokens + i);
-          for (int64_t x = 1; x <= b1 - b0; ++x) v += __ldcg(first + 2 * x * (kRows * kMaxTokens) + i);
-          write(i, v);
+      const int outs = kRows * a.n;
+      auto sum_of = [&](int r, int b) {
+        float v = 0.0f;
+#pragma unroll
+        for (int x = 0; x < kGWarps; ++x) v += s_red[buf][x][r][b];
+        return v;
+      };
+      if (whole) {
+        for (int i = tid; i < outs; i += kGThreads) write(i % kRows, i / kRows, sum_of(i % kRows, i / kRows));
+      } else {
+        for (int i = tid; i < outs; i += kGThreads) mine[i % kRows * kMaxTokens + i / kRows] = sum_of(i % kRows, i / kRows);
+        __syncthreads();
+        if (tid == 0) {
+          __threadfence();
+          s_last = atomicAdd(ticket, 1) == static_cast<int>(run1 - run0);
+        }
+        __syncthreads();
+        if (s_last) {
+          __threadfence();
+          if (tid == 0) *ticket = 0;
+          for (int i = tid; i < outs; i += kGThreads) write(i % kRows, i / kRows, joined(i % kRows * kMaxTokens + i / kRows));
         }
       }
     }
+#pragma unroll
+    for (int m = 0; m < kMT; ++m)
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[m][nt][e] = 0.0f;
     buf ^= 1;
     seg = end;
   }
@@ -569,7 +617,7 @@ int row_groups_of(const Layout& l, int sms) {
 }
 
 struct GPlan {
-  int mt, slabs, slab_chunks, slab_blocks, row_sets, smem;
+  int mt, slabs, slab_chunks, slab_blocks, row_sets, solo, aligned, smem;
 };
 
 GPlan plan_of(const GroupDense& g, int n) {
@@ -586,6 +634,19 @@ GPlan plan_of(const GroupDense& g, int n) {
   const int64_t last = l.chunks - (p.slabs - 1) * p.slab_chunks;
   const int64_t most = std::max<int64_t>(1, p.row_sets * last / kGWarps);
   p.slab_blocks = static_cast<int>(std::min<int64_t>(std::max(1, g.sms / p.slabs), most));
+  p.solo = p.row_sets >= p.slab_blocks * kGWarps;
+  // Whole row sets leave blocks idle for part of the last round; cut ones cost a join of about
+  // 2.5 us at the run's end. At 5 TB/s a microsecond is 5 MB of records.
+  const int per = (p.row_sets + p.slab_blocks - 1) / p.slab_blocks;
+  const double idle = static_cast<double>(per) * p.slab_blocks / p.row_sets - 1.0;
+  p.aligned = !p.solo && p.row_sets >= p.slab_blocks && idle * l.group_bytes * l.row_groups < 2.5 * 5e6;
+  if (!p.solo && p.row_sets < p.slab_blocks) {
+    // fewer row sets than blocks: a block each, if a block's records stay few
+    if (static_cast<double>(l.group_bytes) * p.mt * p.slabs < 2.5 * 50e3 * p.slabs) {
+      p.slab_blocks = p.row_sets;
+      p.aligned = 1;
+    }
+  }
   return p;
 }
 
@@ -671,7 +732,7 @@ Status gdense_fill(GroupDense* g, const GroupDenseSrc& src) {
   size_t part = 0, tickets = 0, slabs = 0;
   for (int n = 1; n <= kMaxTokens; ++n) {
     const GPlan p = plan_of(*g, n);
-    part = std::max<size_t>(part, static_cast<size_t>(p.slabs) * p.slab_blocks * 2 * 16 * p.mt * kMaxTokens * 4);
+    part = std::max<size_t>(part, static_cast<size_t>(p.slabs) * p.slab_blocks * (p.solo ? kGWarps : 1) * 2 * 16 * p.mt * kMaxTokens * 4);
     tickets = std::max<size_t>(tickets, static_cast<size_t>(p.slabs) * p.row_sets * 4);
     if (p.slabs > 1) slabs = std::max<size_t>(slabs, static_cast<size_t>(p.slabs) * n * g->rows * 4);
     WB_CUDA(cudaFuncSetAttribute(kernel_of(*g, n, p.mt), cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -735,6 +796,8 @@ Status gdense_forward(GroupDense* g, int n, const float* x, int64_t x_ld, float*
     a.slab_chunks = p.slab_chunks;
     a.slab_blocks = p.slab_blocks;
     a.row_sets = p.row_sets;
+    a.solo = p.solo;
+    a.aligned = p.aligned;
     WB_TRY(g_launch(kernel_of(*g, a.n, p.mt), dim3(p.slabs * p.slab_blocks), kGThreads, p.smem, st, a));
     if (p.slabs > 1) WB_TRY(g_launch(k_group_slabs, dim3((g->rows + 255) / 256, a.n), 256, 0, st, a));
   }
