@@ -308,9 +308,6 @@ WELVET_API welvet_status welvet_b200_gdense_mount(int32_t in, int32_t out, int32
  * `stream`. Made for 1..8 rows; more rows run in passes of 8 over the weights. */
 WELVET_API welvet_status welvet_b200_gdense_execute_device(welvet_b200_gdense* g, int32_t rows, const float* x_dev,
                                                            int64_t x_ld, float* pre_dev, float* post_dev, void* stream);
-/* Synchronizes `stream`; status 4 (cleared by the report) if a weight copy of an earlier call did not
- * arrive within the kernel's wait limit. */
-WELVET_API welvet_status welvet_b200_gdense_check_error(welvet_b200_gdense* g, void* stream);
 WELVET_API void welvet_b200_gdense_release(welvet_b200_gdense* g);
 
 /* ---------------------------------------------------------------- multi-GPU (one box)

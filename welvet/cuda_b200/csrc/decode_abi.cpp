@@ -285,13 +285,6 @@ welvet_status welvet_b200_gdense_execute_device(welvet_b200_gdense* g, int32_t r
   });
 }
 
-welvet_status welvet_b200_gdense_check_error(welvet_b200_gdense* g, void* stream) {
-  return guarded([&] {
-    if (!g || !g->g) return wb::Status::Invalid("group dense: nil handle");
-    return wb::gdense_check_error(g->g, static_cast<cudaStream_t>(stream));
-  });
-}
-
 void welvet_b200_gdense_release(welvet_b200_gdense* g) {
   if (!g) return;
   delete g->g;

@@ -2,7 +2,6 @@
 #include "gdense.hpp"
 
 #include "codec.cuh"
-#include "pipeline.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -31,7 +30,7 @@ constexpr int kChunk = 256, kUnit = 64;
 
 struct Layout {
   int row_groups, chunks, units;  // units of 64 inputs in all
-  int sg, shift, sets;            // inputs of a scale set and its logarithm, sets of a record
+  int sg, sets;                   // inputs of a scale set, sets of a record
   int tail;                       // bytes of a record's scales and zero points
   int64_t group_bytes;            // records of a row group
 };
@@ -42,7 +41,6 @@ Layout layout_of(int rows, int cols, int group, int code) {
   l.units = (cols + kUnit - 1) / kUnit;
   l.chunks = (cols + kChunk - 1) / kChunk;
   l.sg = group % 256 == 0 ? 256 : (group % 128 == 0 ? 128 : (group % 64 == 0 ? 64 : 32));
-  l.shift = l.sg == 256 ? 8 : (l.sg == 128 ? 7 : (l.sg == 64 ? 6 : 5));
   l.sets = kChunk / l.sg;
   l.tail = l.sets * (code == kCodeUint4 ? 48 : 32);
   l.group_bytes = static_cast<int64_t>(l.units) * 512 + static_cast<int64_t>(l.chunks) * l.tail;
@@ -98,27 +96,26 @@ __global__ void __launch_bounds__(128) k_group_build(const __grid_constant__ Bui
 // ---------------------------------------------------------------- matrix-vector product
 //
 // HBM bound: in * out / 2 bytes of codes and 2 (Uint4: 3) bytes per group of scales are read once,
-// for 2 in out flops per token. A warp copies records into its own ring of shared memory (one bulk
-// copy each, issued by one lane) and multiplies them on the register path of the tensor cores:
-// codes become exact f16 A fragments, x is two f16 parts (22 bits) after scaling each token's
-// chunk by a power of two, part p of token b in column 2 b + p, so that a thread's pair of
-// accumulators is one token. Products are exact; a scale set's sum (fp32, at most 256 products)
-// is multiplied by its scale and added to the row's fp32 sum.
+// for 2 in out flops per token. A warp loads a record straight into registers, in fragment order,
+// one record ahead of the one it multiplies on the register path of the tensor cores: codes become
+// exact f16 A fragments, x is two f16 parts (22 bits) after scaling each token's chunk by a power
+// of two, part p of token b in column 2 b + p, so that a thread's pair of accumulators is one
+// token. Products are exact; a scale set's sum (fp32, at most 256 products) is multiplied by its
+// scale and added to the row's fp32 sum. (Records copied to rings of shared memory by the bulk
+// engine, 8 warps a block, were slower on layers below 100 MB: the ring leaves half the warps.)
 // tcgen05 needs N >= 8 and M = 128 rows of dequantised weights in shared or tensor memory; at 1..8
 // tokens the conversion is the work, and the register path takes its result without a store.
 //
-// The records (row set by row set, chunk by chunk) are cut into equal runs. Layers that give every
-// warp a row set or more make the runs the warps', which then never wait for one another; smaller
-// ones make them the blocks', whose warps take every eighth record and add their sums in shared
-// memory. Row sets that a run's ends cut are joined through global memory by the last run to come,
-// in run order; small layers avoid that with runs of whole row sets. The weight copies start before
-// the previous kernel's end is waited for.
+// The records (row group by row group, chunk by chunk) are cut into equal runs. Layers that give
+// every warp a row group or more make the runs the warps', which then never wait for one another;
+// smaller ones make them the blocks', whose warps take every 16th record and add their sums in
+// shared memory. Row groups that a run's ends cut are joined through global memory by the last run
+// to come, in run order; small layers avoid that with runs of whole row groups. The first weight
+// loads start before the previous kernel's end is waited for.
 constexpr int kMaxTokens = 8;
-constexpr int kGWarps = 8;
+constexpr int kGWarps = 16;
 constexpr int kGThreads = 32 * kGWarps;
-constexpr int kRecord = 2048 + 8 * 48;  // the longest record
-constexpr int kGStages = 6;             // records in a warp's ring
-constexpr int kXBytes = 90 * 1024;      // shared memory for x
+constexpr int kXBytes = 200 * 1024;  // shared memory for x
 
 struct GArgs {
   const uint8_t* w;
@@ -133,13 +130,11 @@ struct GArgs {
   int slabs;         // parts of the inputs whose x fits shared memory, each with its own blocks
   int slab_chunks;   // chunks of a slab (the last one may have fewer)
   int slab_blocks;   // blocks of a slab
-  int row_sets;
   int solo;          // runs are the warps', not the blocks'
-  int aligned;       // (blocks') runs are whole row sets
-  float* part;       // [runs][2][rows of a set][8]
-  int* tickets;      // [slabs][row_sets], zero between calls
+  int aligned;       // (blocks') runs are whole row groups
+  float* part;       // [runs][2][16][8]
+  int* tickets;      // [slabs][row groups], zero between calls
   float* slab_sum;   // [slabs][n][rows], with more than one slab
-  int* err;
 };
 
 __device__ __forceinline__ void g_write(const GArgs& a, int o, int b, float y) {
@@ -191,92 +186,116 @@ __device__ __forceinline__ void g_decode(uint32_t w, __half2 z0, __half2 z1, uin
   }
 }
 
-// kNT n8 tiles of tokens (1: up to 4 tokens, 2: up to 8), kMT row groups a warp (a row set). kSub:
-// sums are scaled every 32 inputs (scale sets of 32) or every unit of 64 (longer ones). kScale: the
-// scales' type.
-template <int kCode, int kNT, int kMT, int kSub, int kScale>
+__device__ __forceinline__ uint4 ld_weights(const uint8_t* p) {
+  uint4 r;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+
+// A lane's share of a record: its codes of the four units, and the scales and zero points of rows g
+// and g + 8 for each set of kSub inputs.
+template <int kCode, int kSub>
+struct GRecord {
+  static constexpr int kSets = kChunk / kSub;
+  uint4 codes[4];
+  uint32_t scales[kSets];
+  uint32_t zeros[kCode == kCodeUint4 ? (kSets + 1) / 2 : 1];  // two sets a word
+};
+
+// The words of kN sets that lie together.
+template <int kN>
+__device__ __forceinline__ void ld_words(const uint8_t* p, uint32_t* w) {
+#pragma unroll
+  for (int i = 0; i < kN; i += 4) {
+    if constexpr (kN >= 4) asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]) : "l"(p + 4 * i));
+    else if constexpr (kN == 2) asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "l"(p));
+    else asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(w[0]) : "l"(p));
+  }
+}
+
+// kNT n8 tiles of tokens (1: up to 4 tokens, 2: up to 8). kSub: inputs of a scale set (32, 64, 128
+// or 256). kScale: the scales' type.
+template <int kCode, int kNT, int kSub, int kScale>
 __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_constant__ GArgs a) {
-  constexpr int kStages = kGStages / kMT;
-  constexpr int kRows = 16 * kMT;
-  extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ __align__(8) uint64_t bars[kGWarps][kStages];
-  __shared__ float s_red[2][kGWarps][kRows][4 * kNT];
+  using Record = GRecord<kCode, kSub>;
+  extern __shared__ __align__(128) uint8_t sx[];  // x parts: [2 n columns][slab inputs] f16
+  __shared__ float s_red[2][kGWarps][16][4 * kNT];
   __shared__ __align__(16) uint8_t s_zero[kChunk * 2];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
-  uint8_t* const ring = smem + w * (kGStages * kRecord);
-  uint8_t* const sx = smem + kGWarps * kGStages * kRecord;  // x parts: [2 n columns][slab inputs] f16
   const int slab = blockIdx.x / a.slab_blocks, rank = blockIdx.x - slab * a.slab_blocks;
   const int c_first = slab * a.slab_chunks, chunks = min(a.slab_chunks, a.l.chunks - c_first);
   const int pitch = a.slab_chunks * (kChunk * 2) + 64;  // bytes of a column; two columns fill the banks
   float* const sxs = reinterpret_cast<float*>(sx + 2 * a.n * pitch);  // [token][chunk] 2^-e
 
   asm volatile("griddepcontrol.launch_dependents;");
-  if (tid < kChunk / 8) *reinterpret_cast<uint4*>(s_zero + 16 * tid) = make_uint4(0, 0, 0, 0);
-  if (lane == 0) {
-#pragma unroll
-    for (int s = 0; s < kStages; ++s) pipe::mbar_init(&bars[w][s], 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  __syncwarp();
-
-  // this block's or this warp's run of records, and the warp's share of it: every step-th from `first`
-  const int64_t total = static_cast<int64_t>(a.row_sets) * chunks;
-  const int64_t runs = a.solo ? a.slab_blocks * kGWarps : a.slab_blocks, run = a.solo ? rank * kGWarps + w : rank;
-  auto run_start = [&](int64_t i) { return a.aligned ? i * a.row_sets / runs * chunks : i * total / runs; };
-  const int64_t r0 = run_start(run), r1 = run_start(run + 1);
+  // this block's or this warp's run of records, and the warp's share of it: every step-th from first_rec
+  const int total = a.l.row_groups * chunks;
+  const int runs = a.solo ? a.slab_blocks * kGWarps : a.slab_blocks, run = a.solo ? rank * kGWarps + w : rank;
+  auto run_start = [&](int i) {
+    return a.aligned ? static_cast<int>(static_cast<int64_t>(i) * a.l.row_groups / runs) * chunks
+                     : static_cast<int>(static_cast<int64_t>(i) * total / runs);
+  };
+  const int r0 = run_start(run), r1 = run_start(run + 1);
   const int step = a.solo ? 1 : kGWarps;
-  const int64_t first_rec = a.solo ? r0 : r0 + w;
-  int set = static_cast<int>(first_rec / chunks), ch = static_cast<int>(first_rec - static_cast<int64_t>(set) * chunks);
-  int64_t issued = first_rec;
-  const int rec_bytes = 2048 + a.l.tail, last_bytes = 512 * (a.l.units - (a.l.chunks - 1) * (kChunk / kUnit)) + a.l.tail;
-  const int to_last = a.l.chunks - 1 - c_first;
-  const uint8_t* src = a.w + static_cast<int64_t>(set) * kMT * a.l.group_bytes + static_cast<int64_t>(c_first + ch) * rec_bytes;
-  uint64_t policy;
-  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
-  auto issue = [&](int stage) {
-    if (issued < r1) {
-      if (lane == 0) {
-        const int bytes = ch == to_last ? last_bytes : rec_bytes;
-        const int groups = kMT == 1 ? 1 : min(kMT, a.l.row_groups - set * kMT);
-        uint64_t* bar = &bars[w][stage];
-        pipe::mbar_expect_tx(bar, bytes * groups);
-        pipe::bulk_load_hint(ring + stage * kMT * kRecord, src, bytes, bar, policy);
-        if (kMT > 1 && groups > 1) pipe::bulk_load_hint(ring + (stage * kMT + 1) * kRecord, src + a.l.group_bytes, bytes, bar, policy);
-      }
-      issued += step;
-      ch += step;
-      src += step * rec_bytes;
-      if (ch >= chunks) {
-        do {
-          ch -= chunks;
-          ++set;
-        } while (ch >= chunks);
-        src = a.w + static_cast<int64_t>(set) * kMT * a.l.group_bytes + static_cast<int64_t>(c_first + ch) * rec_bytes;
-      }
+  const int first_rec = a.solo ? r0 : r0 + w;
+
+  // loads, one record ahead
+  const int rec_bytes = 2048 + a.l.tail, last_units = a.l.units - (a.l.chunks - 1) * (kChunk / kUnit);
+  const int to_last = last_units < kChunk / kUnit ? a.l.chunks - 1 - c_first : -1;  // the chunk that is short
+  int rg = first_rec / chunks, ch = first_rec - rg * chunks;
+  const uint8_t* src = a.w + rg * a.l.group_bytes + static_cast<int64_t>(c_first + ch) * rec_bytes + lane * 16;
+  const int step_bytes = step * rec_bytes, to_scales = g * (4 * Record::kSets) - lane * 16, to_zeros = 32 * Record::kSets + g * (2 * Record::kSets) - lane * 16;
+  int loaded = first_rec;
+  auto load = [&](Record& r) {
+    if (loaded >= r1) return;
+    const uint8_t* tl = src + 2048;
+    if (ch != to_last) {
+#pragma unroll
+      for (int u = 0; u < kChunk / kUnit; ++u) r.codes[u] = ld_weights(src + u * 512);
+    } else {  // codes of absent units are zero; their x is zero too
+#pragma unroll
+      for (int u = 0; u < kChunk / kUnit; ++u) r.codes[u] = u < last_units ? ld_weights(src + u * 512) : make_uint4(0, 0, 0, 0);
+      tl = src + last_units * 512;
+    }
+    ld_words<Record::kSets>(tl + to_scales, r.scales);
+    if constexpr (kCode == kCodeUint4) {
+      if constexpr (Record::kSets == 1) r.zeros[0] = *reinterpret_cast<const uint16_t*>(tl + to_zeros);
+      else ld_words<Record::kSets / 2>(tl + to_zeros, r.zeros);
+    }
+    loaded += step;
+    ch += step;
+    src += step_bytes;
+    if (ch >= chunks) {
+      do {
+        ch -= chunks;
+        ++rg;
+      } while (ch >= chunks);
+      src = a.w + rg * a.l.group_bytes + static_cast<int64_t>(c_first + ch) * rec_bytes + lane * 16;
     }
   };
-#pragma unroll
-  for (int s = 0; s < kStages; ++s) issue(s);
+  Record rec_a, rec_b;  // in turn the one at work and the one ahead
+  load(rec_a);
+  if (tid < kChunk / 8) *reinterpret_cast<uint4*>(s_zero + 16 * tid) = make_uint4(0, 0, 0, 0);
 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // x: a warp takes a token's chunk at a time, eight inputs a lane
   const bool vec = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.x_ld & 3) == 0;
-  constexpr int kFly = 8;  // chunks whose loads are in flight together
+  constexpr int kFly = 4;  // chunks whose loads are in flight together
   for (int i0 = w; i0 < a.n * chunks; i0 += kFly * kGWarps) {
     float v[kFly][8];
 #pragma unroll
     for (int y = 0; y < kFly; ++y) {
       const int i = i0 + y * kGWarps, b = i / chunks, c = i - b * chunks;
       const int k0 = (c_first + c) * kChunk + 8 * lane;
-      const float* src = a.x + b * a.x_ld + k0;
+      const float* xs = a.x + b * a.x_ld + k0;
       const bool on = i < a.n * chunks;
       if (vec && on && k0 + 8 <= a.cols) {
-        *reinterpret_cast<float4*>(v[y]) = ld_dep4(src);
-        *reinterpret_cast<float4*>(v[y] + 4) = ld_dep4(src + 4);
+        *reinterpret_cast<float4*>(v[y]) = ld_dep4(xs);
+        *reinterpret_cast<float4*>(v[y] + 4) = ld_dep4(xs + 4);
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[y][e] = on && k0 + e < a.cols ? ld_dep(src + e) : 0.0f;
+        for (int e = 0; e < 8; ++e) v[y][e] = on && k0 + e < a.cols ? ld_dep(xs + e) : 0.0f;
       }
     }
 #pragma unroll
@@ -319,164 +338,116 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
     xcol[nt] = on ? sx + (8 * nt + g) * pitch + 16 * t : s_zero + 16 * t;
     xstep[nt] = on ? kChunk * 2 : 0;
   }
-  float acc[kMT][kNT][4];
+  float acc[kNT][4];
 #pragma unroll
-  for (int m = 0; m < kMT; ++m)
+  for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) acc[m][nt][e] = 0.0f;
+    for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
 
-  int stage = 0;
-  uint32_t phase = 0;
   int buf = 0;
-  int64_t next = first_rec;  // the warp's next record
-  int64_t rs = r0 / chunks;
-  for (int64_t seg = r0; seg < r1; ++rs) {  // row sets of the run
-    const int64_t set_end = (rs + 1) * chunks, end = set_end < r1 ? set_end : r1;
-    const bool whole = seg == rs * chunks && end == set_end;
-    for (; next < end; next += step) {
-      const int c = static_cast<int>(next - rs * chunks), chunk = c_first + c;
-      const int units = min(kChunk / kUnit, a.l.units - chunk * (kChunk / kUnit));
-      pipe::mbar_wait(&bars[w][stage], phase, a.err, 40);
-      __syncwarp();
-      const uint8_t* rec = ring + stage * kMT * kRecord;
+  int next = first_rec;  // the warp's next record
+  bool turn = false;
+  int rs = r0 / chunks;
+  for (int seg = r0; seg < r1; ++rs) {  // row groups of the run
+    const int set_begin = rs * chunks, set_end = set_begin + chunks, end = min(set_end, r1);
+    const bool whole = seg == set_begin && end == set_end;
+    auto record = [&](const Record& r, Record& ahead) {
+      const int c = next - set_begin;
+      load(ahead);
       const uint8_t* xp[kNT];
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) xp[nt] = xcol[nt] + c * xstep[nt];
-      float sum[kMT][kNT][4];  // the record's, in units of the thread's token's 2^-e
+      float sum[kNT][4];  // the record's, in units of the thread's token's 2^-e
+      float part[kNT][4];
 #pragma unroll
-      for (int m = 0; m < kMT; ++m)
+      for (int u = 0; u < kChunk / kUnit; ++u) {
+        uint4 xb[kNT][2];
 #pragma unroll
-        for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sum[m][nt][e] = 0.0f;
-      // `full`: all four units are there, and nothing stands between their instructions
-      auto record = [&](auto full) {
-        constexpr bool kFull = decltype(full)::value;
-        const int tail_at = kFull ? 2048 : units * 512;
-        // sets of 32: the lane's eight scales and zero points of two rows at once
-        uint4 sc[kMT][2], zp[kMT];
-        if constexpr (kSub == 32) {
-#pragma unroll
-          for (int m = 0; m < kMT; ++m) {
-            const uint8_t* tl = rec + m * kRecord + tail_at;
-            sc[m][0] = *reinterpret_cast<const uint4*>(tl + 32 * g);
-            sc[m][1] = *reinterpret_cast<const uint4*>(tl + 32 * g + 16);
-            if constexpr (kCode == kCodeUint4) zp[m] = *reinterpret_cast<const uint4*>(tl + 256 + 16 * g);
-          }
+        for (int nt = 0; nt < kNT; ++nt) {
+          const uint4* xs = reinterpret_cast<const uint4*>(xp[nt] + u * (kUnit * 2));
+          xb[nt][0] = xs[0];
+          xb[nt][1] = xs[4];
         }
-        auto word_of = [](const uint4& q, int i) { return i == 0 ? q.x : (i == 1 ? q.y : (i == 2 ? q.z : q.w)); };
 #pragma unroll
-        for (int u = 0; u < kChunk / kUnit; ++u) {
-          float part[kMT][kNT][4];
-          if (!kFull && u >= units) break;
-          uint4 xb[kNT][2];
-#pragma unroll
-          for (int nt = 0; nt < kNT; ++nt) {
-            const uint4* src = reinterpret_cast<const uint4*>(xp[nt] + u * (kUnit * 2));
-            xb[nt][0] = src[0];
-            xb[nt][1] = src[4];
+        for (int hf = 0; hf < 2; ++hf) {  // halves of the unit
+          constexpr int kS = kSub;
+          const int k = u * kUnit + 32 * hf, set = k / kS;  // constants once unrolled
+          const bool begins = k % kS == 0, ends = (k + 32) % kS == 0;
+          __half2 z0 = __float2half2_rn(1032.0f), z1 = __float2half2_rn(-72.0f);
+          if constexpr (kCode == kCodeUint4) {
+            const uint32_t z = r.zeros[set >> 1] >> (16 * (set & 1));
+            z0 = __half2half2(__ushort_as_half(static_cast<unsigned short>(0x6400u | (z & 0xffu))));
+            z1 = __hneg2(__half2half2(__ushort2half_rn(static_cast<unsigned short>(64u + ((z >> 8) & 0xffu)))));
           }
 #pragma unroll
-          for (int m = 0; m < kMT; ++m) {
-            const uint8_t* mr = rec + m * kRecord;
-            const uint4 codes = *reinterpret_cast<const uint4*>(mr + u * 512 + lane * 16);
+          for (int jj = 0; jj < 2; ++jj) {
+            const int j = 2 * hf + jj;
+            const uint32_t word = j == 0 ? r.codes[u].x : (j == 1 ? r.codes[u].y : (j == 2 ? r.codes[u].z : r.codes[u].w));
+            uint32_t fr[4];
+            g_decode<kCode>(word, z0, z1, fr);
 #pragma unroll
-            for (int hf = 0; hf < 2; ++hf) {  // halves of the unit: sets of 32 inputs end with each
-              const int sidx = kSub == 32 ? 2 * u + hf : (u * kUnit) >> a.l.shift;
-              __half2 z0 = __float2half2_rn(1032.0f), z1 = __float2half2_rn(-72.0f);
-              if constexpr (kCode == kCodeUint4) {
-                uint32_t z;
-                if constexpr (kSub == 32) z = word_of(zp[m], u) >> (16 * hf) & 0xffffu;
-                else z = *reinterpret_cast<const uint16_t*>(mr + tail_at + a.l.sets * 32 + 2 * (g * a.l.sets + sidx));
-                z0 = __half2half2(__ushort_as_half(static_cast<unsigned short>(0x6400u | (z & 0xffu))));
-                z1 = __half2half2(__ushort2half_rn(static_cast<unsigned short>(64u + (z >> 8))));
-                z1 = __hneg2(z1);
-              }
-#pragma unroll
-              for (int jj = 0; jj < 2; ++jj) {
-                const int j = 2 * hf + jj;
-                const uint32_t word = j == 0 ? codes.x : (j == 1 ? codes.y : (j == 2 ? codes.z : codes.w));
-                uint32_t fr[4];
-                g_decode<kCode>(word, z0, z1, fr);
-#pragma unroll
-                for (int nt = 0; nt < kNT; ++nt) {
-                  const uint4 x = xb[nt][j >> 1];
-                  const uint32_t b0 = j & 1 ? x.z : x.x, b1 = j & 1 ? x.w : x.y;
-                  if (jj == 0 && (kSub == 32 || hf == 0)) g_mma0(part[m][nt], fr, b0, b1);
-                  else g_mma(part[m][nt], fr, b0, b1);
-                }
-              }
-              if (kSub == 32 || hf == 1) {
-                uint32_t s2;
-                if constexpr (kSub == 32) s2 = word_of(sc[m][u >> 1], 2 * (u & 1) + hf);
-                else s2 = *reinterpret_cast<const uint32_t*>(mr + tail_at + 4 * (g * a.l.sets + sidx));
-                const float s0 = scale_value(static_cast<uint16_t>(s2), kScale), s1 = scale_value(static_cast<uint16_t>(s2 >> 16), kScale);
-#pragma unroll
-                for (int nt = 0; nt < kNT; ++nt) {
-                  sum[m][nt][0] += part[m][nt][0] * s0;
-                  sum[m][nt][1] += part[m][nt][1] * s0;
-                  sum[m][nt][2] += part[m][nt][2] * s1;
-                  sum[m][nt][3] += part[m][nt][3] * s1;
-                }
-              }
+            for (int nt = 0; nt < kNT; ++nt) {
+              const uint4 x = xb[nt][hf];
+              const uint32_t b0 = jj ? x.z : x.x, b1 = jj ? x.w : x.y;
+              if (jj == 0 && begins) g_mma0(part[nt], fr, b0, b1);
+              else g_mma(part[nt], fr, b0, b1);
             }
           }
+          if (ends) {
+            const uint32_t s2 = r.scales[set];
+            const float s0 = scale_value(static_cast<uint16_t>(s2), kScale), s1 = scale_value(static_cast<uint16_t>(s2 >> 16), kScale);
+#pragma unroll
+            for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) sum[nt][e] = (set == 0 ? 0.0f : sum[nt][e]) + part[nt][e] * (e < 2 ? s0 : s1);
+          }
         }
-      };
-      if (units == kChunk / kUnit) record(std::true_type{});
-      else record(std::false_type{});
+      }
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
         const float xs = 4 * nt + t < a.n ? sxs[(4 * nt + t) * a.slab_chunks + c] : 0.0f;
 #pragma unroll
-        for (int m = 0; m < kMT; ++m)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) acc[m][nt][e] += sum[m][nt][e] * xs;
+        for (int e = 0; e < 4; ++e) acc[nt][e] += sum[nt][e] * xs;
       }
-      __syncwarp();
-      issue(stage);
-      if (++stage == kStages) {
-        stage = 0;
-        phase ^= 1u;
-      }
+    };
+    for (; next < end; next += step) {
+      if (turn) record(rec_b, rec_a);
+      else record(rec_a, rec_b);
+      turn = !turn;
     }
-    const int64_t slot = 2 * (static_cast<int64_t>(slab) * runs + run);  // of `part`
-    const int64_t run0 = whole ? 0 : ((rs * chunks + 1) * runs - 1) / total, run1 = whole ? 0 : (set_end * runs - 1) / total;
-    int* const ticket = a.tickets + static_cast<int64_t>(slab) * a.row_sets + rs;
+    const int run0 = whole ? 0 : static_cast<int>((static_cast<int64_t>(set_begin + 1) * runs - 1) / total);
+    const int run1 = whole ? 0 : static_cast<int>((static_cast<int64_t>(set_end) * runs - 1) / total);
+    int* const ticket = a.tickets + static_cast<int64_t>(slab) * a.l.row_groups + rs;
     auto write = [&](int r, int b, float v) {
-      const int o = static_cast<int>(rs) * kRows + r;
+      const int o = rs * 16 + r;
       if (o >= a.rows) return;
       if (a.slabs == 1) g_write(a, o, b, v);
       else a.slab_sum[(static_cast<int64_t>(slab) * a.n + b) * a.rows + o] = v;
     };
-    // The runs that cut a row set leave their sums in order of the runs; the last one to come adds
+    // The runs that cut a row group leave their sums in order of the runs; the last one to come adds
     // them: the first run's lie in its second slot, the others' in their first.
-    float* const mine = a.part + (slot + (seg == rs * chunks ? 1 : 0)) * (kRows * kMaxTokens);
-    const float* const cut = a.part + 2 * (static_cast<int64_t>(slab) * runs + run0) * (kRows * kMaxTokens);
+    constexpr int kSlot = 16 * kMaxTokens;
+    float* const mine = a.part + (2 * (static_cast<int64_t>(slab) * runs + run) + (seg == set_begin ? 1 : 0)) * kSlot;
+    const float* const cut = a.part + 2 * (static_cast<int64_t>(slab) * runs + run0) * kSlot;
     auto joined = [&](int i) {
-      float v = __ldcg(cut + kRows * kMaxTokens + i);
-      for (int64_t x = 1; x <= run1 - run0; ++x) v += __ldcg(cut + 2 * x * (kRows * kMaxTokens) + i);
+      float v = __ldcg(cut + kSlot + i);
+      for (int x = 1; x <= run1 - run0; ++x) v += __ldcg(cut + 2ll * x * kSlot + i);
       return v;
     };
     if (a.solo) {
       bool last = true;
       if (!whole) {
 #pragma unroll
-        for (int m = 0; m < kMT; ++m)
+        for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-          for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              mine[(16 * m + g + 8 * e) * kMaxTokens + 4 * nt + t] = acc[m][nt][2 * e] + acc[m][nt][2 * e + 1];
+          for (int e = 0; e < 2; ++e) mine[(g + 8 * e) * kMaxTokens + 4 * nt + t] = acc[nt][2 * e] + acc[nt][2 * e + 1];
         __syncwarp();
         int before = 0;
         if (lane == 0) {
           __threadfence();
           before = atomicAdd(ticket, 1);
         }
-        last = __shfl_sync(0xffffffffu, before, 0) == static_cast<int>(run1 - run0);
+        last = __shfl_sync(0xffffffffu, before, 0) == run1 - run0;
         if (last) {
           __threadfence();
           if (lane == 0) *ticket = 0;
@@ -484,55 +455,47 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
       }
       if (last) {
 #pragma unroll
-        for (int m = 0; m < kMT; ++m)
-#pragma unroll
-          for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int r = 16 * m + g + 8 * e, b = 4 * nt + t;
-              if (b < a.n) write(r, b, whole ? acc[m][nt][2 * e] + acc[m][nt][2 * e + 1] : joined(r * kMaxTokens + b));
-            }
-      }
-    } else {
-      // the row set's sums over the warps
-#pragma unroll
-      for (int m = 0; m < kMT; ++m)
-#pragma unroll
         for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
-            s_red[buf][w][16 * m + g + 8 * e][4 * nt + t] = acc[m][nt][2 * e] + acc[m][nt][2 * e + 1];
+          for (int e = 0; e < 2; ++e) {
+            const int r = g + 8 * e, b = 4 * nt + t;
+            if (b < a.n) write(r, b, whole ? acc[nt][2 * e] + acc[nt][2 * e + 1] : joined(r * kMaxTokens + b));
+          }
+      }
+    } else {
+      // the row group's sums over the warps
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) s_red[buf][w][g + 8 * e][4 * nt + t] = acc[nt][2 * e] + acc[nt][2 * e + 1];
       __syncthreads();
-      const int outs = kRows * a.n;
-      auto sum_of = [&](int r, int b) {
-        float v = 0.0f;
+      const int r = tid & 15, b = tid >> 4;  // 16 rows x at most 8 tokens: one output a thread
+      float v = 0.0f;
+      if (b < a.n) {
 #pragma unroll
         for (int x = 0; x < kGWarps; ++x) v += s_red[buf][x][r][b];
-        return v;
-      };
+      }
       if (whole) {
-        for (int i = tid; i < outs; i += kGThreads) write(i % kRows, i / kRows, sum_of(i % kRows, i / kRows));
+        if (b < a.n) write(r, b, v);
       } else {
-        for (int i = tid; i < outs; i += kGThreads) mine[i % kRows * kMaxTokens + i / kRows] = sum_of(i % kRows, i / kRows);
+        if (b < a.n) mine[r * kMaxTokens + b] = v;
         __syncthreads();
         if (tid == 0) {
           __threadfence();
-          s_last = atomicAdd(ticket, 1) == static_cast<int>(run1 - run0);
+          s_last = atomicAdd(ticket, 1) == run1 - run0;
         }
         __syncthreads();
         if (s_last) {
           __threadfence();
           if (tid == 0) *ticket = 0;
-          for (int i = tid; i < outs; i += kGThreads) write(i % kRows, i / kRows, joined(i % kRows * kMaxTokens + i / kRows));
+          if (b < a.n) write(r, b, joined(r * kMaxTokens + b));
         }
       }
     }
 #pragma unroll
-    for (int m = 0; m < kMT; ++m)
+    for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-      for (int nt = 0; nt < kNT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[m][nt][e] = 0.0f;
+      for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
     buf ^= 1;
     seg = end;
   }
@@ -610,40 +573,31 @@ GroupDense::~GroupDense() {
 
 namespace {
 
-// Row groups a warp takes together: two share the reads of x and a record's bookkeeping, unless the
-// layer has too few records for every warp.
-int row_groups_of(const Layout& l, int sms) {
-  return static_cast<int64_t>(l.row_groups / 2) * l.chunks >= static_cast<int64_t>(sms) * kGWarps ? 2 : 1;
-}
-
 struct GPlan {
-  int mt, slabs, slab_chunks, slab_blocks, row_sets, solo, aligned, smem;
+  int slabs, slab_chunks, slab_blocks, solo, aligned, smem;
 };
 
-GPlan plan_of(const GroupDense& g, int n) {
-  const Layout l = layout_of(g.rows, g.cols, g.group, g.code);
+GPlan plan_of(const GroupDense& g, const Layout& l, int n) {
   GPlan p;
-  p.mt = row_groups_of(l, g.sms);
-  p.row_sets = (l.row_groups + p.mt - 1) / p.mt;
   const int fit = (kXBytes - 2 * n * 64) / (n * (2 * kChunk * 2 + 4));  // chunks of x in shared memory
   p.slabs = (l.chunks + fit - 1) / fit;
   p.slab_chunks = (l.chunks + p.slabs - 1) / p.slabs;
   p.slabs = (l.chunks + p.slab_chunks - 1) / p.slab_chunks;
-  p.smem = kGWarps * kGStages * kRecord + 2 * n * (p.slab_chunks * kChunk * 2 + 64) + n * p.slab_chunks * 4;
+  p.smem = 2 * n * (p.slab_chunks * kChunk * 2 + 64) + n * p.slab_chunks * 4;
   // every warp of a block has a record or more
   const int64_t last = l.chunks - (p.slabs - 1) * p.slab_chunks;
-  const int64_t most = std::max<int64_t>(1, p.row_sets * last / kGWarps);
+  const int64_t most = std::max<int64_t>(1, l.row_groups * last / kGWarps);
   p.slab_blocks = static_cast<int>(std::min<int64_t>(std::max(1, g.sms / p.slabs), most));
-  p.solo = p.row_sets >= p.slab_blocks * kGWarps;
-  // Whole row sets leave blocks idle for part of the last round; cut ones cost a join of about
-  // 2.5 us at the run's end. At 5 TB/s a microsecond is 5 MB of records.
-  const int per = (p.row_sets + p.slab_blocks - 1) / p.slab_blocks;
-  const double idle = static_cast<double>(per) * p.slab_blocks / p.row_sets - 1.0;
-  p.aligned = !p.solo && p.row_sets >= p.slab_blocks && idle * l.group_bytes * l.row_groups < 2.5 * 5e6;
-  if (!p.solo && p.row_sets < p.slab_blocks) {
-    // fewer row sets than blocks: a block each, if a block's records stay few
-    if (static_cast<double>(l.group_bytes) * p.mt * p.slabs < 2.5 * 50e3 * p.slabs) {
-      p.slab_blocks = p.row_sets;
+  p.solo = l.row_groups >= p.slab_blocks * kGWarps;
+  p.aligned = 0;
+  if (!p.solo) {
+    // Whole row groups leave blocks idle for part of the last round; cut ones cost a join of about
+    // 2.5 us at the run's end. At 5 TB/s a microsecond is 5 MB of records.
+    const int per = (l.row_groups + p.slab_blocks - 1) / p.slab_blocks;
+    const double idle = static_cast<double>(per) * p.slab_blocks / l.row_groups - 1.0;
+    p.aligned = l.row_groups >= p.slab_blocks && idle * l.group_bytes * l.row_groups < 2.5 * 5e6;
+    if (l.row_groups < p.slab_blocks && l.group_bytes < 2.5 * 50e3) {  // one row group a block, if that is little
+      p.slab_blocks = l.row_groups;
       p.aligned = 1;
     }
   }
@@ -652,21 +606,20 @@ GPlan plan_of(const GroupDense& g, int n) {
 
 using GKernel = void (*)(GArgs);
 
-template <int kCode, int kSub, int kScale>
-GKernel kernel_of(int n, int mt) {
-  if (n > 4) return mt == 2 ? k_group_gemv<kCode, 2, 2, kSub, kScale> : k_group_gemv<kCode, 2, 1, kSub, kScale>;
-  return mt == 2 ? k_group_gemv<kCode, 1, 2, kSub, kScale> : k_group_gemv<kCode, 1, 1, kSub, kScale>;
-}
-
 template <int kSub, int kScale>
-GKernel kernel_of(int code, int n, int mt) {
-  if (code == kCodeFp4) return kernel_of<kCodeFp4, kSub, kScale>(n, mt);
-  return code == kCodeInt4 ? kernel_of<kCodeInt4, kSub, kScale>(n, mt) : kernel_of<kCodeUint4, kSub, kScale>(n, mt);
+GKernel kernel_of(int code, int n) {
+  if (code == kCodeFp4) return n > 4 ? k_group_gemv<kCodeFp4, 2, kSub, kScale> : k_group_gemv<kCodeFp4, 1, kSub, kScale>;
+  if (code == kCodeInt4) return n > 4 ? k_group_gemv<kCodeInt4, 2, kSub, kScale> : k_group_gemv<kCodeInt4, 1, kSub, kScale>;
+  return n > 4 ? k_group_gemv<kCodeUint4, 2, kSub, kScale> : k_group_gemv<kCodeUint4, 1, kSub, kScale>;
 }
 
-GKernel kernel_of(const GroupDense& g, int n, int mt) {
-  if (g.scale_type == kScaleF16) return g.group % 64 == 0 ? kernel_of<64, kScaleF16>(g.code, n, mt) : kernel_of<32, kScaleF16>(g.code, n, mt);
-  return g.group % 64 == 0 ? kernel_of<64, kScaleBF16>(g.code, n, mt) : kernel_of<32, kScaleBF16>(g.code, n, mt);
+template <int kScale>
+GKernel kernel_of(int sg, int code, int n) {
+  return sg == 32 ? kernel_of<32, kScale>(code, n) : (sg == 64 ? kernel_of<64, kScale>(code, n) : (sg == 128 ? kernel_of<128, kScale>(code, n) : kernel_of<256, kScale>(code, n)));
+}
+
+GKernel kernel_of(const GroupDense& g, const Layout& l, int n) {
+  return g.scale_type == kScaleF16 ? kernel_of<kScaleF16>(l.sg, g.code, n) : kernel_of<kScaleBF16>(l.sg, g.code, n);
 }
 
 template <typename K>
@@ -731,20 +684,18 @@ Status gdense_fill(GroupDense* g, const GroupDenseSrc& src) {
   // workspaces for every number of tokens
   size_t part = 0, tickets = 0, slabs = 0;
   for (int n = 1; n <= kMaxTokens; ++n) {
-    const GPlan p = plan_of(*g, n);
-    part = std::max<size_t>(part, static_cast<size_t>(p.slabs) * p.slab_blocks * (p.solo ? kGWarps : 1) * 2 * 16 * p.mt * kMaxTokens * 4);
-    tickets = std::max<size_t>(tickets, static_cast<size_t>(p.slabs) * p.row_sets * 4);
+    const GPlan p = plan_of(*g, b.l, n);
+    part = std::max<size_t>(part, static_cast<size_t>(p.slabs) * p.slab_blocks * (p.solo ? kGWarps : 1) * 2 * 16 * kMaxTokens * 4);
+    tickets = std::max<size_t>(tickets, static_cast<size_t>(p.slabs) * b.l.row_groups * 4);
     if (p.slabs > 1) slabs = std::max<size_t>(slabs, static_cast<size_t>(p.slabs) * n * g->rows * 4);
-    WB_CUDA(cudaFuncSetAttribute(kernel_of(*g, n, p.mt), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 kGWarps * kGStages * kRecord + kXBytes + 1024));
+    WB_CUDA(cudaFuncSetAttribute(kernel_of(*g, b.l, n), cudaFuncAttributeMaxDynamicSharedMemorySize, kXBytes));
   }
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-  WB_CUDA(cudaMalloc(&g->work, 256 + up(tickets) + up(part) + up(slabs)));
-  g->err = reinterpret_cast<int*>(g->work);
-  g->tickets = reinterpret_cast<int*>(g->work + 256);
-  g->part = reinterpret_cast<float*>(g->work + 256 + up(tickets));
-  g->slab_sum = reinterpret_cast<float*>(g->work + 256 + up(tickets) + up(part));
-  WB_CUDA(cudaMemset(g->work, 0, 256 + up(tickets)));
+  WB_CUDA(cudaMalloc(&g->work, up(tickets) + up(part) + up(slabs)));
+  g->tickets = reinterpret_cast<int*>(g->work);
+  g->part = reinterpret_cast<float*>(g->work + up(tickets));
+  g->slab_sum = reinterpret_cast<float*>(g->work + up(tickets) + up(part));
+  WB_CUDA(cudaMemset(g->work, 0, up(tickets)));
   return cuda_status(cudaDeviceSynchronize(), "group dense mount");
 }
 
@@ -785,34 +736,21 @@ Status gdense_forward(GroupDense* g, int n, const float* x, int64_t x_ld, float*
   a.part = g->part;
   a.tickets = g->tickets;
   a.slab_sum = g->slab_sum;
-  a.err = g->err;
   for (int b = 0; b < n; b += kMaxTokens) {
     a.n = std::min(n - b, kMaxTokens);
     a.x = x + b * x_ld;
     a.pre = pre ? pre + static_cast<int64_t>(b) * g->rows : nullptr;
     a.post = post + static_cast<int64_t>(b) * g->rows;
-    const GPlan p = plan_of(*g, a.n);
+    const GPlan p = plan_of(*g, a.l, a.n);
     a.slabs = p.slabs;
     a.slab_chunks = p.slab_chunks;
     a.slab_blocks = p.slab_blocks;
-    a.row_sets = p.row_sets;
     a.solo = p.solo;
     a.aligned = p.aligned;
-    WB_TRY(g_launch(kernel_of(*g, a.n, p.mt), dim3(p.slabs * p.slab_blocks), kGThreads, p.smem, st, a));
+    WB_TRY(g_launch(kernel_of(*g, a.l, a.n), dim3(p.slabs * p.slab_blocks), kGThreads, p.smem, st, a));
     if (p.slabs > 1) WB_TRY(g_launch(k_group_slabs, dim3((g->rows + 255) / 256, a.n), 256, 0, st, a));
   }
   return Status::Ok();
-}
-
-Status gdense_check_error(GroupDense* g, cudaStream_t st) {
-  WB_CUDA(cudaSetDevice(g->device));
-  int e = 0;
-  WB_CUDA(cudaMemcpyAsync(&e, g->err, 4, cudaMemcpyDeviceToHost, st));
-  WB_CUDA(cudaStreamSynchronize(st));
-  if (e == 0) return Status::Ok();
-  WB_CUDA(cudaMemsetAsync(g->err, 0, 4, st));
-  WB_CUDA(cudaStreamSynchronize(st));
-  return Status::Internal("group dense: pipeline wait timed out (stage code " + std::to_string(e) + ")");
 }
 
 Status group_quantize(int rows, int cols, int group, int code, int scale_type, const float* W, uint8_t* codes, void* scales,

@@ -23,7 +23,6 @@ struct GroupDense {
   int bias_len = 0;
   int sms = 148;
   uint8_t* work = nullptr;   // the one allocation behind what follows
-  int* err = nullptr;        // a timed-out copy wait of an earlier call
   int* tickets = nullptr;
   float* part = nullptr;
   float* slab_sum = nullptr;
@@ -43,9 +42,6 @@ Status gdense_mount(int device, int rows, int cols, int group, int code, int sca
                     GroupDense** out);
 // x [n][cols] (rows x_ld apart), pre (may be null) and post [n][rows].
 Status gdense_forward(GroupDense* g, int n, const float* x, int64_t x_ld, float* pre, float* post, cudaStream_t st);
-
-// Synchronizes the stream; reports and clears a copy wait that timed out in an earlier call.
-Status gdense_check_error(GroupDense* g, cudaStream_t st);
 
 // W [rows][cols] float32 -> codes, scales, zeros (Uint4) in the layout gdense_mount takes.
 Status group_quantize(int rows, int cols, int group, int code, int scale_type, const float* W, uint8_t* codes, void* scales,

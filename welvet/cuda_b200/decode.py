@@ -47,7 +47,6 @@ _sig("welvet_b200_group_quantize", _ST, c_int32, c_int32, c_int32, c_int32, c_in
 _sig("welvet_b200_gdense_mount", _ST, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
      c_int32, c_void_p, c_size_t, POINTER(c_void_p))
 _sig("welvet_b200_gdense_execute_device", _ST, c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p)
-_sig("welvet_b200_gdense_check_error", _ST, c_void_p, c_void_p)
 _sig("welvet_b200_gdense_release", None, c_void_p)
 
 _append, _attend, _evict, _gemv = (_L.welvet_b200_kv_append, _L.welvet_b200_kv_attend, _L.welvet_b200_kv_evict,
@@ -257,10 +256,6 @@ class GroupDense:
         st = _gemv(self._h, rows, xp, x_ld, None if pre is None else pre.data_ptr(), y.data_ptr(), _stream(stream, x))
         if st.code != OK:
             _fail(st)
-
-    def check_error(self, stream=None) -> None:
-        """Synchronizes and raises (code 4) if a weight copy of an earlier call timed out."""
-        check(_L.welvet_b200_gdense_check_error(self._h, _stream(stream)))
 
     def release(self) -> None:
         if self._h:
