@@ -173,12 +173,17 @@ __device__ __forceinline__ void g_decode(uint32_t w, __half2 z0, __half2 z1, uin
         : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]) : "r"(w));
   } else {
     const uint32_t v = w >> 8;
+    // (x & mask) | 0x6400: one three-input operation
+    auto code = [](uint32_t x, uint32_t mask) {
+      uint32_t y;
+      asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(y) : "r"(x), "r"(mask), "r"(0x64006400u));
+      return *reinterpret_cast<__half2*>(&y);
+    };
     const __half2 sixteenth = __float2half2_rn(0.0625f);
-    auto h = [](uint32_t x) { return *reinterpret_cast<__half2*>(&x); };
-    const __half2 r0 = __hsub2(h((w & 0x000f000fu) | 0x64006400u), z0);
-    const __half2 r1 = __hfma2(h((w & 0x00f000f0u) | 0x64006400u), sixteenth, z1);
-    const __half2 r2 = __hsub2(h((v & 0x000f000fu) | 0x64006400u), z0);
-    const __half2 r3 = __hfma2(h((v & 0x00f000f0u) | 0x64006400u), sixteenth, z1);
+    const __half2 r0 = __hsub2(code(w, 0x000f000fu), z0);
+    const __half2 r1 = __hfma2(code(w, 0x00f000f0u), sixteenth, z1);
+    const __half2 r2 = __hsub2(code(v, 0x000f000fu), z0);
+    const __half2 r3 = __hfma2(code(v, 0x00f000f0u), sixteenth, z1);
     a[0] = *reinterpret_cast<const uint32_t*>(&r0);
     a[1] = *reinterpret_cast<const uint32_t*>(&r1);
     a[2] = *reinterpret_cast<const uint32_t*>(&r2);
