@@ -633,3 +633,68 @@ def test_attend_many_sequences(D):
     pages = [t.float().cpu() for t in (kp, vp)]
     want, _, bound = attend64(q, pages[0], pages[1], table, lens, 0.125)
     assert np.all(np.abs(out.cpu().numpy() - want) <= bound)
+
+
+@pytest.mark.parametrize("kv,lens,keep,page", [(1, [70000], 20000, 64), (2, [30001, 5, 250000], 29999, 16), (40, [3000, 2500, 10, 2049], 2048, 32)])
+def test_evict_long_and_many(D, kv, lens, keep, page):
+    """Heads spread over a cluster of blocks, keys beyond what shared memory holds, and more heads than SMs,
+    against one stable sort."""
+    import torch
+    dim, n = 16, len(lens)
+    per = -(-max(lens) // page)
+    S = per * page
+    g = torch.Generator(device="cuda").manual_seed(kv)
+    kp = torch.randint(0, 256, (n * per, page, kv, dim), generator=g, device="cuda", dtype=torch.uint8)
+    vp = torch.randint(0, 256, kp.shape, generator=g, device="cuda", dtype=torch.uint8)
+    table = torch.randperm(n * per, generator=g, device="cuda").reshape(n, per).to(torch.int32)
+    w = (torch.rand((n, kv, S), generator=g, device="cuda") * 50).floor() * 0.25  # many ties
+    pos = torch.arange(S, device="cuda", dtype=torch.int32).expand(n, kv, S).contiguous()
+    lens_t = i32(lens)
+    k0, v0, w0 = kp.clone(), vp.clone(), w.clone()
+    c = D.PagedKV(kp.view(torch.float8_e4m3fn), vp.view(torch.float8_e4m3fn), table, lens_t, num_heads=kv, seen=i32(lens), weights=w, positions=pos)
+    c.evict(keep, sinks=3, recent=keep // 5)
+    c.check_error()
+    assert lens_t.tolist() == [min(x, keep) for x in lens]
+    for b, L in enumerate(lens):
+        t = table[b].long()
+        old_k, old_v = k0[t].reshape(S, kv, dim), v0[t].reshape(S, kv, dim)
+        new_k, new_v = kp[t].reshape(S, kv, dim), vp[t].reshape(S, kv, dim)
+        m = min(L, keep)
+        for h in range(kv):
+            src = torch.arange(m, device="cuda")
+            if L > keep:
+                j = torch.arange(L, device="cuda")
+                key = torch.where((j < 3) | (j >= L - keep // 5), torch.inf, w0[b, h, :L])
+                stays = torch.zeros(L, dtype=torch.bool, device="cuda")
+                stays[torch.sort(key, descending=True, stable=True).indices[:keep]] = True
+                src[~stays[:keep]] = keep + torch.nonzero(stays[keep:]).flatten()
+            assert torch.equal(pos[b, h, :m].long(), src)
+            assert torch.equal(w[b, h, :m], w0[b, h, src])
+            assert torch.equal(new_k[:m, h], old_k[src, h]) and torch.equal(new_v[:m, h], old_v[src, h])
+
+
+def test_evict_again_and_again(D):
+    """Two hundred calls with one new token between them: the tickets and lengths stay in step."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(1)
+    n, kv, dim, page, per, keep = 3, 2, 64, 16, 6, 64
+    kp = torch.randn((n * per, page, kv, dim), generator=g, device="cuda")
+    vp, table = kp.clone(), torch.arange(n * per, device="cuda", dtype=torch.int32).reshape(n, per)
+    lens, seen = i32([60, 0, 30]), i32([60, 0, 30])
+    w, pos = torch.rand((n, kv, per * page), generator=g, device="cuda"), torch.zeros((n, kv, per * page), dtype=torch.int32, device="cuda")
+    pos[:] = torch.arange(per * page, device="cuda", dtype=torch.int32)
+    c = D.PagedKV(kp, vp, table, lens, num_heads=4, seen=seen, weights=w, positions=pos)
+    q, out = torch.randn((n, 4, dim), generator=g, device="cuda"), torch.empty((n, 4, dim), device="cuda")
+    for step in range(200):
+        k = torch.randn((n, kv, dim), generator=g, device="cuda")
+        c.append(k, k)
+        c.attend(q, out, accumulate=True)
+        c.evict(keep, budget=keep + 7, sinks=2, recent=16)
+    c.check_error()
+    assert seen.tolist() == [260, 200, 230]
+    assert all(keep <= x <= keep + 7 for x in lens.tolist())
+    for b in range(n):
+        for h in range(kv):
+            p = pos[b, h, : lens.tolist()[b]].tolist()
+            assert len(set(p)) == len(p) and {0, 1} <= set(p)
+            assert set(range(seen.tolist()[b] - 16, seen.tolist()[b])) <= set(p)

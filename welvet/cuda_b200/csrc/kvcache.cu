@@ -2,6 +2,9 @@
 #include "kvcache.hpp"
 #include "kvcache.cuh"
 
+#include <cooperative_groups.h>
+
+#include <algorithm>
 #include <cmath>
 
 namespace wb {
@@ -156,181 +159,325 @@ __global__ void __launch_bounds__(kAppendThreads) k_append(const __grid_constant
 struct EvictParams {
   KvEvictArgs a;
   KvView c;
-  int32_t* moves;
-  int32_t* n_moves;
+  int32_t* moves;    // [num_seqs][num_kv][2][max_slots / 2]: slots to fill, slots to take
+  int32_t* n_moves;  // [num_seqs][num_kv]; -1: not cut
+  int* tickets;      // [num_seqs], zero between calls
+  int cached;        // keys a block keeps in shared memory (0: read again in each pass)
 };
 
-constexpr int kEvictThreads = 1024;
-constexpr int kRadixBits = 11;  // three passes over a 32-bit key: 11 + 11 + 10 bits
+constexpr int kEvictThreads = 512;
+constexpr int kEvictWarps = kEvictThreads / 32;
+constexpr int kRadixBins = 2048;      // three passes over a 32-bit key: 11 + 11 + 10 bits
+constexpr int kEvictCache = 24 * 1024;  // keys: 96 KB
 
 // The order in which slots stay: protected ones first, then by weight; larger keys stay. NaN counts
 // as -infinity, -0 as 0.
-__device__ __forceinline__ uint32_t evict_key(const EvictParams& p, int64_t rec, int j, int seen) {
-  const int pos = p.a.positions_in[rec + j];
-  if (pos < p.a.sinks || pos >= seen - p.a.recent) return 0xffffffffu;
-  const float w = p.a.weights_in[rec + j];
+__device__ __forceinline__ uint32_t evict_key(float w, int pos, int sinks, int recent_from) {
+  if (pos < sinks || pos >= recent_from) return 0xffffffffu;
   if (isnan(w)) return 0x007fffffu;
   const uint32_t u = __float_as_uint(w + 0.0f);
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-// Exclusive sum of v over the block's threads; *total the whole sum.
-__device__ __forceinline__ int block_scan(int v, int* s_warp, int* total) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int x = v;
+// Rows of one (sequence, key-value head): slots `take` to slots `fill`, 16 bytes a lane where the
+// layout allows it. A group of lanes takes a row; kFly rows a group are in flight.
+template <int kSize, bool kVec, int kFly>
+__device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kv, const int32_t* fill, const int32_t* take,
+                                          int n, int worker, int workers) {
+  const KvView& c = p.c;
+  const int64_t rec = (static_cast<int64_t>(b) * c.num_kv + kv) * c.max_slots;
+  const int32_t* table = c.table + b * c.table_stride;
+  const int lane = threadIdx.x & 31;
+  const int bytes = c.head_dim * kSize;
+  auto row_of = [&](int slot, int64_t* k, int64_t* v) {
+    const int page_at = slot / c.page_size, in = slot - page_at * c.page_size;
+    const int page = table[page_at];
+    if (page < 0 || page >= c.num_pages) return false;
+    *k = (page * c.k.page + in * c.k.slot + kv * c.k.head) * kSize;
+    *v = (page * c.v.page + in * c.v.slot + kv * c.v.head) * kSize;
+    return true;
+  };
+  if constexpr (kVec) {
+    const int lanes = bytes >= 512 ? 32 : (bytes > 128 ? (bytes > 256 ? 32 : 16) : 8);  // of a row
+    const int groups = 32 / lanes, sub = lane / lanes, at = 16 * (lane % lanes);
+    for (int i0 = worker * groups * kFly; i0 < n; i0 += workers * groups * kFly) {
+      int64_t kt[kFly], vt[kFly], kf[kFly], vf[kFly];
+      int to[kFly], from[kFly];
+      bool ok[kFly];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
-  }
-  __syncthreads();
-  if (lane == 31) s_warp[w] = x;
-  __syncthreads();
-  if (w == 0) {
-    int y = lane < static_cast<int>(blockDim.x) / 32 ? s_warp[lane] : 0;
+      for (int x = 0; x < kFly; ++x) {
+        const int i = i0 + x * groups + sub;
+        ok[x] = i < n;
+        to[x] = ok[x] ? fill[i] : 0;
+        from[x] = ok[x] ? take[i] : 0;
+      }
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int z = __shfl_up_sync(0xffffffffu, y, o);
-      if (lane >= o) y += z;
+      for (int x = 0; x < kFly; ++x) {
+        if (!ok[x]) continue;
+        if (lane % lanes == 0) {
+          c.weights[rec + to[x]] = p.a.weights_in[rec + from[x]];
+          c.positions[rec + to[x]] = p.a.positions_in[rec + from[x]];
+        }
+        ok[x] = row_of(to[x], &kt[x], &vt[x]) && row_of(from[x], &kf[x], &vf[x]);
+        if (!ok[x]) atomicCAS(c.err, 0, kKvErrPage);
+      }
+      for (int o = at; o < bytes; o += 16 * lanes) {
+        uint4 k[kFly], v[kFly];
+#pragma unroll
+        for (int x = 0; x < kFly; ++x)
+          if (ok[x]) {
+            k[x] = *reinterpret_cast<const uint4*>(c.k.base + kf[x] + o);
+            v[x] = *reinterpret_cast<const uint4*>(c.v.base + vf[x] + o);
+          }
+#pragma unroll
+        for (int x = 0; x < kFly; ++x)
+          if (ok[x]) {
+            *reinterpret_cast<uint4*>(c.k.base + kt[x] + o) = k[x];
+            *reinterpret_cast<uint4*>(c.v.base + vt[x] + o) = v[x];
+          }
+      }
     }
-    s_warp[lane] = y;
+  } else {
+    for (int i = worker; i < n; i += workers) {
+      const int to = fill[i], from = take[i];
+      if (lane == 0) {
+        c.weights[rec + to] = p.a.weights_in[rec + from];
+        c.positions[rec + to] = p.a.positions_in[rec + from];
+      }
+      int64_t kt, vt, kf, vf;
+      if (!(row_of(to, &kt, &vt) && row_of(from, &kf, &vf))) {
+        if (lane == 0) atomicCAS(c.err, 0, kKvErrPage);
+        continue;
+      }
+      for (int o = lane; o < bytes; o += 32) {
+        c.k.base[kt + o] = c.k.base[kf + o];
+        c.v.base[vt + o] = c.v.base[vf + o];
+      }
+    }
   }
-  __syncthreads();
-  *total = s_warp[31];
-  return x - v + (w > 0 ? s_warp[w - 1] : 0);
 }
 
-// One block per (sequence, kv head): the keep-th largest key by radix selection, then, in slot
-// order, the slots below keep that go (to fill) and those above it that stay (to take). Both
-// lists are equally long, and no slot is in both, so the moves can run in any order.
-__global__ void __launch_bounds__(kEvictThreads) k_evict_select(const __grid_constant__ EvictParams p) {
-  __shared__ int hist[1 << kRadixBits];
-  __shared__ int s_warp[32];
+// A cluster of blocks per (sequence, key-value head), each with its share of the slots: the keep-th
+// largest key by radix selection (histograms added over the cluster through distributed shared
+// memory), then, in slot order, the slots below keep that go (to fill) and those above it that stay
+// (to take). Both lists are equally long and no slot is in both, so the rows can move in any order.
+// A cluster of one block moves them itself; larger ones leave the lists to k_evict_move.
+// Latency bound: 8 bytes a slot are read, the rest is a dozen barriers.
+template <int kSize, bool kVec>
+__global__ void __launch_bounds__(kEvictThreads, 2) k_evict_select(const __grid_constant__ EvictParams p) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  extern __shared__ uint32_t s_keys[];
+  __shared__ __align__(16) int s_hist[3][kRadixBins];
+  __shared__ int s_warp[kEvictWarps], s_warp2[kEvictWarps];
   __shared__ uint32_t s_prefix;
   __shared__ int s_rest;
+  __shared__ int s_ties;      // of this block
+  __shared__ int s_lists[2];  // slots of this block to fill, to take
   const KvView& c = p.c;
-  const int kv = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int kv = blockIdx.x / ranks, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, w = tid >> 5;
   const int row = b * c.num_kv + kv;
   const int64_t rec = static_cast<int64_t>(row) * c.max_slots;
-  int len = p.a.lens_in[b];
-  if (len < 0 || len > c.max_slots) {
-    if (tid == 0) atomicCAS(c.err, 0, kKvErrSlot);
-    len = len < 0 ? 0 : c.max_slots;
-  }
+  asm volatile("griddepcontrol.launch_dependents;");
+  for (int i = tid; i < 3 * kRadixBins; i += kEvictThreads) (&s_hist[0][0])[i] = 0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int given = p.a.lens_in[b], keep = p.a.keep, recent_from = c.seen[b] - p.a.recent;
+  const int len = min(max(given, 0), c.max_slots);
+  if (len != given && tid == 0) atomicCAS(c.err, 0, kKvErrSlot);
   const bool cut = len > p.a.budget;
-  const int keep = p.a.keep, seen = c.seen[b];
-  if (p.a.weights_in != c.weights || p.a.positions_in != c.positions) {
-    // separate records: what stays in place is copied (the moves write the filled slots later)
-    const int n = cut ? keep : len;
-    for (int j = tid; j < n; j += kEvictThreads) {
-      c.weights[rec + j] = p.a.weights_in[rec + j];
-      c.positions[rec + j] = p.a.positions_in[rec + j];
+  // this block's slots, and each warp's: multiples of 32
+  const int per = ((len + ranks - 1) / ranks + 31) & ~31;
+  const int lo = min(rank * per, len), hi = min(lo + per, len);
+  const int per_warp = (((hi - lo) + kEvictWarps - 1) / kEvictWarps + 31) & ~31;
+  const int wlo = min(lo + w * per_warp, hi), whi = min(wlo + per_warp, hi);
+  const bool apart = p.a.weights_in != c.weights || p.a.positions_in != c.positions;
+  const int stays_to = cut ? keep : len;  // separate records: what stays in place is copied
+  auto key_at = [&](int j) -> uint32_t {
+    if (p.cached) return s_keys[j - lo];
+    return evict_key(p.a.weights_in[rec + j], p.a.positions_in[rec + j], p.a.sinks, recent_from);
+  };
+  if (cut || apart) {
+#pragma unroll 4
+    for (int j = lo + tid; j < hi; j += kEvictThreads) {
+      const float weight = p.a.weights_in[rec + j];
+      const int pos = p.a.positions_in[rec + j];
+      if (apart && j < stays_to) {
+        c.weights[rec + j] = weight;
+        c.positions[rec + j] = pos;
+      }
+      const uint32_t k = evict_key(weight, pos, p.a.sinks, recent_from);
+      if (cut && p.cached) s_keys[j - lo] = k;
     }
   }
+  // The last (head, block) of a sequence to have read its length writes the new one.
+  auto leave = [&] {
+    if (tid == 0 && atomicAdd(p.tickets + b, 1) == c.num_kv * ranks - 1) {
+      p.tickets[b] = 0;
+      c.lens[b] = stays_to;
+    }
+  };
   if (!cut) {
-    if (tid == 0) p.n_moves[row] = -1;
-    return;
+    if (rank == 0 && tid == 0) p.n_moves[row] = -1;
+    leave();
+    return;  // the whole cluster does
   }
+  __syncthreads();
+
+
   uint32_t prefix = 0;  // of the keep-th largest key
   int rest = keep;      // how many of the keys with this prefix stay
+#pragma unroll
   for (int pass = 0; pass < 3; ++pass) {
     const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
     const int bits = pass == 2 ? 10 : 11;
-    for (int i = tid; i < (1 << kRadixBits); i += kEvictThreads) hist[i] = 0;
-    __syncthreads();
-    for (int j = tid; j < len; j += kEvictThreads) {
-      const uint32_t k = evict_key(p, rec, j, seen);
+    int* hist = s_hist[pass];
+    for (int j = lo + tid; j < hi; j += kEvictThreads) {
+      const uint32_t k = key_at(j);
       if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1u)], 1);
     }
-    __syncthreads();
-    // bins from the top: thread t takes the two bins below 2t from the top
-    const int n = 1 << bits;
-    int a0 = 0, a1 = 0;
-    const int top = n - 1 - 2 * tid;
-    if (top >= 1) {
-      a0 = hist[top];
-      a1 = hist[top - 1];
+    if (ranks > 1) cluster.sync();
+    else __syncthreads();
+    // bins from the top, four a thread
+    const int top = (1 << bits) - 1 - 4 * tid;
+    int n[4] = {0, 0, 0, 0};
+    if (top >= 3) {
+      for (int r = 0; r < ranks; ++r) {
+        const int* h = ranks > 1 ? cluster.map_shared_rank(hist, r) : hist;
+        const int4 q = *reinterpret_cast<const int4*>(h + top - 3);
+        n[0] += q.w;
+        n[1] += q.z;
+        n[2] += q.y;
+        n[3] += q.x;
+      }
     }
-    int total;
-    const int before = block_scan(a0 + a1, s_warp, &total);
-    if (top >= 1 && before < rest && before + a0 + a1 >= rest) {
-      const bool second = before + a0 < rest;
-      s_prefix = (prefix << bits) | static_cast<uint32_t>(second ? top - 1 : top);
-      s_rest = rest - before - (second ? a0 : 0);
+    const int mine = n[0] + n[1] + n[2] + n[3];
+    int x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) s_warp[w] = x;
+    __syncthreads();
+    int before = x - mine;
+#pragma unroll
+    for (int i = 0; i < kEvictWarps; ++i)
+      if (i < w) before += s_warp[i];
+    if (top >= 3 && before < rest && before + mine >= rest) {
+      int e = 0, left = rest - before;
+#pragma unroll
+      for (int i = 0; i < 3; ++i)
+        if (e == i && left > n[i]) {
+          left -= n[i];
+          ++e;
+        }
+      s_prefix = (prefix << bits) | static_cast<uint32_t>(top - e);
+      s_rest = left;
     }
     __syncthreads();
     prefix = s_prefix;
     rest = s_rest;
     __syncthreads();
   }
+
   // keys above the threshold stay, and the first `rest` slots whose key equals it
+  int ties = 0;
+  for (int j0 = wlo; j0 < whi; j0 += 32) ties += __popc(__ballot_sync(0xffffffffu, j0 + lane < whi && key_at(min(j0 + lane, whi - 1)) == prefix));
+  if (lane == 0) s_warp[w] = ties;
+  __syncthreads();
+  int ties_before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kEvictWarps; ++i) {
+    if (i < w) ties_before += s_warp[i];
+    all += s_warp[i];
+  }
+  if (tid == 0) s_ties = all;
+  if (ranks > 1) {
+    cluster.sync();
+    for (int r = 0; r < rank; ++r) ties_before += *cluster.map_shared_rank(&s_ties, r);
+  }
+  __syncthreads();
+  auto flags_at = [&](int j0, int& seen_ties, uint32_t& f, uint32_t& g) {
+    const int j = j0 + lane;
+    const uint32_t k = j < whi ? key_at(j) : 0u;
+    const uint32_t tie = __ballot_sync(0xffffffffu, j < whi && k == prefix);
+    const int order = seen_ties + __popc(tie & ((1u << lane) - 1u));
+    const bool stays = j < whi && (k > prefix || (k == prefix && order < rest));
+    f = __ballot_sync(0xffffffffu, j < whi && j < keep && !stays);
+    g = __ballot_sync(0xffffffffu, j >= keep && stays);
+    seen_ties += __popc(tie);
+  };
+  int n_fill = 0, n_take = 0, seen_ties = ties_before;
+  for (int j0 = wlo; j0 < whi; j0 += 32) {
+    uint32_t f, g;
+    flags_at(j0, seen_ties, f, g);
+    n_fill += __popc(f);
+    n_take += __popc(g);
+  }
+  __syncthreads();
+  if (lane == 0) {
+    s_warp[w] = n_fill;
+    s_warp2[w] = n_take;
+  }
+  __syncthreads();
+  int fill_at = 0, take_at = 0, fills = 0, takes = 0;
+#pragma unroll
+  for (int i = 0; i < kEvictWarps; ++i) {
+    if (i < w) {
+      fill_at += s_warp[i];
+      take_at += s_warp2[i];
+    }
+    fills += s_warp[i];
+    takes += s_warp2[i];
+  }
+  if (tid == 0) {
+    s_lists[0] = fills;
+    s_lists[1] = takes;
+  }
+  int moved = fills;
+  if (ranks > 1) {
+    cluster.sync();
+    moved = 0;
+    for (int r = 0; r < ranks; ++r) {
+      const int* l = cluster.map_shared_rank(s_lists, r);
+      if (r < rank) {
+        fill_at += l[0];
+        take_at += l[1];
+      }
+      moved += l[0];
+    }
+  }
   int32_t* fill = p.moves + static_cast<int64_t>(row) * 2 * (c.max_slots / 2);
   int32_t* take = fill + c.max_slots / 2;
-  int ties = 0, n_fill = 0, n_take = 0;
-  for (int j0 = 0; j0 < len; j0 += kEvictThreads) {
-    const int j = j0 + tid;
-    const uint32_t k = j < len ? evict_key(p, rec, j, seen) : 0u;
-    int total;
-    const int tie = j < len && k == prefix;
-    const int order = ties + block_scan(tie, s_warp, &total);
-    ties += total;
-    const bool stays = j < len && (k > prefix || (tie && order < rest));
-    const int f = j < keep && !stays, g = j >= keep && stays;
-    int both;
-    const int at = block_scan(f | (g << 16), s_warp, &both);
-    if (f) fill[n_fill + (at & 0xffff)] = j;
-    if (g) take[n_take + (at >> 16)] = j;
-    n_fill += both & 0xffff;
-    n_take += both >> 16;
+  seen_ties = ties_before;
+  for (int j0 = wlo; j0 < whi; j0 += 32) {
+    uint32_t f, g;
+    flags_at(j0, seen_ties, f, g);
+    const uint32_t below = (1u << lane) - 1u;
+    if ((f >> lane) & 1) fill[fill_at + __popc(f & below)] = j0 + lane;
+    if ((g >> lane) & 1) take[take_at + __popc(g & below)] = j0 + lane;
+    fill_at += __popc(f);
+    take_at += __popc(g);
   }
-  if (tid == 0) p.n_moves[row] = n_fill;
+  if (ranks == 1) {
+    __syncthreads();  // the block's own lists
+    move_rows<kSize, kVec, 1>(p, b, kv, fill, take, moved, w, kEvictWarps);
+  } else {
+    if (rank == 0 && tid == 0) p.n_moves[row] = moved;
+    cluster.sync();  // no block leaves while another reads its shared memory
+  }
+  leave();
 }
 
-// Moves rows: a warp per (slot to fill), keys then values, 16 bytes a lane where the layout
-// allows it. Block (0, 0, b) sets the new length.
 template <int kSize, bool kVec>
-__global__ void __launch_bounds__(256) k_evict_move(const __grid_constant__ EvictParams p) {
+__global__ void __launch_bounds__(256, 4) k_evict_move(const __grid_constant__ EvictParams p) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const KvView& c = p.c;
   const int kv = blockIdx.y, b = blockIdx.z, row = b * c.num_kv + kv;
-  const int n = p.n_moves[row];
-  if (kv == 0 && blockIdx.x == 0 && threadIdx.x == 0) {
-    const int len = p.a.lens_in[b];
-    c.lens[b] = n >= 0 ? p.a.keep : (len < 0 ? 0 : (len > c.max_slots ? c.max_slots : len));
-  }
   const int32_t* fill = p.moves + static_cast<int64_t>(row) * 2 * (c.max_slots / 2);
-  const int32_t* take = fill + c.max_slots / 2;
-  const int lane = threadIdx.x & 31;
-  const int64_t rec = static_cast<int64_t>(row) * c.max_slots;
-  const int32_t* table = c.table + b * c.table_stride;
-  for (int i = blockIdx.x * 8 + (threadIdx.x >> 5); i < n; i += gridDim.x * 8) {
-    const int to = fill[i], from = take[i];
-    const int64_t pt = table[to / c.page_size], pf = table[from / c.page_size];
-    if (lane == 0) {
-      c.weights[rec + to] = p.a.weights_in[rec + from];
-      c.positions[rec + to] = p.a.positions_in[rec + from];
-    }
-    if (pt < 0 || pt >= c.num_pages || pf < 0 || pf >= c.num_pages) {
-      if (lane == 0) atomicCAS(c.err, 0, kKvErrPage);
-      continue;
-    }
-    const int st = to % c.page_size, sf = from % c.page_size;
-    uint8_t* kt = c.k.base + (pt * c.k.page + st * c.k.slot + kv * c.k.head) * kSize;
-    const uint8_t* kf = c.k.base + (pf * c.k.page + sf * c.k.slot + kv * c.k.head) * kSize;
-    uint8_t* vt = c.v.base + (pt * c.v.page + st * c.v.slot + kv * c.v.head) * kSize;
-    const uint8_t* vf = c.v.base + (pf * c.v.page + sf * c.v.slot + kv * c.v.head) * kSize;
-    const int bytes = c.head_dim * kSize;
-    if constexpr (kVec) {
-      for (int o = 16 * lane; o < bytes; o += 512) {
-        *reinterpret_cast<uint4*>(kt + o) = *reinterpret_cast<const uint4*>(kf + o);
-        *reinterpret_cast<uint4*>(vt + o) = *reinterpret_cast<const uint4*>(vf + o);
-      }
-    } else {
-      for (int o = lane; o < bytes; o += 32) {
-        kt[o] = kf[o];
-        vt[o] = vf[o];
-      }
-    }
-  }
+  move_rows<kSize, kVec, 2>(p, b, kv, fill, fill + c.max_slots / 2, p.n_moves[row], blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8);
 }
 
 bool f32_aligned(const float* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0; }
@@ -354,7 +501,7 @@ static Status kv_alloc(KvCache* c) {
     return at;
   };
   WB_TRY(attend_plan(c));
-  const size_t err = take(4), ticket = take(4);
+  const size_t err = take(4), ticket = take(4), evict_tickets = take(v.positions ? static_cast<size_t>(v.num_seqs) * 4 : 0);
   const size_t part = take(c->part_bytes);  // from here on nothing needs to start as zero
   const size_t spans = take(c->span_bytes);
   const size_t scores = take(v.weights ? rows * v.max_slots * 4 : 0), lse = take(v.weights ? rows * 4 : 0);
@@ -362,6 +509,7 @@ static Status kv_alloc(KvCache* c) {
   WB_CUDA(cudaMalloc(&c->work, bytes));
   c->err = reinterpret_cast<int*>(c->work + err);
   c->ticket = reinterpret_cast<int*>(c->work + ticket);
+  c->evict_tickets = reinterpret_cast<int*>(c->work + evict_tickets);
   c->spans = c->work + spans;
   c->part = reinterpret_cast<float*>(c->work + part);
   c->scores = reinterpret_cast<float*>(c->work + scores);
@@ -428,23 +576,47 @@ Status kv_evict(KvCache* c, const KvEvictArgs& a, cudaStream_t st) {
   if (!p.a.positions_in) p.a.positions_in = p.c.positions;
   p.moves = c->moves;
   p.n_moves = c->n_moves;
-  k_evict_select<<<dim3(p.c.num_kv, p.c.num_seqs), kEvictThreads, 0, st>>>(p);
-  WB_TRY(cuda_status(cudaGetLastError(), "kv evict launch"));
+  p.tickets = c->evict_tickets;
   const int size = kv_size(c->type);
   const bool vec = p.c.head_dim * size % 16 == 0 && pool_aligned(p.c.k, size, 16) && pool_aligned(p.c.v, size, 16);
-  int blocks = (p.c.max_slots / 2 + 7) / 8;
-  if (blocks > 64) blocks = 64;
-  if (blocks < 1) blocks = 1;
-  const dim3 grid(blocks, p.c.num_kv, p.c.num_seqs);
-  auto go = [&](auto size_c) {
+  // One block a head unless that leaves SMs idle or a block's keys do not fit its shared memory.
+  const int64_t heads = static_cast<int64_t>(p.c.num_seqs) * p.c.num_kv;
+  int ranks = 1;
+  while (ranks < 8 && ((heads * ranks < 148 && p.c.max_slots / ranks > 2048) || p.c.max_slots / ranks > kEvictCache - 32)) ranks *= 2;
+  const int per = ((p.c.max_slots + ranks - 1) / ranks + 31) & ~31;
+  p.cached = per <= kEvictCache;
+  auto go = [&](auto size_c, auto vec_c) -> Status {
     constexpr int S = decltype(size_c)::value;
-    if (vec) k_evict_move<S, true><<<grid, 256, 0, st>>>(p);
-    else k_evict_move<S, false><<<grid, 256, 0, st>>>(p);
+    constexpr bool V = decltype(vec_c)::value;
+    auto* select = k_evict_select<S, V>;
+    WB_CUDA(cudaFuncSetAttribute(select, cudaFuncAttributeMaxDynamicSharedMemorySize, kEvictCache * 4));
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim = {static_cast<unsigned>(ranks), 1, 1};
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(p.c.num_kv * ranks, p.c.num_seqs);
+    cfg.blockDim = dim3(kEvictThreads);
+    cfg.dynamicSmemBytes = p.cached ? per * 4 : 0;
+    cfg.stream = st;
+    cfg.attrs = at;
+    cfg.numAttrs = 2;
+    WB_TRY(cuda_status(cudaLaunchKernelEx(&cfg, select, p), "kv evict launch"));
+    if (ranks == 1) return Status::Ok();
+    cfg.gridDim = dim3(static_cast<unsigned>(std::min<int64_t>((p.c.max_slots / 2 + 63) / 64, std::max<int64_t>(1, 148 * 8 / heads))),
+                       p.c.num_kv, p.c.num_seqs);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    cfg.numAttrs = 1;
+    return cuda_status(cudaLaunchKernelEx(&cfg, k_evict_move<S, V>, p), "kv evict move launch");
   };
-  if (size == 4) go(std::integral_constant<int, 4>{});
-  else if (size == 2) go(std::integral_constant<int, 2>{});
-  else go(std::integral_constant<int, 1>{});
-  return cuda_status(cudaGetLastError(), "kv evict move launch");
+  auto by_size = [&](auto vec_c) -> Status {
+    if (size == 4) return go(std::integral_constant<int, 4>{}, vec_c);
+    if (size == 2) return go(std::integral_constant<int, 2>{}, vec_c);
+    return go(std::integral_constant<int, 1>{}, vec_c);
+  };
+  return vec ? by_size(std::true_type{}) : by_size(std::false_type{});
 }
 
 Status kv_check_error(KvCache* c, cudaStream_t st) {

@@ -63,6 +63,7 @@ struct KvCache {
   float* lse = nullptr;          // [num_seqs][num_heads]
   int32_t* moves = nullptr;      // evict: [num_seqs][num_kv][2][max_slots / 2] slots to fill, slots to take
   int32_t* n_moves = nullptr;    // [num_seqs][num_kv]
+  int* evict_tickets = nullptr;  // [num_seqs], zero between calls
   ~KvCache();
 };
 
