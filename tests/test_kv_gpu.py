@@ -698,3 +698,37 @@ def test_evict_again_and_again(D):
             p = pos[b, h, : lens.tolist()[b]].tolist()
             assert len(set(p)) == len(p) and {0, 1} <= set(p)
             assert set(range(seen.tolist()[b] - 16, seen.tolist()[b])) <= set(p)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("dim", [64, 80, 96, 128, 256])
+@pytest.mark.parametrize("page", [16, 48, 20, 64])
+def test_attend_pages_and_groups(D, dtype, dim, page):
+    """Every constant width, pages that hold whole 16-slot tiles and pages that end inside one, head groups
+    that fill a tile of eight in part, exactly and more than once."""
+    import torch
+    rng = np.random.default_rng(dim + page)
+    lens = [131, 64, 33, 400]
+    for H, kv in ((3, 1), (16, 2), (20, 2)):
+        per = -(-400 // page)
+        kp, vp, table = make_cache(rng, dtype, 4, per, page, kv, dim, layout="heads" if page == 48 else "slots")
+        q = torch.from_numpy(rng.standard_normal((4, H, dim)).astype(np.float32)).cuda()
+        out = torch.full((4, H, dim), float("nan"), device="cuda")
+        c = D.PagedKV(kp, vp, table, i32(lens), num_heads=H)
+        c.attend(q, out)
+        c.check_error()
+        want, _, bound = attend64(q, kp, vp, table, lens, 1.0 / math.sqrt(dim))
+        assert np.all(np.abs(out.cpu().numpy() - want) <= bound), (H, kv)
+
+
+def test_attend_pools_of_different_layout(D):
+    """Keys by slot, values by head: the pools' strides differ."""
+    import torch
+    rng = np.random.default_rng(31)
+    kp, _, table = make_cache(rng, "bf16", 2, 8, 32, 4, 128)
+    vp = torch.from_numpy(rng.standard_normal((kp.shape[0], 4, 32, 128)).astype(np.float32)).cuda().to(torch.bfloat16).transpose(1, 2)
+    q = torch.from_numpy(rng.standard_normal((2, 8, 128)).astype(np.float32)).cuda()
+    out = torch.empty((2, 8, 128), device="cuda")
+    D.PagedKV(kp, vp, table, i32([250, 77]), num_heads=8).attend(q, out)
+    want, _, bound = attend64(q, kp, vp, table, [250, 77], 128 ** -0.5)
+    assert np.all(np.abs(out.cpu().numpy() - want) <= bound)

@@ -16,9 +16,15 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+struct KvBytes {  // a pool's strides in bytes
+  uint32_t page, slot, head;
+};
+
 struct AttendParams {
   KvAttendArgs a;
   KvView c;
+  KvBytes kb, vb;  // tiled form
+  int same;        // the two pools have the same strides
   int splits;      // simple form
   float* part;     // partial results: o, m, l
   float* scores;   // with accumulate: [num_seqs][num_heads][max_slots], units of log2
@@ -254,22 +260,23 @@ struct Tiled {
   static constexpr bool kBF16 = std::is_same_v<T, __nv_bfloat16>;
   static constexpr bool kFP8 = std::is_same_v<T, __nv_fp8_e4m3>;
   using M = std::conditional_t<kFP8, __half, T>;  // MMA operand type
-  static constexpr int kRow = DP * static_cast<int>(sizeof(T));  // bytes of a row in shared memory (at most, unpadded)
+  static constexpr int kRow = DP * static_cast<int>(sizeof(T));  // bytes of a row
+  static constexpr bool kSwz = kRow % 128 == 0;                  // with kFull: chunks xored by the key
+  // the longest pitch of a row in shared memory
+  static constexpr int kPitch = kFull ? (kSwz ? kRow : 16 * (((kRow / 16 + 1) & ~1) + 1)) : (kRow == 64 ? 80 : kRow);
   static constexpr int kWarps = kRow <= 512 ? 4 : 2;
-  static constexpr int kStages = kRow <= 128 ? 4 : 3;
+  static constexpr int kSub = kRow <= 128 ? 2 : 1;      // 16-key blocks of a warp's tile
+  static constexpr int kStages = kRow <= 256 || kRow > 384 ? 3 : 2;
   static constexpr int kDP = DP;
   static constexpr int kThreads = 32 * kWarps;
-  static constexpr int kBlocks = kRow <= 128 ? 3 : (kRow <= 256 && DP <= 128 ? 2 : 1);  // of an SM: what registers allow
-  static constexpr int kKeys = 16 * kWarps;  // keys of a block tile
-  static constexpr int kLanes = kRow < 128 ? kRow / 16 : 8;  // lanes that copy a row
-  static constexpr bool kSwz = kRow % 128 == 0;              // with kFull: chunks xored by the key
+  static constexpr int kBlocks = kRow <= 384 && DP <= 128 ? 2 : 1;  // of an SM (three, with 168 registers a thread, cost more)
+  static constexpr int kKeys = 16 * kSub * kWarps;  // keys of a block tile
+  static constexpr int kLanes = kRow <= 64 ? 4 : 8;  // lanes that copy a row
   static constexpr int kSets = kBF16 ? 2 : 1;
-  static constexpr int kSteps = kF32 ? DP / 8 : DP / 16;  // MMA steps over a head's dims
+  static constexpr int kSteps = kF32 ? DP / 8 : (kFP8 ? (DP / 16 + 1) & ~1 : DP / 16);  // MMA steps over a head's dims
   static constexpr float kBias = kF32 || kBF16 ? 0.0f : 15.0f;  // log2 of the weights' scale
-  static constexpr int kRowMax = kRow == 64 ? 80 : kRow;  // the longest pitch of a row
-  static constexpr int kRing = kStages * kWarps * 2 * 16 * kRowMax;
-  static constexpr int kSmemQ = kSets * kSteps * 512, kSmemO = 8 * DP * 4;
-  static constexpr int kSmem = kRing + kSmemQ + kSmemO;
+  static constexpr int kRing = kStages * kWarps * kSub * 32 * kPitch;
+  static constexpr int kSmem = kRing + kSets * kSteps * 512;  // and the query's fragments
 };
 
 // Beginning and finishing a unit costs a block about as much as kOver tiles: the list that the
@@ -280,7 +287,7 @@ constexpr int kOver = 4;
 // A tile's place in that list: `at`, of sequence b, unit u, tile of the unit's nt.
 struct Cursor {
   int b, u, kv, hg, tile, nt, len, lo, first;
-  long long at;
+  int at;
 };
 
 __device__ __forceinline__ void cursor_seq(const AttendParams& p, int keys, Cursor& c) {
@@ -316,9 +323,8 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
   using G = Tiled<T, DP, kFull>;
   using M = typename G::M;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ long long s_sum[G::kWarps], s_rest[G::kWarps];
-  __shared__ long long s_off;
-  __shared__ int s_b;
+  __shared__ int s_sum[G::kWarps], s_rest[G::kWarps];
+  __shared__ int s_b, s_off;
   __shared__ float s_m[G::kWarps][8], s_l[G::kWarps][8], s_mult[8];
   __shared__ uint32_t s_ok[G::kWarps][G::kStages];
   const KvView& c = p.c;
@@ -329,42 +335,41 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
   // 16-byte chunks xored by the key; others with a pitch of an odd number of chunks. Both keep
   // ldmatrix free of bank conflicts.
   const int pad_chunks = (chunks + 1) & ~1;  // the MMAs read whole steps of 32 bytes
-  const bool swz = kFull ? G::kSwz : (row_bytes & 127) == 0 || 16 * (pad_chunks + 1) > G::kRowMax;
+  const bool swz = kFull ? G::kSwz : (row_bytes & 127) == 0 || 16 * (pad_chunks + 1) > G::kPitch;
   const int pitch = swz ? (row_bytes + 127) & ~127 : 16 * (pad_chunks + 1);
   // offset of chunk ch + x of row r, x a constant of a loop whose bits ch leaves clear
   auto chunk_at = [&](int r, int ch, int x) -> uint32_t {
     if constexpr (kFull && G::kSwz) return (r * pitch + ((ch ^ (r & 7)) << 4) ^ ((x & 7) << 4)) + (x >> 3) * 128;
     else return r * pitch + ((swz ? (ch + x) ^ (r & 7) : ch + x) << 4);
   };
-  uint8_t* const ring = smem + w * (G::kStages * 32 * pitch);
+  uint8_t* const ring = smem + w * (G::kStages * G::kSub * 32 * pitch);
   const uint32_t ring_addr = pipe::smem_u32(ring);
   uint4* const sq = reinterpret_cast<uint4*>(smem + G::kRing);
-  float* const so = reinterpret_cast<float*>(smem + G::kRing + G::kSmemQ);
 
   asm volatile("griddepcontrol.launch_dependents;");
   if (pad_chunks != chunks) {  // columns that no copy writes
-    for (int i = lane; i < G::kStages * 32; i += 32)
+    for (int i = lane; i < G::kStages * G::kSub * 32; i += 32)
       *reinterpret_cast<uint4*>(ring + i * pitch + ((swz ? chunks ^ (i & 7) : chunks) << 4)) = make_uint4(0, 0, 0, 0);
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // This block's run of the list: all units' places, then the sequence that the run begins in.
   // With no more sequences than threads both come from one reading of the lengths.
-  auto places = [&](int b) -> long long {
+  auto places = [&](int b) {
     if (b >= c.num_seqs) return 0;
     Cursor s;
     s.b = b;
     cursor_seq(p, G::kKeys, s);
-    return static_cast<long long>(s.nt + kOver) * p.units;
+    return (s.nt + kOver) * p.units;
   };
-  long long mine = places(tid), scan = mine, rest = 0;
+  int mine = places(tid), scan = mine, rest = 0;
   for (int b = tid + G::kThreads; b < c.num_seqs; b += G::kThreads) rest += places(b);
   if (blockIdx.x == 0)
     for (int b = tid; b < c.num_seqs; b += G::kThreads)
       if (c.lens[b] < 0 || c.lens[b] > c.max_slots) atomicCAS(c.err, 0, kKvErrSlot);
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, scan, o);
+    const int y = __shfl_up_sync(0xffffffffu, scan, o);
     if (lane >= o) scan += y;
   }
 #pragma unroll
@@ -372,7 +377,7 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
   if (lane == 31) s_sum[w] = scan;
   if (lane == 0) s_rest[w] = rest;
   __syncthreads();
-  long long before = 0, chunk = 0, total = 0;
+  int before = 0, chunk = 0, total = 0;
 #pragma unroll
   for (int i = 0; i < G::kWarps; ++i) {
     if (i < w) before += s_sum[i];
@@ -382,25 +387,26 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
   total += chunk;
   // A unit cut into P runs costs about P / 14 tiles of joining: runs are at least
   // as long as balances that, and never empty.
-  const float tiles = static_cast<float>(total) / static_cast<float>(static_cast<long long>(c.num_seqs) * p.units);
+  const float tiles = static_cast<float>(total) / static_cast<float>(c.num_seqs * p.units);
   const int shortest = max(1, static_cast<int>(sqrtf(tiles * (1.0f / 14.0f))));
-  const long long n_cta = max(1ll, min(static_cast<long long>(gridDim.x), total / shortest));
-  auto run_start = [&](long long i) { return i * total / n_cta; };
-  if (blockIdx.x >= n_cta) return;
-  const long long t0 = run_start(blockIdx.x), t1 = run_start(blockIdx.x + 1);
-  for (long long base = 0, acc = 0;;) {
-    const long long end = acc + before + scan;  // of this thread's sequence
+  const int n_cta = max(1, min(static_cast<int>(gridDim.x), total / shortest));
+  const int rank = blockIdx.x;
+  if (rank >= n_cta) return;
+  const int t0 = static_cast<int>(static_cast<int64_t>(rank) * total / n_cta);
+  const int t1 = static_cast<int>(static_cast<int64_t>(rank + 1) * total / n_cta);
+  for (int base = 0, acc = 0;;) {
+    const int end = acc + before + scan;  // of this thread's sequence
     if (end - mine <= t0 && t0 < end) {
-      s_b = static_cast<int>(base) + tid;
+      s_b = base + tid;
       s_off = t0 - (end - mine);
     }
     acc += chunk;
     if (t0 < acc) break;
     base += G::kThreads;
-    mine = scan = places(static_cast<int>(base) + tid);
+    mine = scan = places(base + tid);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, scan, o);
+      const int y = __shfl_up_sync(0xffffffffu, scan, o);
       if (lane >= o) scan += y;
     }
     __syncthreads();
@@ -417,8 +423,8 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
   Cursor cur;
   cur.b = s_b;
   cursor_seq(p, G::kKeys, cur);
-  cur.u = static_cast<int>(s_off / (cur.nt + kOver));
-  cur.tile = static_cast<int>(s_off - static_cast<long long>(cur.u) * (cur.nt + kOver)) - kOver;
+  cur.u = s_off / (cur.nt + kOver);
+  cur.tile = s_off - cur.u * (cur.nt + kOver) - kOver;
   cur.kv = cur.u / p.head_groups;
   cur.hg = cur.u - cur.kv * p.head_groups;
   cur.at = t0;
@@ -428,85 +434,99 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
   }
   Cursor nxt = cur;
 
-  // Copies the warp's 16 keys and values of the tile at `nxt`; rows that the mask leaves out are
+  // Copies the warp's keys and values of the tile at `nxt`; rows that the mask leaves out are
   // zeros (their contents, even NaN, must not reach the sums).
   const bool one_page = c.page_size % 16 == 0 && !(p.a.window > 0 && c.positions);
+  constexpr int kRows = 32 / G::kLanes;  // rows copied at a time
+  const int lr = lane / G::kLanes, lc = lane % G::kLanes;
+  auto page_of = [&](int j, int& in) {
+    const int slot_page = p.page_shift >= 0 ? j >> p.page_shift : j / c.page_size;
+    in = j - slot_page * c.page_size;
+    return c.table[nxt.b * c.table_stride + slot_page];
+  };
+  auto offset = [](const KvBytes& s, int page, int in, int kv) {  // 32 x 32 -> 64 bit products
+    return static_cast<uint64_t>(static_cast<uint32_t>(page)) * s.page + static_cast<uint64_t>(static_cast<uint32_t>(in)) * s.slot +
+           static_cast<uint64_t>(static_cast<uint32_t>(kv)) * s.head;
+  };
   auto issue = [&](int stage) {
     if (nxt.at < t1) {
-      const int kv = nxt.kv, j0 = (nxt.first + nxt.tile) * G::kKeys + 16 * w;
-      const uint32_t dst = ring_addr + stage * 32 * pitch;
-      constexpr int kRows = 32 / G::kLanes;  // rows copied at a time
-      const int lr = lane / G::kLanes, lc = lane % G::kLanes;
-      uint32_t okm;
-      if (one_page) {
-        // the 16 slots lie in one page, and their rows a stride apart
-        const int from = min(max(nxt.lo - j0, 0), 16), to = min(max(nxt.len - j0, 0), 16);
-        okm = ((1u << to) - 1u) & ~((1u << from) - 1u);
-        int page = 0, in = 0;
-        if (okm != 0) {
-          const int slot_page = p.page_shift >= 0 ? j0 >> p.page_shift : j0 / c.page_size;
-          page = c.table[nxt.b * c.table_stride + slot_page];
-          in = j0 - slot_page * c.page_size;
-          if (page < 0 || page >= c.num_pages) {
-            if (lane == 0) atomicCAS(c.err, 0, kKvErrPage);
-            page = in = 0;
-            okm = 0;
-          }
-        }
-        const uint8_t* ks = c.k.base + (page * c.k.page + (in + lr) * c.k.slot + kv * c.k.head) * static_cast<int64_t>(sizeof(T)) + 16 * lc;
-        const uint8_t* vs = c.v.base + (page * c.v.page + (in + lr) * c.v.slot + kv * c.v.head) * static_cast<int64_t>(sizeof(T)) + 16 * lc;
-        const int64_t kstep = c.k.slot * (kRows * static_cast<int64_t>(sizeof(T))), vstep = c.v.slot * (kRows * static_cast<int64_t>(sizeof(T)));
+      uint32_t ok_all = 0;
 #pragma unroll
-        for (int r0 = 0; r0 < 16; r0 += kRows) {
-          const int n = (okm >> (r0 + lr)) & 1 ? 16 : 0;
-#pragma unroll
-          for (int x = 0; x < G::kRow / 16; x += G::kLanes) {
-            if (kFull || x + lc < chunks) {
-              uint32_t at;
-              if constexpr (kFull && G::kSwz) at = (r0 + lr) * pitch + (((lc ^ lr) ^ (r0 & 7)) << 4) + 16 * x;
-              else at = (r0 + lr) * pitch + ((swz ? (x + lc) ^ ((r0 + lr) & 7) : x + lc) << 4);
-              cp16(dst + at, ks + 16 * x, n);
-              cp16(dst + 16 * pitch + at, vs + 16 * x, n);
+      for (int sb = 0; sb < G::kSub; ++sb) {
+        const int j0 = (nxt.first + nxt.tile) * G::kKeys + 16 * (G::kSub * w + sb);
+        const uint32_t dst = ring_addr + (stage * G::kSub + sb) * 32 * pitch;
+        uint32_t okm;
+        if (one_page) {
+          // the 16 slots lie in one page, and their rows a stride apart
+          const int from = min(max(nxt.lo - j0, 0), 16), to = min(max(nxt.len - j0, 0), 16);
+          okm = ((1u << to) - 1u) & ~((1u << from) - 1u);
+          int page = 0, in = 0;
+          if (okm != 0) {
+            page = page_of(j0, in);
+            if (page < 0 || page >= c.num_pages) {
+              if (lane == 0) atomicCAS(c.err, 0, kKvErrPage);
+              page = in = 0;
+              okm = 0;
             }
           }
-          ks += kstep;
-          vs += vstep;
-        }
-      } else {
-        const int j = j0 + (lane & 15);
-        bool ok = j >= nxt.lo && j < nxt.len;
-        int64_t koff = 0, voff = 0;
-        if (ok) {
-          const int slot_page = p.page_shift >= 0 ? j >> p.page_shift : j / c.page_size;
-          const int page = c.table[nxt.b * c.table_stride + slot_page];
-          const int in = j - slot_page * c.page_size;
-          if (p.a.window > 0 && c.positions) {
-            const int64_t rec = (static_cast<int64_t>(nxt.b) * c.num_kv + kv) * c.max_slots + j;
-            ok = c.positions[rec] > c.seen[nxt.b] - 1 - p.a.window;
-          }
-          if (page < 0 || page >= c.num_pages) {
-            atomicCAS(c.err, 0, kKvErrPage);
-            ok = false;
-          }
-          if (ok) {
-            koff = (page * c.k.page + in * c.k.slot + kv * c.k.head) * static_cast<int64_t>(sizeof(T));
-            voff = (page * c.v.page + in * c.v.slot + kv * c.v.head) * static_cast<int64_t>(sizeof(T));
-          }
-        }
-        okm = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+          const uint64_t ko = offset(p.kb, page, in + lr, nxt.kv);
+          const uint8_t* ks = c.k.base + ko + 16 * lc;
+          const uint8_t* vs = c.v.base + (p.same ? ko : offset(p.vb, page, in + lr, nxt.kv)) + 16 * lc;
 #pragma unroll
-        for (int r0 = 0; r0 < 16; r0 += kRows) {
-          const int r = r0 + lr;
-          const int64_t ko = __shfl_sync(0xffffffffu, koff, r), vo = __shfl_sync(0xffffffffu, voff, r);
-          const int n = (okm >> r) & 1 ? 16 : 0;
-          for (int ch = lc; ch < chunks; ch += G::kLanes) {
-            const uint32_t at = r * pitch + ((swz ? ch ^ (r & 7) : ch) << 4);
-            cp16(dst + at, c.k.base + ko + 16 * ch, n);
-            cp16(dst + 16 * pitch + at, c.v.base + vo + 16 * ch, n);
+          for (int r0 = 0; r0 < 16; r0 += kRows) {
+            const int n = (okm >> (r0 + lr)) & 1 ? 16 : 0;
+#pragma unroll
+            for (int x = 0; x < G::kRow / 16; x += G::kLanes) {
+              if (((kFull && G::kRow / 16 - x >= G::kLanes)) || x + lc < chunks) {
+                uint32_t at;
+                if constexpr (kFull && G::kSwz) at = (r0 + lr) * pitch + (((lc ^ lr) ^ (r0 & 7)) << 4) + 16 * x;
+                else at = (r0 + lr) * pitch + ((swz ? (x + lc) ^ ((r0 + lr) & 7) : x + lc) << 4);
+                cp16(dst + at, ks + 16 * x, n);
+                cp16(dst + 16 * pitch + at, vs + 16 * x, n);
+              }
+            }
+            ks += static_cast<uint64_t>(p.kb.slot) * kRows;
+            vs += static_cast<uint64_t>(p.vb.slot) * kRows;
+          }
+        } else {
+          const int j = j0 + (lane & 15);
+          bool ok = j >= nxt.lo && j < nxt.len;
+          uint64_t ko = 0, vo = 0;
+          if (ok) {
+            int in;
+            const int page = page_of(j, in);
+            if (p.a.window > 0 && c.positions) {
+              const int64_t rec = (static_cast<int64_t>(nxt.b) * c.num_kv + nxt.kv) * c.max_slots + j;
+              ok = c.positions[rec] > c.seen[nxt.b] - 1 - p.a.window;
+            }
+            if (page < 0 || page >= c.num_pages) {
+              atomicCAS(c.err, 0, kKvErrPage);
+              ok = false;
+            }
+            if (ok) {
+              ko = offset(p.kb, page, in, nxt.kv);
+              vo = p.same ? ko : offset(p.vb, page, in, nxt.kv);
+            }
+          }
+          okm = __ballot_sync(0xffffffffu, ok) & 0xffffu;
+#pragma unroll
+          for (int r0 = 0; r0 < 16; r0 += kRows) {
+            const int r = r0 + lr;
+            const uint64_t kr = __shfl_sync(0xffffffffu, ko, r), vr = p.same ? kr : __shfl_sync(0xffffffffu, vo, r);
+            const int n = (okm >> r) & 1 ? 16 : 0;
+#pragma unroll
+            for (int x = 0; x < G::kRow / 16; x += G::kLanes) {
+              if (x + lc < chunks) {
+                const uint32_t at = r * pitch + ((swz ? (x + lc) ^ (r & 7) : x + lc) << 4);
+                cp16(dst + at, c.k.base + kr + 16 * (x + lc), n);
+                cp16(dst + 16 * pitch + at, c.v.base + vr + 16 * (x + lc), n);
+              }
+            }
           }
         }
+        ok_all |= okm << (16 * sb);
       }
-      if (lane == 0) s_ok[w][stage] = okm;
+      if (lane == 0) s_ok[w][stage] = ok_all;
       cursor_next(p, G::kKeys, nxt);
     }
     cp_commit();
@@ -518,9 +538,11 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
   float m = -INFINITY, l = 0.0f, mult = 0.0f, slope = 0.0f;
   int stage = 0, q_pos = 0;
   bool fresh = true;  // the unit's query is not in shared memory yet
-  long long unit_start = 0;
+  int unit_start = 0;
 
   while (cur.at < t1) {
+    __syncwarp();  // the slot of the tile before has been read by every lane
+    issue(stage == 0 ? G::kStages - 1 : stage - 1);
     const int kv = cur.kv, h0 = 8 * cur.hg;
     const int heads = p.group - h0 < 8 ? p.group - h0 : 8;  // of this unit
     const int head = kv * p.group + h0;                      // the first of them
@@ -536,64 +558,68 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
       l = 0.0f;
       const float* q = p.a.q + cur.b * p.a.q_ld + static_cast<int64_t>(head) * D;
       const float base = p.a.scale * c.k_scale * kLog2e;
-      if constexpr (G::kF32 || G::kBF16) {
-        if (tid < 8) s_mult[tid] = base;
-      } else {
+      // kPer threads a head, each with its share of the head's fragments
+      constexpr int kPer = G::kThreads / 8, kVals = G::kF32 ? 2 : 4, kEnt = (G::kSteps * 4 + kPer - 1) / kPer;
+      const int h = tid / kPer;
+      float v[kEnt][kVals];
+      float mx = 0.0f;
+#pragma unroll
+      for (int x = 0; x < kEnt; ++x) {
+        const int i = tid % kPer + x * kPer, step = i >> 2, tt = i & 3;
+#pragma unroll
+        for (int y = 0; y < kVals; ++y) {
+          const int d = G::kF32 ? 8 * step + tt + 4 * y : 16 * step + (G::kFP8 ? 4 * tt + y : 2 * tt + (y & 1) + 8 * (y >> 1));
+          v[x][y] = h < heads && d < D ? q[h * D + d] : 0.0f;
+          mx = fmaxf(mx, fabsf(v[x][y]));
+        }
+      }
+      float f = 1.0f;
+      if constexpr (!G::kF32 && !G::kBF16) {
         // a power of two that brings the head's largest |q| to [2^13, 2^14)
-        constexpr int kPer = G::kThreads / 8;
-        const int h = tid / kPer;
-        float mx = 0.0f;
-        if (h < heads)
-          for (int d = tid % kPer; d < D; d += kPer) mx = fmaxf(mx, fabsf(q[h * D + d]));
 #pragma unroll
         for (int x = kPer / 2; x > 0; x >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, x));
-        int e = 0;
-        if (mx > 0.0f && mx < INFINITY) e = min(126, max(-126, 13 - ilogbf(mx)));
-        if (tid % kPer == 0) {
-          s_mult[h] = ldexpf(1.0f, e);
-        }
+        if (mx > 0.0f && mx < INFINITY) f = ldexpf(1.0f, min(126, 13 - ilogbf(mx)));
+        if (tid % kPer == 0) s_mult[h] = f;
       }
-      __syncthreads();
-      for (int i = tid; i < G::kSteps * 32; i += G::kThreads) {
-        const int step = i >> 5, gg = (i & 31) >> 2, tt = i & 3;
-        auto value = [&](int d) { return gg < heads && d < D ? q[gg * D + d] : 0.0f; };
+#pragma unroll
+      for (int x = 0; x < kEnt; ++x) {
+        const int i = tid % kPer + x * kPer;
+        if (i >= G::kSteps * 4) break;
+        const int at = (i >> 2) * 32 + 4 * h + (i & 3);
         if constexpr (G::kF32) {
           uint32_t a[4];
-          tf32_parts(value(8 * step + tt), a[0], a[1]);
-          tf32_parts(value(8 * step + 4 + tt), a[2], a[3]);
-          sq[i] = make_uint4(a[0], a[1], a[2], a[3]);
+          tf32_parts(v[x][0], a[0], a[1]);
+          tf32_parts(v[x][1], a[2], a[3]);
+          sq[at] = make_uint4(a[0], a[1], a[2], a[3]);
+        } else if constexpr (G::kBF16) {
+          uint32_t lo[3], hi[3];
+          parts3(v[x][0], v[x][1], lo);
+          parts3(v[x][2], v[x][3], hi);
+          sq[at] = make_uint4(lo[0], lo[1], hi[0], hi[1]);
+          sq[G::kSteps * 32 + at] = make_uint4(lo[2], 0u, hi[2], 0u);
         } else {
-          const int d0 = 16 * step + (G::kFP8 ? 4 * tt : 2 * tt), d1 = d0 + (G::kFP8 ? 2 : 8);
-          if constexpr (G::kBF16) {
-            uint32_t x[3], y[3];
-            parts3(value(d0), value(d0 + 1), x);
-            parts3(value(d1), value(d1 + 1), y);
-            sq[i] = make_uint4(x[0], x[1], y[0], y[1]);
-            sq[G::kSteps * 32 + i] = make_uint4(x[2], 0u, y[2], 0u);
-          } else {
-            const float f = s_mult[gg];
-            uint32_t x[2], y[2];
-            parts2(value(d0) * f, value(d0 + 1) * f, x);
-            parts2(value(d1) * f, value(d1 + 1) * f, y);
-            sq[i] = make_uint4(x[0], x[1], y[0], y[1]);
-          }
+          uint32_t lo[2], hi[2];
+          parts2(v[x][0] * f, v[x][1] * f, lo);
+          parts2(v[x][2] * f, v[x][3] * f, hi);
+          sq[at] = make_uint4(lo[0], lo[1], hi[0], hi[1]);
         }
       }
+      __syncthreads();
       mult = G::kF32 || G::kBF16 ? base : base / s_mult[g];
       slope = p.a.alibi ? alibi_slope(head + g, c.num_heads) * kLog2e : 0.0f;
-      __syncthreads();
     }
 
-    cp_wait<G::kStages - 2>();
+    cp_wait<G::kStages - 1>();
     __syncwarp();
-    const uint32_t kbase = ring_addr + stage * 32 * pitch, vbase = kbase + 16 * pitch;
+    const uint32_t kbase = ring_addr + stage * G::kSub * 32 * pitch, vbase = kbase + 16 * pitch;
     const uint32_t okm = s_ok[w][stage];
-    const int j0 = (cur.first + cur.tile) * G::kKeys + 16 * w;
+    const int j0 = (cur.first + cur.tile) * G::kKeys + 16 * G::kSub * w;
+    constexpr int kN = 2 * G::kSub;  // blocks of eight keys
 
     // scores of keys j0 + 8 n + 2 t + e for head g
-    float s[2][4];
+    float s[kN][4];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < kN; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
     if constexpr (G::kF32) {
@@ -604,10 +630,10 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
           *reinterpret_cast<uint4*>(a0) = sq[st * 32 + lane];
           *reinterpret_cast<uint4*>(a1) = sq[(st + 1) * 32 + lane];
 #pragma unroll
-          for (int n = 0; n < 2; ++n) {
+          for (int n = 0; n < kN; ++n) {
             // four chunks (16 dims) of eight keys
             uint32_t k[4], hi[4], lo[4];
-            ldsm4(k, kbase + chunk_at(8 * n + (lane & 7), lane >> 3, 2 * st));
+            ldsm4(k, kbase + (n >> 1) * 32 * pitch + chunk_at(8 * (n & 1) + (lane & 7), lane >> 3, 2 * st));
 #pragma unroll
             for (int e = 0; e < 4; ++e) tf32_parts(__uint_as_float(k[e]), hi[e], lo[e]);
             mma(M(), s[n], a0, hi[0], hi[1]);
@@ -623,16 +649,18 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
 #pragma unroll
       for (int st = 0; st < G::kSteps; st += 2) {
         if (16 * st < D) {
-          uint32_t k[4];
-          ldsm4(k, kbase + chunk_at(8 * ((lane >> 3) & 1) + (lane & 7), lane >> 4, st));
+          uint32_t k[G::kSub][4];
+#pragma unroll
+          for (int sb = 0; sb < G::kSub; ++sb)
+            ldsm4(k[sb], kbase + sb * 32 * pitch + chunk_at(8 * ((lane >> 3) & 1) + (lane & 7), lane >> 4, st));
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             uint32_t a[4];
             *reinterpret_cast<uint4*>(a) = sq[(st + x) * 32 + lane];
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
+            for (int n = 0; n < kN; ++n) {
               uint32_t b0, b1;
-              e4m3_pairs(k[2 * x + n], b0, b1);
+              e4m3_pairs(k[n >> 1][2 * x + (n & 1)], b0, b1);
               mma(M(), s[n], a, b0, b1);
             }
           }
@@ -642,36 +670,38 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
 #pragma unroll
       for (int st = 0; st < G::kSteps; ++st) {
         if (16 * st < D) {
-          uint32_t k[4];
-          ldsm4(k, kbase + chunk_at(8 * (lane >> 4) + (lane & 7), (lane >> 3) & 1, 2 * st));
+          uint32_t k[G::kSub][4];
+#pragma unroll
+          for (int sb = 0; sb < G::kSub; ++sb)
+            ldsm4(k[sb], kbase + sb * 32 * pitch + chunk_at(8 * (lane >> 4) + (lane & 7), (lane >> 3) & 1, 2 * st));
 #pragma unroll
           for (int x = 0; x < G::kSets; ++x) {
             uint32_t a[4];
             *reinterpret_cast<uint4*>(a) = sq[(x * G::kSteps + st) * 32 + lane];
-            mma(M(), s[0], a, k[0], k[1]);
-            mma(M(), s[1], a, k[2], k[3]);
+#pragma unroll
+            for (int n = 0; n < kN; ++n) mma(M(), s[n], a, k[n >> 1][2 * (n & 1)], k[n >> 1][2 * (n & 1) + 1]);
           }
         }
       }
     }
-    float z[2][2];
+    float z[kN][2];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < kN; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) z[n][e] = (s[n][e] + s[n][e + 2]) * mult;
     if (p.a.alibi) {
       const int32_t* pos = c.positions ? c.positions + (static_cast<int64_t>(cur.b) * c.num_kv + kv) * c.max_slots : nullptr;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < kN; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int i = 8 * n + 2 * t + e;
           if ((okm >> i) & 1) z[n][e] -= slope * static_cast<float>(q_pos - (pos ? pos[j0 + i] : j0 + i));
         }
     }
-    if (okm != 0xffffu) {
+    if (okm != (G::kSub == 2 ? 0xffffffffu : 0xffffu)) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < kN; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           if (!((okm >> (8 * n + 2 * t + e)) & 1)) z[n][e] = -INFINITY;
@@ -679,12 +709,14 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
     if (p.a.accumulate && g < heads) {
       float* sc = p.scores + (static_cast<int64_t>(cur.b) * c.num_heads + head + g) * c.max_slots + j0;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int n = 0; n < kN; ++n)
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           if (j0 + 8 * n + 2 * t + e < cur.len) sc[8 * n + 2 * t + e] = z[n][e];
     }
-    float mx = fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[1][0], z[1][1]));
+    float mx = fmaxf(z[0][0], z[0][1]);
+#pragma unroll
+    for (int n = 1; n < kN; ++n) mx = fmaxf(mx, fmaxf(z[n][0], z[n][1]));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     if (__any_sync(0xffffffffu, mx > m)) {
@@ -698,9 +730,9 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
       m = m_new;
     }
     const float ref = (m == -INFINITY ? 0.0f : m) - G::kBias;
-    float pw[2][2];
+    float pw[kN][2];
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+    for (int n = 0; n < kN; ++n)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         pw[n][e] = exp2_fast(z[n][e] - ref);
@@ -710,16 +742,17 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
     // o += weights . values
     if constexpr (G::kF32) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+      for (int n = 0; n < kN; ++n) {
         uint32_t a[4];  // k index t is key 2 t, t + 4 is key 2 t + 1
         tf32_parts(pw[n][0], a[0], a[1]);
         tf32_parts(pw[n][1], a[2], a[3]);
-        const int r0 = 8 * n + 2 * t, r1 = r0 + 1;
+        const int r0 = 8 * (n & 1) + 2 * t, r1 = r0 + 1;
+        const uint32_t vb = vbase + (n >> 1) * 32 * pitch;
 #pragma unroll
         for (int i = 0; i < DP / 8; ++i) {
           if (8 * i < D) {
-            const float v0 = __uint_as_float(lds32(vbase + chunk_at(r0, g >> 2, 2 * i) + 4 * (g & 3)));
-            const float v1 = __uint_as_float(lds32(vbase + chunk_at(r1, g >> 2, 2 * i) + 4 * (g & 3)));
+            const float v0 = __uint_as_float(lds32(vb + chunk_at(r0, g >> 2, 2 * i) + 4 * (g & 3)));
+            const float v1 = __uint_as_float(lds32(vb + chunk_at(r1, g >> 2, 2 * i) + 4 * (g & 3)));
             uint32_t h0, l0, h1, l1;
             tf32_parts(v0, h0, l0);
             tf32_parts(v1, h1, l1);
@@ -729,113 +762,132 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
         }
       }
     } else {
-      uint32_t a[G::kSets][4];
-      if constexpr (G::kBF16) {
-        uint32_t x[3], y[3];
-        parts3(pw[0][0], pw[0][1], x);
-        parts3(pw[1][0], pw[1][1], y);
-        a[0][0] = x[0]; a[0][1] = x[1]; a[0][2] = y[0]; a[0][3] = y[1];
-        a[1][0] = x[2]; a[1][1] = 0u; a[1][2] = y[2]; a[1][3] = 0u;
-      } else {
-        uint32_t x[2], y[2];
-        parts2(pw[0][0], pw[0][1], x);
-        parts2(pw[1][0], pw[1][1], y);
-        a[0][0] = x[0]; a[0][1] = x[1]; a[0][2] = y[0]; a[0][3] = y[1];
-      }
-      const int r = 8 * ((lane >> 3) & 1) + (lane & 7);
 #pragma unroll
-      for (int i = 0; i < DP / 8; i += G::kFP8 ? 4 : 2) {
-        if (8 * i < D) {
-          uint32_t v[4];
-          ldsm4t(v, vbase + chunk_at(r, lane >> 4, G::kFP8 ? i / 2 : i));
-          if constexpr (G::kFP8) {
-            // a register holds dims 2 g, 2 g + 1 of keys 2 t, 2 t + 1: regroup the bytes by dim
+      for (int sb = 0; sb < G::kSub; ++sb) {
+        const float(&p0)[2] = pw[2 * sb], (&p1)[2] = pw[2 * sb + 1];
+        const uint32_t vb = vbase + sb * 32 * pitch;
+        uint32_t a[G::kSets][4];
+        if constexpr (G::kBF16) {
+          uint32_t x[3], y[3];
+          parts3(p0[0], p0[1], x);
+          parts3(p1[0], p1[1], y);
+          a[0][0] = x[0]; a[0][1] = x[1]; a[0][2] = y[0]; a[0][3] = y[1];
+          a[1][0] = x[2]; a[1][1] = 0u; a[1][2] = y[2]; a[1][3] = 0u;
+        } else {
+          uint32_t x[2], y[2];
+          parts2(p0[0], p0[1], x);
+          parts2(p1[0], p1[1], y);
+          a[0][0] = x[0]; a[0][1] = x[1]; a[0][2] = y[0]; a[0][3] = y[1];
+        }
+        const int r = 8 * ((lane >> 3) & 1) + (lane & 7);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              uint32_t e0, o0, e1, o1;
-              e4m3_pairs(__byte_perm(v[2 * x], 0, 0x3120), e0, o0);
-              e4m3_pairs(__byte_perm(v[2 * x + 1], 0, 0x3120), e1, o1);
-              mma(M(), o[i + 2 * x], a[0], e0, e1);
-              mma(M(), o[i + 2 * x + 1], a[0], o0, o1);
-            }
-          } else {
+        for (int i = 0; i < DP / 8; i += G::kFP8 ? 4 : 2) {
+          if (8 * i < D) {
+            uint32_t v[4];
+            ldsm4t(v, vb + chunk_at(r, lane >> 4, G::kFP8 ? i / 2 : i));
+            if constexpr (G::kFP8) {
+              // a register holds dims 2 g, 2 g + 1 of keys 2 t, 2 t + 1: regroup the bytes by dim
 #pragma unroll
-            for (int x = 0; x < G::kSets; ++x) {
-              mma(M(), o[i], a[x], v[0], v[1]);
-              mma(M(), o[i + 1], a[x], v[2], v[3]);
+              for (int x = 0; x < 2; ++x) {
+                if (i + 2 * x >= DP / 8) break;
+                uint32_t e0, o0, e1, o1;
+                e4m3_pairs(__byte_perm(v[2 * x], 0, 0x3120), e0, o0);
+                e4m3_pairs(__byte_perm(v[2 * x + 1], 0, 0x3120), e1, o1);
+                mma(M(), o[i + 2 * x], a[0], e0, e1);
+                mma(M(), o[i + 2 * x + 1], a[0], o0, o1);
+              }
+            } else {
+#pragma unroll
+              for (int x = 0; x < G::kSets; ++x) {
+                mma(M(), o[i], a[x], v[0], v[1]);
+                mma(M(), o[i + 1], a[x], v[2], v[3]);
+              }
             }
           }
         }
       }
     }
-    __syncwarp();  // the stage is read; its slot can be filled again
-    issue(stage + G::kStages - 1 >= G::kStages ? stage - 1 : stage + G::kStages - 1);
-    stage = stage + 1 == G::kStages ? 0 : stage + 1;
-
     const bool unit_ends = cur.tile + 1 == cur.nt;
     if (unit_ends || cur.at + 1 == t1) {
-      // join the warps: each adds its sums in turn
+      // Join the warps: each leaves its sums in the slot it has just read (rows of D values, turned by
+      // four per head against bank conflicts), then every thread adds the four of its values.
       l += __shfl_xor_sync(0xffffffffu, l, 1);
       l += __shfl_xor_sync(0xffffffffu, l, 2);
       if (t == 0) {
         s_m[w][g] = m;
         s_l[w][g] = l;
       }
-      __syncthreads();
-      float mm = s_m[0][g], ll = 0.0f;
+      uint8_t* const scratch = ring + stage * G::kSub * 32 * pitch;
+      float* const mine = reinterpret_cast<float*>(scratch) + g * D;
+      __syncwarp();
 #pragma unroll
-      for (int i = 1; i < G::kWarps; ++i) mm = fmaxf(mm, s_m[i][g]);
-      const float r = mm == -INFINITY ? 0.0f : mm;
-#pragma unroll
-      for (int i = 0; i < G::kWarps; ++i) ll += s_l[i][g] * exp2f(s_m[i][g] - r);
-      const float f = exp2f(m - r);
-      for (int x = 0; x < G::kWarps; ++x) {
-        if (x == w) {
-#pragma unroll
-          for (int i = 0; i < DP / 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int d = G::kFP8 ? 16 * (i >> 1) + 4 * t + 2 * e + (i & 1) : 8 * i + 2 * t + e;
-              float v = (o[i][e] + o[i][e + 2]) * f;
-              if (w > 0) v += so[g * DP + d];
-              so[g * DP + d] = v;
-            }
+      for (int i = 0; i < DP / 8; i += G::kFP8 ? 2 : 1) {
+        if (8 * i >= D) break;
+        int d = (G::kFP8 ? 8 * i + 4 * t : 8 * i + 2 * t) + 4 * g;
+        if (d >= D) d -= D;
+        const float2 a = make_float2(o[i][0] + o[i][2], o[i][1] + o[i][3]);
+        if constexpr (G::kFP8) {
+          *reinterpret_cast<float4*>(mine + d) = make_float4(a.x, o[i + 1][0] + o[i + 1][2], a.y, o[i + 1][1] + o[i + 1][3]);
+        } else {
+          *reinterpret_cast<float2*>(mine + d) = a;
         }
-        __syncthreads();
       }
-      const int seg = cur.b * p.units + cur.u;
-      float* out = p.a.out + cur.b * p.a.out_ld + static_cast<int64_t>(head) * D;
-      float* lse = p.lse + static_cast<int64_t>(cur.b) * c.num_heads + head;
-      if (t == 0 && w == 0) s_mult[g] = ll;  // reuse: the unit's sum and maximum
-      if (t == 0 && w == 0) s_m[0][g] = mm;
       __syncthreads();
-      if (unit_ends && unit_start >= t0) {
-        for (int i = tid; i < heads * D; i += G::kThreads) {
-          const int h = i / D, d = i - h * D;
-          out[i] = s_mult[h] == 0.0f ? 0.0f : so[h * DP + d] * (c.v_scale / s_mult[h]);
+      const bool whole = unit_ends && unit_start >= t0;
+      float* out = p.a.out + cur.b * p.a.out_ld + static_cast<int64_t>(head) * D;
+      // a block leaves at most two partial units: one that began before its run, one that goes on after it
+      const int stride = D + 4;  // 16-byte rows
+      float* dst = p.part + (2ll * rank + (unit_start >= t0 ? 1 : 0)) * 8 * stride;
+      const int d4 = D / 4;
+      for (int i = tid; i < heads * d4; i += G::kThreads) {
+        const int h = i / d4, d = 4 * (i - h * d4);
+        float mm = s_m[0][h];
+#pragma unroll
+        for (int x = 1; x < G::kWarps; ++x) mm = fmaxf(mm, s_m[x][h]);
+        const float r = mm == -INFINITY ? 0.0f : mm;
+        int at = d + 4 * h;
+        if (at >= D) at -= D;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        float ll = 0.0f;
+#pragma unroll
+        for (int x = 0; x < G::kWarps; ++x) {
+          const float f = exp2f(s_m[x][h] - r);
+          const float4 y = *reinterpret_cast<const float4*>(smem + (x * G::kStages + stage) * (G::kSub * 32 * pitch) + (h * D + at) * 4);
+          v.x += y.x * f;
+          v.y += y.y * f;
+          v.z += y.z * f;
+          v.w += y.w * f;
+          ll += s_l[x][h] * f;
         }
-        if (p.a.accumulate && tid < heads)
-          lse[tid] = s_mult[tid] == 0.0f ? INFINITY : (s_m[0][tid] == -INFINITY ? 0.0f : s_m[0][tid]) - G::kBias + log2f(s_mult[tid]);
-      } else {
-        // a block leaves at most two partial units: one that began before its run, one that goes on after it
-        const int stride = D + 4;  // 16-byte rows
-        float* dst = p.part + (2ll * blockIdx.x + (unit_start >= t0 ? 1 : 0)) * 8 * stride;
-        for (int i = tid; i < heads * D; i += G::kThreads) {
-          const int h = i / D, d = i - h * D;
-          dst[h * stride + d] = so[h * DP + d];
-        }
-        if (tid < heads) {
-          dst[tid * stride + D] = s_m[0][tid];
-          dst[tid * stride + D + 1] = s_mult[tid];
+        if (whole) {
+          const float f = ll == 0.0f ? 0.0f : c.v_scale / ll;
+          float* to = out + h * D + d;
+          to[0] = ll == 0.0f ? 0.0f : v.x * f;
+          to[1] = ll == 0.0f ? 0.0f : v.y * f;
+          to[2] = ll == 0.0f ? 0.0f : v.z * f;
+          to[3] = ll == 0.0f ? 0.0f : v.w * f;
+          if (p.a.accumulate && d == 0)
+            p.lse[static_cast<int64_t>(cur.b) * c.num_heads + head + h] = ll == 0.0f ? INFINITY : r - G::kBias + log2f(ll);
+        } else {
+          *reinterpret_cast<float4*>(dst + h * stride + d) = v;
+          if (d == 0) {
+            dst[h * stride + D] = mm;
+            dst[h * stride + D + 1] = ll;
+          }
         }
       }
       if (unit_start >= t0 && tid == 0) {  // the block that began the unit says where its parts are
-        const long long c1 = ((unit_start + cur.nt) * n_cta - 1) / total;
-        p.spans[seg] = make_int2(static_cast<int>(blockIdx.x), static_cast<int>(c1 - blockIdx.x) + 1);
+        const int last = static_cast<int>((static_cast<int64_t>(unit_start + cur.nt) * n_cta - 1) / total);
+        p.spans[cur.b * p.units + cur.u] = make_int2(rank, last - rank + 1);
       }
-      __syncthreads();  // before the next unit's query replaces what was read here
+      __syncthreads();  // the slots are copies' again, and the next unit's query may come
+      if (pad_chunks != chunks) {
+        for (int i = lane; i < G::kSub * 32; i += 32)
+          *reinterpret_cast<uint4*>(scratch + i * pitch + ((swz ? chunks ^ (i & 7) : chunks) << 4)) = make_uint4(0, 0, 0, 0);
+      }
       fresh = true;
     }
+    stage = stage + 1 == G::kStages ? 0 : stage + 1;
     cursor_next(p, G::kKeys, cur);
   }
   cp_wait<0>();
@@ -919,9 +971,14 @@ int simple_splits(const KvView& v) {
   return s < 1 ? 1 : static_cast<int>(s);
 }
 
-// The tiled form copies rows in 16-byte pieces.
+// The tiled form copies rows in 16-byte pieces and multiplies 32-bit strides and counts.
 bool tiled(const KvView& v, KvType type) {
   const int size = kv_size(type);
+  for (const KvPool& p : {v.k, v.v})
+    for (int64_t s : {p.page, p.slot, p.head})
+      if (s * size > 0xffffffffll) return false;
+  const int64_t units = static_cast<int64_t>(v.num_seqs) * v.num_heads;
+  if (units * (v.max_slots / 64 + 1 + kOver) > 0x7fffffffll) return false;
   return v.head_dim % 8 == 0 && v.head_dim * size % 16 == 0 && pool_aligned(v.k, size, 16) && pool_aligned(v.v, size, 16);
 }
 
@@ -930,6 +987,8 @@ Status by_shape(const KvView& v, KvType type, F&& f) {
   return by_type(type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     if (v.head_dim == 64) return f(Tiled<T, 64, true>{}, k_attend_tiled<T, 64, true>);
+    if (v.head_dim == 80) return f(Tiled<T, 80, true>{}, k_attend_tiled<T, 80, true>);
+    if (v.head_dim == 96) return f(Tiled<T, 96, true>{}, k_attend_tiled<T, 96, true>);
     if (v.head_dim == 128) return f(Tiled<T, 128, true>{}, k_attend_tiled<T, 128, true>);
     if (v.head_dim == 256) return f(Tiled<T, 256, true>{}, k_attend_tiled<T, 256, true>);
     if (v.head_dim < 64) return f(Tiled<T, 64, false>{}, k_attend_tiled<T, 64, false>);
@@ -1000,6 +1059,13 @@ Status kv_attend(KvCache* c, const KvAttendArgs& a, cudaStream_t st) {
   p.spans = reinterpret_cast<int2*>(c->spans);
   const unsigned B = v.num_seqs, H = v.num_heads;
   if (c->attend_tiled) {
+    const int64_t size = kv_size(c->type);
+    auto bytes = [&](const KvPool& q) {
+      return KvBytes{static_cast<uint32_t>(q.page * size), static_cast<uint32_t>(q.slot * size), static_cast<uint32_t>(q.head * size)};
+    };
+    p.kb = bytes(v.k);
+    p.vb = bytes(v.v);
+    p.same = p.kb.page == p.vb.page && p.kb.slot == p.vb.slot && p.kb.head == p.vb.head;
     WB_TRY(by_shape(v, c->type, [&](auto g, auto* kernel) {
       using G = decltype(g);
       WB_TRY(launch_after(kernel, dim3(c->attend_blocks), G::kThreads, G::kSmem, st, p));
