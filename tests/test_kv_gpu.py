@@ -732,3 +732,23 @@ def test_attend_pools_of_different_layout(D):
     D.PagedKV(kp, vp, table, i32([250, 77]), num_heads=8).attend(q, out)
     want, _, bound = attend64(q, kp, vp, table, [250, 77], 128 ** -0.5)
     assert np.all(np.abs(out.cpu().numpy() - want) <= bound)
+
+
+@pytest.mark.parametrize("dim", [33, 66, 64, 130])
+@pytest.mark.parametrize("shift", [0, 1])
+def test_append_rotates_q_in_place(D, dim, shift):
+    """q_out = q, on rows that 16-byte accesses can serve and on rows that they cannot."""
+    import torch
+    rng = np.random.default_rng(dim)
+    n, H, kv, page = 7, 24, 2, 16
+    kp, vp, table = make_cache(rng, "f16", n, 2, page, kv, dim)
+    rows = rng.standard_normal((n, H * dim + shift)).astype(np.float32)
+    g = torch.from_numpy(rows).cuda()[:, shift:]
+    k = torch.zeros((n, kv, dim), device="cuda")
+    pos = np.arange(n) * 1001 + 5
+    c = D.PagedKV(kp, vp, table, i32([3] * n), num_heads=H, seen=i32(pos))
+    c.append(k, k, q=g, q_out=g, theta=10000.0)
+    x = rows[:, shift:].reshape(n, H, dim).astype(np.float64)
+    want = rotate64(x, pos.astype(np.float64), 10000.0)
+    got = g.cpu().numpy().reshape(n, H, dim)
+    assert np.all(np.abs(got - want) <= rotation_bound(x, 10000.0) + EPS * np.abs(want))

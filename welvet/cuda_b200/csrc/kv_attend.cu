@@ -31,10 +31,9 @@ struct AttendParams {
   float* lse;      // [num_seqs][num_heads]
   // tiled form
   int group;       // query heads per key-value head
-  int units;       // num_kv * head groups of 8: work units of a sequence
-  int head_groups;
+  int head_groups; // of eight query heads of a key-value head
   int page_shift;  // log2(page_size), or -1
-  int2* spans;     // [num_seqs][units]: first block and number of blocks of a unit
+  int2* spans;     // [num_seqs][num_kv]: first run and number of runs of a unit
 };
 
 // ---------------------------------------------------------------- one query head a block
@@ -151,20 +150,37 @@ __global__ void k_attend_join(const __grid_constant__ AttendParams p) {
   if (threadIdx.x == 0 && p.a.accumulate) p.lse[static_cast<int64_t>(b) * c.num_heads + h] = l == 0.0f ? INFINITY : ref + log2f(l);
 }
 
-// weights[j] = weights_in[j] + sum over the group's heads of 2^(score - lse), heads in order.
-__global__ void k_attend_weights(const __grid_constant__ AttendParams p) {
+// weights[j] = weights_in[j] + sum over the group's heads of 2^(score - lse), heads in order, for
+// every step-th slot from `first`.
+__device__ __forceinline__ void add_weights(const AttendParams& p, int b, int kv, const float* lse, int first, int step) {
   const KvView& c = p.c;
-  const int kv = blockIdx.y, b = blockIdx.z, group = c.num_heads / c.num_kv;
+  const int group = c.num_heads / c.num_kv;
   int len = c.lens[b];
   len = len < 0 ? 0 : (len > c.max_slots ? c.max_slots : len);
   const int lo = p.a.window > 0 && !c.positions ? len - p.a.window : 0;  // slots below have no score
   const int64_t rec = (static_cast<int64_t>(b) * c.num_kv + kv) * c.max_slots;
-  const int64_t row = static_cast<int64_t>(b) * c.num_heads + kv * group;
-  for (int j = blockIdx.x * blockDim.x + threadIdx.x; j < len; j += gridDim.x * blockDim.x) {
-    float s = p.a.weights_in[rec + j];
-    for (int i = 0; i < group && j >= lo; ++i) s += exp2f(p.scores[(row + i) * c.max_slots + j] - p.lse[row + i]);
-    c.weights[rec + j] = s;
+  const float* scores = p.scores + (static_cast<int64_t>(b) * c.num_heads + kv * group) * c.max_slots;
+  constexpr int kFly = 4;
+  for (int j0 = first; j0 < len; j0 += kFly * step) {
+    float s[kFly];
+#pragma unroll
+    for (int x = 0; x < kFly; ++x) s[x] = j0 + x * step < len ? p.a.weights_in[rec + j0 + x * step] : 0.0f;
+    for (int i = 0; i < group; ++i) {
+#pragma unroll
+      for (int x = 0; x < kFly; ++x) {
+        const int j = j0 + x * step;
+        if (j >= lo && j < len) s[x] += exp2f(scores[static_cast<int64_t>(i) * c.max_slots + j] - lse[i]);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < kFly; ++x)
+      if (j0 + x * step < len) c.weights[rec + j0 + x * step] = s[x];
   }
+}
+
+__global__ void k_attend_weights(const __grid_constant__ AttendParams p) {
+  add_weights(p, blockIdx.z, blockIdx.y, p.lse + static_cast<int64_t>(blockIdx.z) * p.c.num_heads + blockIdx.y * (p.c.num_heads / p.c.num_kv),
+              blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
 }
 
 // ---------------------------------------------------------------- tiled form
@@ -180,10 +196,11 @@ __global__ void k_attend_weights(const __grid_constant__ AttendParams p) {
 // The register-path MMA is used, not tcgen05: with 8 query rows an M = 128 tile would be 94 %
 // padding, and at HBM speed the warp MMAs of a 16-key tile take about a third of its time.
 //
-// Work is cut into tiles of 16 keys per warp; the grid's blocks take equal runs of all tiles of
-// all (sequence, key-value head) units, so that ragged lengths balance. A unit that lies within
-// one block is finished there; otherwise each block leaves its partial (o, m, l) and a second
-// kernel joins them in block order. (Joined by the last block to arrive, behind a counter, one
+// Work is cut into tiles of 16 or 32 keys per warp; the tiles of all (sequence, key-value head) units
+// are cut into equal runs, so that ragged lengths balance. A block takes a run; where a key-value
+// head has more than eight query heads, neighbouring blocks take the same run with eight each, so
+// that the second reads the rows from L2. A unit that lies within one run is finished there;
+// otherwise each run leaves its partial (o, m, l) and a second kernel joins them in run order. (Joined by the last block to arrive, behind a counter, one
 // sequence of 131072 slots took 53 us, the registers of that code among it.)
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -279,14 +296,15 @@ struct Tiled {
   static constexpr int kSmem = kRing + kSets * kSteps * 512;  // and the query's fragments
 };
 
-// Beginning and finishing a unit costs a block about as much as kOver tiles: the list that the
+// Beginning and finishing a unit costs a block about as much as kOver tiles (the ragged batch of 64
+// took 57.6, 53.9, 57.8 and 64.6 us with 1, 2, 4 and 7): the list that the
 // blocks divide has kOver places before each unit's tiles, so that runs of short units (one tile
 // each) get fewer of them.
-constexpr int kOver = 4;
+constexpr int kOver = 2;
 
 // A tile's place in that list: `at`, of sequence b, unit u, tile of the unit's nt.
 struct Cursor {
-  int b, u, kv, hg, tile, nt, len, lo, first;
+  int b, kv, tile, nt, len, lo, first;
   int at;
 };
 
@@ -304,11 +322,8 @@ __device__ __forceinline__ void cursor_next(const AttendParams& p, int keys, Cur
   if (++c.tile < c.nt) return;
   c.tile = 0;
   c.at += kOver;
-  ++c.u;
-  if (++c.hg < p.head_groups) return;
-  c.hg = 0;
   if (++c.kv < p.c.num_kv) return;
-  c.kv = c.u = 0;
+  c.kv = 0;
   if (++c.b < p.c.num_seqs) cursor_seq(p, keys, c);
 }
 
@@ -360,7 +375,7 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
     Cursor s;
     s.b = b;
     cursor_seq(p, G::kKeys, s);
-    return (s.nt + kOver) * p.units;
+    return (s.nt + kOver) * c.num_kv;
   };
   int mine = places(tid), scan = mine, rest = 0;
   for (int b = tid + G::kThreads; b < c.num_seqs; b += G::kThreads) rest += places(b);
@@ -385,15 +400,15 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
     total += s_rest[i];
   }
   total += chunk;
-  // A unit cut into P runs costs about P / 14 tiles of joining: runs are at least
-  // as long as balances that, and never empty.
-  const float tiles = static_cast<float>(total) / static_cast<float>(c.num_seqs * p.units);
-  const int shortest = max(1, static_cast<int>(sqrtf(tiles * (1.0f / 14.0f))));
-  const int n_cta = max(1, min(static_cast<int>(gridDim.x), total / shortest));
-  const int rank = blockIdx.x;
-  if (rank >= n_cta) return;
-  const int t0 = static_cast<int>(static_cast<int64_t>(rank) * total / n_cta);
-  const int t1 = static_cast<int>(static_cast<int64_t>(rank + 1) * total / n_cta);
+  // A unit cut into P runs costs about P / 50 tiles of joining: runs are at least as long as
+  // balances that, and never empty.
+  const float tiles = static_cast<float>(total) / static_cast<float>(c.num_seqs * c.num_kv);
+  const int shortest = max(1, static_cast<int>(sqrtf(tiles * (1.0f / 50.0f))));
+  const int n_runs = max(1, min(static_cast<int>(gridDim.x) / p.head_groups, total / shortest));
+  const int run = blockIdx.x / p.head_groups, hg = blockIdx.x - run * p.head_groups;
+  if (run >= n_runs) return;
+  const int t0 = static_cast<int>(static_cast<int64_t>(run) * total / n_runs);
+  const int t1 = static_cast<int>(static_cast<int64_t>(run + 1) * total / n_runs);
   for (int base = 0, acc = 0;;) {
     const int end = acc + before + scan;  // of this thread's sequence
     if (end - mine <= t0 && t0 < end) {
@@ -423,10 +438,8 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
   Cursor cur;
   cur.b = s_b;
   cursor_seq(p, G::kKeys, cur);
-  cur.u = s_off / (cur.nt + kOver);
-  cur.tile = s_off - cur.u * (cur.nt + kOver) - kOver;
-  cur.kv = cur.u / p.head_groups;
-  cur.hg = cur.u - cur.kv * p.head_groups;
+  cur.kv = s_off / (cur.nt + kOver);
+  cur.tile = s_off - cur.kv * (cur.nt + kOver) - kOver;
   cur.at = t0;
   if (cur.tile < 0) {
     cur.at -= cur.tile;
@@ -543,7 +556,7 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
   while (cur.at < t1) {
     __syncwarp();  // the slot of the tile before has been read by every lane
     issue(stage == 0 ? G::kStages - 1 : stage - 1);
-    const int kv = cur.kv, h0 = 8 * cur.hg;
+    const int kv = cur.kv, h0 = 8 * hg;
     const int heads = p.group - h0 < 8 ? p.group - h0 : 8;  // of this unit
     const int head = kv * p.group + h0;                      // the first of them
     if (fresh) {
@@ -835,9 +848,9 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
       __syncthreads();
       const bool whole = unit_ends && unit_start >= t0;
       float* out = p.a.out + cur.b * p.a.out_ld + static_cast<int64_t>(head) * D;
-      // a block leaves at most two partial units: one that began before its run, one that goes on after it
+      // a run leaves at most two partial units: one that began before it, one that goes on after it
       const int stride = D + 4;  // 16-byte rows
-      float* dst = p.part + (2ll * rank + (unit_start >= t0 ? 1 : 0)) * 8 * stride;
+      float* dst = p.part + (2ll * blockIdx.x + (unit_start >= t0 ? 1 : 0)) * 8 * stride;
       const int d4 = D / 4;
       for (int i = tid; i < heads * d4; i += G::kThreads) {
         const int h = i / d4, d = 4 * (i - h * d4);
@@ -876,9 +889,9 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
           }
         }
       }
-      if (unit_start >= t0 && tid == 0) {  // the block that began the unit says where its parts are
-        const int last = static_cast<int>((static_cast<int64_t>(unit_start + cur.nt) * n_cta - 1) / total);
-        p.spans[cur.b * p.units + cur.u] = make_int2(rank, last - rank + 1);
+      if (unit_start >= t0 && hg == 0 && tid == 0) {  // the run that began the unit says where its parts are
+        const int last = static_cast<int>((static_cast<int64_t>(unit_start + cur.nt) * n_runs - 1) / total);
+        p.spans[cur.b * c.num_kv + kv] = make_int2(run, last - run + 1);
       }
       __syncthreads();  // the slots are copies' again, and the next unit's query may come
       if (pad_chunks != chunks) {
@@ -893,24 +906,52 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
   cp_wait<0>();
 }
 
-// Joins the parts of one (unit, head) in order: the unit's first block left its second slot, the
-// others their first. Four warps take the parts in turn, sums are added in warp order.
+// What is left once all runs are done. Blocks below num_heads join the parts of one query head in
+// order (the unit's first run left its second slot, the others their first; four warps take the
+// parts in turn, sums are added in warp order). The others, with accumulate, add the attention
+// weights of a key-value head's slots; the normalisers of split units they make for themselves.
+constexpr int kMaxGroup = 128;  // query heads of a key-value head that the weights' blocks can hold
+
 template <int kBias>
-__global__ void __launch_bounds__(128) k_attend_join_parts(const __grid_constant__ AttendParams p) {
+__global__ void __launch_bounds__(128) k_attend_finish(const __grid_constant__ AttendParams p) {
   __shared__ float s_o[4][256];
   __shared__ float s_m[4], s_l[4];
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const KvView& c = p.c;
-  const int h = blockIdx.x, b = blockIdx.y, D = c.head_dim, stride = D + 4;
-  const int kv = h / p.group, hg = (h - kv * p.group) >> 3, row = (h - kv * p.group) & 7;
-  const int2 span = p.spans[static_cast<int64_t>(b) * p.units + kv * p.head_groups + hg];
-  if (span.y <= 1) return;
+  const int b = blockIdx.y, D = c.head_dim, stride = D + 4;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const float* first = p.part + (static_cast<int64_t>(span.x) * 2 * 8 + row) * stride;
-  auto part_of = [&](int i) { return first + static_cast<int64_t>(2 * i + (i == 0)) * 8 * stride; };
+  // row of part i of query head r of a key-value head
+  auto part_of = [&](int first_run, int r, int i) {
+    return p.part + ((static_cast<int64_t>(first_run + i) * p.head_groups + (r >> 3)) * 2 + (i == 0)) * 8 * stride + (r & 7) * stride;
+  };
+  if (static_cast<int>(blockIdx.x) >= c.num_heads) {
+    const int at = blockIdx.x - c.num_heads, kv = at % c.num_kv, chunk = at / c.num_kv, chunks = (gridDim.x - c.num_heads) / c.num_kv;
+    const int2 span = p.spans[static_cast<int64_t>(b) * c.num_kv + kv];
+    float* lse = &s_o[0][0];
+    for (int r = w; r < p.group; r += 4) {
+      if (span.y <= 1) {
+        if (lane == 0) lse[r] = p.lse[static_cast<int64_t>(b) * c.num_heads + kv * p.group + r];
+        continue;
+      }
+      float m = -INFINITY, l = 0.0f;
+      for (int i = lane; i < span.y; i += 32) m = fmaxf(m, __ldcg(part_of(span.x, r, i) + D));
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+      const float ref = m == -INFINITY ? 0.0f : m;
+      for (int i = lane; i < span.y; i += 32) l += __ldcg(part_of(span.x, r, i) + D + 1) * exp2f(__ldcg(part_of(span.x, r, i) + D) - ref);
+      l = warp_sum(l);
+      if (lane == 0) lse[r] = l == 0.0f ? INFINITY : ref - kBias + log2f(l);
+    }
+    __syncthreads();
+    add_weights(p, b, kv, lse, chunk * 128 + threadIdx.x, chunks * 128);
+    return;
+  }
+  const int h = blockIdx.x, kv = h / p.group, r = h - kv * p.group;
+  const int2 span = p.spans[static_cast<int64_t>(b) * c.num_kv + kv];
+  if (span.y <= 1) return;
   float m = -INFINITY;
-  for (int i = threadIdx.x; i < span.y; i += 128) m = fmaxf(m, __ldcg(part_of(i) + D));
+  for (int i = threadIdx.x; i < span.y; i += 128) m = fmaxf(m, __ldcg(part_of(span.x, r, i) + D));
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
   if (lane == 0) s_m[w] = m;
@@ -921,20 +962,20 @@ __global__ void __launch_bounds__(128) k_attend_join_parts(const __grid_constant
   float l = 0.0f;
   constexpr int kBatch = 8;
   for (int i0 = w; i0 < span.y; i0 += 4 * kBatch) {
-    float4 r[kBatch][2];
+    float4 row[kBatch][2];
     float f[kBatch], ls[kBatch];
 #pragma unroll
     for (int x = 0; x < kBatch; ++x) {
       const int i = i0 + 4 * x;
       f[x] = ls[x] = 0.0f;
-      r[x][0] = r[x][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      row[x][0] = row[x][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (i < span.y) {
-        const float* src = part_of(i);
+        const float* src = part_of(span.x, r, i);
         f[x] = __ldcg(src + D);
         ls[x] = __ldcg(src + D + 1);
 #pragma unroll
         for (int e = 0; e < 2; ++e)
-          if (4 * lane + 128 * e < D) r[x][e] = __ldcg(reinterpret_cast<const float4*>(src + 4 * lane + 128 * e));
+          if (4 * lane + 128 * e < D) row[x][e] = __ldcg(reinterpret_cast<const float4*>(src + 4 * lane + 128 * e));
       }
     }
 #pragma unroll
@@ -944,10 +985,10 @@ __global__ void __launch_bounds__(128) k_attend_join_parts(const __grid_constant
       l += ls[x] * fx;
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        v[e].x += r[x][e].x * fx;
-        v[e].y += r[x][e].y * fx;
-        v[e].z += r[x][e].z * fx;
-        v[e].w += r[x][e].w * fx;
+        v[e].x += row[x][e].x * fx;
+        v[e].y += row[x][e].y * fx;
+        v[e].z += row[x][e].z * fx;
+        v[e].w += row[x][e].w * fx;
       }
     }
   }
@@ -960,7 +1001,6 @@ __global__ void __launch_bounds__(128) k_attend_join_parts(const __grid_constant
   const float f = l == 0.0f ? 0.0f : c.v_scale / l;
   float* out = p.a.out + b * p.a.out_ld + static_cast<int64_t>(h) * D;
   for (int d = threadIdx.x; d < D; d += 128) out[d] = l == 0.0f ? 0.0f : (s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d]) * f;
-  if (threadIdx.x == 0 && p.a.accumulate) p.lse[static_cast<int64_t>(b) * c.num_heads + h] = l == 0.0f ? INFINITY : ref - kBias + log2f(l);
 }
 
 int simple_splits(const KvView& v) {
@@ -977,8 +1017,9 @@ bool tiled(const KvView& v, KvType type) {
   for (const KvPool& p : {v.k, v.v})
     for (int64_t s : {p.page, p.slot, p.head})
       if (s * size > 0xffffffffll) return false;
-  const int64_t units = static_cast<int64_t>(v.num_seqs) * v.num_heads;
+  const int64_t units = static_cast<int64_t>(v.num_seqs) * v.num_kv;
   if (units * (v.max_slots / 64 + 1 + kOver) > 0x7fffffffll) return false;
+  if (v.num_heads / v.num_kv > kMaxGroup) return false;
   return v.head_dim % 8 == 0 && v.head_dim * size % 16 == 0 && pool_aligned(v.k, size, 16) && pool_aligned(v.v, size, 16);
 }
 
@@ -995,22 +1036,6 @@ Status by_shape(const KvView& v, KvType type, F&& f) {
     if (v.head_dim < 128) return f(Tiled<T, 128, false>{}, k_attend_tiled<T, 128, false>);
     return f(Tiled<T, 256, false>{}, k_attend_tiled<T, 256, false>);
   });
-}
-
-// A launch that may start while the kernel before it still runs (it waits for its results itself).
-template <typename K, typename P>
-Status launch_after(K* kernel, dim3 grid, int threads, int smem, cudaStream_t st, const P& p) {
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p), "kv launch");
 }
 
 int head_groups(const KvView& v) { return (v.num_heads / v.num_kv + 7) / 8; }
@@ -1032,11 +1057,12 @@ Status attend_plan(KvCache* c) {
     WB_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, G::kThreads, G::kSmem));
     WB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c->device));
     if (per_sm < 1) return Status::Internal("kv attend: the kernel does not fit");
-    const int64_t units = static_cast<int64_t>(v.num_kv) * head_groups(v);
-    const int64_t most = v.num_seqs * units * ((v.max_slots + G::kKeys - 1) / G::kKeys);
-    c->attend_blocks = static_cast<int>(std::min<int64_t>(static_cast<int64_t>(per_sm) * sms, most));
+    const int64_t units = static_cast<int64_t>(v.num_seqs) * v.num_kv;
+    const int64_t most = units * ((v.max_slots + G::kKeys - 1) / G::kKeys + kOver);
+    const int hg = head_groups(v);
+    c->attend_blocks = static_cast<int>(std::min<int64_t>(std::max(1, per_sm * sms / hg), most)) * hg;
     c->part_bytes = static_cast<size_t>(c->attend_blocks) * 2 * 8 * (v.head_dim + 4) * 4;
-    c->span_bytes = static_cast<size_t>(v.num_seqs) * units * 8;
+    c->span_bytes = static_cast<size_t>(units) * 8;
     return Status::Ok();
   });
 }
@@ -1054,7 +1080,6 @@ Status kv_attend(KvCache* c, const KvAttendArgs& a, cudaStream_t st) {
   p.lse = c->lse;
   p.group = v.num_heads / v.num_kv;
   p.head_groups = head_groups(v);
-  p.units = v.num_kv * p.head_groups;
   p.page_shift = (v.page_size & (v.page_size - 1)) == 0 ? 31 - __builtin_clz(v.page_size) : -1;
   p.spans = reinterpret_cast<int2*>(c->spans);
   const unsigned B = v.num_seqs, H = v.num_heads;
@@ -1070,8 +1095,9 @@ Status kv_attend(KvCache* c, const KvAttendArgs& a, cudaStream_t st) {
       using G = decltype(g);
       WB_TRY(launch_after(kernel, dim3(c->attend_blocks), G::kThreads, G::kSmem, st, p));
       // a unit of one tile is never cut
-      if (v.max_slots <= G::kKeys) return Status::Ok();
-      return launch_after(k_attend_join_parts<static_cast<int>(G::kBias)>, dim3(H, B), 128, 0, st, p);
+      if (v.max_slots <= G::kKeys && !a.accumulate) return Status::Ok();
+      const int chunks = a.accumulate ? std::min((v.max_slots + 1023) / 1024, 64) : 0;
+      return launch_after(k_attend_finish<static_cast<int>(G::kBias)>, dim3(H + v.num_kv * chunks, B), 128, 0, st, p);
     }));
   } else {
     p.splits = simple_splits(v);
@@ -1081,10 +1107,10 @@ Status kv_attend(KvCache* c, const KvAttendArgs& a, cudaStream_t st) {
       return cuda_status(cudaGetLastError(), "kv attend launch");
     }));
     k_attend_join<<<dim3(H, B), 128, 0, st>>>(p);
-  }
-  if (a.accumulate) {
-    const unsigned blocks = (v.max_slots + 255) / 256;
-    k_attend_weights<<<dim3(blocks < 64 ? blocks : 64, v.num_kv, B), 256, 0, st>>>(p);
+    if (a.accumulate) {
+      const unsigned blocks = (v.max_slots + 255) / 256;
+      k_attend_weights<<<dim3(blocks < 64 ? blocks : 64, v.num_kv, B), 256, 0, st>>>(p);
+    }
   }
   return cuda_status(cudaGetLastError(), "kv attend launch");
 }

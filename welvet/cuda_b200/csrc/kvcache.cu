@@ -38,115 +38,145 @@ __global__ void __launch_bounds__(kAppendThreads) k_append(const __grid_constant
   __shared__ float s_cos[kMaxPairs], s_sin[kMaxPairs];
   __shared__ int s_last;
   const KvView& c = p.c;
-  const int t = blockIdx.x;
+  const int t = blockIdx.x, tid = threadIdx.x;
   const int D = c.head_dim, half = p.half;
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int kv_heads = c.num_kv, heads = 2 * kv_heads + (p.a.q ? c.num_heads : 0);
+  auto source = [&](int h) {
+    return h < kv_heads ? p.a.k + t * p.a.k_ld + static_cast<int64_t>(h) * D
+                        : (h < 2 * kv_heads ? p.a.v + t * p.a.v_ld + static_cast<int64_t>(h - kv_heads) * D
+                                            : p.a.q + t * p.a.q_ld + static_cast<int64_t>(h - 2 * kv_heads) * D);
+  };
+  // An item is four dims of a head's lower half and their partners; the first items' loads go out
+  // before the row's place and angles are looked up.
+  constexpr int kFly = 4;
+  const int per = D / 8, h2 = D / 2, items = heads * per;
+  float4 lo[kFly], hi[kFly];
+  auto load = [&](int first) {
+#pragma unroll
+    for (int x = 0; x < kFly; ++x) {
+      const int w = first + x * kAppendThreads;
+      if (w >= items) continue;
+      const int h = w / per;
+      const float* src = source(h) + 4 * (w - h * per);
+      lo[x] = *reinterpret_cast<const float4*>(src);
+      hi[x] = *reinterpret_cast<const float4*>(src + h2);
+    }
+  };
+  if constexpr (kVec) {
+    if (t < p.a.rows) load(tid);
+  }
   // the row's sequence: the last s with cu[s] <= t
   int seq = t, i = 0;
   bool live = t < p.a.rows;
   if (p.a.cu) {
-    int lo = 0, hi = c.num_seqs;  // cu[lo] <= t < cu[hi] is what a row of a sequence has
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (p.a.cu[mid] <= t) lo = mid; else hi = mid;
+    int a = 0, b = c.num_seqs;  // cu[a] <= t < cu[b] is what a row of a sequence has
+    while (b - a > 1) {
+      const int mid = (a + b) >> 1;
+      if (p.a.cu[mid] <= t) a = mid; else b = mid;
     }
-    seq = lo;
+    seq = a;
     i = t - p.a.cu[seq];
     live = live && i >= 0 && t < p.a.cu[seq + 1];
   }
   if (live) {
     const int64_t slot = static_cast<int64_t>(p.a.start[seq]) + i;
     const int64_t pos = static_cast<int64_t>(p.a.start_seen[seq]) + i;
-    int64_t page = -1;
-    if (slot >= 0 && slot < c.max_slots) {
-      page = c.table[seq * c.table_stride + slot / c.page_size];
-      if (page < 0 || page >= c.num_pages) {
-        page = -1;
-        if (threadIdx.x == 0) atomicCAS(c.err, 0, kKvErrPage);
-      }
-    } else if (threadIdx.x == 0) {
-      atomicCAS(c.err, 0, kKvErrSlot);
-    }
-    for (int d = threadIdx.x; d < half; d += kAppendThreads) {
+    for (int d = tid; d < half; d += kAppendThreads) {
       const double u = static_cast<double>(pos) * p.rope.turns[d];
       sincospif(static_cast<float>(u - 2.0 * rint(0.5 * u)), &s_sin[d], &s_cos[d]);
     }
+    int64_t page = -1;
+    const bool in_range = slot >= 0 && slot < c.max_slots;
+    const int at_page = in_range ? static_cast<int>(slot) / c.page_size : 0, in_page = in_range ? static_cast<int>(slot) - at_page * c.page_size : 0;
+    if (in_range) {
+      page = c.table[seq * c.table_stride + at_page];
+      if (page < 0 || page >= c.num_pages) {
+        page = -1;
+        if (tid == 0) atomicCAS(c.err, 0, kKvErrPage);
+      }
+    } else if (tid == 0) {
+      atomicCAS(c.err, 0, kKvErrSlot);
+    }
     __syncthreads();
-    const int in_page = static_cast<int>(slot % c.page_size);
     T* kd = reinterpret_cast<T*>(c.k.base) + page * c.k.page + in_page * c.k.slot;
     T* vd = reinterpret_cast<T*>(c.v.base) + page * c.v.page + in_page * c.v.slot;
     const float ks = 1.0f / c.k_scale, vs = 1.0f / c.v_scale;
-    const float* k = p.a.k + t * p.a.k_ld;
-    const float* v = p.a.v + t * p.a.v_ld;
-    const float* q = p.a.q ? p.a.q + t * p.a.q_ld : nullptr;
     float* qo = p.a.q_out + t * p.a.q_out_ld;
-    const int heads = 2 * c.num_kv + (q ? c.num_heads : 0);
     if constexpr (kVec) {
-      // a thread takes 4 dims of the lower half and their partners (values: 4 + 4 dims)
-      const int per = D / 8, h2 = D / 2;
-      for (int w = threadIdx.x; w < heads * per; w += kAppendThreads) {
-        const int h = w / per, d = 4 * (w - h * per);
-        const bool is_v = h >= c.num_kv && h < 2 * c.num_kv;
-        const float* src = h < c.num_kv ? k + h * D : (is_v ? v + (h - c.num_kv) * D : q + (h - 2 * c.num_kv) * D);
-        const float4 lo = *reinterpret_cast<const float4*>(src + d);
-        const float4 hi = *reinterpret_cast<const float4*>(src + d + h2);
-        float a[4] = {lo.x, lo.y, lo.z, lo.w}, b[4] = {hi.x, hi.y, hi.z, hi.w};
-        if (!is_v && half > 0) {
+      for (int first = tid; first < items; first += kFly * kAppendThreads) {
+        if (first != tid) load(first);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float cs = s_cos[d + e], sn = s_sin[d + e], x0 = a[e], x1 = b[e];
-            a[e] = x0 * cs - x1 * sn;
-            b[e] = x0 * sn + x1 * cs;
+        for (int x = 0; x < kFly; ++x) {
+          const int w = first + x * kAppendThreads;
+          if (w >= items) continue;
+          const int h = w / per, d = 4 * (w - h * per);
+          const bool is_v = h >= kv_heads && h < 2 * kv_heads;
+          float a[4] = {lo[x].x, lo[x].y, lo[x].z, lo[x].w}, b[4] = {hi[x].x, hi[x].y, hi[x].z, hi[x].w};
+          if (!is_v && half > 0) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float cs = s_cos[d + e], sn = s_sin[d + e], x0 = a[e], x1 = b[e];
+              a[e] = x0 * cs - x1 * sn;
+              b[e] = x0 * sn + x1 * cs;
+            }
           }
-        }
-        if (h >= 2 * c.num_kv) {
-          float* o = qo + (h - 2 * c.num_kv) * D;
-          *reinterpret_cast<float4*>(o + d) = make_float4(a[0], a[1], a[2], a[3]);
-          *reinterpret_cast<float4*>(o + d + h2) = make_float4(b[0], b[1], b[2], b[3]);
-        } else if (page >= 0) {
-          T* o = is_v ? vd + (h - c.num_kv) * c.v.head : kd + h * c.k.head;
-          const float s = is_v ? vs : ks;
-          store4<T>(o + d, a, s);
-          store4<T>(o + d + h2, b, s);
+          if (h >= 2 * kv_heads) {
+            float* o = qo + static_cast<int64_t>(h - 2 * kv_heads) * D;
+            *reinterpret_cast<float4*>(o + d) = make_float4(a[0], a[1], a[2], a[3]);
+            *reinterpret_cast<float4*>(o + d + h2) = make_float4(b[0], b[1], b[2], b[3]);
+          } else if (page >= 0) {
+            T* o = is_v ? vd + (h - kv_heads) * c.v.head : kd + h * c.k.head;
+            const float s = is_v ? vs : ks;
+            store4<T>(o + d, a, s);
+            store4<T>(o + d + h2, b, s);
+          }
         }
       }
     } else {
-      for (int w = threadIdx.x; w < heads * D; w += kAppendThreads) {
-        const int h = w / D, d = w - h * D;
-        const bool is_v = h >= c.num_kv && h < 2 * c.num_kv;
-        const float* src = h < c.num_kv ? k + h * D : (is_v ? v + (h - c.num_kv) * D : q + (h - 2 * c.num_kv) * D);
-        float x = src[d];
-        if (!is_v && d < 2 * half) {
-          const int e = d < half ? d : d - half;
-          const float other = src[d < half ? d + half : e];
-          x = d < half ? x * s_cos[e] - other * s_sin[e] : other * s_sin[e] + x * s_cos[e];
+      // a pair of dims (d, d + n / 2) a thread, so that q may be rotated in place
+      const int pairs = (D + 1) / 2;
+      for (int w = tid; w < heads * pairs; w += kAppendThreads) {
+        const int h = w / pairs, d0 = w - h * pairs, d1 = d0 + D / 2;
+        const bool is_v = h >= kv_heads && h < 2 * kv_heads;
+        const bool odd = d0 == D / 2;  // the unpaired last dim of an odd width
+        const float* src = source(h);
+        float a = odd ? 0.0f : src[d0], b = odd ? src[D - 1] : src[d1];
+        if (!is_v && half > 0 && !odd) {
+          const float x0 = a, x1 = b;
+          a = x0 * s_cos[d0] - x1 * s_sin[d0];
+          b = x0 * s_sin[d0] + x1 * s_cos[d0];
         }
-        if (h >= 2 * c.num_kv) qo[(h - 2 * c.num_kv) * D + d] = x;
-        else if (page >= 0) {
-          if (is_v) vd[(h - c.num_kv) * c.v.head + d] = to_stored<T>(x * vs);
-          else kd[h * c.k.head + d] = to_stored<T>(x * ks);
+        const int db = odd ? D - 1 : d1;
+        if (h >= 2 * kv_heads) {
+          float* o = qo + static_cast<int64_t>(h - 2 * kv_heads) * D;
+          if (!odd) o[d0] = a;
+          o[db] = b;
+        } else if (page >= 0) {
+          T* o = is_v ? vd + (h - kv_heads) * c.v.head : kd + h * c.k.head;
+          const float s = is_v ? vs : ks;
+          if (!odd) o[d0] = to_stored<T>(a * s);
+          o[db] = to_stored<T>(b * s);
         }
       }
     }
-    if (slot >= 0 && slot < c.max_slots) {
-      for (int h = threadIdx.x; h < c.num_kv; h += kAppendThreads) {
-        const int64_t at = (static_cast<int64_t>(seq) * c.num_kv + h) * c.max_slots + slot;
+    if (in_range) {
+      for (int h = tid; h < kv_heads; h += kAppendThreads) {
+        const int64_t at = (static_cast<int64_t>(seq) * kv_heads + h) * c.max_slots + slot;
         if (c.positions) c.positions[at] = static_cast<int32_t>(pos);
         if (c.weights) c.weights[at] = 0.0f;
       }
     }
   }
-  // The last block to finish advances the lengths: start may be lens itself, which every block
-  // has read by then.
+  // The last block to finish advances the lengths: start may be lens itself, which every thread of
+  // every block has read by then.
   __syncthreads();
-  if (threadIdx.x == 0) {
-    __threadfence();
-    s_last = atomicAdd(p.ticket, 1) == static_cast<int>(gridDim.x) - 1;
-  }
+  if (tid == 0) s_last = atomicAdd(p.ticket, 1) == static_cast<int>(gridDim.x) - 1;
   __syncthreads();
   if (!s_last) return;
-  __threadfence();
-  if (threadIdx.x == 0) *p.ticket = 0;
-  for (int s = threadIdx.x; s < c.num_seqs; s += kAppendThreads) {
+  if (tid == 0) *p.ticket = 0;
+  for (int s = tid; s < c.num_seqs; s += kAppendThreads) {
     const int n = p.a.cu ? p.a.cu[s + 1] - p.a.cu[s] : 1;
     const int64_t len = static_cast<int64_t>(p.a.start[s]) + n, tot = static_cast<int64_t>(p.a.start_seen[s]) + n;
     c.lens[s] = static_cast<int32_t>(len < c.max_slots ? len : c.max_slots);
@@ -167,6 +197,7 @@ struct EvictParams {
 
 constexpr int kEvictThreads = 512;
 constexpr int kEvictWarps = kEvictThreads / 32;
+constexpr int kMaxRanks = 8;          // blocks of a cluster
 constexpr int kRadixBins = 2048;      // three passes over a 32-bit key: 11 + 11 + 10 bits
 constexpr int kEvictCache = 24 * 1024;  // keys: 96 KB
 
@@ -271,7 +302,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) k_evict_select(const __grid_
   __shared__ __align__(16) int s_hist[3][kRadixBins];
   __shared__ int s_warp[kEvictWarps], s_warp2[kEvictWarps];
   __shared__ uint32_t s_prefix;
-  __shared__ int s_rest;
+  __shared__ int s_rest, s_same;
   __shared__ int s_ties;      // of this block
   __shared__ int s_lists[2];  // slots of this block to fill, to take
   const KvView& c = p.c;
@@ -342,13 +373,18 @@ __global__ void __launch_bounds__(kEvictThreads, 2) k_evict_select(const __grid_
     const int top = (1 << bits) - 1 - 4 * tid;
     int n[4] = {0, 0, 0, 0};
     if (top >= 3) {
-      for (int r = 0; r < ranks; ++r) {
-        const int* h = ranks > 1 ? cluster.map_shared_rank(hist, r) : hist;
-        const int4 q = *reinterpret_cast<const int4*>(h + top - 3);
-        n[0] += q.w;
-        n[1] += q.z;
-        n[2] += q.y;
-        n[3] += q.x;
+      int4 q[kMaxRanks];
+#pragma unroll
+      for (int r = 0; r < kMaxRanks; ++r) {
+        q[r] = make_int4(0, 0, 0, 0);
+        if (r < ranks) q[r] = *reinterpret_cast<const int4*>((ranks > 1 ? cluster.map_shared_rank(hist, r) : hist) + top - 3);
+      }
+#pragma unroll
+      for (int r = 0; r < kMaxRanks; ++r) {
+        n[0] += q[r].w;
+        n[1] += q[r].z;
+        n[2] += q[r].y;
+        n[3] += q[r].x;
       }
     }
     const int mine = n[0] + n[1] + n[2] + n[3];
@@ -374,6 +410,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) k_evict_select(const __grid_
         }
       s_prefix = (prefix << bits) | static_cast<uint32_t>(top - e);
       s_rest = left;
+      s_same = e == 0 ? n[0] : (e == 1 ? n[1] : (e == 2 ? n[2] : n[3]));
     }
     __syncthreads();
     prefix = s_prefix;
@@ -381,23 +418,31 @@ __global__ void __launch_bounds__(kEvictThreads, 2) k_evict_select(const __grid_
     __syncthreads();
   }
 
-  // keys above the threshold stay, and the first `rest` slots whose key equals it
-  int ties = 0;
-  for (int j0 = wlo; j0 < whi; j0 += 32) ties += __popc(__ballot_sync(0xffffffffu, j0 + lane < whi && key_at(min(j0 + lane, whi - 1)) == prefix));
-  if (lane == 0) s_warp[w] = ties;
-  __syncthreads();
-  int ties_before = 0, all = 0;
+  // Keys above the threshold stay, and the first `rest` slots whose key equals it; where all of those
+  // stay (no ties but within the kept), their order is not needed.
+  int ties_before = 0;
+  if (s_same != rest) {
+    int ties = 0;
+    for (int j0 = wlo; j0 < whi; j0 += 32) ties += __popc(__ballot_sync(0xffffffffu, j0 + lane < whi && key_at(min(j0 + lane, whi - 1)) == prefix));
+    if (lane == 0) s_warp[w] = ties;
+    __syncthreads();
+    int all = 0;
 #pragma unroll
-  for (int i = 0; i < kEvictWarps; ++i) {
-    if (i < w) ties_before += s_warp[i];
-    all += s_warp[i];
+    for (int i = 0; i < kEvictWarps; ++i) {
+      if (i < w) ties_before += s_warp[i];
+      all += s_warp[i];
+    }
+    if (tid == 0) s_ties = all;
+    if (ranks > 1) {
+      cluster.sync();
+      int t[kMaxRanks];
+#pragma unroll
+      for (int r = 0; r < kMaxRanks; ++r) t[r] = r < rank ? *cluster.map_shared_rank(&s_ties, r) : 0;
+#pragma unroll
+      for (int r = 0; r < kMaxRanks; ++r) ties_before += t[r];
+    }
+    __syncthreads();
   }
-  if (tid == 0) s_ties = all;
-  if (ranks > 1) {
-    cluster.sync();
-    for (int r = 0; r < rank; ++r) ties_before += *cluster.map_shared_rank(&s_ties, r);
-  }
-  __syncthreads();
   auto flags_at = [&](int j0, int& seen_ties, uint32_t& f, uint32_t& g) {
     const int j = j0 + lane;
     const uint32_t k = j < whi ? key_at(j) : 0u;
@@ -412,6 +457,10 @@ __global__ void __launch_bounds__(kEvictThreads, 2) k_evict_select(const __grid_
   for (int j0 = wlo; j0 < whi; j0 += 32) {
     uint32_t f, g;
     flags_at(j0, seen_ties, f, g);
+    if (p.cached && lane == 0) {  // kept where the warp's keys were
+      s_keys[j0 - lo] = f;
+      s_keys[j0 - lo + 1] = g;
+    }
     n_fill += __popc(f);
     n_take += __popc(g);
   }
@@ -439,13 +488,23 @@ __global__ void __launch_bounds__(kEvictThreads, 2) k_evict_select(const __grid_
   if (ranks > 1) {
     cluster.sync();
     moved = 0;
-    for (int r = 0; r < ranks; ++r) {
-      const int* l = cluster.map_shared_rank(s_lists, r);
-      if (r < rank) {
-        fill_at += l[0];
-        take_at += l[1];
+    int f[kMaxRanks], g[kMaxRanks];
+#pragma unroll
+    for (int r = 0; r < kMaxRanks; ++r) {
+      f[r] = g[r] = 0;
+      if (r < ranks) {
+        const int* l = cluster.map_shared_rank(s_lists, r);
+        f[r] = l[0];
+        g[r] = l[1];
       }
-      moved += l[0];
+    }
+#pragma unroll
+    for (int r = 0; r < kMaxRanks; ++r) {
+      if (r < rank) {
+        fill_at += f[r];
+        take_at += g[r];
+      }
+      moved += f[r];
     }
   }
   int32_t* fill = p.moves + static_cast<int64_t>(row) * 2 * (c.max_slots / 2);
@@ -453,7 +512,12 @@ __global__ void __launch_bounds__(kEvictThreads, 2) k_evict_select(const __grid_
   seen_ties = ties_before;
   for (int j0 = wlo; j0 < whi; j0 += 32) {
     uint32_t f, g;
-    flags_at(j0, seen_ties, f, g);
+    if (p.cached) {
+      f = s_keys[j0 - lo];
+      g = s_keys[j0 - lo + 1];
+    } else {
+      flags_at(j0, seen_ties, f, g);
+    }
     const uint32_t below = (1u << lane) - 1u;
     if ((f >> lane) & 1) fill[fill_at + __popc(f & below)] = j0 + lane;
     if ((g >> lane) & 1) take[take_at + __popc(g & below)] = j0 + lane;
@@ -560,9 +624,7 @@ Status kv_append(KvCache* c, const KvAppendArgs& a, cudaStream_t st) {
   return by_type(c->type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     const int blocks = a.rows > 0 ? a.rows : 1;  // no row: the lengths are still carried over
-    if (vec) k_append<T, true><<<blocks, kAppendThreads, 0, st>>>(p);
-    else k_append<T, false><<<blocks, kAppendThreads, 0, st>>>(p);
-    return cuda_status(cudaGetLastError(), "kv append launch");
+    return launch_after(vec ? k_append<T, true> : k_append<T, false>, dim3(blocks), kAppendThreads, 0, st, p);
   });
 }
 
@@ -582,7 +644,7 @@ Status kv_evict(KvCache* c, const KvEvictArgs& a, cudaStream_t st) {
   // One block a head unless that leaves SMs idle or a block's keys do not fit its shared memory.
   const int64_t heads = static_cast<int64_t>(p.c.num_seqs) * p.c.num_kv;
   int ranks = 1;
-  while (ranks < 8 && ((heads * ranks < 148 && p.c.max_slots / ranks > 2048) || p.c.max_slots / ranks > kEvictCache - 32)) ranks *= 2;
+  while (ranks < kMaxRanks && ((heads * ranks < 148 && p.c.max_slots / ranks > 2048) || p.c.max_slots / ranks > kEvictCache - 32)) ranks *= 2;
   const int per = ((p.c.max_slots + ranks - 1) / ranks + 31) & ~31;
   p.cached = per <= kEvictCache;
   auto go = [&](auto size_c, auto vec_c) -> Status {

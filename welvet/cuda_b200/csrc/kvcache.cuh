@@ -66,4 +66,20 @@ Status by_type(KvType t, F&& f) {
   return Status::Internal("kv: type");
 }
 
+// A launch that may start while the kernel before it still runs (it waits for its results itself).
+template <typename K, typename P>
+Status launch_after(K* kernel, dim3 grid, int threads, int smem, cudaStream_t st, const P& p) {
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p), "kv launch");
+}
+
 } // namespace wb
