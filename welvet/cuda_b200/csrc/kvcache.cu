@@ -329,16 +329,26 @@ __global__ void __launch_bounds__(kEvictThreads, 2) k_evict_select(const __grid_
     return evict_key(p.a.weights_in[rec + j], p.a.positions_in[rec + j], p.a.sinks, recent_from);
   };
   if (cut || apart) {
-#pragma unroll 4
-    for (int j = lo + tid; j < hi; j += kEvictThreads) {
-      const float weight = p.a.weights_in[rec + j];
-      const int pos = p.a.positions_in[rec + j];
-      if (apart && j < stays_to) {
-        c.weights[rec + j] = weight;
-        c.positions[rec + j] = pos;
+    constexpr int kFly = 8;  // slots whose loads are in flight together (the stores may alias them)
+    for (int j0 = lo + tid; j0 < hi; j0 += kFly * kEvictThreads) {
+      float weight[kFly];
+      int pos[kFly];
+#pragma unroll
+      for (int x = 0; x < kFly; ++x) {
+        const int j = j0 + x * kEvictThreads;
+        weight[x] = j < hi ? p.a.weights_in[rec + j] : 0.0f;
+        pos[x] = j < hi ? p.a.positions_in[rec + j] : 0;
       }
-      const uint32_t k = evict_key(weight, pos, p.a.sinks, recent_from);
-      if (cut && p.cached) s_keys[j - lo] = k;
+#pragma unroll
+      for (int x = 0; x < kFly; ++x) {
+        const int j = j0 + x * kEvictThreads;
+        if (j >= hi) break;
+        if (apart && j < stays_to) {
+          c.weights[rec + j] = weight[x];
+          c.positions[rec + j] = pos[x];
+        }
+        if (cut && p.cached) s_keys[j - lo] = evict_key(weight[x], pos[x], p.a.sinks, recent_from);
+      }
     }
   }
   // The last (head, block) of a sequence to have read its length writes the new one.
