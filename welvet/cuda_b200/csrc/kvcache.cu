@@ -300,6 +300,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) k_evict_select(const __grid_
   cg::cluster_group cluster = cg::this_cluster();
   extern __shared__ uint32_t s_keys[];
   __shared__ __align__(16) int s_hist[3][kRadixBins];
+  __shared__ int s_group[3][kRadixBins / 32];
   __shared__ int s_warp[kEvictWarps], s_warp2[kEvictWarps];
   __shared__ uint32_t s_prefix;
   __shared__ int s_rest, s_same;
@@ -377,50 +378,54 @@ __global__ void __launch_bounds__(kEvictThreads, 2) k_evict_select(const __grid_
       const uint32_t k = key_at(j);
       if (pass == 0 || (k >> (shift + bits)) == prefix) atomicAdd(&hist[(k >> shift) & ((1u << bits) - 1u)], 1);
     }
+    // sums of 32 bins each, then one warp finds the group and the bin, adding over the cluster
+    __syncthreads();
+    const int4 four = *reinterpret_cast<const int4*>(hist + 4 * tid);
+    int sum = four.x + four.y + four.z + four.w;
+#pragma unroll
+    for (int o = 1; o < 8; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((lane & 7) == 0) s_group[pass][tid >> 3] = sum;
     if (ranks > 1) cluster.sync();
     else __syncthreads();
-    // bins from the top, four a thread
-    const int top = (1 << bits) - 1 - 4 * tid;
-    int n[4] = {0, 0, 0, 0};
-    if (top >= 3) {
-      int4 q[kMaxRanks];
+    if (w == 0) {
+      auto total = [&](const int* at) {  // of one counter over the cluster
+        int q[kMaxRanks];
 #pragma unroll
-      for (int r = 0; r < kMaxRanks; ++r) {
-        q[r] = make_int4(0, 0, 0, 0);
-        if (r < ranks) q[r] = *reinterpret_cast<const int4*>((ranks > 1 ? cluster.map_shared_rank(hist, r) : hist) + top - 3);
-      }
+        for (int r = 0; r < kMaxRanks; ++r) q[r] = r < ranks ? *(ranks > 1 ? cluster.map_shared_rank(at, r) : at) : 0;
+        int n = 0;
 #pragma unroll
-      for (int r = 0; r < kMaxRanks; ++r) {
-        n[0] += q[r].w;
-        n[1] += q[r].z;
-        n[2] += q[r].y;
-        n[3] += q[r].x;
-      }
-    }
-    const int mine = n[0] + n[1] + n[2] + n[3];
-    int x = mine;
+        for (int r = 0; r < kMaxRanks; ++r) n += q[r];
+        return n;
+      };
+      // lane i holds n, the i-th from the top; the lane in which `left` is used up
+      auto find = [&](int n, int& left) {
+        int x = n;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    if (lane == 31) s_warp[w] = x;
-    __syncthreads();
-    int before = x - mine;
-#pragma unroll
-    for (int i = 0; i < kEvictWarps; ++i)
-      if (i < w) before += s_warp[i];
-    if (top >= 3 && before < rest && before + mine >= rest) {
-      int e = 0, left = rest - before;
-#pragma unroll
-      for (int i = 0; i < 3; ++i)
-        if (e == i && left > n[i]) {
-          left -= n[i];
-          ++e;
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, x, o);
+          if (lane >= o) x += y;
         }
-      s_prefix = (prefix << bits) | static_cast<uint32_t>(top - e);
-      s_rest = left;
-      s_same = e == 0 ? n[0] : (e == 1 ? n[1] : (e == 2 ? n[2] : n[3]));
+        const int at = __ffs(__ballot_sync(0xffffffffu, x >= left)) - 1;
+        left -= __shfl_sync(0xffffffffu, x - n, at);
+        return at;
+      };
+      int left = rest;
+      const int upper = total(&s_group[pass][kRadixBins / 32 - 1 - 2 * lane]), lower = total(&s_group[pass][kRadixBins / 32 - 2 - 2 * lane]);
+      const int pair = find(upper + lower, left);
+      const int in_upper = __shfl_sync(0xffffffffu, upper, pair);
+      int group = kRadixBins / 32 - 1 - 2 * pair;
+      if (left > in_upper) {
+        left -= in_upper;
+        --group;
+      }
+      const int n = total(hist + 32 * group + 31 - lane);
+      const int bin = find(n, left);
+      const int same = __shfl_sync(0xffffffffu, n, bin);
+      if (lane == 0) {
+        s_prefix = (prefix << bits) | static_cast<uint32_t>(32 * group + 31 - bin);
+        s_rest = left;
+        s_same = same;
+      }
     }
     __syncthreads();
     prefix = s_prefix;
