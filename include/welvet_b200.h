@@ -284,6 +284,19 @@ WELVET_API welvet_status welvet_b200_kv_evict(welvet_b200_kv* kv, int32_t keep, 
 WELVET_API welvet_status welvet_b200_kv_check_error(welvet_b200_kv* kv, void* stream);
 WELVET_API void welvet_b200_kv_release(welvet_b200_kv* kv);
 
+/* An MHA cell's step over a cache of its head counts and width. decode: one new token per sequence,
+ * x_dev [num_seqs][d_model] -> attn_dev [num_seqs][q_dim] (may be NULL), y_dev [num_seqs][d_model]:
+ * projections, rotary and append, attention with the cell's mask, position kind and scale (mask 3's
+ * window is max_seq_len), output projection; accumulate as in kv_attend. prefill: `tokens` rows of a
+ * prompt for a sequence that holds nothing yet, attended among themselves as in mha_execute_device
+ * (tokens <= the cell's max_seq_len) and appended. The first call for a number of rows allocates the
+ * cell's work buffers. */
+WELVET_API welvet_status welvet_b200_mha_decode_device(welvet_b200_mha* s, welvet_b200_kv* kv, const float* x_dev,
+                                                       float* attn_dev, float* y_dev, int32_t accumulate, void* stream);
+WELVET_API welvet_status welvet_b200_mha_prefill_device(welvet_b200_mha* s, welvet_b200_kv* kv, int32_t sequence,
+                                                        int32_t tokens, const float* x_dev, float* attn_dev,
+                                                        float* y_dev, void* stream);
+
 /* ---------------------------------------------------------------- 4-bit Dense with group scales
  *
  * No counterpart in the reference (one scale per tensor). y = act(sum over groups of scale *

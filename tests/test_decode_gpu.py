@@ -1,0 +1,150 @@
+"""An MHA cell's prompt and decode steps over a paged cache against the cell's own forward of the whole
+sequence and against 64-bit sums, and the example that runs the operators together."""
+import os
+import sys
+
+import numpy as np
+import pytest
+
+from conftest import ROOT
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def D(wb):
+    import welvet.cuda_b200.decode as decode
+    return decode
+
+
+def cache_for(D, n, heads, kv, dim, slots, dtype, page=16, records=False):
+    import torch
+    per = -(-slots // page)
+    k = torch.zeros((n * per + 1, page, kv, dim), dtype=dtype, device="cuda")
+    table = torch.randperm(n * per, device="cuda").reshape(n, per).to(torch.int32)
+    z = lambda: torch.zeros(n, dtype=torch.int32, device="cuda")  # noqa: E731
+    kw = {}
+    if records:
+        kw = dict(weights=torch.zeros((n, kv, per * page), device="cuda"),
+                  positions=torch.zeros((n, kv, per * page), dtype=torch.int32, device="cuda"))
+    return D.PagedKV(k, torch.zeros_like(k), table, z(), num_heads=heads, seen=z(), **kw)
+
+
+@pytest.mark.parametrize("pos", [0, 2, 3, 1])
+@pytest.mark.parametrize("mask,max_seq", [(1, 200), (3, 20), (2, 200), (4, 200)])
+def test_cell_steps_equal_the_whole_forward(D, wb, pos, mask, max_seq):
+    """A prompt and single tokens over a float32 cache give the rows that the cell's forward of the whole
+    sequence gives (causal rows; mask 2's last row sees everything up to itself, as a step does).
+
+    The cell's attention is in 64 bits, the cache's in 32 (keys, values and query to 24 bits, scores to
+    about 2^-20 of |q||k| / sqrt(dim) ~ 10): 1e-4 of the largest output holds both, and the projections'
+    2^-18 bound between other batch sizes."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(pos * 10 + mask)
+    d_model, heads, kv, dim, total, first = 256, 4, 2, 64, 60, 13
+    w = [torch.randn((r, d_model), generator=g, device="cuda") * 0.08 for r in (heads * dim, kv * dim, kv * dim)]
+    w.append(torch.randn((d_model, heads * dim), generator=g, device="cuda") * 0.08)
+    cell = wb.MhaCell(*w, d_model, heads, kv, dim, max_seq, mask, pos, wb.FP8E4M3)
+    x = torch.randn((total, d_model), generator=g, device="cuda")
+    seen = total if mask != 3 else max_seq  # the cell's ring holds max_seq positions of one forward
+    cache = cache_for(D, 1, heads, kv, dim, 100, torch.float32)
+    y, attn = torch.empty((first, d_model), device="cuda"), torch.empty((first, heads * dim), device="cuda")
+    D.mha_prefill(cell, cache, 0, x[:first].contiguous(), y, attn)
+    got_y, got_a = [y], [attn]
+    for t in range(first, seen):
+        y, attn = torch.empty((1, d_model), device="cuda"), torch.empty((1, heads * dim), device="cuda")
+        D.mha_decode(cell, cache, x[t: t + 1], y, attn)
+        got_y.append(y)
+        got_a.append(attn)
+    cache.check_error()
+    assert cache.lens.tolist() == [seen] and cache.seen.tolist() == [seen]
+    if mask == 2:  # full: each step is compared with the last row of its own prefix
+        for t in (first, first + 1, seen - 1):
+            ye, ae = torch.empty((t + 1, d_model), device="cuda"), torch.empty((t + 1, heads * dim), device="cuda")
+            cell.execute_device(x[: t + 1].contiguous(), 1, t + 1, ye, ae)
+            for a, b in ((got_a[t - first + 1], ae[-1:]), (got_y[t - first + 1], ye[-1:])):
+                assert float((a - b).abs().max()) <= 1e-4 * float(b.abs().max())
+        return
+    ye, ae = torch.empty((seen, d_model), device="cuda"), torch.empty((seen, heads * dim), device="cuda")
+    cell.execute_device(x[:seen].contiguous(), 1, seen, ye, ae)
+    for a, b in ((torch.cat(got_a), ae), (torch.cat(got_y), ye)):
+        assert float((a - b).abs().max()) <= 1e-4 * float(b.abs().max())
+
+
+def test_window_cell_forgets(D, wb):
+    """mask 3: tokens max_seq_len back no longer count."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(5)
+    d_model, heads, dim, window = 128, 2, 64, 8
+    w = [torch.randn((128, 128), generator=g, device="cuda") * 0.1 for _ in range(4)]
+    cell = wb.MhaCell(*w, d_model, heads, heads, dim, window, 3, 1, wb.FP8E4M3)  # no positions: rows decide
+    x = torch.randn((30, d_model), generator=g, device="cuda")
+    outs = []
+    for drop in (0, 15):  # a cache that never saw the first tokens gives the same last step
+        cache = cache_for(D, 1, heads, heads, dim, 64, torch.bfloat16)
+        for t in range(drop, 30):
+            y = torch.empty((1, d_model), device="cuda")
+            D.mha_decode(cell, cache, x[t: t + 1], y)
+        outs.append(y)
+    assert float((outs[0] - outs[1]).abs().max()) <= 2e-6 * float(outs[0].abs().max())
+
+
+def test_refusals(D, wb):
+    import torch
+    w = [torch.zeros((128, 128), device="cuda") for _ in range(4)]
+    cell = wb.MhaCell(*w, 128, 2, 2, 64, 64, 1, 0, wb.FP8E4M3)
+    cache = cache_for(D, 3, 2, 2, 64, 32, torch.bfloat16)
+    other = cache_for(D, 3, 4, 2, 64, 32, torch.bfloat16)
+    x, y = torch.zeros((3, 128), device="cuda"), torch.zeros((3, 128), device="cuda")
+    for f in (lambda: D.mha_decode(cell, other, x, y), lambda: D.mha_decode(cell, cache, x, y, accumulate=True),
+              lambda: D.mha_prefill(cell, cache, 3, x, y), lambda: D.mha_prefill(cell, cache, -1, x, y),
+              lambda: D.mha_prefill(cell, cache, 0, torch.zeros((40, 128), device="cuda"), torch.zeros((40, 128), device="cuda"))):
+        with pytest.raises(wb.WelvetError) as e:
+            f()
+        assert e.value.code == 1
+    for a in ((x[:2], y), (x, y[:, :64]), (x.half(), y)):
+        with pytest.raises(ValueError):
+            D.mha_decode(cell, cache, *a)
+    assert cache.lens.tolist() == [0, 0, 0]
+
+
+def test_example(D):
+    """Replays of the captured step keep the budget, are finite, and repeat bit for bit."""
+    import torch
+    sys.path.insert(0, os.path.join(ROOT, "examples"))
+    import decode_step
+    layer, outs = decode_step.run(steps=40, budget=48, d_model=256, heads=4, kv_heads=2, inter=512, prompts=(60, 1, 20), quiet=True)
+    again = decode_step.run(steps=40, budget=48, d_model=256, heads=4, kv_heads=2, inter=512, prompts=(60, 1, 20), quiet=True)[1]
+    assert all(torch.isfinite(o).all() for o in outs)
+    for a, b in zip(outs, again):
+        assert torch.equal(a, b)
+    # one step before the capture and 40 replays (the capture itself runs nothing)
+    assert layer.cache.seen.tolist() == [101, 42, 61]
+    assert all(x <= 56 for x in layer.cache.lens.tolist()) and layer.cache.lens.tolist()[1] == 42
+
+
+def test_example_without_eviction_equals_single_steps(D, wb):
+    """The captured and the plain step agree bit for bit, and follow the cell and layers called one by one."""
+    import torch
+    sys.path.insert(0, os.path.join(ROOT, "examples"))
+    import decode_step
+    res = []
+    for captured in (False, True):
+        layer = decode_step.Layer(256, 4, 2, 512, (9, 3), 64, 8, seed=3)
+        g = torch.Generator(device="cuda").manual_seed(9)
+        for s, n in enumerate((9, 3)):
+            layer.prompt(s, torch.randn((n, 256), generator=g, device="cuda"))
+        x = torch.randn((2, 256), generator=g, device="cuda")
+        layer.step(x, evict=False)
+        if captured:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                layer.step(x, evict=False)
+        outs = []
+        for _ in range(5):
+            graph.replay() if captured else layer.step(x, evict=False)
+            outs.append(layer.out.clone())
+            x.copy_(layer.out)
+        res.append(outs)
+    for a, b in zip(*res):
+        assert torch.equal(a, b)

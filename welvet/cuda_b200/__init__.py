@@ -388,6 +388,7 @@ class MhaCell:
         else:
             keep = [_f32(t) for t in (Q, K, V, O)]
             ptrs = [_np_ptr(t) for t in keep]
+        self.d_model = d_model
         check(_L.welvet_b200_mha_mount(d_model, num_heads, num_kv_heads, head_dim, max_seq_len, mask, pos, dtype,
                                        *ptrs, 1 if on_dev else 0, byref(self._h)))
 

@@ -4,9 +4,13 @@
 #include "../../../include/welvet_b200.h"
 
 #include "comm.hpp"
+#include "kvcache.hpp"
 #include "sharded.hpp"
 #include "volume.hpp"
 
+struct welvet_b200_kv {
+  wb::KvCache* c;
+};
 struct welvet_b200_volume {
   wb::Volume* v;
 };

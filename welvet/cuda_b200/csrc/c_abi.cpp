@@ -2,7 +2,7 @@
 //
 // Reference boundary replaced: include/welvet_c.h + src/interop/c_abi.cpp. Status mapping
 // and "no C++ exception crosses C" follow c_abi.cpp:41-47 and model_session.cpp:87-100.
-#include "../../../include/welvet_b200.h"
+#include "abi_handles.hpp"
 
 #include "cells.hpp"
 #include "codec.hpp"
@@ -479,6 +479,24 @@ welvet_status welvet_b200_mha_execute_device(welvet_b200_mha* s, int32_t batch, 
     WB_CUDA(cudaSetDevice(s->cell.device));
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     return wb::mha_forward_device(&s->cell, batch, seq, x_dev, attn_dev, y_dev, st);
+  });
+}
+
+welvet_status welvet_b200_mha_decode_device(welvet_b200_mha* s, welvet_b200_kv* kv, const float* x_dev, float* attn_dev,
+                                            float* y_dev, int32_t accumulate, void* stream) {
+  return guarded([&] {
+    if (!s || !kv || !kv->c || !x_dev || !y_dev) return wb::Status::Invalid("mha: invalid argument");
+    WB_CUDA(cudaSetDevice(s->cell.device));
+    return wb::mha_decode_device(&s->cell, kv->c, x_dev, attn_dev, y_dev, accumulate != 0, static_cast<cudaStream_t>(stream));
+  });
+}
+
+welvet_status welvet_b200_mha_prefill_device(welvet_b200_mha* s, welvet_b200_kv* kv, int32_t sequence, int32_t tokens,
+                                             const float* x_dev, float* attn_dev, float* y_dev, void* stream) {
+  return guarded([&] {
+    if (!s || !kv || !kv->c || !x_dev || !y_dev) return wb::Status::Invalid("mha: invalid argument");
+    WB_CUDA(cudaSetDevice(s->cell.device));
+    return wb::mha_prefill_device(&s->cell, kv->c, sequence, tokens, x_dev, attn_dev, y_dev, static_cast<cudaStream_t>(stream));
   });
 }
 

@@ -404,6 +404,67 @@ Status mha_forward_device(MhaCell* c, int batch, int seq, const float* x, float*
   return forward_device(c->o, bs, attn_out, qd, y, y, &c->io_o, st, false);
 }
 
+static Status mha_cache_fits(const MhaCell& c, const KvCache& kv) {
+  const MhaConfig& g = c.cfg;
+  const KvView& v = kv.view;
+  if (v.num_heads != g.num_heads || v.num_kv != g.num_kv_heads || v.head_dim != g.head_dim)
+    return Status::Invalid("mha: the cache's head counts or width are not the cell's");
+  if (kv.device != c.device) return Status::Invalid("mha: the cache is on another device");
+  if (g.softmax != 0) return Status::Unsupported("mha: a cached step needs Softmax attention (not sigmoid)");
+  return Status::Ok();
+}
+
+static double mha_theta(const MhaConfig& g) { return g.pos == 0 || g.pos == 3 ? g.rope_theta : 0.0; }
+
+Status mha_decode_device(MhaCell* c, KvCache* kv, const float* x, float* attn, float* y, bool accumulate, cudaStream_t st) {
+  WB_TRY(mha_cache_fits(*c, *kv));
+  const MhaConfig& g = c->cfg;
+  const int rows = kv->view.num_seqs, qd = g.num_heads * g.head_dim, kvd = g.num_kv_heads * g.head_dim;
+  if (accumulate && !kv->view.weights) return Status::Invalid("mha: the cache has no weights to accumulate");
+  WB_TRY(mha_reserve(c, rows, st));
+  WB_TRY(forward_device(c->q, rows, x, g.d_model, c->qb, c->qb, &c->io_q, st, false));
+  WB_TRY(forward_device(c->k, rows, x, g.d_model, c->kb, c->kb, &c->io_k, st, false));
+  WB_TRY(forward_device(c->v, rows, x, g.d_model, c->vb, c->vb, &c->io_v, st, false));
+  KvAppendArgs ap;
+  ap.rows = rows;
+  ap.k = c->kb;
+  ap.v = c->vb;
+  ap.q = c->qb;
+  ap.q_out = c->qb;
+  ap.k_ld = ap.v_ld = kvd;
+  ap.q_ld = ap.q_out_ld = qd;
+  ap.theta = mha_theta(g);
+  WB_TRY(kv_append(kv, ap, st));
+  float* attn_out = attn ? attn : c->attn;
+  KvAttendArgs at;
+  at.q = c->qb;
+  at.out = attn_out;
+  at.q_ld = at.out_ld = qd;
+  at.scale = static_cast<float>(g.scale_override);
+  // the masks as the newest position sees them: only the window leaves keys out
+  at.window = g.mask == 3 ? (g.window > 0 ? g.window : g.max_seq_len) : 0;
+  at.alibi = g.pos == 2 || g.pos == 3;
+  at.accumulate = accumulate;
+  WB_TRY(kv_attend(kv, at, st));
+  return forward_device(c->o, rows, attn_out, qd, y, y, &c->io_o, st, false);
+}
+
+Status mha_prefill_device(MhaCell* c, KvCache* kv, int sequence, int tokens, const float* x, float* attn, float* y,
+                          cudaStream_t st) {
+  WB_TRY(mha_cache_fits(*c, *kv));
+  if (sequence < 0 || sequence >= kv->view.num_seqs) return Status::Invalid("mha: no such sequence in the cache");
+  if (tokens > kv->view.max_slots) return Status::Invalid("mha: the prompt is longer than a sequence's slots");
+  WB_TRY(mha_forward_device(c, 1, tokens, x, attn, y, st));
+  KvAppendArgs ap;
+  ap.rows = tokens;
+  ap.k = c->kb;
+  ap.v = c->vb;
+  ap.k_ld = ap.v_ld = static_cast<int64_t>(c->cfg.num_kv_heads) * c->cfg.head_dim;
+  ap.theta = mha_theta(c->cfg);
+  ap.only = sequence;
+  return kv_append(kv, ap, st);
+}
+
 Status rmsnorm_gamma(int device, int dim, DType dt, const float* gamma, double** gamma64_dev, cudaStream_t st) {
   return rmsnorm_gamma_src(device, dim, dt, f32_src(gamma, false), gamma64_dev, st);
 }

@@ -8,6 +8,7 @@
 
 #include "cell_kernels.hpp"
 #include "dense.hpp"
+#include "kvcache.hpp"
 
 namespace wb {
 
@@ -90,6 +91,15 @@ Status mha_reserve(MhaCell* c, int bs, cudaStream_t st);
 // x [batch*seq][d_model] (device) -> attn [bs][q_dim] (pre) and y [bs][d_model] (post).
 Status mha_forward_device(MhaCell* c, int batch, int seq, const float* x, float* attn, float* y,
                           cudaStream_t st, const SplitNorm* norm = nullptr);
+
+// The cell over a paged cache (kvcache.hpp) of its own head counts and width, whose keys and values
+// outlive the call. Decode: one new token per sequence, x [num_seqs][d_model]: projections, rotary
+// and append, attention over each sequence's slots (the cell's mask, position kind and scale),
+// output projection. Prefill: a prompt of `tokens` rows for one sequence that holds nothing yet:
+// the cell's own attention among them, and their keys and values into the cache.
+Status mha_decode_device(MhaCell* c, KvCache* kv, const float* x, float* attn, float* y, bool accumulate, cudaStream_t st);
+Status mha_prefill_device(MhaCell* c, KvCache* kv, int sequence, int tokens, const float* x, float* attn, float* y,
+                          cudaStream_t st);
 
 // gamma f32 [dim] quantized with `dt` then decoded to f64 as the reference's gamma store.
 Status rmsnorm_gamma(int device, int dim, DType dt, const float* gamma, double** gamma64_dev, cudaStream_t st);

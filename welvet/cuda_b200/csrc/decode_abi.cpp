@@ -1,6 +1,6 @@
 // decode_abi.cpp -- extern "C" entry points of the decode step: the paged key-value cache
 // (kvcache.hpp) and the 4-bit group-scaled Dense layer (gdense.hpp).
-#include "../../../include/welvet_b200.h"
+#include "abi_handles.hpp"
 
 #include "dense.hpp"
 #include "gdense.hpp"
@@ -12,9 +12,6 @@
 #include <new>
 #include <string>
 
-struct welvet_b200_kv {
-  wb::KvCache* c;
-};
 struct welvet_b200_gdense {
   wb::GroupDense* g;
 };

@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_append(const __grid_constant
     if (t < p.a.rows) load(tid);
   }
   // the row's sequence: the last s with cu[s] <= t
-  int seq = t, i = 0;
+  int seq = p.a.only >= 0 ? p.a.only : t, i = p.a.only >= 0 ? t : 0;
   bool live = t < p.a.rows;
   if (p.a.cu) {
     int a = 0, b = c.num_seqs;  // cu[a] <= t < cu[b] is what a row of a sequence has
@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_append(const __grid_constant
   if (!s_last) return;
   if (tid == 0) *p.ticket = 0;
   for (int s = tid; s < c.num_seqs; s += kAppendThreads) {
-    const int n = p.a.cu ? p.a.cu[s + 1] - p.a.cu[s] : 1;
+    const int n = p.a.cu ? p.a.cu[s + 1] - p.a.cu[s] : (p.a.only < 0 ? 1 : (s == p.a.only ? p.a.rows : 0));
     const int64_t len = static_cast<int64_t>(p.a.start[s]) + n, tot = static_cast<int64_t>(p.a.start_seen[s]) + n;
     c.lens[s] = static_cast<int32_t>(len < c.max_slots ? len : c.max_slots);
     if (c.seen != c.lens) c.seen[s] = static_cast<int32_t>(tot);

@@ -80,6 +80,7 @@ struct KvAppendArgs {
   float* q_out = nullptr;
   int64_t k_ld = 0, v_ld = 0, q_ld = 0, q_out_ld = 0;
   const int32_t* cu = nullptr;  // [num_seqs + 1] first row of each sequence; null: one row each
+  int only = -1;                // >= 0: every row is this sequence's (cu null)
   double theta = 0.0;           // <= 0: no rotation
   const int32_t* start = nullptr;       // slots in use before the call (null: lens)
   const int32_t* start_seen = nullptr;  // tokens seen before the call (null: seen)

@@ -49,6 +49,9 @@ _sig("welvet_b200_gdense_mount", _ST, c_int32, c_int32, c_int32, c_int32, c_int3
 _sig("welvet_b200_gdense_execute_device", _ST, c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p)
 _sig("welvet_b200_gdense_release", None, c_void_p)
 
+_sig("welvet_b200_mha_decode_device", _ST, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p)
+_sig("welvet_b200_mha_prefill_device", _ST, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p)
+
 _append, _attend, _evict, _gemv = (_L.welvet_b200_kv_append, _L.welvet_b200_kv_attend, _L.welvet_b200_kv_evict,
                                    _L.welvet_b200_gdense_execute_device)
 _F32, _I32 = torch.float32, torch.int32
@@ -196,6 +199,26 @@ class PagedKV:
             self.release()
         except Exception:
             pass
+
+
+def _mha_rows(cell_d: int, rows: int, x, y, attn, width: int):
+    for t, w, what in ((x, cell_d, "x"), (y, cell_d, "y"), (attn, width, "attn")):
+        if t is not None and (t.dtype is not _F32 or not t.is_cuda or not t.is_contiguous() or t.shape != (rows, w)):
+            raise ValueError(f"{what}: expected a contiguous float32 CUDA tensor ({rows}, {w})")
+    return x.data_ptr(), None if attn is None else attn.data_ptr(), y.data_ptr()
+
+
+def mha_decode(cell, cache: PagedKV, x, y, attn=None, *, accumulate: bool = False, stream=None) -> None:
+    """One new token per sequence through an MhaCell over a cache: x, y [sequences, d_model]."""
+    xp, ap, yp = _mha_rows(cell.d_model, cache.num_seqs, x, y, attn, cache._qw)
+    check(_L.welvet_b200_mha_decode_device(cell._h, cache._h, xp, ap, yp, 1 if accumulate else 0, _stream(stream, x)))
+
+
+def mha_prefill(cell, cache: PagedKV, sequence: int, x, y, attn=None, *, stream=None) -> None:
+    """A prompt x [tokens, d_model] through an MhaCell, its keys and values into a sequence of the cache that
+    holds nothing yet."""
+    xp, ap, yp = _mha_rows(cell.d_model, x.shape[0], x, y, attn, cache._qw)
+    check(_L.welvet_b200_mha_prefill_device(cell._h, cache._h, sequence, x.shape[0], xp, ap, yp, _stream(stream, x)))
 
 
 def group_quantize(W, group: int, code: int, scale_dtype=torch.bfloat16, stream=None):
