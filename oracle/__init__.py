@@ -15,6 +15,7 @@ from __future__ import annotations
 import ctypes
 import os
 import subprocess
+import unittest
 from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int64, c_size_t, c_uint8, c_uint64, c_void_p
 
 import numpy as np
@@ -97,6 +98,8 @@ def ref():
     """The reference's own codec / store / Dense session, compiled from its sources."""
     global _ref
     if _ref is None:
+        if not ref_available():
+            raise unittest.SkipTest("oracle/_ref is not built (the reference tree is absent)")
         R = ctypes.CDLL(REF_SO)
         for n in ("ref_e4m3_encode", "ref_e5m2_encode", "ref_fp4_encode"):
             getattr(R, n).restype = c_uint8
