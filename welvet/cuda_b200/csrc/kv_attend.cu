@@ -8,12 +8,15 @@
 #include "kvcache.hpp"
 #include "pipeline.cuh"
 
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <cmath>
 
 namespace wb {
 namespace {
 
+constexpr int kMaxCluster = 8;  // blocks of a cluster
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct KvBytes {  // a pool's strides in bytes
@@ -33,6 +36,7 @@ struct AttendParams {
   int group;       // query heads per key-value head
   int head_groups; // of eight query heads of a key-value head
   int page_shift;  // log2(page_size), or -1
+  int cluster;     // blocks of a unit that join through distributed shared memory (0: runs)
   int2* spans;     // [num_seqs][num_kv]: first run and number of runs of a unit
 };
 
@@ -200,7 +204,9 @@ __global__ void k_attend_weights(const __grid_constant__ AttendParams p) {
 // are cut into equal runs, so that ragged lengths balance. A block takes a run; where a key-value
 // head has more than eight query heads, neighbouring blocks take the same run with eight each, so
 // that the second reads the rows from L2. A unit that lies within one run is finished there;
-// otherwise each run leaves its partial (o, m, l) and a second kernel joins them in run order. (Joined by the last block to arrive, behind a counter, one
+// otherwise each run leaves its partial (o, m, l) and a second kernel joins them in run order.
+// Small caches (attend_plan says when) instead give each unit a cluster of blocks with equal shares
+// of its tiles, which join through distributed shared memory: one launch. (Joined by the last block to arrive, behind a counter, one
 // sequence of 131072 slots took 53 us, the registers of that code among it.)
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
@@ -286,7 +292,9 @@ struct Tiled {
   static constexpr int kStages = kRow <= 256 || kRow > 384 ? 3 : 2;
   static constexpr int kDP = DP;
   static constexpr int kThreads = 32 * kWarps;
-  static constexpr int kBlocks = kRow <= 384 && DP <= 128 ? 2 : 1;  // of an SM (three, with 168 registers a thread, cost more)
+  // of an SM: three where a tile is small enough for 168 registers (160-byte rows; 128-byte rows, two
+  // blocks of keys a warp, took 245 us for 157)
+  static constexpr int kBlocks = kRow == 160 ? 3 : (kRow <= 384 && DP <= 128 ? 2 : 1);
   static constexpr int kKeys = 16 * kSub * kWarps;  // keys of a block tile
   static constexpr int kLanes = kRow <= 64 ? 4 : 8;  // lanes that copy a row
   static constexpr int kSets = kBF16 ? 2 : 1;
@@ -333,6 +341,59 @@ __device__ __forceinline__ float exp2_fast(float x) {  // ex2.approx: 2 ulp, 2^-
   return y;
 }
 
+// Each block of a cluster adds its share of the values over all of them, in rank order. Out of line:
+// its registers are not the main loop's.
+template <typename G>
+__device__ __noinline__ void join_cluster(const AttendParams& p, float* s_o, float* s_bm, float* s_bl, int heads, int D, float* out,
+                                          float* lse) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = static_cast<int>(cluster.block_rank()), d4 = D / 4;
+  for (int i = rank * G::kThreads + threadIdx.x; i < heads * d4; i += p.cluster * G::kThreads) {
+    const int h = i / d4, d = 4 * (i - h * d4);
+    float m[kMaxCluster], mm = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < kMaxCluster; ++r) {
+      m[r] = r < p.cluster ? cluster.map_shared_rank(s_bm, r)[h] : -INFINITY;
+      mm = fmaxf(mm, m[r]);
+    }
+    const float ref = mm == -INFINITY ? 0.0f : mm;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float ll = 0.0f;
+#pragma unroll
+    for (int r0 = 0; r0 < kMaxCluster; r0 += 4) {
+      float l[4];
+      float4 o[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        l[x] = 0.0f;
+        o[x] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (r0 + x < p.cluster) {
+          l[x] = cluster.map_shared_rank(s_bl, r0 + x)[h];
+          o[x] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(s_o, r0 + x) + h * D + d);
+        }
+      }
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        if (l[x] == 0.0f) continue;  // no key allowed there, or no tile
+        const float f = exp2f(m[r0 + x] - ref);
+        v.x += o[x].x * f;
+        v.y += o[x].y * f;
+        v.z += o[x].z * f;
+        v.w += o[x].w * f;
+        ll += l[x] * f;
+      }
+    }
+    const float f = ll == 0.0f ? 0.0f : p.c.v_scale / ll;
+    float* to = out + h * D + d;
+    to[0] = ll == 0.0f ? 0.0f : v.x * f;
+    to[1] = ll == 0.0f ? 0.0f : v.y * f;
+    to[2] = ll == 0.0f ? 0.0f : v.z * f;
+    to[3] = ll == 0.0f ? 0.0f : v.w * f;
+    if (lse && d == 0) lse[h] = ll == 0.0f ? INFINITY : ref - G::kBias + log2f(ll);
+  }
+}
+
 template <typename T, int DP, bool kFull>
 __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kFull>::kBlocks) k_attend_tiled(const __grid_constant__ AttendParams p) {
   using G = Tiled<T, DP, kFull>;
@@ -340,6 +401,7 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int s_sum[G::kWarps], s_rest[G::kWarps];
   __shared__ int s_b, s_off;
+  __shared__ float s_bm[8], s_bl[8];  // the block's maximum and sum per head, for its cluster
   __shared__ float s_m[G::kWarps][8], s_l[G::kWarps][8], s_mult[8];
   __shared__ uint32_t s_ok[G::kWarps][G::kStages];
   const KvView& c = p.c;
@@ -377,75 +439,90 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
     cursor_seq(p, G::kKeys, s);
     return (s.nt + kOver) * c.num_kv;
   };
-  int mine = places(tid), scan = mine, rest = 0;
-  for (int b = tid + G::kThreads; b < c.num_seqs; b += G::kThreads) rest += places(b);
-  if (blockIdx.x == 0)
-    for (int b = tid; b < c.num_seqs; b += G::kThreads)
-      if (c.lens[b] < 0 || c.lens[b] > c.max_slots) atomicCAS(c.err, 0, kKvErrSlot);
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, scan, o);
-    if (lane >= o) scan += y;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
-  if (lane == 31) s_sum[w] = scan;
-  if (lane == 0) s_rest[w] = rest;
-  __syncthreads();
-  int before = 0, chunk = 0, total = 0;
-#pragma unroll
-  for (int i = 0; i < G::kWarps; ++i) {
-    if (i < w) before += s_sum[i];
-    chunk += s_sum[i];
-    total += s_rest[i];
-  }
-  total += chunk;
-  // A unit cut into P runs costs about P / 50 tiles of joining: runs are at least as long as
-  // balances that, and never empty.
-  const float tiles = static_cast<float>(total) / static_cast<float>(c.num_seqs * c.num_kv);
-  const int shortest = max(1, static_cast<int>(sqrtf(tiles * (1.0f / 50.0f))));
-  const int n_runs = max(1, min(static_cast<int>(gridDim.x) / p.head_groups, total / shortest));
-  const int run = blockIdx.x / p.head_groups, hg = blockIdx.x - run * p.head_groups;
-  if (run >= n_runs) return;
-  const int t0 = static_cast<int>(static_cast<int64_t>(run) * total / n_runs);
-  const int t1 = static_cast<int>(static_cast<int64_t>(run + 1) * total / n_runs);
-  for (int base = 0, acc = 0;;) {
-    const int end = acc + before + scan;  // of this thread's sequence
-    if (end - mine <= t0 && t0 < end) {
-      s_b = base + tid;
-      s_off = t0 - (end - mine);
-    }
-    acc += chunk;
-    if (t0 < acc) break;
-    base += G::kThreads;
-    mine = scan = places(base + tid);
+  Cursor cur;
+  int t0, t1, n_runs = 1, run = 0, hg, total = 0;
+  if (p.cluster > 0) {
+    const int unit = blockIdx.x / p.cluster, rank = blockIdx.x - unit * p.cluster;
+    hg = unit % p.head_groups;
+    cur.b = unit / p.head_groups / c.num_kv;
+    cur.kv = unit / p.head_groups - cur.b * c.num_kv;
+    cursor_seq(p, G::kKeys, cur);
+    t0 = rank * cur.nt / p.cluster;
+    t1 = (rank + 1) * cur.nt / p.cluster;
+    cur.at = cur.tile = t0;
+    if (tid == 0 && (c.lens[cur.b] < 0 || c.lens[cur.b] > c.max_slots)) atomicCAS(c.err, 0, kKvErrSlot);
+  } else {
+    int mine = places(tid), scan = mine, rest = 0;
+    for (int b = tid + G::kThreads; b < c.num_seqs; b += G::kThreads) rest += places(b);
+    if (blockIdx.x == 0)
+      for (int b = tid; b < c.num_seqs; b += G::kThreads)
+        if (c.lens[b] < 0 || c.lens[b] > c.max_slots) atomicCAS(c.err, 0, kKvErrSlot);
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, scan, o);
       if (lane >= o) scan += y;
     }
-    __syncthreads();
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
     if (lane == 31) s_sum[w] = scan;
+    if (lane == 0) s_rest[w] = rest;
     __syncthreads();
-    before = chunk = 0;
+    int before = 0, chunk = 0;
 #pragma unroll
     for (int i = 0; i < G::kWarps; ++i) {
       if (i < w) before += s_sum[i];
       chunk += s_sum[i];
+      total += s_rest[i];
+    }
+    total += chunk;
+    // A unit cut into P runs costs about P / 50 tiles of joining: runs are at least as long as
+    // balances that, and never empty.
+    const float tiles = static_cast<float>(total) / static_cast<float>(c.num_seqs * c.num_kv);
+    const int shortest = max(1, static_cast<int>(sqrtf(tiles * (1.0f / 50.0f))));
+    n_runs = max(1, min(static_cast<int>(gridDim.x) / p.head_groups, total / shortest));
+    run = blockIdx.x / p.head_groups;
+    hg = blockIdx.x - run * p.head_groups;
+    if (run >= n_runs) return;
+    t0 = static_cast<int>(static_cast<int64_t>(run) * total / n_runs);
+    t1 = static_cast<int>(static_cast<int64_t>(run + 1) * total / n_runs);
+    for (int base = 0, acc = 0;;) {
+      const int end = acc + before + scan;  // of this thread's sequence
+      if (end - mine <= t0 && t0 < end) {
+        s_b = base + tid;
+        s_off = t0 - (end - mine);
+      }
+      acc += chunk;
+      if (t0 < acc) break;
+      base += G::kThreads;
+      mine = scan = places(base + tid);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += y;
+      }
+      __syncthreads();
+      if (lane == 31) s_sum[w] = scan;
+      __syncthreads();
+      before = chunk = 0;
+#pragma unroll
+      for (int i = 0; i < G::kWarps; ++i) {
+        if (i < w) before += s_sum[i];
+        chunk += s_sum[i];
+      }
+    }
+    __syncthreads();
+    cur.b = s_b;
+    cursor_seq(p, G::kKeys, cur);
+    cur.kv = s_off / (cur.nt + kOver);
+    cur.tile = s_off - cur.kv * (cur.nt + kOver) - kOver;
+    cur.at = t0;
+    if (cur.tile < 0) {
+      cur.at -= cur.tile;
+      cur.tile = 0;
     }
   }
-  __syncthreads();
-  Cursor cur;
-  cur.b = s_b;
-  cursor_seq(p, G::kKeys, cur);
-  cur.kv = s_off / (cur.nt + kOver);
-  cur.tile = s_off - cur.kv * (cur.nt + kOver) - kOver;
-  cur.at = t0;
-  if (cur.tile < 0) {
-    cur.at -= cur.tile;
-    cur.tile = 0;
-  }
   Cursor nxt = cur;
+  const int cur_b = cur.b, cur_kv = cur.kv;  // a cluster's unit
 
   // Copies the warp's keys and values of the tile at `nxt`; rows that the mask leaves out are
   // zeros (their contents, even NaN, must not reach the sums).
@@ -872,7 +949,13 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
           v.w += y.w * f;
           ll += s_l[x][h] * f;
         }
-        if (whole) {
+        if (p.cluster > 0) {
+          *reinterpret_cast<float4*>(reinterpret_cast<float*>(sq) + h * D + d) = v;
+          if (d == 0) {
+            s_bm[h] = mm;
+            s_bl[h] = ll;
+          }
+        } else if (whole) {
           const float f = ll == 0.0f ? 0.0f : c.v_scale / ll;
           float* to = out + h * D + d;
           to[0] = ll == 0.0f ? 0.0f : v.x * f;
@@ -889,7 +972,7 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
           }
         }
       }
-      if (unit_start >= t0 && hg == 0 && tid == 0) {  // the run that began the unit says where its parts are
+      if (p.cluster == 0 && unit_start >= t0 && hg == 0 && tid == 0) {  // the run that began the unit says where its parts are
         const int last = static_cast<int>((static_cast<int64_t>(unit_start + cur.nt) * n_runs - 1) / total);
         p.spans[cur.b * c.num_kv + kv] = make_int2(run, last - run + 1);
       }
@@ -904,6 +987,21 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
     cursor_next(p, G::kKeys, cur);
   }
   cp_wait<0>();
+  if (p.cluster == 0) return;
+
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int heads = min(p.group - 8 * hg, 8), head = cur_kv * p.group + 8 * hg, rank = static_cast<int>(cluster.block_rank());
+  if (t0 == t1 && tid < 8) {  // a block without tiles has nothing to add
+    s_bm[tid] = -INFINITY;
+    s_bl[tid] = 0.0f;
+  }
+  cluster.sync();
+  join_cluster<G>(p, reinterpret_cast<float*>(sq), s_bm, s_bl, heads, D,
+                  p.a.out + cur_b * p.a.out_ld + static_cast<int64_t>(head) * D,
+                  p.a.accumulate ? p.lse + static_cast<int64_t>(cur_b) * c.num_heads + head : nullptr);
+  if (p.a.accumulate && rank == 0 && hg == 0 && tid == 0) p.spans[cur_b * c.num_kv + cur_kv] = make_int2(0, 1);
+  cluster.sync();  // no block leaves while another reads its shared memory
 }
 
 // What is left once all runs are done. Blocks below num_heads join the parts of one query head in
@@ -1062,6 +1160,28 @@ Status attend_plan(KvCache* c) {
     const int hg = head_groups(v);
     c->attend_blocks = static_cast<int>(std::min<int64_t>(std::max(1, per_sm * sms / hg), most)) * hg;
     c->part_bytes = static_cast<size_t>(c->attend_blocks) * 2 * 8 * (v.head_dim + 4) * 4;
+    // Clusters where all of them are resident together and a block's tiles are so few that ragged
+    // lengths cannot cost more than the second launch (one sequence of 500 slots, 16 heads: 6.0 us
+    // against 7.9; with 16 tiles a block they are the slower form, 19 us against 17).
+    const int64_t tiles = (v.max_slots + G::kKeys - 1) / G::kKeys;
+    int size = kMaxCluster;
+    while (size > 1 && (units * hg * size > static_cast<int64_t>(per_sm) * sms || size > tiles)) size /= 2;
+    if (size > 1 && tiles <= 4 * size) {
+      cudaLaunchConfig_t cfg{};
+      cudaLaunchAttribute at[1];
+      at[0].id = cudaLaunchAttributeClusterDimension;
+      cfg.blockDim = dim3(G::kThreads);
+      cfg.dynamicSmemBytes = G::kSmem;
+      cfg.attrs = at;
+      cfg.numAttrs = 1;
+      for (int fit = 0; size > 1; size /= 2) {
+        at[0].val.clusterDim = {static_cast<unsigned>(size), 1, 1};
+        cfg.gridDim = dim3(static_cast<unsigned>(units * hg * size));
+        WB_CUDA(cudaOccupancyMaxActiveClusters(&fit, kernel, &cfg));
+        if (fit >= units * hg) break;
+      }
+      if (size > 1 && tiles <= 4 * size) c->attend_cluster = size;
+    }
     c->span_bytes = static_cast<size_t>(units) * 8;
     return Status::Ok();
   });
@@ -1093,9 +1213,11 @@ Status kv_attend(KvCache* c, const KvAttendArgs& a, cudaStream_t st) {
     p.same = p.kb.page == p.vb.page && p.kb.slot == p.vb.slot && p.kb.head == p.vb.head;
     WB_TRY(by_shape(v, c->type, [&](auto g, auto* kernel) {
       using G = decltype(g);
-      WB_TRY(launch_after(kernel, dim3(c->attend_blocks), G::kThreads, G::kSmem, st, p));
+      p.cluster = c->attend_cluster;
+      const int blocks = p.cluster > 0 ? v.num_seqs * v.num_kv * p.head_groups * p.cluster : c->attend_blocks;
+      WB_TRY(launch_after(kernel, dim3(blocks), G::kThreads, G::kSmem, st, p, p.cluster));
       // a unit of one tile is never cut
-      if (v.max_slots <= G::kKeys && !a.accumulate) return Status::Ok();
+      if ((p.cluster > 0 || v.max_slots <= G::kKeys) && !a.accumulate) return Status::Ok();
       const int chunks = a.accumulate ? std::min((v.max_slots + 1023) / 1024, 64) : 0;
       return launch_after(k_attend_finish<static_cast<int>(G::kBias)>, dim3(H + v.num_kv * chunks, B), 128, 0, st, p);
     }));

@@ -68,8 +68,8 @@ Status by_type(KvType t, F&& f) {
 
 // A launch that may start while the kernel before it still runs (it waits for its results itself).
 template <typename K, typename P>
-Status launch_after(K* kernel, dim3 grid, int threads, int smem, cudaStream_t st, const P& p) {
-  cudaLaunchAttribute at[1];
+Status launch_after(K* kernel, dim3 grid, int threads, int smem, cudaStream_t st, const P& p, int cluster = 0) {
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
@@ -77,8 +77,10 @@ Status launch_after(K* kernel, dim3 grid, int threads, int smem, cudaStream_t st
   cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim = {static_cast<unsigned>(cluster), 1, 1};
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
   return cuda_status(cudaLaunchKernelEx(&cfg, kernel, p), "kv launch");
 }
 

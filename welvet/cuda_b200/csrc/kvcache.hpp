@@ -56,6 +56,7 @@ struct KvCache {
   // attend (kv_attend.cu)
   bool attend_tiled = false;
   int attend_blocks = 0;         // blocks of the tiled form
+  int attend_cluster = 0;        // blocks of a unit's cluster (0: runs of tiles)
   size_t part_bytes = 0, span_bytes = 0;
   float* part = nullptr;         // partial results
   void* spans = nullptr;         // where each unit's parts are
