@@ -108,14 +108,15 @@ __global__ void __launch_bounds__(128) k_group_build(const __grid_constant__ Bui
 //
 // The records (row group by row group, chunk by chunk) are cut into equal runs. Layers that give
 // every warp a row group or more make the runs the warps', which then never wait for one another;
-// smaller ones make them the blocks', whose warps take every 16th record and add their sums in
-// shared memory. Row groups that a run's ends cut are joined through global memory by the last run
+// smaller ones make them the blocks', whose warps take every 16th record and leave their sums in
+// shared memory, where those of up to eight row groups are added and finished together. Row groups that a run's ends cut are joined through global memory by the last run
 // to come, in run order; small layers avoid that with runs of whole row groups. The first weight
 // loads start before the previous kernel's end is waited for.
 constexpr int kMaxTokens = 8;
 constexpr int kGWarps = 16;
 constexpr int kGThreads = 32 * kGWarps;
-constexpr int kXBytes = 200 * 1024;  // shared memory for x
+constexpr int kXBytes = 140 * 1024;  // shared memory for x
+constexpr int kHold = 8;             // row groups whose sums wait in shared memory for one barrier
 
 struct GArgs {
   const uint8_t* w;
@@ -224,7 +225,6 @@ template <int kCode, int kNT, int kSub, int kScale>
 __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_constant__ GArgs a) {
   using Record = GRecord<kCode, kSub>;
   extern __shared__ __align__(128) uint8_t sx[];  // x parts: [2 n columns][slab inputs] f16
-  __shared__ float s_red[2][kGWarps][16][4 * kNT];
   __shared__ __align__(16) uint8_t s_zero[kChunk * 2];
   __shared__ int s_last;
   const int tid = threadIdx.x, lane = tid & 31, w = tid >> 5, g = lane >> 2, t = lane & 3;
@@ -232,6 +232,8 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
   const int c_first = slab * a.slab_chunks, chunks = min(a.slab_chunks, a.l.chunks - c_first);
   const int pitch = a.slab_chunks * (kChunk * 2) + 64;  // bytes of a column; two columns fill the banks
   float* const sxs = reinterpret_cast<float*>(sx + 2 * a.n * pitch);  // [token][chunk] 2^-e
+  constexpr int kOuts = 16 * 4 * kNT;  // sums of a row group: [row][token]
+  float* const s_red = sxs + (a.n * a.slab_chunks + 3) / 4 * 4;  // [kHold][warp][kOuts], not with runs of the warps
 
   asm volatile("griddepcontrol.launch_dependents;");
   // this block's or this warp's run of records, and the warp's share of it: every step-th from first_rec
@@ -286,6 +288,7 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // x: a warp takes a token's chunk at a time, eight inputs a lane
   const bool vec = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.x_ld & 3) == 0;
+  const bool vec2 = (reinterpret_cast<uintptr_t>(a.x) & 7) == 0 && (a.x_ld & 1) == 0;
   constexpr int kFly = 4;  // chunks whose loads are in flight together
   for (int i0 = w; i0 < a.n * chunks; i0 += kFly * kGWarps) {
     float v[kFly][8];
@@ -298,6 +301,9 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
       if (vec && on && k0 + 8 <= a.cols) {
         *reinterpret_cast<float4*>(v[y]) = ld_dep4(xs);
         *reinterpret_cast<float4*>(v[y] + 4) = ld_dep4(xs + 4);
+      } else if (vec2 && on && k0 + 8 <= a.cols) {
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) asm volatile("ld.global.v2.f32 {%0, %1}, [%2];" : "=f"(v[y][e]), "=f"(v[y][e + 1]) : "l"(xs + e));
       } else {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[y][e] = on && k0 + e < a.cols ? ld_dep(xs + e) : 0.0f;
@@ -349,7 +355,26 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
 #pragma unroll
     for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
 
-  int buf = 0;
+  auto write = [&](int rs, int r, int b, float v) {
+    const int o = rs * 16 + r;
+    if (o >= a.rows) return;
+    if (a.slabs == 1) g_write(a, o, b, v);
+    else a.slab_sum[(static_cast<int64_t>(slab) * a.n + b) * a.rows + o] = v;
+  };
+  // The runs that cut a row group leave their sums; the last one to come adds them in run order. A
+  // run has two slots: the second for a row group that begins in it, the first for one that goes on.
+  constexpr int kSlot = 16 * kMaxTokens;
+  auto run_of = [&](int rec) { return static_cast<int>((static_cast<int64_t>(rec + 1) * runs - 1) / total); };
+  auto slot_of = [&](int begin) { return a.part + (2 * (static_cast<int64_t>(slab) * runs + run) + (begin >= r0 ? 1 : 0)) * kSlot; };
+  auto ticket_of = [&](int rs) { return a.tickets + static_cast<int64_t>(slab) * a.l.row_groups + rs; };
+  auto joined = [&](int begin, int i) {
+    const int run0 = run_of(begin), run1 = run_of(begin + chunks - 1);
+    const float* cut = a.part + 2 * (static_cast<int64_t>(slab) * runs + run0) * kSlot + i;
+    float v = __ldcg(cut + kSlot);
+    for (int x = 1; x <= run1 - run0; ++x) v += __ldcg(cut + 2ll * x * kSlot);
+    return v;
+  };
+  int held = 0;          // row groups in s_red
   int next = first_rec;  // the warp's next record
   bool turn = false;
   int rs = r0 / chunks;
@@ -420,42 +445,23 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
       else record(rec_a, rec_b);
       turn = !turn;
     }
-    const int run0 = whole ? 0 : static_cast<int>((static_cast<int64_t>(set_begin + 1) * runs - 1) / total);
-    const int run1 = whole ? 0 : static_cast<int>((static_cast<int64_t>(set_end) * runs - 1) / total);
-    int* const ticket = a.tickets + static_cast<int64_t>(slab) * a.l.row_groups + rs;
-    auto write = [&](int r, int b, float v) {
-      const int o = rs * 16 + r;
-      if (o >= a.rows) return;
-      if (a.slabs == 1) g_write(a, o, b, v);
-      else a.slab_sum[(static_cast<int64_t>(slab) * a.n + b) * a.rows + o] = v;
-    };
-    // The runs that cut a row group leave their sums in order of the runs; the last one to come adds
-    // them: the first run's lie in its second slot, the others' in their first.
-    constexpr int kSlot = 16 * kMaxTokens;
-    float* const mine = a.part + (2 * (static_cast<int64_t>(slab) * runs + run) + (seg == set_begin ? 1 : 0)) * kSlot;
-    const float* const cut = a.part + 2 * (static_cast<int64_t>(slab) * runs + run0) * kSlot;
-    auto joined = [&](int i) {
-      float v = __ldcg(cut + kSlot + i);
-      for (int x = 1; x <= run1 - run0; ++x) v += __ldcg(cut + 2ll * x * kSlot + i);
-      return v;
-    };
     if (a.solo) {
       bool last = true;
       if (!whole) {
 #pragma unroll
         for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) mine[(g + 8 * e) * kMaxTokens + 4 * nt + t] = acc[nt][2 * e] + acc[nt][2 * e + 1];
+          for (int e = 0; e < 2; ++e) slot_of(set_begin)[(g + 8 * e) * kMaxTokens + 4 * nt + t] = acc[nt][2 * e] + acc[nt][2 * e + 1];
         __syncwarp();
         int before = 0;
         if (lane == 0) {
           __threadfence();
-          before = atomicAdd(ticket, 1);
+          before = atomicAdd(ticket_of(rs), 1);
         }
-        last = __shfl_sync(0xffffffffu, before, 0) == run1 - run0;
+        last = __shfl_sync(0xffffffffu, before, 0) == run_of(set_end - 1) - run_of(set_begin);
         if (last) {
           __threadfence();
-          if (lane == 0) *ticket = 0;
+          if (lane == 0) *ticket_of(rs) = 0;
         }
       }
       if (last) {
@@ -464,44 +470,54 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int r = g + 8 * e, b = 4 * nt + t;
-            if (b < a.n) write(r, b, whole ? acc[nt][2 * e] + acc[nt][2 * e + 1] : joined(r * kMaxTokens + b));
+            if (b < a.n) write(rs, r, b, whole ? acc[nt][2 * e] + acc[nt][2 * e + 1] : joined(set_begin, r * kMaxTokens + b));
           }
       }
     } else {
-      // the row group's sums over the warps
+      float* const to = s_red + (held * kGWarps + w) * kOuts;
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) s_red[buf][w][g + 8 * e][4 * nt + t] = acc[nt][2 * e] + acc[nt][2 * e + 1];
-      __syncthreads();
-      const int r = tid & 15, b = tid >> 4;  // 16 rows x at most 8 tokens: one output a thread
-      float v = 0.0f;
-      if (b < a.n) {
+        for (int e = 0; e < 2; ++e) to[(g + 8 * e) * (4 * kNT) + 4 * nt + t] = acc[nt][2 * e] + acc[nt][2 * e + 1];
+      if (++held == kHold || end == r1) {
+        // add the warps' sums of the row groups held, finish those that are whole
+        __syncthreads();
+        const int first_rs = rs + 1 - held;
+        for (int i = tid; i < held * kOuts; i += kGThreads) {
+          const int x = i / kOuts, at = i - x * kOuts, r = at / (4 * kNT), b = at - r * (4 * kNT);
+          if (b >= a.n) continue;
+          float v = 0.0f;
 #pragma unroll
-        for (int x = 0; x < kGWarps; ++x) v += s_red[buf][x][r][b];
-      }
-      if (whole) {
-        if (b < a.n) write(r, b, v);
-      } else {
-        if (b < a.n) mine[r * kMaxTokens + b] = v;
-        __syncthreads();
-        if (tid == 0) {
-          __threadfence();
-          s_last = atomicAdd(ticket, 1) == run1 - run0;
+          for (int y = 0; y < kGWarps; ++y) v += s_red[(x * kGWarps + y) * kOuts + at];
+          const int begin = (first_rs + x) * chunks;
+          if (begin >= r0 && begin + chunks <= r1) write(first_rs + x, r, b, v);
+          else slot_of(begin)[r * kMaxTokens + b] = v;
         }
-        __syncthreads();
-        if (s_last) {
-          __threadfence();
-          if (tid == 0) *ticket = 0;
-          if (b < a.n) write(r, b, joined(r * kMaxTokens + b));
+        // at most the first and the last row group of the run are cut
+        for (int x = 0; x < held; ++x) {
+          const int cut_rs = first_rs + x, begin = cut_rs * chunks;
+          if (begin >= r0 && begin + chunks <= r1) continue;
+          __syncthreads();
+          if (tid == 0) {
+            __threadfence();
+            s_last = atomicAdd(ticket_of(cut_rs), 1) == run_of(begin + chunks - 1) - run_of(begin);
+          }
+          __syncthreads();
+          if (s_last) {
+            __threadfence();
+            if (tid == 0) *ticket_of(cut_rs) = 0;
+            const int r = tid & 15, b = tid >> 4;
+            if (b < a.n) write(cut_rs, r, b, joined(begin, r * kMaxTokens + b));
+          }
         }
+        held = 0;
+        if (end < r1) __syncthreads();  // before the next sums are left there
       }
     }
 #pragma unroll
     for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) acc[nt][e] = 0.0f;
-    buf ^= 1;
     seg = end;
   }
 }
@@ -588,14 +604,15 @@ GPlan plan_of(const GroupDense& g, const Layout& l, int n) {
   p.slabs = (l.chunks + fit - 1) / fit;
   p.slab_chunks = (l.chunks + p.slabs - 1) / p.slabs;
   p.slabs = (l.chunks + p.slab_chunks - 1) / p.slab_chunks;
-  p.smem = 2 * n * (p.slab_chunks * kChunk * 2 + 64) + n * p.slab_chunks * 4;
   // every warp of a block has a record or more
   const int64_t last = l.chunks - (p.slabs - 1) * p.slab_chunks;
   const int64_t most = std::max<int64_t>(1, l.row_groups * last / kGWarps);
   p.slab_blocks = static_cast<int>(std::min<int64_t>(std::max(1, g.sms / p.slabs), most));
   p.solo = l.row_groups >= p.slab_blocks * kGWarps;
   p.aligned = 0;
+  p.smem = 2 * n * (p.slab_chunks * kChunk * 2 + 64) + (n * p.slab_chunks + 3) / 4 * 16;
   if (!p.solo) {
+    p.smem += kHold * kGWarps * 16 * (n > 4 ? 8 : 4) * 4;
     // Whole row groups leave blocks idle for part of the last round; cut ones cost a join of about
     // 2.5 us at the run's end. At 5 TB/s a microsecond is 5 MB of records.
     const int per = (l.row_groups + p.slab_blocks - 1) / p.slab_blocks;
@@ -693,7 +710,7 @@ Status gdense_fill(GroupDense* g, const GroupDenseSrc& src) {
     part = std::max<size_t>(part, static_cast<size_t>(p.slabs) * p.slab_blocks * (p.solo ? kGWarps : 1) * 2 * 16 * kMaxTokens * 4);
     tickets = std::max<size_t>(tickets, static_cast<size_t>(p.slabs) * b.l.row_groups * 4);
     if (p.slabs > 1) slabs = std::max<size_t>(slabs, static_cast<size_t>(p.slabs) * n * g->rows * 4);
-    WB_CUDA(cudaFuncSetAttribute(kernel_of(*g, b.l, n), cudaFuncAttributeMaxDynamicSharedMemorySize, kXBytes));
+    WB_CUDA(cudaFuncSetAttribute(kernel_of(*g, b.l, n), cudaFuncAttributeMaxDynamicSharedMemorySize, kXBytes + kHold * kGWarps * 16 * 8 * 4 + 64));
   }
   auto up = [](size_t n) { return (n + 255) / 256 * 256; };
   WB_CUDA(cudaMalloc(&g->work, up(tickets) + up(part) + up(slabs)));
