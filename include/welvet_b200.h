@@ -312,13 +312,15 @@ WELVET_API welvet_status welvet_b200_group_quantize(int32_t in, int32_t out, int
 
 typedef struct welvet_b200_gdense welvet_b200_gdense;
 /* Copies the arrays (device or host per weights_on_device; zeros with Uint4 only) into the layout
- * the kernels read. bias: host, rows o < bias_len, as in welvet_dense_mount. Synchronous. */
+ * the kernels read. bias: host, rows o < bias_len, as in welvet_dense_mount. Synchronous, on the
+ * default stream: device arrays must have been written by then. */
 WELVET_API welvet_status welvet_b200_gdense_mount(int32_t in, int32_t out, int32_t group, int32_t code,
                                                   int32_t scale_dtype, int32_t act, const uint8_t* codes,
                                                   const void* scales, const uint8_t* zeros, int32_t weights_on_device,
                                                   const double* bias, size_t bias_len, welvet_b200_gdense** g_out);
 /* x_dev [rows][in] (rows x_ld apart) -> pre_dev (may be NULL), post_dev [rows][out], asynchronous on
- * `stream`. Made for 1..8 rows; more rows run in passes of 8 over the weights. */
+ * `stream`; allocates nothing, can be captured, must not overlap another call on the same handle, and
+ * the outputs must not overlap x. Made for 1..8 rows; more rows run in passes of 8 over the weights. */
 WELVET_API welvet_status welvet_b200_gdense_execute_device(welvet_b200_gdense* g, int32_t rows, const float* x_dev,
                                                            int64_t x_ld, float* pre_dev, float* post_dev, void* stream);
 WELVET_API void welvet_b200_gdense_release(welvet_b200_gdense* g);

@@ -752,3 +752,53 @@ def test_append_rotates_q_in_place(D, dim, shift):
     want = rotate64(x, pos.astype(np.float64), 10000.0)
     got = g.cpu().numpy().reshape(n, H, dim)
     assert np.all(np.abs(got - want) <= rotation_bound(x, 10000.0) + EPS * np.abs(want))
+
+
+def test_create_without_memory_leaves_no_trace(D, wb):
+    """Workspaces that no GPU holds: the create fails, and the next cache's launches are not blamed for it."""
+    import ctypes
+
+    import torch
+    big = D._KvDesc(dtype=3, num_heads=60000, num_kv_heads=60000, head_dim=64, page_size=1024, num_pages=10, num_seqs=60000,
+                    pages_per_seq=1024, k_pages=4096, v_pages=4096, k_strides=(ctypes.c_int64 * 3)(2 ** 32, 2 ** 22, 64),
+                    v_strides=(ctypes.c_int64 * 3)(2 ** 32, 2 ** 22, 64), k_scale=1.0, v_scale=1.0, page_table=4096,
+                    table_stride=1024, lens=4096, weights=4096)
+    h = ctypes.c_void_p()
+    st = wb.lib().welvet_b200_kv_create(ctypes.byref(big), ctypes.byref(h))
+    assert st.code == 4 and not h
+    rng = np.random.default_rng(41)
+    kp, vp, table = make_cache(rng, "bf16", 1, 2, 16, 1, 33)  # the form with plain launches
+    q = torch.from_numpy(rng.standard_normal((1, 2, 33)).astype(np.float32)).cuda()
+    out = torch.empty((1, 2, 33), device="cuda")
+    D.PagedKV(kp, vp, table, i32([20]), num_heads=2).attend(q, out)
+    want, _, bound = attend64(q, kp, vp, table, [20], 33 ** -0.5)
+    assert np.all(np.abs(out.cpu().numpy() - want) <= bound)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("n,kv,per", [(1, 1, 2), (1, 4, 30), (3, 2, 8), (2, 8, 33)])
+def test_attend_small_caches(D, dtype, n, kv, per):
+    """Caches small enough for clusters: lengths that leave some of their blocks without a tile, windows that
+    start inside one, weights summed."""
+    import torch
+    rng = np.random.default_rng(n * 100 + per)
+    H, dim, page = kv * 3, 128, 16
+    S = per * page
+    kp, vp, table = make_cache(rng, dtype, n, per, page, kv, dim)
+    q = torch.from_numpy(rng.standard_normal((n, H, dim)).astype(np.float32)).cuda()
+    out = torch.empty((n, H, dim), device="cuda")
+    w = torch.zeros((n, kv, S), device="cuda")
+    lens = i32([0] * n)
+    c = D.PagedKV(kp, vp, table, lens, num_heads=H, weights=w)
+    for base, window in ((S, 0), (1, 0), (S - 1, 0), (S // 2 + 1, 37), (0, 0), (17, 5)):
+        now = [max(0, base - 5 * i) for i in range(n)]
+        lens.copy_(i32(now))
+        w.zero_()
+        c.attend(q, out, window=window, accumulate=True)
+        want, ws, bound = attend64(q, kp, vp, table, now, dim ** -0.5, window)
+        assert np.all(np.abs(out.cpu().numpy() - want) <= bound)
+        got = w.cpu().numpy()
+        for b, L in enumerate(now):
+            np.testing.assert_allclose(got[b, :, :L], ws[b].reshape(kv, 3, L).sum(1), rtol=2e-4, atol=4 * EPS)
+            assert not got[b, :, L:].any()
+    c.check_error()

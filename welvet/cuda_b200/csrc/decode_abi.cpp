@@ -91,8 +91,8 @@ welvet_status welvet_b200_kv_create(const welvet_b200_kv_desc* desc, welvet_b200
     if (d.table_stride < d.pages_per_seq && d.num_seqs > 1) return wb::Status::Invalid("kv: table_stride < pages_per_seq");
     if (!d.page_table || !d.lens) return wb::Status::Invalid("kv: nil page_table or lens");
     if (d.positions && !d.seen) return wb::Status::Invalid("kv: positions without seen");
-    if (!(d.k_scale > 0.0f) || !(d.v_scale > 0.0f) || !std::isfinite(d.k_scale) || !std::isfinite(d.v_scale))
-      return wb::Status::Invalid("kv: k_scale and v_scale must be positive and finite");
+    if (!(d.k_scale > 0.0f) || !(d.v_scale > 0.0f) || !std::isnormal(d.k_scale) || !std::isnormal(d.v_scale))
+      return wb::Status::Invalid("kv: k_scale and v_scale must be positive, finite and normal");
     wb::KvView v;
     const auto type = static_cast<wb::KvType>(d.dtype);
     WB_TRY(pool_of("k_pages", d.k_pages, d.k_strides, d, wb::kv_size(type), &v.k));
@@ -226,6 +226,7 @@ static wb::Status group_shape(int32_t in, int32_t out, int32_t group, int32_t co
     return wb::Status::Unsupported("group dense: scale dtype id " + std::to_string(scale_dtype) + " (Float16 or BFloat16)");
   if (group != 32 && (group <= 0 || group % 64 != 0))
     return wb::Status::Unsupported("group dense: group must be 32 or a multiple of 64");
+  if (group > (1 << 20)) return wb::Status::Unsupported("group dense: group > 2^20");
   return wb::Status::Ok();
 }
 

@@ -736,6 +736,7 @@ Status gdense_mount(int device, int rows, int cols, int group, int code, int sca
   g->act = act;
   const Status st = gdense_fill(g, src);
   if (!st.ok()) {
+    cudaGetLastError();  // a failed allocation must not be taken for a later launch's error
     delete g;
     return st;
   }

@@ -155,8 +155,9 @@ __global__ void k_attend_join(const __grid_constant__ AttendParams p) {
 }
 
 // weights[j] = weights_in[j] + sum over the group's heads of 2^(score - lse), heads in order, for
-// every step-th slot from `first`.
-__device__ __forceinline__ void add_weights(const AttendParams& p, int b, int kv, const float* lse, int first, int step) {
+// every step-th slot from `first`. The first slots' loads go out before `ready` (which makes lse).
+template <typename F>
+__device__ __forceinline__ void add_weights(const AttendParams& p, int b, int kv, const float* lse, int first, int step, F&& ready) {
   const KvView& c = p.c;
   const int group = c.num_heads / c.num_kv;
   int len = c.lens[b];
@@ -164,16 +165,33 @@ __device__ __forceinline__ void add_weights(const AttendParams& p, int b, int kv
   const int lo = p.a.window > 0 && !c.positions ? len - p.a.window : 0;  // slots below have no score
   const int64_t rec = (static_cast<int64_t>(b) * c.num_kv + kv) * c.max_slots;
   const float* scores = p.scores + (static_cast<int64_t>(b) * c.num_heads + kv * group) * c.max_slots;
-  constexpr int kFly = 4;
-  for (int j0 = first; j0 < len; j0 += kFly * step) {
-    float s[kFly];
+  constexpr int kFly = 4, kHeads = 4;  // slots and heads in flight together
+  float s[kFly], z[kHeads][kFly];
+  auto load = [&](int j0, int i0) {
 #pragma unroll
-    for (int x = 0; x < kFly; ++x) s[x] = j0 + x * step < len ? p.a.weights_in[rec + j0 + x * step] : 0.0f;
-    for (int i = 0; i < group; ++i) {
+    for (int i = 0; i < kHeads; ++i)
 #pragma unroll
       for (int x = 0; x < kFly; ++x) {
         const int j = j0 + x * step;
-        if (j >= lo && j < len) s[x] += exp2f(scores[static_cast<int64_t>(i) * c.max_slots + j] - lse[i]);
+        z[i][x] = i0 + i < group && j >= lo && j < len ? scores[static_cast<int64_t>(i0 + i) * c.max_slots + j] : -INFINITY;
+      }
+  };
+  auto start = [&](int j0) {
+#pragma unroll
+    for (int x = 0; x < kFly; ++x) s[x] = j0 + x * step < len ? p.a.weights_in[rec + j0 + x * step] : 0.0f;
+    load(j0, 0);
+  };
+  if (first < len) start(first);
+  ready();
+  for (int j0 = first; j0 < len; j0 += kFly * step) {
+    if (j0 != first) start(j0);
+    for (int i0 = 0; i0 < group; i0 += kHeads) {
+      if (i0 > 0) load(j0, i0);
+#pragma unroll
+      for (int i = 0; i < kHeads; ++i) {
+        const float l = i0 + i < group ? lse[i0 + i] : 0.0f;
+#pragma unroll
+        for (int x = 0; x < kFly; ++x) s[x] += exp2f(z[i][x] - l);
       }
     }
 #pragma unroll
@@ -184,7 +202,7 @@ __device__ __forceinline__ void add_weights(const AttendParams& p, int b, int kv
 
 __global__ void k_attend_weights(const __grid_constant__ AttendParams p) {
   add_weights(p, blockIdx.z, blockIdx.y, p.lse + static_cast<int64_t>(blockIdx.z) * p.c.num_heads + blockIdx.y * (p.c.num_heads / p.c.num_kv),
-              blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x);
+              blockIdx.x * blockDim.x + threadIdx.x, gridDim.x * blockDim.x, [] {});
 }
 
 // ---------------------------------------------------------------- tiled form
@@ -1025,24 +1043,30 @@ __global__ void __launch_bounds__(128) k_attend_finish(const __grid_constant__ A
   };
   if (static_cast<int>(blockIdx.x) >= c.num_heads) {
     const int at = blockIdx.x - c.num_heads, kv = at % c.num_kv, chunk = at / c.num_kv, chunks = (gridDim.x - c.num_heads) / c.num_kv;
-    const int2 span = p.spans[static_cast<int64_t>(b) * c.num_kv + kv];
     float* lse = &s_o[0][0];
-    for (int r = w; r < p.group; r += 4) {
-      if (span.y <= 1) {
-        if (lane == 0) lse[r] = p.lse[static_cast<int64_t>(b) * c.num_heads + kv * p.group + r];
-        continue;
-      }
-      float m = -INFINITY, l = 0.0f;
-      for (int i = lane; i < span.y; i += 32) m = fmaxf(m, __ldcg(part_of(span.x, r, i) + D));
+    add_weights(p, b, kv, lse, chunk * 128 + threadIdx.x, chunks * 128, [&] {
+      const int2 span = p.spans[static_cast<int64_t>(b) * c.num_kv + kv];
+      for (int r = w; r < p.group; r += 4) {
+        if (span.y <= 1) {
+          if (lane == 0) lse[r] = p.lse[static_cast<int64_t>(b) * c.num_heads + kv * p.group + r];
+          continue;
+        }
+        float m = -INFINITY, l = 0.0f;
+        for (int i = lane; i < span.y; i += 32) {  // a lane's parts, then the lanes'
+          const float* part = part_of(span.x, r, i) + D;
+          const float pm = __ldcg(part), pl = __ldcg(part + 1), both = fmaxf(m, pm), ref = both == -INFINITY ? 0.0f : both;
+          l = l * exp2f(m - ref) + pl * exp2f(pm - ref);
+          m = both;
+        }
+        float all = m;
 #pragma unroll
-      for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-      const float ref = m == -INFINITY ? 0.0f : m;
-      for (int i = lane; i < span.y; i += 32) l += __ldcg(part_of(span.x, r, i) + D + 1) * exp2f(__ldcg(part_of(span.x, r, i) + D) - ref);
-      l = warp_sum(l);
-      if (lane == 0) lse[r] = l == 0.0f ? INFINITY : ref - kBias + log2f(l);
-    }
-    __syncthreads();
-    add_weights(p, b, kv, lse, chunk * 128 + threadIdx.x, chunks * 128);
+        for (int x = 16; x > 0; x >>= 1) all = fmaxf(all, __shfl_xor_sync(0xffffffffu, all, x));
+        const float ref = all == -INFINITY ? 0.0f : all;
+        l = warp_sum(l * exp2f(m - ref));
+        if (lane == 0) lse[r] = l == 0.0f ? INFINITY : ref - kBias + log2f(l);
+      }
+      __syncthreads();
+    });
     return;
   }
   const int h = blockIdx.x, kv = h / p.group, r = h - kv * p.group;
@@ -1058,7 +1082,7 @@ __global__ void __launch_bounds__(128) k_attend_finish(const __grid_constant__ A
   const float ref = m == -INFINITY ? 0.0f : m;
   float4 v[2] = {};
   float l = 0.0f;
-  constexpr int kBatch = 8;
+  constexpr int kBatch = 4;
   for (int i0 = w; i0 < span.y; i0 += 4 * kBatch) {
     float4 row[kBatch][2];
     float f[kBatch], ls[kBatch];

@@ -607,6 +607,7 @@ Status kv_create(int device, KvType type, const KvView& view, KvCache** out) {
   c->view = view;
   const Status st = kv_alloc(c);
   if (!st.ok()) {
+    cudaGetLastError();  // a failed allocation must not be taken for a later launch's error
     delete c;
     return st;
   }
