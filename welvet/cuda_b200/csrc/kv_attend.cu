@@ -264,6 +264,23 @@ __device__ __forceinline__ void mma(float, float (&d)[4], const uint32_t (&a)[4]
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// The same from zero.
+__device__ __forceinline__ void mma0(__half, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma0(__nv_bfloat16, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+__device__ __forceinline__ void mma0(float, float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 // x = part 0 + part 1 in tf32 (22 bits); the MMA reads the upper 19 bits of part 1.
 __device__ __forceinline__ void tf32_parts(float x, uint32_t& hi, uint32_t& lo) {
   asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
@@ -642,7 +659,7 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
 #pragma unroll
   for (int s = 0; s < G::kStages - 1; ++s) issue(s);
 
-  float o[DP / 8][4];
+  float o[DP / 8][2];
   float m = -INFINITY, l = 0.0f, mult = 0.0f, slope = 0.0f;
   int stage = 0, q_pos = 0;
   bool fresh = true;  // the unit's query is not in shared memory yet
@@ -661,7 +678,7 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
 #pragma unroll
       for (int i = 0; i < DP / 8; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+        for (int e = 0; e < 2; ++e) o[i][e] = 0.0f;
       m = -INFINITY;
       l = 0.0f;
       const float* q = p.a.q + cur.b * p.a.q_ld + static_cast<int64_t>(head) * D;
@@ -834,7 +851,7 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
 #pragma unroll
       for (int i = 0; i < DP / 8; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] *= corr;
+        for (int e = 0; e < 2; ++e) o[i][e] *= corr;
       m = m_new;
     }
     const float ref = (m == -INFINITY ? 0.0f : m) - G::kBias;
@@ -847,52 +864,69 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
         l += pw[n][e];
       }
 
-    // o += weights . values
+    // o += weights . values. The MMAs' accumulators cut their sums short of the last bit: a tile's
+    // sum starts from zero and is added to o (both parts of the weights at once) in rounded fp32, or
+    // runs of hundreds of tiles would lose a digit (E4M3, 30k..131k slots: 3.3e-6 of the result).
     if constexpr (G::kF32) {
+      uint32_t a[kN][4];  // k index t is key 2 t, t + 4 is key 2 t + 1
 #pragma unroll
       for (int n = 0; n < kN; ++n) {
-        uint32_t a[4];  // k index t is key 2 t, t + 4 is key 2 t + 1
-        tf32_parts(pw[n][0], a[0], a[1]);
-        tf32_parts(pw[n][1], a[2], a[3]);
-        const int r0 = 8 * (n & 1) + 2 * t, r1 = r0 + 1;
-        const uint32_t vb = vbase + (n >> 1) * 32 * pitch;
+        tf32_parts(pw[n][0], a[n][0], a[n][1]);
+        tf32_parts(pw[n][1], a[n][2], a[n][3]);
+      }
 #pragma unroll
-        for (int i = 0; i < DP / 8; ++i) {
-          if (8 * i < D) {
+      for (int i = 0; i < DP / 8; ++i) {
+        if (8 * i < D) {
+          float d[4];
+#pragma unroll
+          for (int n = 0; n < kN; ++n) {
+            const int r0 = 8 * (n & 1) + 2 * t, r1 = r0 + 1;
+            const uint32_t vb = vbase + (n >> 1) * 32 * pitch;
             const float v0 = __uint_as_float(lds32(vb + chunk_at(r0, g >> 2, 2 * i) + 4 * (g & 3)));
             const float v1 = __uint_as_float(lds32(vb + chunk_at(r1, g >> 2, 2 * i) + 4 * (g & 3)));
             uint32_t h0, l0, h1, l1;
             tf32_parts(v0, h0, l0);
             tf32_parts(v1, h1, l1);
-            mma(M(), o[i], a, h0, h1);
-            mma(M(), o[i], a, l0, l1);
+            if (n == 0) mma0(M(), d, a[n], l0, l1);
+            else mma(M(), d, a[n], l0, l1);
+            mma(M(), d, a[n], h0, h1);
           }
+          o[i][0] += d[0] + d[2];
+          o[i][1] += d[1] + d[3];
         }
       }
     } else {
+      uint32_t a[G::kSub][G::kSets][4];
 #pragma unroll
       for (int sb = 0; sb < G::kSub; ++sb) {
         const float(&p0)[2] = pw[2 * sb], (&p1)[2] = pw[2 * sb + 1];
-        const uint32_t vb = vbase + sb * 32 * pitch;
-        uint32_t a[G::kSets][4];
         if constexpr (G::kBF16) {
           uint32_t x[3], y[3];
           parts3(p0[0], p0[1], x);
           parts3(p1[0], p1[1], y);
-          a[0][0] = x[0]; a[0][1] = x[1]; a[0][2] = y[0]; a[0][3] = y[1];
-          a[1][0] = x[2]; a[1][1] = 0u; a[1][2] = y[2]; a[1][3] = 0u;
+          a[sb][0][0] = x[0]; a[sb][0][1] = x[1]; a[sb][0][2] = y[0]; a[sb][0][3] = y[1];
+          a[sb][1][0] = x[2]; a[sb][1][1] = 0u; a[sb][1][2] = y[2]; a[sb][1][3] = 0u;
         } else {
           uint32_t x[2], y[2];
           parts2(p0[0], p0[1], x);
           parts2(p1[0], p1[1], y);
-          a[0][0] = x[0]; a[0][1] = x[1]; a[0][2] = y[0]; a[0][3] = y[1];
+          a[sb][0][0] = x[0]; a[sb][0][1] = x[1]; a[sb][0][2] = y[0]; a[sb][0][3] = y[1];
         }
-        const int r = 8 * ((lane >> 3) & 1) + (lane & 7);
+      }
+      const int r = 8 * ((lane >> 3) & 1) + (lane & 7);
+      constexpr int kWide = G::kFP8 ? 4 : 2;  // n8 tiles of an ldmatrix
 #pragma unroll
-        for (int i = 0; i < DP / 8; i += G::kFP8 ? 4 : 2) {
-          if (8 * i < D) {
+      for (int i = 0; i < DP / 8; i += kWide) {
+        if (8 * i < D) {
+          float d[kWide][4];
+#pragma unroll
+          for (int sb = 0; sb < G::kSub; ++sb) {
             uint32_t v[4];
-            ldsm4t(v, vb + chunk_at(r, lane >> 4, G::kFP8 ? i / 2 : i));
+            ldsm4t(v, vbase + sb * 32 * pitch + chunk_at(r, lane >> 4, G::kFP8 ? i / 2 : i));
+            auto add = [&](int x, const uint32_t(&w)[4], uint32_t b0, uint32_t b1, bool first) {
+              if (first) mma0(M(), d[x], w, b0, b1);
+              else mma(M(), d[x], w, b0, b1);
+            };
             if constexpr (G::kFP8) {
               // a register holds dims 2 g, 2 g + 1 of keys 2 t, 2 t + 1: regroup the bytes by dim
 #pragma unroll
@@ -901,16 +935,23 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
                 uint32_t e0, o0, e1, o1;
                 e4m3_pairs(__byte_perm(v[2 * x], 0, 0x3120), e0, o0);
                 e4m3_pairs(__byte_perm(v[2 * x + 1], 0, 0x3120), e1, o1);
-                mma(M(), o[i + 2 * x], a[0], e0, e1);
-                mma(M(), o[i + 2 * x + 1], a[0], o0, o1);
+                add(2 * x, a[sb][0], e0, e1, sb == 0);
+                add(2 * x + 1, a[sb][0], o0, o1, sb == 0);
               }
             } else {
 #pragma unroll
-              for (int x = 0; x < G::kSets; ++x) {
-                mma(M(), o[i], a[x], v[0], v[1]);
-                mma(M(), o[i + 1], a[x], v[2], v[3]);
+              for (int x = 0; x < G::kSets; ++x) {  // the least part first
+                const int set = G::kSets - 1 - x;
+                add(0, a[sb][set], v[0], v[1], sb == 0 && x == 0);
+                add(1, a[sb][set], v[2], v[3], sb == 0 && x == 0);
               }
             }
+          }
+#pragma unroll
+          for (int x = 0; x < kWide; ++x) {
+            if (i + x >= DP / 8) break;
+            o[i + x][0] += d[x][0] + d[x][2];
+            o[i + x][1] += d[x][1] + d[x][3];
           }
         }
       }
@@ -933,9 +974,9 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
         if (8 * i >= D) break;
         int d = (G::kFP8 ? 8 * i + 4 * t : 8 * i + 2 * t) + 4 * g;
         if (d >= D) d -= D;
-        const float2 a = make_float2(o[i][0] + o[i][2], o[i][1] + o[i][3]);
+        const float2 a = make_float2(o[i][0], o[i][1]);
         if constexpr (G::kFP8) {
-          *reinterpret_cast<float4*>(mine + d) = make_float4(a.x, o[i + 1][0] + o[i + 1][2], a.y, o[i + 1][1] + o[i + 1][3]);
+          *reinterpret_cast<float4*>(mine + d) = make_float4(a.x, o[i + 1][0], a.y, o[i + 1][1]);
         } else {
           *reinterpret_cast<float2*>(mine + d) = a;
         }
