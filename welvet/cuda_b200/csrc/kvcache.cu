@@ -33,13 +33,14 @@ constexpr int kAppendThreads = 256;
 // One block per new token: the token's angles once into shared memory, then its key, value and
 // query heads, pair (d, d + half) by pair. HBM bound: 4 B read per element, the page's type
 // written (and 4 B for q). kVec: four consecutive pairs a thread (16-byte accesses).
-template <typename T, bool kVec>
-__global__ void __launch_bounds__(kAppendThreads) k_append(const __grid_constant__ AppendParams p) {
+// kDim: the width, 0 where it is not a constant (13k prompt tokens of 48 heads of 128: 74 us, 90 without).
+template <typename T, bool kVec, int kDim>
+__global__ void __launch_bounds__(kAppendThreads, 4) k_append(const __grid_constant__ AppendParams p) {
   __shared__ float s_cos[kMaxPairs], s_sin[kMaxPairs];
   __shared__ int s_last;
   const KvView& c = p.c;
   const int t = blockIdx.x, tid = threadIdx.x;
-  const int D = c.head_dim, half = p.half;
+  const int D = kDim > 0 ? kDim : c.head_dim, half = p.half;
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int kv_heads = c.num_kv, heads = 2 * kv_heads + (p.a.q ? c.num_heads : 0);
@@ -211,8 +212,9 @@ __device__ __forceinline__ uint32_t evict_key(float w, int pos, int sinks, int r
 }
 
 // Rows of one (sequence, key-value head): slots `take` to slots `fill`, 16 bytes a lane where the
-// layout allows it. A group of lanes takes a row; kFly rows a group are in flight.
-template <int kSize, bool kVec, int kFly>
+// layout allows it. A group of lanes takes a row; the next row's place is looked up while this
+// one's values are on their way.
+template <int kSize, bool kVec>
 __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kv, const int32_t* fill, const int32_t* take,
                                           int n, int worker, int workers) {
   const KvView& c = p.c;
@@ -229,44 +231,59 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kv, c
     return true;
   };
   if constexpr (kVec) {
-    const int lanes = bytes >= 512 ? 32 : (bytes > 128 ? (bytes > 256 ? 32 : 16) : 8);  // of a row
-    const int groups = 32 / lanes, sub = lane / lanes, at = 16 * (lane % lanes);
-    for (int i0 = worker * groups * kFly; i0 < n; i0 += workers * groups * kFly) {
-      int64_t kt[kFly], vt[kFly], kf[kFly], vf[kFly];
-      int to[kFly], from[kFly];
-      bool ok[kFly];
-#pragma unroll
-      for (int x = 0; x < kFly; ++x) {
-        const int i = i0 + x * groups + sub;
-        ok[x] = i < n;
-        to[x] = ok[x] ? fill[i] : 0;
-        from[x] = ok[x] ? take[i] : 0;
+    const int lanes = bytes > 256 ? 32 : (bytes > 128 ? 16 : 8);  // of a row
+    const int groups = 32 / lanes, at = 16 * (lane % lanes), step = workers * groups;
+    struct Row {  // slots and pages
+      int to, from, to_page, to_in, from_page, from_in;
+    };
+    auto fetch = [&](int i) {
+      Row r;
+      r.to = fill[i];
+      r.from = take[i];
+      const int pt = r.to / c.page_size, pf = r.from / c.page_size;
+      r.to_in = r.to - pt * c.page_size;
+      r.from_in = r.from - pf * c.page_size;
+      r.to_page = table[pt];
+      r.from_page = table[pf];
+      return r;
+    };
+    auto address = [&](const KvPool& q, int page, int in) { return q.base + (page * q.page + in * q.slot + kv * q.head) * kSize + at; };
+    int i = worker * groups + lane / lanes;
+    Row row{};
+    if (i < n) row = fetch(i);
+    for (; i < n; i += step) {
+      uint4 k{}, v{};
+      float weight = 0.0f;
+      int pos = 0;
+      if (at == 0) {
+        weight = p.a.weights_in[rec + row.from];
+        pos = p.a.positions_in[rec + row.from];
       }
-#pragma unroll
-      for (int x = 0; x < kFly; ++x) {
-        if (!ok[x]) continue;
-        if (lane % lanes == 0) {
-          c.weights[rec + to[x]] = p.a.weights_in[rec + from[x]];
-          c.positions[rec + to[x]] = p.a.positions_in[rec + from[x]];
+      const bool ok = row.to_page >= 0 && row.to_page < c.num_pages && row.from_page >= 0 && row.from_page < c.num_pages;
+      if (!ok) atomicCAS(c.err, 0, kKvErrPage);
+      const uint8_t* const kf = address(c.k, row.from_page, row.from_in);
+      const uint8_t* const vf = address(c.v, row.from_page, row.from_in);
+      if (ok && at < bytes) {
+        k = *reinterpret_cast<const uint4*>(kf);
+        v = *reinterpret_cast<const uint4*>(vf);
+      }
+      Row ahead{};
+      if (i + step < n) ahead = fetch(i + step);
+      if (at == 0) {
+        c.weights[rec + row.to] = weight;
+        c.positions[rec + row.to] = pos;
+      }
+      if (ok && at < bytes) {
+        uint8_t* const kt = address(c.k, row.to_page, row.to_in);
+        uint8_t* const vt = address(c.v, row.to_page, row.to_in);
+        *reinterpret_cast<uint4*>(kt) = k;
+        *reinterpret_cast<uint4*>(vt) = v;
+        for (int o = 16 * lanes; at + o < bytes; o += 16 * lanes) {
+          *reinterpret_cast<uint4*>(kt + o) = *reinterpret_cast<const uint4*>(kf + o);
+          *reinterpret_cast<uint4*>(vt + o) = *reinterpret_cast<const uint4*>(vf + o);
         }
-        ok[x] = row_of(to[x], &kt[x], &vt[x]) && row_of(from[x], &kf[x], &vf[x]);
-        if (!ok[x]) atomicCAS(c.err, 0, kKvErrPage);
       }
-      for (int o = at; o < bytes; o += 16 * lanes) {
-        uint4 k[kFly], v[kFly];
-#pragma unroll
-        for (int x = 0; x < kFly; ++x)
-          if (ok[x]) {
-            k[x] = *reinterpret_cast<const uint4*>(c.k.base + kf[x] + o);
-            v[x] = *reinterpret_cast<const uint4*>(c.v.base + vf[x] + o);
-          }
-#pragma unroll
-        for (int x = 0; x < kFly; ++x)
-          if (ok[x]) {
-            *reinterpret_cast<uint4*>(c.k.base + kt[x] + o) = k[x];
-            *reinterpret_cast<uint4*>(c.v.base + vt[x] + o) = v[x];
-          }
-      }
+      row = ahead;
     }
   } else {
     for (int i = worker; i < n; i += workers) {
@@ -541,7 +558,7 @@ __global__ void __launch_bounds__(kEvictThreads, 2) k_evict_select(const __grid_
   }
   if (ranks == 1) {
     __syncthreads();  // the block's own lists
-    move_rows<kSize, kVec, 1>(p, b, kv, fill, take, moved, w, kEvictWarps);
+    move_rows<kSize, kVec>(p, b, kv, fill, take, moved, w, kEvictWarps);
   } else {
     if (rank == 0 && tid == 0) p.n_moves[row] = moved;
     cluster.sync();  // no block leaves while another reads its shared memory
@@ -556,7 +573,7 @@ __global__ void __launch_bounds__(256, 4) k_evict_move(const __grid_constant__ E
   const KvView& c = p.c;
   const int kv = blockIdx.y, b = blockIdx.z, row = b * c.num_kv + kv;
   const int32_t* fill = p.moves + static_cast<int64_t>(row) * 2 * (c.max_slots / 2);
-  move_rows<kSize, kVec, 2>(p, b, kv, fill, fill + c.max_slots / 2, p.n_moves[row], blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8);
+  move_rows<kSize, kVec>(p, b, kv, fill, fill + c.max_slots / 2, p.n_moves[row], blockIdx.x * 8 + (threadIdx.x >> 5), gridDim.x * 8);
 }
 
 bool f32_aligned(const float* p, int64_t ld) { return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 4 == 0; }
@@ -640,7 +657,8 @@ Status kv_append(KvCache* c, const KvAppendArgs& a, cudaStream_t st) {
   return by_type(c->type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     const int blocks = a.rows > 0 ? a.rows : 1;  // no row: the lengths are still carried over
-    return launch_after(vec ? k_append<T, true> : k_append<T, false>, dim3(blocks), kAppendThreads, 0, st, p);
+    auto* kernel = !vec ? k_append<T, false, 0> : (p.c.head_dim == 128 ? k_append<T, true, 128> : (p.c.head_dim == 64 ? k_append<T, true, 64> : k_append<T, true, 0>));
+    return launch_after(kernel, dim3(blocks), kAppendThreads, 0, st, p);
   });
 }
 
