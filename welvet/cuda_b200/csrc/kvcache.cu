@@ -213,7 +213,9 @@ __device__ __forceinline__ uint32_t evict_key(float w, int pos, int sinks, int r
 
 // Rows of one (sequence, key-value head): slots `take` to slots `fill`, 16 bytes a lane where the
 // layout allows it. A group of lanes takes a row; the next row's place is looked up while this
-// one's values are on their way.
+// one's values are on their way. Rows lie in random order, and a narrow one is a short access: of 24
+// E4M3 heads of 128 cut from 40k..65k slots to 16k the move takes 32 us at about 3.5 TB/s of read and
+// written rows (38 us with the look-up in line).
 template <int kSize, bool kVec>
 __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kv, const int32_t* fill, const int32_t* take,
                                           int n, int worker, int workers) {
@@ -310,7 +312,9 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kv, c
 // memory), then, in slot order, the slots below keep that go (to fill) and those above it that stay
 // (to take). Both lists are equally long and no slot is in both, so the rows can move in any order.
 // A cluster of one block moves them itself; larger ones leave the lists to k_evict_move.
-// Latency bound: 8 bytes a slot are read, the rest is a dozen barriers.
+// Latency bound: 8 bytes a slot are read, the rest is a dozen barriers. About 24 us of the 56
+// at 24 heads of 40k..65k slots (10 MB read, eight blocks a head); 32 sequences x 8 heads of 1025..1056
+// slots cut to 1024 take 9 us with their rows, in one launch.
 template <int kSize, bool kVec>
 __global__ void __launch_bounds__(kEvictThreads, 2) k_evict_select(const __grid_constant__ EvictParams p) {
   namespace cg = cooperative_groups;
