@@ -238,7 +238,8 @@ typedef struct welvet_b200_kv_desc {
   const int32_t* page_table; /* [num_seqs][pages_per_seq], rows table_stride apart */
   int64_t table_stride;
   int32_t* lens;         /* [num_seqs] slots in use */
-  int32_t* seen;         /* [num_seqs] tokens seen, >= lens once slots were evicted; NULL: lens */
+  int32_t* seen;         /* [num_seqs] tokens seen, >= lens once slots were evicted; NULL: lens. With
+                            positions an array of its own */
   float* weights;        /* [num_seqs][num_kv_heads][max_slots] accumulated attention weight, or NULL */
   int32_t* positions;    /* same shape: the token position a slot holds (needs seen), or NULL: the
                             slot index. Eviction needs weights, positions and seen */
@@ -261,8 +262,10 @@ WELVET_API welvet_status welvet_b200_kv_append(welvet_b200_kv* kv, int32_t rows,
 
 /* Attention of one new token per sequence: q, out [num_seqs][num_heads * head_dim] float32, rows
  * q_ld / out_ld apart; softmax over the sequence's slots of scale * q.k (scale <= 0: head_dim^-0.5).
- * window > 0 keeps positions above (query position - window), the query's position being seen - 1;
- * alibi adds the MHA cell's linear biases. A sequence with no slot allowed gets zeros. accumulate:
+ * window > 0 keeps positions above (query position - window), the query's position being seen - 1
+ * (without positions the last slot's, lens - 1); alibi adds the MHA cell's linear biases. A sequence
+ * with no slot allowed gets zeros. What slots that are not allowed hold, even NaN, does not matter; an
+ * infinity or NaN in an allowed one can make the rows of the heads that read it NaN. accumulate:
  * weights[slot] = weights_in[slot] (NULL: weights) + the slot's attention weights summed over the
  * query heads of its key-value head, for slots below lens. */
 WELVET_API welvet_status welvet_b200_kv_attend(welvet_b200_kv* kv, const float* q, int64_t q_ld, float* out,
@@ -305,7 +308,8 @@ WELVET_API welvet_status welvet_b200_mha_prefill_device(welvet_b200_mha* s, welv
  * may be shorter); scales Float16 (2) or BFloat16 (3). codes [out][(in + 1) / 2] bytes, low nibble =
  * even input; scales and zeros [out][ceil(in / group)]. */
 
-/* Round-to-nearest quantisation of W_dev [out][in] float32 into those arrays (device). */
+/* Round-to-nearest quantisation of W_dev [out][in] float32 into those arrays (device). A group that
+ * holds an infinity or NaN gets a NaN scale. */
 WELVET_API welvet_status welvet_b200_group_quantize(int32_t in, int32_t out, int32_t group, int32_t code,
                                                     int32_t scale_dtype, const float* W_dev, uint8_t* codes_dev,
                                                     void* scales_dev, uint8_t* zeros_dev, void* stream);

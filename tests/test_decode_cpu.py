@@ -66,3 +66,17 @@ def test_group_arguments():
         64, 4, 64, code, 2, act, FAKE, FAKE, zeros, 1, bias, n, ctypes.byref(h)).code
     assert m(15, None) == 1 and m(14, FAKE) == 1 and m(16, None, act=7) == 1 and m(16, None, n=3) == 1
     assert L.welvet_b200_group_quantize(64, 4, 64, 15, 2, FAKE, FAKE, FAKE, None, None).code == 1
+
+
+def test_positions_need_a_seen_of_their_own():
+    h = ctypes.c_void_p()
+    st = W.lib().welvet_b200_kv_create(ctypes.byref(desc(positions=FAKE, seen=FAKE, lens=FAKE)), ctypes.byref(h))
+    assert st.code == 1 and b"of its own" in st.message and not h
+
+
+@pytest.mark.parametrize("in_,out", [((1 << 31) - 1, 16), (64, (1 << 31) - 1), ((1 << 30) + 1, 16)])
+def test_group_sizes_past_the_index_range(in_, out):
+    L = W.lib()
+    assert L.welvet_b200_group_quantize(in_, out, 64, 14, 2, FAKE, FAKE, FAKE, None, None).code == 2
+    h = ctypes.c_void_p()
+    assert L.welvet_b200_gdense_mount(in_, out, 64, 14, 2, -1, FAKE, FAKE, None, 1, None, 0, ctypes.byref(h)).code == 2 and not h

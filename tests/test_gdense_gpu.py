@@ -282,3 +282,24 @@ def test_refusals(D, wb):
         with pytest.raises(ValueError):
             g.forward(*a)
     g.forward(x[:0], y[:0])  # no rows: nothing to do
+
+
+@pytest.mark.parametrize("scale_dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("code", ["int4", "uint4", "fp4"])
+def test_quantize_does_not_hide_what_is_not_finite(D, code, scale_dtype):
+    """A group with an infinity or NaN gets a NaN scale, and its row's result is NaN; no other changes."""
+    import torch
+    rng = np.random.default_rng(61)
+    W = torch.from_numpy(rng.standard_normal((20, 200)).astype(np.float32)).cuda()
+    dt = torch.float16 if scale_dtype == "f16" else torch.bfloat16
+    want = D.group_quantize(W, 64, D.CODES[code], dt)
+    W[3, 70], W[7, 199], W[11, 0] = float("nan"), float("inf"), float("-inf")
+    got = D.group_quantize(W, 64, D.CODES[code], dt)
+    bad = torch.zeros((20, 4), dtype=torch.bool, device="cuda")
+    bad[3, 1] = bad[7, 3] = bad[11, 0] = True
+    assert torch.equal(torch.isnan(got[1]), bad)
+    assert torch.equal(got[1][~bad], want[1][~bad])
+    layer = D.GroupDense.from_codes(got[0], got[1], 200, 64, D.CODES[code], zeros=got[2])
+    y = torch.empty((1, 20), device="cuda")
+    layer.forward(torch.ones((1, 200), device="cuda"), y)
+    assert torch.equal(torch.isnan(y[0]), bad.any(1))

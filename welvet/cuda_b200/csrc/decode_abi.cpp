@@ -91,6 +91,7 @@ welvet_status welvet_b200_kv_create(const welvet_b200_kv_desc* desc, welvet_b200
     if (d.table_stride < d.pages_per_seq && d.num_seqs > 1) return wb::Status::Invalid("kv: table_stride < pages_per_seq");
     if (!d.page_table || !d.lens) return wb::Status::Invalid("kv: nil page_table or lens");
     if (d.positions && !d.seen) return wb::Status::Invalid("kv: positions without seen");
+    if (d.positions && d.seen == d.lens) return wb::Status::Invalid("kv: with positions seen must be an array of its own");
     if (!(d.k_scale > 0.0f) || !(d.v_scale > 0.0f) || !std::isnormal(d.k_scale) || !std::isnormal(d.v_scale))
       return wb::Status::Invalid("kv: k_scale and v_scale must be positive, finite and normal");
     wb::KvView v;
@@ -220,6 +221,7 @@ void welvet_b200_kv_release(welvet_b200_kv* kv) {
 
 static wb::Status group_shape(int32_t in, int32_t out, int32_t group, int32_t code, int32_t scale_dtype) {
   if (in <= 0 || out <= 0) return wb::Status::Invalid("group dense: need in > 0 and out > 0");
+  if (in > (1 << 30) || out > (1 << 30)) return wb::Status::Unsupported("group dense: more than 2^30 inputs or outputs");
   if (code != wb::kCodeInt4 && code != wb::kCodeUint4 && code != wb::kCodeFp4)
     return wb::Status::Unsupported("group dense: code dtype id " + std::to_string(code) + " (Int4, Uint4 or FP4)");
   if (scale_dtype != wb::kScaleF16 && scale_dtype != wb::kScaleBF16)

@@ -23,9 +23,9 @@ __device__ __forceinline__ float scale_value(uint16_t bits, int type) {
 // fragments of the unit's four m16n8k16 MMAs), then 16 scales and, for Uint4, 16 zero points
 // per set of sg inputs ([8 rows][set][row, row + 8]), sg being the largest of 32, 64, 128, 256 that
 // divides the group. Records of a row group follow one another, so a warp's piece of work is one
-// contiguous copy. The inputs' order within a unit is the MMAs' own: input 32 (j / 2) + 8 t + 4 (j % 2) + 2 r + e is element e of
-// register r of block j in lane t, so that 8 consecutive inputs of x are a lane's B fragments of two
-// blocks, which span 32 inputs.
+// contiguous copy. The inputs' order within a unit is the MMAs' own: input 32 (j / 2) + 8 t +
+// 4 (j % 2) + 2 r + e is element e of register r of block j in lane t, so that 8 consecutive inputs
+// of x are a lane's B fragments of two blocks, which span 32 inputs.
 constexpr int kChunk = 256, kUnit = 64;
 
 struct Layout {
@@ -114,8 +114,9 @@ __global__ void __launch_bounds__(128) k_group_build(const __grid_constant__ Bui
 // every warp a row group or more make the runs the warps', which then never wait for one another;
 // smaller ones make them the blocks', whose warps take every 16th record and leave their sums in
 // shared memory, where those of up to eight row groups are added and finished together. Row groups
-// that a run's ends cut are joined through global memory by the last run to come, in run order; small layers avoid that with runs of whole row groups. The first weight
-// loads start before the previous kernel's end is waited for.
+// that a run's ends cut are joined through global memory by the last run to come, in run order;
+// small layers avoid that with runs of whole row groups. The first weight loads start before the
+// previous kernel's end is waited for.
 constexpr int kMaxTokens = 8;
 constexpr int kGWarps = 16;
 constexpr int kGThreads = 32 * kGWarps;
@@ -538,8 +539,9 @@ __global__ void __launch_bounds__(256) k_group_slabs(const __grid_constant__ GAr
 }
 
 // The quantiser, run once per matrix and bound by its 4 bytes read per weight. One warp per (row,
-// group): the group's range gives its scale, rounded to the scale's type before
-// the codes are chosen, so that decoding multiplies by what the codes were divided by.
+// group): the group's range gives its scale, rounded to the scale's type before the codes are
+// chosen, so that decoding multiplies by what the codes were divided by. A group that holds an
+// infinity or NaN gets a NaN scale: its row says so, where codes would hide it.
 template <int kCode>
 __global__ void __launch_bounds__(256)
     k_group_quantize(const float* __restrict__ W, int rows, int cols, int group, int groups, int scale_type, uint8_t* codes,
@@ -551,10 +553,13 @@ __global__ void __launch_bounds__(256)
   const float* w = W + static_cast<int64_t>(o) * cols;
   const int k0 = g * group, k1 = k0 + group < cols ? k0 + group : cols;
   float lo = 0.0f, hi = 0.0f;  // zero stays representable
+  bool finite = true;
   for (int k = k0 + lane; k < k1; k += 32) {
     lo = fminf(lo, w[k]);
     hi = fmaxf(hi, w[k]);
+    finite = finite && isfinite(w[k]);
   }
+  finite = __all_sync(0xffffffffu, finite);
 #pragma unroll
   for (int d = 16; d > 0; d >>= 1) {
     lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, d));
@@ -565,6 +570,7 @@ __global__ void __launch_bounds__(256)
   uint16_t bits;
   if (scale_type == kScaleF16) bits = __half_as_ushort(__float2half_rn(fminf(s, 65504.0f)));
   else bits = __bfloat16_as_ushort(__float2bfloat16_rn(fminf(s, 3.3895314e38f)));
+  if (!finite) bits = scale_type == kScaleF16 ? 0x7e00u : 0x7fc0u;
   s = scale_value(bits, scale_type);
   const float zero = kCode == kCodeUint4 && s > 0.0f ? fminf(fmaxf(rintf(-lo / s), 0.0f), 15.0f) : 0.0f;
   if (lane == 0) {

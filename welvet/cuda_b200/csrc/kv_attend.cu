@@ -330,7 +330,6 @@ struct Tiled {
   static constexpr int kWarps = kRow <= 512 ? 4 : 2;
   static constexpr int kSub = kRow <= 128 ? 2 : 1;      // 16-key blocks of a warp's tile
   static constexpr int kStages = kRow <= 256 || kRow > 384 ? 3 : 2;
-  static constexpr int kDP = DP;
   static constexpr int kThreads = 32 * kWarps;
   // of an SM: three where a tile is small enough for 168 registers (160-byte rows; 128-byte rows, two
   // blocks of keys a warp, took 245 us for 157)
@@ -1186,7 +1185,7 @@ bool tiled(const KvView& v, KvType type) {
     for (int64_t s : {p.page, p.slot, p.head})
       if (s * size > 0xffffffffll) return false;
   const int64_t units = static_cast<int64_t>(v.num_seqs) * v.num_kv;
-  if (units * (v.max_slots / 64 + 1 + kOver) > 0x7fffffffll) return false;
+  if (units * (v.max_slots / 32 + 1 + kOver) > 0x7fffffffll) return false;  // a tile has 32 keys or more
   if (v.num_heads / v.num_kv > kMaxGroup) return false;
   return v.head_dim % 8 == 0 && v.head_dim * size % 16 == 0 && pool_aligned(v.k, size, 16) && pool_aligned(v.v, size, 16);
 }
