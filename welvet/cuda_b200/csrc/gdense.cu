@@ -295,14 +295,23 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
   const bool vec = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.x_ld & 3) == 0;
   const bool vec2 = (reinterpret_cast<uintptr_t>(a.x) & 7) == 0 && (a.x_ld & 1) == 0;
   constexpr int kFly = 4;  // chunks whose loads are in flight together
-  for (int i0 = w; i0 < a.n * chunks; i0 += kFly * kGWarps) {
+  const int b_step = kGWarps / chunks, c_step = kGWarps - b_step * chunks;
+  auto advance = [&](int& b, int& c) {
+    b += b_step;
+    c += c_step;
+    if (c >= chunks) {
+      c -= chunks;
+      ++b;
+    }
+  };
+  for (int b0 = w / chunks, c0 = w - b0 * chunks; b0 < a.n;) {
     float v[kFly][8];
+    int b = b0, c = c0;
 #pragma unroll
     for (int y = 0; y < kFly; ++y) {
-      const int i = i0 + y * kGWarps, b = i / chunks, c = i - b * chunks;
       const int k0 = (c_first + c) * kChunk + 8 * lane;
       const float* xs = a.x + b * a.x_ld + k0;
-      const bool on = i < a.n * chunks;
+      const bool on = b < a.n;
       if (vec && on && k0 + 8 <= a.cols) {
         *reinterpret_cast<float4*>(v[y]) = ld_dep4(xs);
         *reinterpret_cast<float4*>(v[y] + 4) = ld_dep4(xs + 4);
@@ -313,34 +322,45 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[y][e] = on && k0 + e < a.cols ? ld_dep(xs + e) : 0.0f;
       }
+      advance(b, c);
     }
 #pragma unroll
     for (int y = 0; y < kFly; ++y) {
-      const int i = i0 + y * kGWarps, b = i / chunks, c = i - b * chunks;
-      if (i >= a.n * chunks) break;
-      float mx = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) mx = fmaxf(mx, isfinite(v[y][e]) ? fabsf(v[y][e]) : 0.0f);
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      if (b0 >= a.n) break;
       // the chunk's largest finite |x| goes to [2^14, 2^15)
-      const int ex = mx > 0.0f ? min(126, 14 - ilogbf(mx)) : 0;
-      const float f = ldexpf(1.0f, ex);
+      uint32_t top = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[y][e]) & 0x7fffffffu);
+      top = __reduce_max_sync(0xffffffffu, top);
+      const bool finite = top < 0x7f800000u;
+      if (!finite) {
+        top = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = max(top, isfinite(v[y][e]) ? __float_as_uint(v[y][e]) & 0x7fffffffu : 0u);
+        top = __reduce_max_sync(0xffffffffu, top);
+      }
+      const int ex = min(126, 141 - static_cast<int>(top >> 23));
+      const float f = __uint_as_float(static_cast<uint32_t>(127 + ex) << 23);  // 2^ex
       uint32_t hi[4], lo[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float p = v[y][2 * e] * f, q = v[y][2 * e + 1] * f;
         const __half2 h = __floats2half2_rn(p, q);
         const float2 r = __half22float2(h);
-        // infinities and NaN stay in the first part
-        const __half2 l = __floats2half2_rn(isfinite(p) ? p - r.x : 0.0f, isfinite(q) ? q - r.y : 0.0f);
+        float dp = p - r.x, dq = q - r.y;
+        if (!finite) {  // infinities and NaN stay in the first part
+          dp = isfinite(p) ? dp : 0.0f;
+          dq = isfinite(q) ? dq : 0.0f;
+        }
+        const __half2 l = __floats2half2_rn(dp, dq);
         hi[e] = *reinterpret_cast<const uint32_t*>(&h);
         lo[e] = *reinterpret_cast<const uint32_t*>(&l);
       }
-      uint8_t* dst = sx + 2 * b * pitch + (c * kChunk + 8 * lane) * 2;
+      uint8_t* dst = sx + 2 * b0 * pitch + (c0 * kChunk + 8 * lane) * 2;
       *reinterpret_cast<uint4*>(dst) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
       *reinterpret_cast<uint4*>(dst + pitch) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      if (lane == 0) sxs[b * a.slab_chunks + c] = ldexpf(1.0f, -ex);
+      if (lane == 0) sxs[b0 * a.slab_chunks + c0] = __uint_as_float(static_cast<uint32_t>(127 - ex) << 23);
+      advance(b0, c0);
     }
   }
   __syncthreads();
