@@ -230,7 +230,7 @@ __global__ void k_attend_weights(const __grid_constant__ AttendParams p) {
 // Small caches (attend_plan says when) instead give each unit a cluster of blocks with equal shares
 // of its tiles, which join through distributed shared memory: one launch. (Joined by the last block
 // to arrive, behind a counter, one sequence of 131072 slots took 53 us, the registers of that code
-// among it; with the second kernel one key-value head's 131072 slots take 37 us.)
+// among it; with the second kernel one key-value head's 131072 slots take 26 us.)
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -1068,15 +1068,20 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
 }
 
 // What is left once all runs are done. Blocks below num_heads join the parts of one query head in
-// order (the unit's first run left its second slot, the others their first; four warps take the
-// parts in turn, sums are added in warp order). The others, with accumulate, add the attention
-// weights of a key-value head's slots; the normalisers of split units they make for themselves.
+// order (the unit's first run left its second slot, the others their first; the warps take the parts
+// in turn, each with its running maximum; their sums are added in warp order). The others, with
+// accumulate, add the attention weights of a key-value head's slots; the normalisers of split units
+// they make for themselves. Latency bound: four warps a block and registers for nine blocks an SM, so
+// that many short joins run at once (64 sequences of 32 heads, ragged: 54.4 us with the attention, 55.4
+// with seven an SM), or sixteen warps where units have many parts (one key-value head of 131072
+// slots, 296 parts: 26.3 us for 41.8; 56 heads of 8191, 5 parts each, with weights: 53.1 for 54.7).
 constexpr int kMaxGroup = 128;  // query heads of a key-value head that the weights' blocks can hold
+constexpr int kManyParts = 4;   // parts of a unit, on average, beyond which sixteen warps join them
 
-template <int kBias>
-__global__ void __launch_bounds__(128) k_attend_finish(const __grid_constant__ AttendParams p) {
-  __shared__ float s_o[4][256];
-  __shared__ float s_m[4], s_l[4];
+template <int kBias, bool kWide, int kW>  // kWide: head_dim > 128
+__global__ void __launch_bounds__(32 * kW, kW == 4 ? 9 : 2) k_attend_finish(const __grid_constant__ AttendParams p) {
+  __shared__ float s_o[kW][kWide ? 256 : 128];
+  __shared__ float s_m[kW], s_l[kW];
   asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const KvView& c = p.c;
@@ -1089,9 +1094,9 @@ __global__ void __launch_bounds__(128) k_attend_finish(const __grid_constant__ A
   if (static_cast<int>(blockIdx.x) >= c.num_heads) {
     const int at = blockIdx.x - c.num_heads, kv = at % c.num_kv, chunk = at / c.num_kv, chunks = (gridDim.x - c.num_heads) / c.num_kv;
     float* lse = &s_o[0][0];
-    add_weights(p, b, kv, lse, chunk * 128 + threadIdx.x, chunks * 128, [&] {
+    add_weights(p, b, kv, lse, chunk * (32 * kW) + threadIdx.x, chunks * (32 * kW), [&] {
       const int2 span = p.spans[static_cast<int64_t>(b) * c.num_kv + kv];
-      for (int r = w; r < p.group; r += 4) {
+      for (int r = w; r < p.group; r += kW) {
         if (span.y <= 1) {
           if (lane == 0) lse[r] = p.lse[static_cast<int64_t>(b) * c.num_heads + kv * p.group + r];
           continue;
@@ -1117,41 +1122,42 @@ __global__ void __launch_bounds__(128) k_attend_finish(const __grid_constant__ A
   const int h = blockIdx.x, kv = h / p.group, r = h - kv * p.group;
   const int2 span = p.spans[static_cast<int64_t>(b) * c.num_kv + kv];
   if (span.y <= 1) return;
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < span.y; i += 128) m = fmaxf(m, __ldcg(part_of(span.x, r, i) + D));
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-  if (lane == 0) s_m[w] = m;
-  __syncthreads();
-  m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  const float ref = m == -INFINITY ? 0.0f : m;
-  float4 v[2] = {};
-  float l = 0.0f;
-  constexpr int kBatch = 4;
-  for (int i0 = w; i0 < span.y; i0 += 4 * kBatch) {
-    float4 row[kBatch][2];
-    float f[kBatch], ls[kBatch];
+  constexpr int kRows = kWide ? 2 : 1, kBatch = 4 / kRows;  // float4s of a lane, parts in flight
+  float4 v[kRows] = {};
+  float m = -INFINITY, l = 0.0f;
+  for (int i0 = w; i0 < span.y; i0 += kW * kBatch) {
+    float4 row[kBatch][kRows];
+    float ms[kBatch], ls[kBatch];
 #pragma unroll
     for (int x = 0; x < kBatch; ++x) {
-      const int i = i0 + 4 * x;
-      f[x] = ls[x] = 0.0f;
-      row[x][0] = row[x][1] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      const int i = i0 + kW * x;
+      ms[x] = -INFINITY;
+      ls[x] = 0.0f;
+#pragma unroll
+      for (int e = 0; e < kRows; ++e) row[x][e] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (i < span.y) {
         const float* src = part_of(span.x, r, i);
-        f[x] = __ldcg(src + D);
+        ms[x] = __ldcg(src + D);
         ls[x] = __ldcg(src + D + 1);
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int e = 0; e < kRows; ++e)
           if (4 * lane + 128 * e < D) row[x][e] = __ldcg(reinterpret_cast<const float4*>(src + 4 * lane + 128 * e));
       }
     }
+    float m_new = m;
+#pragma unroll
+    for (int x = 0; x < kBatch; ++x) m_new = fmaxf(m_new, ms[x]);
+    const float ref = m_new == -INFINITY ? 0.0f : m_new, f = exp2_fast(m - ref);
+    l *= f;
+#pragma unroll
+    for (int e = 0; e < kRows; ++e) v[e] = make_float4(v[e].x * f, v[e].y * f, v[e].z * f, v[e].w * f);
+    m = m_new;
 #pragma unroll
     for (int x = 0; x < kBatch; ++x) {
-      if (i0 + 4 * x >= span.y) break;
-      const float fx = exp2_fast(f[x] - ref);
+      const float fx = exp2_fast(ms[x] - ref);
       l += ls[x] * fx;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
+      for (int e = 0; e < kRows; ++e) {
         v[e].x += row[x][e].x * fx;
         v[e].y += row[x][e].y * fx;
         v[e].z += row[x][e].z * fx;
@@ -1160,14 +1166,29 @@ __global__ void __launch_bounds__(128) k_attend_finish(const __grid_constant__ A
     }
   }
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
+  for (int e = 0; e < kRows; ++e)
     if (4 * lane + 128 * e < D) *reinterpret_cast<float4*>(&s_o[w][4 * lane + 128 * e]) = v[e];
-  if (lane == 0) s_l[w] = l;
+  if (lane == 0) {
+    s_m[w] = m;
+    s_l[w] = l;
+  }
   __syncthreads();
-  l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
-  const float f = l == 0.0f ? 0.0f : c.v_scale / l;
+  m = s_m[0];
+#pragma unroll
+  for (int x = 1; x < kW; ++x) m = fmaxf(m, s_m[x]);
+  const float ref = m == -INFINITY ? 0.0f : m;
   float* out = p.a.out + b * p.a.out_ld + static_cast<int64_t>(h) * D;
-  for (int d = threadIdx.x; d < D; d += 128) out[d] = l == 0.0f ? 0.0f : (s_o[0][d] + s_o[1][d] + s_o[2][d] + s_o[3][d]) * f;
+  for (int d = threadIdx.x; d < D; d += 32 * kW) {
+    float sum = 0.0f;
+    l = 0.0f;
+#pragma unroll
+    for (int x = 0; x < kW; ++x) {
+      const float f = exp2_fast(s_m[x] - ref);
+      l += s_l[x] * f;
+      sum += s_o[x][d] * f;
+    }
+    out[d] = l == 0.0f ? 0.0f : sum * (c.v_scale / l);
+  }
 }
 
 int simple_splits(const KvView& v) {
@@ -1287,8 +1308,14 @@ Status kv_attend(KvCache* c, const KvAttendArgs& a, cudaStream_t st) {
       WB_TRY(launch_after(kernel, dim3(blocks), G::kThreads, G::kSmem, st, p, p.cluster));
       // a unit of one tile is never cut
       if ((p.cluster > 0 || v.max_slots <= G::kKeys) && !a.accumulate) return Status::Ok();
-      const int chunks = a.accumulate ? std::min((v.max_slots + 1023) / 1024, 64) : 0;
-      return launch_after(k_attend_finish<static_cast<int>(G::kBias)>, dim3(H + v.num_kv * chunks, B), 128, 0, st, p);
+      auto finish = [&](auto wide, auto warps) {
+        constexpr int kW = decltype(warps)::value, kSlots = kW == 4 ? 1024 : 2048;  // slots of a block of weights
+        const int chunks = a.accumulate ? std::min((v.max_slots + kSlots - 1) / kSlots, 64) : 0;
+        return launch_after(k_attend_finish<static_cast<int>(G::kBias), decltype(wide)::value, kW>, dim3(H + v.num_kv * chunks, B), 32 * kW, 0, st, p);
+      };
+      const bool many = c->attend_blocks / p.head_groups > kManyParts * static_cast<int64_t>(v.num_seqs) * v.num_kv;
+      auto by_parts = [&](auto wide) { return many ? finish(wide, std::integral_constant<int, 16>{}) : finish(wide, std::integral_constant<int, 4>{}); };
+      return v.head_dim > 128 ? by_parts(std::true_type{}) : by_parts(std::false_type{});
     }));
   } else {
     p.splits = simple_splits(v);
