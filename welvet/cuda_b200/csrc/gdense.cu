@@ -103,10 +103,11 @@ __global__ void __launch_bounds__(128) k_group_build(const __grid_constant__ Bui
 // token. Products are exact; a scale set's sum (fp32, at most 256 products) is multiplied by its
 // scale and added to the row's fp32 sum. (Records copied to rings of shared memory by the bulk
 // engine, 8 warps a block, were slower on layers below 100 MB: the ring leaves half the warps.)
-// Measured at one token: FP4, 16384 -> 65536, groups of 32 (0.6 GB), 107 us, 5.65 TB/s (86 % of a
-// copy); Int4, 4096 -> 4096, groups of 128 (8.7 MB), 5.7 us, of which 1.3 are the bytes and the
-// rest launch, prologue, one pass of loads and the blocks' join; Int4, 16384 -> 65536, groups of 128:
-// 97, 105 and 134 us at 1, 4 and 8 tokens (the second tile of tokens doubles the MMAs).
+// Measured at one token: FP4, 16384 -> 65536, groups of 32 (0.6 GB), 106 us, 5.7 TB/s (87 % of a
+// copy); Int4, 4096 -> 4096, groups of 128 (8.7 MB), 5.3 us, of which 1.3 are the bytes and the
+// rest launch, prologue, one pass of loads and the blocks' join (8.4 at eight tokens: each block makes
+// its own f16 parts of x); Int4, 16384 -> 65536, groups of 128: 97, 103 and 134 us at 1, 4 and 8 tokens
+// (the second tile of tokens doubles the MMAs).
 // tcgen05 needs N >= 8 and M = 128 rows of dequantised weights in shared or tensor memory; at 1..8
 // tokens the conversion is the work, and the register path takes its result without a store.
 //
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
   // x: a warp takes a token's chunk at a time, eight inputs a lane
   const bool vec = (reinterpret_cast<uintptr_t>(a.x) & 15) == 0 && (a.x_ld & 3) == 0;
   const bool vec2 = (reinterpret_cast<uintptr_t>(a.x) & 7) == 0 && (a.x_ld & 1) == 0;
-  constexpr int kFly = 4;  // chunks whose loads are in flight together
+  constexpr int kFly = 4;  // chunks whose loads are in flight together (8: more code to fetch cold, 8 tokens 8.2 -> 8.5 us)
   const int b_step = kGWarps / chunks, c_step = kGWarps - b_step * chunks;
   auto advance = [&](int& b, int& c) {
     b += b_step;
