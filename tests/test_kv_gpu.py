@@ -802,3 +802,27 @@ def test_attend_small_caches(D, dtype, n, kv, per):
             np.testing.assert_allclose(got[b, :, :L], ws[b].reshape(kv, 3, L).sum(1), rtol=2e-4, atol=4 * EPS)
             assert not got[b, :, L:].any()
     c.check_error()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("dim", [128, 256])
+@pytest.mark.parametrize("n,kv,group,longest", [(10, 8, 1, 900), (2, 2, 3, 6000), (1, 1, 9, 20000)])
+def test_attend_joins_few_and_many_parts(D, dtype, dim, n, kv, group, longest):
+    """Units cut into a few parts and into many, narrow and wide, with the attention weights: dz (see
+    attend64) is below 264 * 2^-24 * 20 here, and a weight moves by twice that."""
+    import torch
+    rng = np.random.default_rng(31 + dim + n)
+    page, H = 16, kv * group
+    per = longest // page + 2
+    lens = [max(0, longest - 97 * b * b) for b in range(n)]
+    kp, vp, table = make_cache(rng, dtype, n, per, page, kv, dim)
+    q = torch.from_numpy(rng.standard_normal((n, H, dim)).astype(np.float32)).cuda()
+    out = torch.full((n, H, dim), float("nan"), device="cuda")
+    w = torch.zeros((n, kv, per * page), device="cuda")
+    c = D.PagedKV(kp, vp, table, i32(lens), num_heads=H, weights=w)
+    c.attend(q, out, accumulate=True)
+    want, ws, bound = attend64(q, kp, vp, table, lens, dim ** -0.5)
+    assert np.all(np.abs(out.cpu().numpy() - want) <= bound)
+    got = w.cpu().numpy()
+    for b, L in enumerate(lens):
+        np.testing.assert_allclose(got[b, :, :L], ws[b].reshape(kv, group, L).sum(1), rtol=1e-3, atol=4 * EPS)
