@@ -826,3 +826,36 @@ def test_attend_joins_few_and_many_parts(D, dtype, dim, n, kv, group, longest):
     got = w.cpu().numpy()
     for b, L in enumerate(lens):
         np.testing.assert_allclose(got[b, :, :L], ws[b].reshape(kv, group, L).sum(1), rtol=1e-3, atol=4 * EPS)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("kv,H,dim,theta,seen", [(4, 8, 128, 10000.0, 0), (2, 2, 64, 500000.0, 1000000), (1, 3, 50, 10000.0, 77)])
+def test_append_rounds_as_the_formula_does(D, dtype, kv, H, dim, theta, seen):
+    """Keys, values and queries are bit for bit what the formula gives in fp32, one rounding an operation,
+    with the angle's cosine and sine rounded once from 64 bits; stored after an exact scale."""
+    import torch
+    n, page = 1500, 16
+    half, per = dim // 2, -(-n // page)
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    q, k, v = (torch.randn((n, h, dim), generator=g, device="cuda") * 2 for h in (H, kv, kv))
+    kp, vp = (torch.zeros((per, page, kv, dim), dtype=types()[dtype], device="cuda") for _ in range(2))
+    scale = 1 / 64 if dtype == "f8" else 1.0
+    out = torch.empty_like(q)
+    c = D.PagedKV(kp, vp, torch.arange(per, dtype=torch.int32, device="cuda")[None], i32([0]), num_heads=H, seen=i32([0]), k_scale=scale, v_scale=scale)
+    c.append(k, v, q=q, q_out=out, cu_tokens=i32([0, n]), theta=theta, start=i32([0]), start_seen=i32([seen]))
+    c.check_error()
+    # half turns are a multiple of two plus what is left: the same angle
+    turns = torch.tensor([math.pow(theta, -2.0 * i / dim) / math.pi for i in range(half)], dtype=torch.float64, device="cuda")
+    u = (seen + torch.arange(n, dtype=torch.float64, device="cuda"))[:, None] * turns
+    angle = math.pi * (u - 2.0 * torch.round(0.5 * u))
+    cs, sn = torch.cos(angle).float()[:, None], torch.sin(angle).float()[:, None]
+
+    def rotate(x):
+        a, b = x[..., :half], x[..., half:]
+        return torch.cat([a * cs - b * sn, a * sn + b * cs], -1)
+
+    assert torch.equal(out, rotate(q))
+    for pool, want in ((kp, rotate(k)), (vp, v)):
+        want = want / scale
+        want = (want.clamp(-448, 448) if dtype == "f8" else want).to(types()[dtype])
+        assert torch.equal(pool.reshape(per * page, kv, dim)[:n].float(), want.float())
