@@ -292,8 +292,9 @@ WELVET_API void welvet_b200_kv_release(welvet_b200_kv* kv);
  * projections, rotary and append, attention with the cell's mask, position kind and scale (mask 3's
  * window is max_seq_len), output projection; accumulate as in kv_attend. prefill: `tokens` rows of a
  * prompt for a sequence that holds nothing yet, attended among themselves as in mha_execute_device
- * (tokens <= the cell's max_seq_len) and appended. The first call for a number of rows allocates the
- * cell's work buffers. */
+ * (tokens <= the cell's max_seq_len) and appended. A call of more rows than any before allocates the
+ * cell's work buffers, so it runs once before it is captured; buffers that a captured call of the cell
+ * (these two, mha_execute_device) works on stay where they are until the cell is released. */
 WELVET_API welvet_status welvet_b200_mha_decode_device(welvet_b200_mha* s, welvet_b200_kv* kv, const float* x_dev,
                                                        float* attn_dev, float* y_dev, int32_t accumulate, void* stream);
 WELVET_API welvet_status welvet_b200_mha_prefill_device(welvet_b200_mha* s, welvet_b200_kv* kv, int32_t sequence,

@@ -148,3 +148,56 @@ def test_example_without_eviction_equals_single_steps(D, wb):
         res.append(outs)
     for a, b in zip(*res):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("captured", ["decode", "prefill"])
+def test_a_longer_prompt_leaves_captured_steps_alone(D, wb, captured):
+    """A step (or a prompt) is captured, then prompts longer than any before go through the cell; replays
+    give the bits of a cell that made the same calls without a capture."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(31)
+    d_model, heads, kv, dim, n = 256, 4, 2, 64, 2
+    w = [torch.randn((r, d_model), generator=g, device="cuda") * 0.08 for r in (heads * dim, kv * dim, kv * dim)]
+    w.append(torch.randn((d_model, heads * dim), generator=g, device="cuda") * 0.08)
+    prompt, long = (torch.randn((t, d_model), generator=g, device="cuda") for t in (9, 300))
+    steps = torch.randn((6, n, d_model), generator=g, device="cuda")
+    results = []
+    for capture in (False, True):
+        cell = wb.MhaCell(*w, d_model, heads, kv, dim, 400, 1, 0, wb.FP8E4M3)
+        cache, other = (cache_for(D, s, heads, kv, dim, 400, torch.bfloat16) for s in (n, 1))
+        x = prompt.clone() if captured == "prefill" else steps[0].clone()
+        y, attn = torch.empty_like(x), torch.empty((x.shape[0], heads * dim), device="cuda")
+
+        def call():
+            if captured == "decode":
+                D.mha_decode(cell, cache, x, y, attn)
+            else:
+                cache.lens.zero_()
+                cache.seen.zero_()
+                D.mha_prefill(cell, cache, 1, x, y, attn)
+
+        call()
+        if capture:
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                call()
+        outs = []
+        for i in range(1, 6):
+            if i in (1, 3):  # each longer than all before
+                other.lens.zero_()
+                other.seen.zero_()
+                p = long[: 100 * i].contiguous()
+                D.mha_prefill(cell, other, 0, p, torch.empty_like(p))
+                torch.cuda.synchronize()
+                junk = [torch.full((1 << 16,), float("nan"), device="cuda") for _ in range(64)]  # noqa: F841
+            x.mul_(0.5).add_(steps[i].repeat(5, 1)[: x.shape[0]])
+            graph.replay() if capture else call()
+            outs += [y.clone(), attn.clone()]
+        cache.check_error()
+        outs += [cache.k_pages.float(), cache.lens.clone()]
+        results.append(outs)
+        results.append(cache.page_table)
+    (plain, t0, graphed, t1) = results
+    for a, b in zip(plain[:-2], graphed[:-2]):
+        assert torch.isfinite(a).all() and torch.equal(a, b)
+    assert torch.equal(plain[-2][t0.long()], graphed[-2][t1.long()]) and torch.equal(plain[-1], graphed[-1])

@@ -320,12 +320,18 @@ Status mha_validate(MhaConfig* cfg) {
   return Status::Ok();
 }
 
-void MhaCell::release_work() {
-  cudaSetDevice(device);
+void MhaWork::release_work() {
   free_dev(x_pad); free_dev(qb); free_dev(kb); free_dev(vb); free_dev(attn); free_dev(attn_pad);
   free_dev(Qr); free_dev(Kr); free_dev(Vd);
   io_q.release(); io_k.release(); io_v.release(); io_o.release();
   bs = 0;
+  captured = false;
+}
+
+MhaCell::~MhaCell() {
+  cudaSetDevice(device);
+  release_work();
+  for (MhaWork& w : outgrown) w.release_work();
 }
 
 Status mha_mount(int device, const MhaConfig& cfg_in, DType dt, const float* Q, const float* K, const float* V,
@@ -354,9 +360,20 @@ Status mha_mount_src(int device, const MhaConfig& cfg_in, DType dt, const Weight
 }
 
 Status mha_reserve(MhaCell* c, int bs, cudaStream_t st) {
-  if (c->bs >= bs) return Status::Ok();
-  c->release_work();
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &capture) != cudaSuccess) cudaGetLastError();  // the legacy stream beside a capture
+  const bool capturing = capture == cudaStreamCaptureStatusActive;
+  if (c->bs >= bs) {
+    c->captured |= capturing;
+    return Status::Ok();
+  }
   WB_CUDA(cudaSetDevice(c->device));
+  if (c->captured) {
+    c->outgrown.push_back(*c);
+    static_cast<MhaWork&>(*c) = MhaWork{};
+  } else {
+    c->release_work();
+  }
   const MhaConfig& g = c->cfg;
   const size_t qd = static_cast<size_t>(g.num_heads) * g.head_dim, kvd = static_cast<size_t>(g.num_kv_heads) * g.head_dim;
   const size_t n = static_cast<size_t>(bs);
@@ -377,6 +394,7 @@ Status mha_reserve(MhaCell* c, int bs, cudaStream_t st) {
   c->io_o.max_tb = xsplit_policy() >= 2 ? 128 : 0;  // attention output: fp32, two x planes
   WB_TRY(alloc_io(c->o, bs, &c->io_o, st));
   c->bs = bs;
+  c->captured = capturing;
   return Status::Ok();
 }
 

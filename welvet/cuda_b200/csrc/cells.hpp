@@ -10,6 +10,8 @@
 #include "dense.hpp"
 #include "kvcache.hpp"
 
+#include <vector>
+
 namespace wb {
 
 // A weight matrix as a cell mount reads it: float32 values (host or device) quantized at
@@ -69,17 +71,23 @@ struct MhaConfig {
 // src/layers/mha/mha.cpp:57-85 (defaults and divisibility checks).
 Status mha_validate(MhaConfig* cfg);
 
-struct MhaCell {
-  int device = 0;
-  MhaConfig cfg;
-  WeightStore sq, sk, sv, so;
-  DeviceDense q, k, v, o;
+// Work buffers of an MHA cell's calls of up to `bs` rows.
+struct MhaWork {
   int bs = 0;
   float *x_pad = nullptr, *qb = nullptr, *kb = nullptr, *vb = nullptr, *attn = nullptr, *attn_pad = nullptr;
   double *Qr = nullptr, *Kr = nullptr, *Vd = nullptr;
   DenseIO io_q, io_k, io_v, io_o;  // per-projection staging and scratch
-  void release_work();
-  ~MhaCell() { release_work(); }
+  bool captured = false;           // a graph holds their addresses
+  void release_work();             // the current device's
+};
+
+struct MhaCell : MhaWork {
+  int device = 0;
+  MhaConfig cfg;
+  WeightStore sq, sk, sv, so;
+  DeviceDense q, k, v, o;
+  std::vector<MhaWork> outgrown;  // buffers that a graph still replays on, kept as long as the cell
+  ~MhaCell();
 };
 
 Status mha_mount(int device, const MhaConfig& cfg, DType dt, const float* Q, const float* K, const float* V,
@@ -87,6 +95,8 @@ Status mha_mount(int device, const MhaConfig& cfg, DType dt, const float* Q, con
 // The same from weight sources Q, K, V, O.
 Status mha_mount_src(int device, const MhaConfig& cfg, DType dt, const WeightSrc (&w)[4], MhaCell* c,
                      cudaStream_t st);
+// Work buffers for `bs` rows. Larger ones replace smaller ones, which are freed unless a call was
+// captured on them: a graph replays on the addresses that it was captured with.
 Status mha_reserve(MhaCell* c, int bs, cudaStream_t st);
 // x [batch*seq][d_model] (device) -> attn [bs][q_dim] (pre) and y [bs][d_model] (post).
 Status mha_forward_device(MhaCell* c, int batch, int seq, const float* x, float* attn, float* y,

@@ -4,8 +4,11 @@
 runs three operators over it: `append` (new tokens, rotated and cast, into the pages), `attend`
 (attention of one new token per sequence) and `evict` (cut back to a budget by accumulated
 attention weight). `GroupDense` is a Dense layer of 4-bit codes with one scale per group of
-inputs, for one to eight rows at a time. All calls are asynchronous on the current stream (or
-`stream`) and allocate nothing, so a whole step can be captured in a CUDA graph.
+inputs, for one to eight rows at a time. `mha_decode` and `mha_prefill` run an MHA cell over such a
+cache. All calls are asynchronous on the current stream (or `stream`) and can be captured in a CUDA
+graph. The calls of a cache and of a layer allocate nothing; a cell's allocate its work buffers when
+a call has more rows than any before, so a step runs once before it is captured. Buffers that were
+captured stay until the cell is released: a longer prompt may follow, and the graph replays on.
 """
 from __future__ import annotations
 
