@@ -290,13 +290,19 @@ WELVET_API void welvet_b200_kv_release(welvet_b200_kv* kv);
 /* An MHA cell's step over a cache of its head counts and width. decode: one new token per sequence,
  * x_dev [num_seqs][d_model] -> attn_dev [num_seqs][q_dim] (may be NULL), y_dev [num_seqs][d_model]:
  * projections, rotary and append, attention with the cell's mask, position kind and scale (mask 3's
- * window is max_seq_len), output projection; accumulate as in kv_attend. prefill: `tokens` rows of a
+ * window is max_seq_len), output projection; accumulate as in kv_attend. decode_active: a sequence with
+ * active_dev[s] = 0 ([num_seqs], NULL: none) is left out, as one that has ended or not begun: nothing of
+ * its slots, weights or page-table row is read or written, its rows of attn and y are zeros (with its length
+ * at 0 kv_evict leaves it alone too). prefill: `tokens` rows of a
  * prompt for a sequence that holds nothing yet, attended among themselves as in mha_execute_device
  * (tokens <= the cell's max_seq_len) and appended. A call of more rows than any before allocates the
  * cell's work buffers, so it runs once before it is captured; buffers that a captured call of the cell
  * (these two, mha_execute_device) works on stay where they are until the cell is released. */
 WELVET_API welvet_status welvet_b200_mha_decode_device(welvet_b200_mha* s, welvet_b200_kv* kv, const float* x_dev,
                                                        float* attn_dev, float* y_dev, int32_t accumulate, void* stream);
+WELVET_API welvet_status welvet_b200_mha_decode_active_device(welvet_b200_mha* s, welvet_b200_kv* kv, const float* x_dev,
+                                                              float* attn_dev, float* y_dev, int32_t accumulate,
+                                                              const int32_t* active_dev, void* stream);
 WELVET_API welvet_status welvet_b200_mha_prefill_device(welvet_b200_mha* s, welvet_b200_kv* kv, int32_t sequence,
                                                         int32_t tokens, const float* x_dev, float* attn_dev,
                                                         float* y_dev, void* stream);

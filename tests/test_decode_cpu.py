@@ -80,3 +80,7 @@ def test_group_sizes_past_the_index_range(in_, out):
     assert L.welvet_b200_group_quantize(in_, out, 64, 14, 2, FAKE, FAKE, FAKE, None, None).code == 2
     h = ctypes.c_void_p()
     assert L.welvet_b200_gdense_mount(in_, out, 64, 14, 2, -1, FAKE, FAKE, None, 1, None, 0, ctypes.byref(h)).code == 2 and not h
+
+
+def test_nil_handles_of_a_step_with_flags():
+    assert W.lib().welvet_b200_mha_decode_active_device(None, None, FAKE, None, FAKE, 0, FAKE, None).code == 1

@@ -201,3 +201,75 @@ def test_a_longer_prompt_leaves_captured_steps_alone(D, wb, captured):
     for a, b in zip(plain[:-2], graphed[:-2]):
         assert torch.isfinite(a).all() and torch.equal(a, b)
     assert torch.equal(plain[-2][t0.long()], graphed[-2][t1.long()]) and torch.equal(plain[-1], graphed[-1])
+
+
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_step_leaves_sequences_out(D, wb, accumulate):
+    """Sequences that have ended are left out of a captured step: one whose former pages belong to another
+    now, one whose page-table row is no longer valid, one that is full. The others get the bits of a batch
+    without them, and a sequence joins again when its flag says so."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(41)
+    d_model, heads, kv, dim, n, per, page = 256, 4, 2, 64, 5, 3, 16
+    w = [torch.randn((r, d_model), generator=g, device="cuda") * 0.08 for r in (heads * dim, kv * dim, kv * dim)]
+    w.append(torch.randn((d_model, heads * dim), generator=g, device="cuda") * 0.08)
+    cell = wb.MhaCell(*w, d_model, heads, kv, dim, 64, 1, 0, wb.FP8E4M3)
+    pools = [torch.randn((n * per, page, kv, dim), generator=g, device="cuda") for _ in range(2)]
+    table = torch.arange(n * per, dtype=torch.int32, device="cuda").reshape(n, per).contiguous()
+    table[1] = table[0]  # its pages went to sequence 0
+    table[2] = -1
+    lens = torch.tensor([5, 20, 7, per * page, 30], dtype=torch.int32, device="cuda")
+    flags = torch.tensor([1, 0, 0, 0, 1], dtype=torch.int32, device="cuda")
+    stay = [0, 4]
+    xs = torch.randn((6, n, d_model), generator=g, device="cuda")
+
+    def cache_of(rows, pools):
+        kw = {}
+        if accumulate:
+            kw = dict(weights=torch.full((len(rows), kv, per * page), 0.5, device="cuda"))
+        return D.PagedKV(*[p.clone() for p in pools], table[rows].contiguous(), lens[rows].contiguous(), num_heads=heads,
+                         seen=lens[rows].contiguous() + 3, **kw)
+
+    cache, alone = cache_of(list(range(n)), pools), cache_of(stay, pools)
+    x, y, attn = xs[0].clone(), torch.full((n, d_model), float("nan"), device="cuda"), torch.full((n, heads * dim), float("nan"), device="cuda")
+    step = lambda: D.mha_decode(cell, cache, x, y, attn, accumulate=accumulate, active=flags)  # noqa: E731
+    graph = torch.cuda.CUDAGraph()
+    flags.zero_()
+    step()  # makes the work buffers; nobody takes part
+    assert not y.any() and not attn.any() and torch.equal(cache.lens, lens) and torch.equal(cache.k_pages, pools[0])
+    flags.copy_(torch.tensor([1, 0, 0, 0, 1]))
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(4):
+        x.copy_(xs[i])
+        graph.replay()
+        ya, aa = torch.empty((2, d_model), device="cuda"), torch.empty((2, heads * dim), device="cuda")
+        D.mha_decode(cell, alone, xs[i][stay].contiguous(), ya, aa, accumulate=accumulate)
+        assert torch.equal(y[stay], ya) and torch.equal(attn[stay], aa)
+        assert not y[1:4].any() and not attn[1:4].any()
+    cache.check_error()
+    assert cache.lens.tolist() == [9, 20, 7, 48, 34] and cache.seen.tolist() == [12, 23, 10, 51, 37]
+    for a, b in ((cache.k_pages, alone.k_pages), (cache.v_pages, alone.v_pages)):
+        assert torch.equal(a, b)
+    if accumulate:
+        assert torch.equal(cache.weights[stay], alone.weights) and bool((cache.weights[1:4] == 0.5).all())
+    flags.fill_(0)
+    flags[1] = 1  # again, with pages of its own
+    table2 = cache.page_table
+    table2[1] = torch.arange(per, dtype=torch.int32) + per
+    x.copy_(xs[4])
+    graph.replay()
+    cache.check_error()
+    assert cache.lens.tolist() == [9, 21, 7, 48, 34] and bool(y[1].any()) and not y[0].any() and not y[2:].any()
+
+
+def test_step_flags_are_checked(D, wb):
+    import torch
+    w = [torch.zeros((128, 128), device="cuda") for _ in range(4)]
+    cell = wb.MhaCell(*w, 128, 2, 2, 64, 64, 1, 0, wb.FP8E4M3)
+    cache = cache_for(D, 3, 2, 2, 64, 32, torch.bfloat16)
+    x, y = torch.zeros((3, 128), device="cuda"), torch.zeros((3, 128), device="cuda")
+    for bad in (torch.ones(3, device="cuda"), torch.ones(2, dtype=torch.int32, device="cuda"), torch.ones(3, dtype=torch.int32)):
+        with pytest.raises(ValueError):
+            D.mha_decode(cell, cache, x, y, active=bad)
+    assert cache.lens.tolist() == [0, 0, 0]

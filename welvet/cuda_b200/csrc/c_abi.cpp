@@ -482,13 +482,20 @@ welvet_status welvet_b200_mha_execute_device(welvet_b200_mha* s, int32_t batch, 
   });
 }
 
-welvet_status welvet_b200_mha_decode_device(welvet_b200_mha* s, welvet_b200_kv* kv, const float* x_dev, float* attn_dev,
-                                            float* y_dev, int32_t accumulate, void* stream) {
+welvet_status welvet_b200_mha_decode_active_device(welvet_b200_mha* s, welvet_b200_kv* kv, const float* x_dev, float* attn_dev,
+                                                   float* y_dev, int32_t accumulate, const int32_t* active_dev,
+                                                   void* stream) {
   return guarded([&] {
     if (!s || !kv || !kv->c || !x_dev || !y_dev) return wb::Status::Invalid("mha: invalid argument");
     WB_CUDA(cudaSetDevice(s->cell.device));
-    return wb::mha_decode_device(&s->cell, kv->c, x_dev, attn_dev, y_dev, accumulate != 0, static_cast<cudaStream_t>(stream));
+    return wb::mha_decode_device(&s->cell, kv->c, x_dev, attn_dev, y_dev, accumulate != 0, active_dev,
+                                 static_cast<cudaStream_t>(stream));
   });
+}
+
+welvet_status welvet_b200_mha_decode_device(welvet_b200_mha* s, welvet_b200_kv* kv, const float* x_dev, float* attn_dev,
+                                            float* y_dev, int32_t accumulate, void* stream) {
+  return welvet_b200_mha_decode_active_device(s, kv, x_dev, attn_dev, y_dev, accumulate, nullptr, stream);
 }
 
 welvet_status welvet_b200_mha_prefill_device(welvet_b200_mha* s, welvet_b200_kv* kv, int32_t sequence, int32_t tokens,

@@ -434,7 +434,8 @@ static Status mha_cache_fits(const MhaCell& c, const KvCache& kv) {
 
 static double mha_theta(const MhaConfig& g) { return g.pos == 0 || g.pos == 3 ? g.rope_theta : 0.0; }
 
-Status mha_decode_device(MhaCell* c, KvCache* kv, const float* x, float* attn, float* y, bool accumulate, cudaStream_t st) {
+Status mha_decode_device(MhaCell* c, KvCache* kv, const float* x, float* attn, float* y, bool accumulate,
+                         const int32_t* active, cudaStream_t st) {
   WB_TRY(mha_cache_fits(*c, *kv));
   const MhaConfig& g = c->cfg;
   const int rows = kv->view.num_seqs, qd = g.num_heads * g.head_dim, kvd = g.num_kv_heads * g.head_dim;
@@ -452,6 +453,8 @@ Status mha_decode_device(MhaCell* c, KvCache* kv, const float* x, float* attn, f
   ap.k_ld = ap.v_ld = kvd;
   ap.q_ld = ap.q_out_ld = qd;
   ap.theta = mha_theta(g);
+  ap.active = active;
+  ap.step_lens = kv->step_lens;
   WB_TRY(kv_append(kv, ap, st));
   float* attn_out = attn ? attn : c->attn;
   KvAttendArgs at;
@@ -463,6 +466,7 @@ Status mha_decode_device(MhaCell* c, KvCache* kv, const float* x, float* attn, f
   at.window = g.mask == 3 ? (g.window > 0 ? g.window : g.max_seq_len) : 0;
   at.alibi = g.pos == 2 || g.pos == 3;
   at.accumulate = accumulate;
+  at.lens = active ? kv->step_lens : nullptr;
   WB_TRY(kv_attend(kv, at, st));
   return forward_device(c->o, rows, attn_out, qd, y, y, &c->io_o, st, false);
 }

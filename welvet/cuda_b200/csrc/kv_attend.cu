@@ -1283,6 +1283,7 @@ Status kv_attend(KvCache* c, const KvAttendArgs& a, cudaStream_t st) {
   p.a = a;
   p.c = c->view;
   const KvView& v = c->view;
+  if (a.lens) p.c.lens = const_cast<int32_t*>(a.lens);  // read only
   if (!(p.a.scale > 0.0f)) p.a.scale = static_cast<float>(1.0 / std::sqrt(static_cast<double>(v.head_dim)));
   if (!p.a.weights_in) p.a.weights_in = v.weights;
   p.part = c->part;

@@ -89,6 +89,8 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_append(const __grid_const
     seq = a;
     i = t - p.a.cu[seq];
     live = live && i >= 0 && t < p.a.cu[seq + 1];
+  } else if (p.a.active) {
+    live = live && p.a.active[seq] != 0;
   }
   if (live) {
     const int64_t slot = static_cast<int64_t>(p.a.start[seq]) + i;
@@ -178,9 +180,14 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_append(const __grid_const
   if (!s_last) return;
   if (tid == 0) *p.ticket = 0;
   for (int s = tid; s < c.num_seqs; s += kAppendThreads) {
+    if (p.a.active && p.a.active[s] == 0) {
+      p.a.step_lens[s] = 0;
+      continue;
+    }
     const int n = p.a.cu ? p.a.cu[s + 1] - p.a.cu[s] : (p.a.only < 0 ? 1 : (s == p.a.only ? p.a.rows : 0));
     const int64_t len = static_cast<int64_t>(p.a.start[s]) + n, tot = static_cast<int64_t>(p.a.start_seen[s]) + n;
     c.lens[s] = static_cast<int32_t>(len < c.max_slots ? len : c.max_slots);
+    if (p.a.active) p.a.step_lens[s] = c.lens[s];
     if (c.seen != c.lens) c.seen[s] = static_cast<int32_t>(tot);
   }
 }
@@ -601,7 +608,8 @@ static Status kv_alloc(KvCache* c) {
     return at;
   };
   WB_TRY(attend_plan(c));
-  const size_t err = take(4), ticket = take(4), evict_tickets = take(v.positions ? static_cast<size_t>(v.num_seqs) * 4 : 0);
+  const size_t err = take(4), ticket = take(4), step_lens = take(static_cast<size_t>(v.num_seqs) * 4);
+  const size_t evict_tickets = take(v.positions ? static_cast<size_t>(v.num_seqs) * 4 : 0);
   const size_t part = take(c->part_bytes);  // from here on nothing needs to start as zero
   const size_t spans = take(c->span_bytes);
   const size_t scores = take(v.weights ? rows * v.max_slots * 4 : 0), lse = take(v.weights ? rows * 4 : 0);
@@ -609,6 +617,7 @@ static Status kv_alloc(KvCache* c) {
   WB_CUDA(cudaMalloc(&c->work, bytes));
   c->err = reinterpret_cast<int*>(c->work + err);
   c->ticket = reinterpret_cast<int*>(c->work + ticket);
+  c->step_lens = reinterpret_cast<int32_t*>(c->work + step_lens);
   c->evict_tickets = reinterpret_cast<int*>(c->work + evict_tickets);
   c->spans = c->work + spans;
   c->part = reinterpret_cast<float*>(c->work + part);

@@ -53,6 +53,7 @@ struct KvCache {
   uint8_t* work = nullptr;       // the one allocation behind what follows
   int* err = nullptr;
   int* ticket = nullptr;         // block counter of append (zero between calls)
+  int32_t* step_lens = nullptr;  // [num_seqs] lengths of a step that leaves sequences out
   // attend (kv_attend.cu)
   bool attend_tiled = false;
   int attend_blocks = 0;         // blocks of the tiled form
@@ -85,6 +86,8 @@ struct KvAppendArgs {
   double theta = 0.0;           // <= 0: no rotation
   const int32_t* start = nullptr;       // slots in use before the call (null: lens)
   const int32_t* start_seen = nullptr;  // tokens seen before the call (null: seen)
+  const int32_t* active = nullptr;      // [num_seqs]; 0: this sequence's row is left out (cu null, only < 0)
+  int32_t* step_lens = nullptr;         // with active: lens, 0 for a sequence that is left out
 };
 Status kv_append(KvCache* c, const KvAppendArgs& a, cudaStream_t st);
 
@@ -97,6 +100,7 @@ struct KvAttendArgs {
   int alibi = 0;
   int accumulate = 0;  // weights = weights_in + this step's attention weights
   const float* weights_in = nullptr;  // null: weights
+  const int32_t* lens = nullptr;      // slots to attend to (null: the cache's lens)
 };
 Status kv_attend(KvCache* c, const KvAttendArgs& a, cudaStream_t st);
 

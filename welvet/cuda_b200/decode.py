@@ -53,6 +53,7 @@ _sig("welvet_b200_gdense_execute_device", _ST, c_void_p, c_int32, c_void_p, c_in
 _sig("welvet_b200_gdense_release", None, c_void_p)
 
 _sig("welvet_b200_mha_decode_device", _ST, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p)
+_sig("welvet_b200_mha_decode_active_device", _ST, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_void_p)
 _sig("welvet_b200_mha_prefill_device", _ST, c_void_p, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p)
 
 _append, _attend, _evict, _gemv = (_L.welvet_b200_kv_append, _L.welvet_b200_kv_attend, _L.welvet_b200_kv_evict,
@@ -211,10 +212,12 @@ def _mha_rows(cell_d: int, rows: int, x, y, attn, width: int):
     return x.data_ptr(), None if attn is None else attn.data_ptr(), y.data_ptr()
 
 
-def mha_decode(cell, cache: PagedKV, x, y, attn=None, *, accumulate: bool = False, stream=None) -> None:
-    """One new token per sequence through an MhaCell over a cache: x, y [sequences, d_model]."""
+def mha_decode(cell, cache: PagedKV, x, y, attn=None, *, accumulate: bool = False, active=None, stream=None) -> None:
+    """One new token per sequence through an MhaCell over a cache: x, y [sequences, d_model]. Sequences
+    whose `active` (int32 on the GPU) is 0 are left out: their cache stays as it is, their rows of y are 0."""
     xp, ap, yp = _mha_rows(cell.d_model, cache.num_seqs, x, y, attn, cache._qw)
-    check(_L.welvet_b200_mha_decode_device(cell._h, cache._h, xp, ap, yp, 1 if accumulate else 0, _stream(stream, x)))
+    check(_L.welvet_b200_mha_decode_active_device(cell._h, cache._h, xp, ap, yp, 1 if accumulate else 0,
+                                                  _ints(active, cache.num_seqs, "active"), _stream(stream, x)))
 
 
 def mha_prefill(cell, cache: PagedKV, sequence: int, x, y, attn=None, *, stream=None) -> None:
