@@ -283,7 +283,8 @@ WELVET_API welvet_status welvet_b200_kv_evict(welvet_b200_kv* kv, int32_t keep, 
                                               const int32_t* positions_in, void* stream);
 
 /* Synchronizes `stream`; status 1 (cleared by the report) if an earlier call met a page id outside
- * the pool or a length outside the sequence's slots: those rows were skipped. */
+ * the pool, a length outside the sequence's slots or a prompt for a sequence that holds slots: those
+ * rows were skipped. */
 WELVET_API welvet_status welvet_b200_kv_check_error(welvet_b200_kv* kv, void* stream);
 WELVET_API void welvet_b200_kv_release(welvet_b200_kv* kv);
 
@@ -293,9 +294,10 @@ WELVET_API void welvet_b200_kv_release(welvet_b200_kv* kv);
  * window is max_seq_len), output projection; accumulate as in kv_attend. decode_active: a sequence with
  * active_dev[s] = 0 ([num_seqs], NULL: none) is left out, as one that has ended or not begun: nothing of
  * its slots, weights or page-table row is read or written, its rows of attn and y are zeros (with its length
- * at 0 kv_evict leaves it alone too). prefill: `tokens` rows of a
- * prompt for a sequence that holds nothing yet, attended among themselves as in mha_execute_device
- * (tokens <= the cell's max_seq_len) and appended. A call of more rows than any before allocates the
+ * at 0 kv_evict leaves it alone too). prefill: `tokens` rows of a prompt from position 0, attended among
+ * themselves as in mha_execute_device (tokens <= the cell's max_seq_len) and appended to a sequence whose
+ * length is 0, whatever its seen; its seen becomes `tokens`. One that holds slots keeps them, and
+ * kv_check_error says so. A call of more rows than any before allocates the
  * cell's work buffers, so it runs once before it is captured; buffers that a captured call of the cell
  * (these two, mha_execute_device) works on stay where they are until the cell is released. */
 WELVET_API welvet_status welvet_b200_mha_decode_device(welvet_b200_mha* s, welvet_b200_kv* kv, const float* x_dev,

@@ -273,3 +273,45 @@ def test_step_flags_are_checked(D, wb):
         with pytest.raises(ValueError):
             D.mha_decode(cell, cache, x, y, active=bad)
     assert cache.lens.tolist() == [0, 0, 0]
+
+
+def test_prompt_into_a_row_that_was_used(D, wb):
+    """A row whose length was reset, but not its count of tokens seen, takes a prompt as a new one does: the
+    keys' positions are those of the attention just computed. A row that holds slots keeps them, with an error."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(51)
+    d_model, heads, kv, dim = 256, 4, 2, 64
+    w = [torch.randn((r, d_model), generator=g, device="cuda") * 0.08 for r in (heads * dim, kv * dim, kv * dim)]
+    w.append(torch.randn((d_model, heads * dim), generator=g, device="cuda") * 0.08)
+    cell = wb.MhaCell(*w, d_model, heads, kv, dim, 64, 1, 0, wb.FP8E4M3)
+    x = torch.randn((20, d_model), generator=g, device="cuda")
+    outs = []
+    for used in (False, True):
+        cache = cache_for(D, 3, heads, kv, dim, 64, torch.float32, records=True)
+        cache.page_table.copy_(torch.arange(12, dtype=torch.int32).reshape(3, 4))
+        if used:
+            y = torch.empty((11, d_model), device="cuda")
+            D.mha_prefill(cell, cache, 1, x[:11].flip(0).contiguous(), y)
+            cache.weights.fill_(3.0)
+            cache.lens.zero_()
+        y = torch.empty((7, d_model), device="cuda")
+        D.mha_prefill(cell, cache, 1, x[:7].contiguous(), y)
+        cache.check_error()
+        assert cache.lens.tolist() == [0, 7, 0] and cache.seen.tolist() == [0, 7, 0]
+        assert cache.positions[1, :, :7].tolist() == [list(range(7))] * kv and not cache.weights[1, :, :7].any()
+        only = torch.tensor([0, 1, 0], dtype=torch.int32, device="cuda")
+        for t in range(7, 12):
+            y = torch.empty((3, d_model), device="cuda")
+            D.mha_decode(cell, cache, x[t].expand(3, -1).contiguous(), y, active=only)
+        outs += [y, cache.k_pages[4].clone(), cache.v_pages[4].clone(), cache.lens.clone(), cache.seen.clone()]
+        outs[-3][12:], outs[-4][12:] = 0, 0  # slots not in use
+    for a, b in zip(outs[:5], outs[5:]):
+        assert torch.equal(a, b)
+    k, positions = cache.k_pages.clone(), cache.positions.clone()
+    D.mha_prefill(cell, cache, 1, x[:3].contiguous(), torch.empty((3, d_model), device="cuda"))
+    with pytest.raises(wb.WelvetError) as e:
+        cache.check_error()
+    assert e.value.code == 1 and "holds" in str(e.value)
+    cache.check_error()
+    assert cache.lens.tolist() == [0, 12, 0] and cache.seen.tolist() == [0, 12, 0]
+    assert torch.equal(k, cache.k_pages) and torch.equal(positions, cache.positions)

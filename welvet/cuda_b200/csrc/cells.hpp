@@ -106,8 +106,8 @@ Status mha_forward_device(MhaCell* c, int batch, int seq, const float* x, float*
 // outlive the call. Decode: one new token per sequence, x [num_seqs][d_model]: projections, rotary
 // and append, attention over each sequence's slots (the cell's mask, position kind and scale),
 // output projection; a sequence with active[s] = 0 (device, may be null) is left out: its cache stays
-// as it is, its rows of attn and y are zeros. Prefill: a prompt of `tokens` rows for one sequence that holds nothing yet:
-// the cell's own attention among them, and their keys and values into the cache.
+// as it is, its rows of attn and y are zeros. Prefill: a prompt of `tokens` rows from position 0 for
+// one sequence of length 0: the cell's own attention among them, and their keys and values into the cache.
 Status mha_decode_device(MhaCell* c, KvCache* kv, const float* x, float* attn, float* y, bool accumulate,
                          const int32_t* active, cudaStream_t st);
 Status mha_prefill_device(MhaCell* c, KvCache* kv, int sequence, int tokens, const float* x, float* attn, float* y,

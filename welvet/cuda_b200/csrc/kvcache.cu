@@ -91,10 +91,13 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_append(const __grid_const
     live = live && i >= 0 && t < p.a.cu[seq + 1];
   } else if (p.a.active) {
     live = live && p.a.active[seq] != 0;
+  } else if (p.a.only >= 0 && p.a.start[seq] != 0) {
+    live = false;
+    if (tid == 0) atomicCAS(c.err, 0, kKvErrHeld);
   }
   if (live) {
     const int64_t slot = static_cast<int64_t>(p.a.start[seq]) + i;
-    const int64_t pos = static_cast<int64_t>(p.a.start_seen[seq]) + i;
+    const int64_t pos = static_cast<int64_t>(p.a.only >= 0 ? 0 : p.a.start_seen[seq]) + i;
     const bool in_range = slot >= 0 && slot < c.max_slots;
     const int at_page = in_range ? static_cast<int>(slot) / c.page_size : 0, in_page = in_range ? static_cast<int>(slot) - at_page * c.page_size : 0;
     int64_t page = in_range ? c.table[seq * c.table_stride + at_page] : -1;  // on its way while the angles are taken
@@ -184,8 +187,9 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_append(const __grid_const
       p.a.step_lens[s] = 0;
       continue;
     }
-    const int n = p.a.cu ? p.a.cu[s + 1] - p.a.cu[s] : (p.a.only < 0 ? 1 : (s == p.a.only ? p.a.rows : 0));
-    const int64_t len = static_cast<int64_t>(p.a.start[s]) + n, tot = static_cast<int64_t>(p.a.start_seen[s]) + n;
+    if (p.a.only >= 0 && (s != p.a.only || p.a.start[s] != 0)) continue;
+    const int n = p.a.cu ? p.a.cu[s + 1] - p.a.cu[s] : (p.a.only < 0 ? 1 : p.a.rows);
+    const int64_t len = static_cast<int64_t>(p.a.start[s]) + n, tot = static_cast<int64_t>(p.a.only >= 0 ? 0 : p.a.start_seen[s]) + n;
     c.lens[s] = static_cast<int32_t>(len < c.max_slots ? len : c.max_slots);
     if (p.a.active) p.a.step_lens[s] = c.lens[s];
     if (c.seen != c.lens) c.seen[s] = static_cast<int32_t>(tot);
@@ -736,6 +740,7 @@ Status kv_check_error(KvCache* c, cudaStream_t st) {
   if (e == 0) return Status::Ok();
   WB_CUDA(cudaMemsetAsync(c->err, 0, 4, st));
   WB_CUDA(cudaStreamSynchronize(st));
+  if (e == kKvErrHeld) return Status::Invalid("kv: a prompt for a sequence that holds slots already");
   if (e == kKvErrPage) return Status::Invalid("kv: a page id of the table is outside the pool");
   return Status::Invalid("kv: a length or an append is outside the sequence's slots");
 }

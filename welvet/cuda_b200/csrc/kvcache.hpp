@@ -43,6 +43,7 @@ struct KvView {
 // Error codes that kernels leave in the error word.
 constexpr int kKvErrPage = 1;  // a page id of the table outside [0, num_pages)
 constexpr int kKvErrSlot = 2;  // a length outside [0, max_slots], or an append past the last slot
+constexpr int kKvErrHeld = 3;  // a prompt for a sequence that holds slots already
 
 struct KvCache {
   int device = 0;
@@ -82,7 +83,8 @@ struct KvAppendArgs {
   float* q_out = nullptr;
   int64_t k_ld = 0, v_ld = 0, q_ld = 0, q_out_ld = 0;
   const int32_t* cu = nullptr;  // [num_seqs + 1] first row of each sequence; null: one row each
-  int only = -1;                // >= 0: every row is this sequence's (cu null)
+  int only = -1;                // >= 0: every row is this sequence's, a prompt from position 0 (cu, start,
+                                // start_seen null); one that holds slots already is left as it is
   double theta = 0.0;           // <= 0: no rotation
   const int32_t* start = nullptr;       // slots in use before the call (null: lens)
   const int32_t* start_seen = nullptr;  // tokens seen before the call (null: seen)

@@ -190,7 +190,8 @@ class PagedKV:
             _fail(st)
 
     def check_error(self, stream=None) -> None:
-        """Synchronizes and raises (code 1) if an earlier call met a bad page id or length."""
+        """Synchronizes and raises (code 1) if an earlier call met a bad page id or length, or a prompt for a
+        sequence that holds slots."""
         check(_L.welvet_b200_kv_check_error(self._h, _stream(stream, self.lens)))
 
     def release(self) -> None:
@@ -221,8 +222,8 @@ def mha_decode(cell, cache: PagedKV, x, y, attn=None, *, accumulate: bool = Fals
 
 
 def mha_prefill(cell, cache: PagedKV, sequence: int, x, y, attn=None, *, stream=None) -> None:
-    """A prompt x [tokens, d_model] through an MhaCell, its keys and values into a sequence of the cache that
-    holds nothing yet."""
+    """A prompt x [tokens, d_model] through an MhaCell, its keys and values into a sequence of the cache whose
+    length is 0, from position 0. One that holds slots keeps them; `check_error` says so."""
     xp, ap, yp = _mha_rows(cell.d_model, x.shape[0], x, y, attn, cache._qw)
     check(_L.welvet_b200_mha_prefill_device(cell._h, cache._h, sequence, x.shape[0], xp, ap, yp, _stream(stream, x)))
 
