@@ -254,7 +254,9 @@ WELVET_API welvet_status welvet_b200_kv_create(const welvet_b200_kv_desc* desc, 
  * start_seen[s] + i; afterwards lens = start + n and seen = start_seen + n (start, start_seen NULL:
  * lens and seen themselves, advanced in place). theta > 0 rotates k, and q [rows][num_heads *
  * head_dim] into q_out (may be q), as the MHA cell does (pairs d, d + head_dim/2); values are stored
- * as they are. A slot past max_slots or a page id outside the pool is skipped and recorded. */
+ * as they are. A slot past max_slots or a page id outside the pool is skipped and recorded; so is
+ * what cu_tokens gives a sequence beyond `rows`, and a cu_tokens that decreases: lengths advance by the
+ * rows that there are. */
 WELVET_API welvet_status welvet_b200_kv_append(welvet_b200_kv* kv, int32_t rows, const float* k, int64_t k_ld,
                                                const float* v, int64_t v_ld, const float* q, int64_t q_ld,
                                                float* q_out, int64_t q_out_ld, const int32_t* cu_tokens, double theta,
@@ -283,8 +285,8 @@ WELVET_API welvet_status welvet_b200_kv_evict(welvet_b200_kv* kv, int32_t keep, 
                                               const int32_t* positions_in, void* stream);
 
 /* Synchronizes `stream`; status 1 (cleared by the report) if an earlier call met a page id outside
- * the pool, a length outside the sequence's slots or a prompt for a sequence that holds slots: those
- * rows were skipped. */
+ * the pool, a length outside the sequence's slots, cu_tokens that do not fit the rows or a prompt for a
+ * sequence that holds slots: those rows were skipped. */
 WELVET_API welvet_status welvet_b200_kv_check_error(welvet_b200_kv* kv, void* stream);
 WELVET_API void welvet_b200_kv_release(welvet_b200_kv* kv);
 

@@ -859,3 +859,33 @@ def test_append_rounds_as_the_formula_does(D, dtype, kv, H, dim, theta, seen):
         want = want / scale
         want = (want.clamp(-448, 448) if dtype == "f8" else want).to(types()[dtype])
         assert torch.equal(pool.reshape(per * page, kv, dim)[:n].float(), want.float())
+
+
+@pytest.mark.parametrize("cu,counts", [([0, 2, 7], [2, 3]), ([0, 9, 9], [5, 0]), ([3, 2, 5], [0, 3]), ([-2, 1, 5], [0, 4]),
+                                       ([0, 5, 2 ** 31 - 1], [5, 0]), ([-2 ** 31, 0, 5], [0, 5])])
+def test_append_rows_that_cu_tokens_do_not_fit(D, wb, cu, counts):
+    """Offsets past the rows, below zero or decreasing: lengths advance by the rows that there are, never
+    back, and the error word says so."""
+    import torch
+    rng = np.random.default_rng(19)
+    kv, dim, page, per, rows = 2, 64, 16, 2, 5
+    kp, vp, table = make_cache(rng, "f32", 2, per, page, kv, dim, fill="nan")
+    k = torch.from_numpy(rng.standard_normal((rows, kv, dim)).astype(np.float32)).cuda()
+    lens, seen = i32([4, 6]), i32([10, 20])
+    c = D.PagedKV(kp, vp, table, lens, num_heads=2, seen=seen)
+    c.append(k, k, cu_tokens=i32(cu))
+    with pytest.raises(wb.WelvetError) as e:
+        c.check_error()
+    assert e.value.code == 1 and "cu_tokens" in str(e.value)
+    assert lens.tolist() == [4 + counts[0], 6 + counts[1]] and seen.tolist() == [10 + counts[0], 20 + counts[1]]
+    for b, (first, n) in enumerate(zip((4, 6), counts)):
+        for i in range(n):
+            j = first + i
+            assert torch.equal(kp[int(table[b, j // page]), j % page], k[cu[b] + i])
+    assert int(torch.isfinite(kp[..., 0]).sum()) == sum(counts) * kv
+    c.append(k, k, cu_tokens=i32([0, 2, 5]))
+    c.check_error()
+    # offsets that begin or end within the rows are no error: rows before and after them are nobody's
+    c.append(k, k, cu_tokens=i32([1, 2, 4]))
+    c.check_error()
+    assert lens.tolist() == [4 + counts[0] + 3, 6 + counts[1] + 5]

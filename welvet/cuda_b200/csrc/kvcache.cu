@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_append(const __grid_const
     }
     seq = a;
     i = t - p.a.cu[seq];
-    live = live && i >= 0 && t < p.a.cu[seq + 1];
+    live = live && i >= 0 && i <= t && t < p.a.cu[seq + 1];
   } else if (p.a.active) {
     live = live && p.a.active[seq] != 0;
   } else if (p.a.only >= 0 && p.a.start[seq] != 0) {
@@ -188,7 +188,12 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_append(const __grid_const
       continue;
     }
     if (p.a.only >= 0 && (s != p.a.only || p.a.start[s] != 0)) continue;
-    const int n = p.a.cu ? p.a.cu[s + 1] - p.a.cu[s] : (p.a.only < 0 ? 1 : p.a.rows);
+    int64_t n = p.a.only < 0 ? 1 : p.a.rows;
+    if (p.a.cu) {  // the rows that there are
+      const int64_t from = p.a.cu[s], to = p.a.cu[s + 1];
+      n = from < 0 ? 0 : max(min(to, static_cast<int64_t>(p.a.rows)) - from, static_cast<int64_t>(0));
+      if (n != to - from) atomicCAS(c.err, 0, kKvErrRows);
+    }
     const int64_t len = static_cast<int64_t>(p.a.start[s]) + n, tot = static_cast<int64_t>(p.a.only >= 0 ? 0 : p.a.start_seen[s]) + n;
     c.lens[s] = static_cast<int32_t>(len < c.max_slots ? len : c.max_slots);
     if (p.a.active) p.a.step_lens[s] = c.lens[s];
@@ -740,6 +745,7 @@ Status kv_check_error(KvCache* c, cudaStream_t st) {
   if (e == 0) return Status::Ok();
   WB_CUDA(cudaMemsetAsync(c->err, 0, 4, st));
   WB_CUDA(cudaStreamSynchronize(st));
+  if (e == kKvErrRows) return Status::Invalid("kv append: cu_tokens decreases, is negative or goes past the rows");
   if (e == kKvErrHeld) return Status::Invalid("kv: a prompt for a sequence that holds slots already");
   if (e == kKvErrPage) return Status::Invalid("kv: a page id of the table is outside the pool");
   return Status::Invalid("kv: a length or an append is outside the sequence's slots");

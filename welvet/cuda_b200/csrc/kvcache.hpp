@@ -44,6 +44,7 @@ struct KvView {
 constexpr int kKvErrPage = 1;  // a page id of the table outside [0, num_pages)
 constexpr int kKvErrSlot = 2;  // a length outside [0, max_slots], or an append past the last slot
 constexpr int kKvErrHeld = 3;  // a prompt for a sequence that holds slots already
+constexpr int kKvErrRows = 4;  // cu decreases, is negative or goes past the rows
 
 struct KvCache {
   int device = 0;

@@ -190,8 +190,8 @@ class PagedKV:
             _fail(st)
 
     def check_error(self, stream=None) -> None:
-        """Synchronizes and raises (code 1) if an earlier call met a bad page id or length, or a prompt for a
-        sequence that holds slots."""
+        """Synchronizes and raises (code 1) if an earlier call met a bad page id, length or cu_tokens,
+        or a prompt for a sequence that holds slots."""
         check(_L.welvet_b200_kv_check_error(self._h, _stream(stream, self.lens)))
 
     def release(self) -> None:
