@@ -889,3 +889,24 @@ def test_append_rows_that_cu_tokens_do_not_fit(D, wb, cu, counts):
     c.append(k, k, cu_tokens=i32([1, 2, 4]))
     c.check_error()
     assert lens.tolist() == [4 + counts[0] + 3, 6 + counts[1] + 5]
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("dim", [128, 24, 33])
+@pytest.mark.parametrize("ks,vs", [(0.013, 3.7), (1.0 / 448, 1.0), (2.0 ** -126, 2.0 ** 127), (1e-30, 1e30)])
+def test_append_divides_by_the_scale(D, dtype, dim, ks, vs):
+    """Stored values are x / scale rounded to fp32 and then to the page's type, for scales that are no
+    powers of two as well."""
+    import torch
+    n, kv, page = 300, 3, 16
+    per = -(-n // page)
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    k, v = (torch.randn((n, kv, dim), generator=g, device="cuda") * s for s in (ks * 40, min(vs, 1e30) * 40))
+    kp, vp = (torch.zeros((per, page, kv, dim), dtype=types()[dtype], device="cuda") for _ in range(2))
+    c = D.PagedKV(kp, vp, torch.arange(per, dtype=torch.int32, device="cuda")[None], i32([0]), num_heads=kv, k_scale=ks, v_scale=vs)
+    c.append(k, v, cu_tokens=i32([0, n]))
+    c.check_error()
+    for pool, x, scale in ((kp, k, ks), (vp, v, vs)):
+        want = (x / torch.tensor(scale, dtype=torch.float32, device="cuda")).float()
+        want = (want.clamp(-448, 448) if dtype == "f8" else want).to(types()[dtype])
+        assert torch.equal(pool.reshape(per * page, kv, dim)[:n].float(), want.float())

@@ -43,7 +43,8 @@ __device__ __forceinline__ void rotate(float& a, float& b, float cs, float sn) {
 // query heads, pair (d, d + half) by pair. HBM bound: 4 B read per element, the page's type
 // written (and 4 B for q). kVec: four consecutive pairs a thread (16-byte accesses).
 // kDim: the width, 0 where it is not a constant (13k prompt tokens of 48 heads of 128: 74 us, 90 without).
-template <typename T, bool kVec, int kDim>
+// kDiv: the scales are not both powers of two.
+template <typename T, bool kVec, int kDim, bool kDiv>
 __global__ void __launch_bounds__(kAppendThreads, 4) k_append(const __grid_constant__ AppendParams p) {
   __shared__ float s_cos[kMaxPairs], s_sin[kMaxPairs];
   __shared__ int s_last;
@@ -138,9 +139,9 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_append(const __grid_const
             *reinterpret_cast<float4*>(o + d + h2) = make_float4(b[0], b[1], b[2], b[3]);
           } else if (page >= 0) {
             T* o = is_v ? vd + (h - kv_heads) * c.v.head : kd + h * c.k.head;
-            const float s = is_v ? vs : ks;
-            store4<T>(o + d, a, s);
-            store4<T>(o + d + h2, b, s);
+            const float scale = kDiv ? (is_v ? c.v_scale : c.k_scale) : 0.0f, inv = kDiv ? 0.0f : (is_v ? vs : ks);
+            store4<T, kDiv>(o + d, a, scale, inv);
+            store4<T, kDiv>(o + d + h2, b, scale, inv);
           }
         }
       }
@@ -161,9 +162,9 @@ __global__ void __launch_bounds__(kAppendThreads, 4) k_append(const __grid_const
           o[db] = b;
         } else if (page >= 0) {
           T* o = is_v ? vd + (h - kv_heads) * c.v.head : kd + h * c.k.head;
-          const float s = is_v ? vs : ks;
-          if (!odd) o[d0] = to_stored<T>(a * s);
-          o[db] = to_stored<T>(b * s);
+          const float scale = kDiv ? (is_v ? c.v_scale : c.k_scale) : 0.0f, inv = kDiv ? 0.0f : (is_v ? vs : ks);
+          if (!odd) o[d0] = to_stored<T>(over<kDiv>(a, scale, inv));
+          o[db] = to_stored<T>(over<kDiv>(b, scale, inv));
         }
       }
     }
@@ -679,7 +680,13 @@ Status kv_append(KvCache* c, const KvAppendArgs& a, cudaStream_t st) {
   return by_type(c->type, [&](auto* t) {
     using T = std::remove_pointer_t<decltype(t)>;
     const int blocks = a.rows > 0 ? a.rows : 1;  // no row: the lengths are still carried over
-    auto* kernel = !vec ? k_append<T, false, 0> : (p.c.head_dim == 128 ? k_append<T, true, 128> : (p.c.head_dim == 64 ? k_append<T, true, 64> : k_append<T, true, 0>));
+    // both reciprocals exact: the fraction of a power of two is one half
+    int e;
+    const bool exact = std::frexp(p.c.k_scale, &e) == 0.5f && std::frexp(p.c.v_scale, &e) == 0.5f;
+    auto* kernel = !vec ? (exact ? k_append<T, false, 0, false> : k_append<T, false, 0, true>)
+                        : (!exact ? k_append<T, true, 0, true>
+                                  : (p.c.head_dim == 128 ? k_append<T, true, 128, false>
+                                                         : (p.c.head_dim == 64 ? k_append<T, true, 64, false> : k_append<T, true, 0, false>)));
     return launch_after(kernel, dim3(blocks), kAppendThreads, 0, st, p);
   });
 }

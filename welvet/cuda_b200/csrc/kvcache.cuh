@@ -27,18 +27,27 @@ __device__ __forceinline__ T to_stored(float x) {
   else return __nv_fp8_e4m3(x);
 }
 
-// Four values x * s to consecutive elements (aligned to four elements).
-template <typename T>
-__device__ __forceinline__ void store4(T* dst, const float (&x)[4], float s) {
+// What a page's values are divided by. The reciprocal of a power of two is exact, and one product
+// gives the quotient; other scales divide (kDiv), so that a value between two codes goes to the side
+// that x / scale rounds to.
+template <bool kDiv>
+__device__ __forceinline__ float over(float x, float scale, float inv) {
+  return kDiv ? __fdiv_rn(x, scale) : x * inv;
+}
+
+// Four values over the scale to consecutive elements (aligned to four elements).
+template <typename T, bool kDiv>
+__device__ __forceinline__ void store4(T* dst, const float (&x)[4], float scale, float inv) {
+  auto f = [&](int i) { return over<kDiv>(x[i], scale, inv); };
   if constexpr (std::is_same_v<T, float>) {
-    *reinterpret_cast<float4*>(dst) = make_float4(x[0] * s, x[1] * s, x[2] * s, x[3] * s);
+    *reinterpret_cast<float4*>(dst) = make_float4(f(0), f(1), f(2), f(3));
   } else if constexpr (sizeof(T) == 2) {
     union { T t[4]; uint2 u; } o;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o.t[i] = to_stored<T>(x[i] * s);
+    for (int i = 0; i < 4; ++i) o.t[i] = to_stored<T>(f(i));
     *reinterpret_cast<uint2*>(dst) = o.u;
   } else {
-    const __nv_fp8x4_e4m3 o(make_float4(x[0] * s, x[1] * s, x[2] * s, x[3] * s));
+    const __nv_fp8x4_e4m3 o(make_float4(f(0), f(1), f(2), f(3)));
     *reinterpret_cast<__nv_fp8x4_e4m3*>(dst) = o;
   }
 }
