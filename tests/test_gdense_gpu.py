@@ -303,3 +303,24 @@ def test_quantize_does_not_hide_what_is_not_finite(D, code, scale_dtype):
     y = torch.empty((1, 20), device="cuda")
     layer.forward(torch.ones((1, 200), device="cuda"), y)
     assert torch.equal(torch.isnan(y[0]), bad.any(1))
+
+
+@pytest.mark.parametrize("code", ["int4", "uint4", "fp4"])
+@pytest.mark.parametrize("n", [1, 8])
+@pytest.mark.parametrize("scale,size", [(1e31, 1e-12), (1e36, 1e-30), (2e38, 1e-35), (1e-35, 1e25), (1e-38, 1e37), (1e-30, 1e-3)])
+def test_scales_at_the_ends_of_their_range(D, code, n, scale, size):
+    """BFloat16 scales near the largest and smallest floats, with x that makes the results ordinary numbers."""
+    import torch
+    rng = np.random.default_rng(17)
+    rows, cols, group = 100, 700, 64
+    codes, _, zeros, W = make(rng, rows, cols, group, code, "bf16")
+    s = torch.from_numpy((rng.uniform(0.5, 1.0, (rows, 11)) * scale).astype(np.float32)).to(torch.bfloat16)
+    c = np.stack([codes & 15, codes >> 4], -1).reshape(rows, -1)[:, :cols].astype(np.int64)
+    which = np.arange(cols) // group
+    v = FP4[c] if code == "fp4" else np.where(c > 7, c - 16, c) if code == "int4" else c - zeros[:, which].astype(np.float64)
+    W = v * s.double().numpy()[:, which]
+    g = mount(D, codes, s, zeros, cols, group, code)
+    x = (rng.standard_normal((n, cols)) * size).astype(np.float32)
+    y = torch.full((n, rows), float("nan"), device="cuda")
+    g.forward(torch.from_numpy(x).cuda(), y)
+    check(y.cpu().numpy(), x, W, (scale, size))

@@ -28,6 +28,10 @@ __device__ __forceinline__ float scale_value(uint16_t bits, int type) {
 // of x are a lane's B fragments of two blocks, which span 32 inputs.
 constexpr int kChunk = 256, kUnit = 64;
 
+// BFloat16 scales of which some are 2^96 or more; their records keep sets of 32 inputs, so that this
+// rare kind needs one width of set only.
+constexpr int kScaleLarge = 4;
+
 struct Layout {
   int row_groups, chunks, units;  // units of 64 inputs in all
   int sg, sets;                   // inputs of a scale set, sets of a record
@@ -35,12 +39,12 @@ struct Layout {
   int64_t group_bytes;            // records of a row group
 };
 
-Layout layout_of(int rows, int cols, int group, int code) {
+Layout layout_of(int rows, int cols, int group, int code, int scale_type) {
   Layout l;
   l.row_groups = (rows + 15) / 16;
   l.units = (cols + kUnit - 1) / kUnit;
   l.chunks = (cols + kChunk - 1) / kChunk;
-  l.sg = group % 256 == 0 ? 256 : (group % 128 == 0 ? 128 : (group % 64 == 0 ? 64 : 32));
+  l.sg = scale_type == kScaleLarge ? 32 : group % 256 == 0 ? 256 : (group % 128 == 0 ? 128 : (group % 64 == 0 ? 64 : 32));
   l.sets = kChunk / l.sg;
   l.tail = l.sets * (code == kCodeUint4 ? 48 : 32);
   l.group_bytes = static_cast<int64_t>(l.units) * 512 + static_cast<int64_t>(l.chunks) * l.tail;
@@ -93,6 +97,16 @@ __global__ void __launch_bounds__(128) k_group_build(const __grid_constant__ Bui
   }
 }
 
+// *large = 1 if a finite BFloat16 scale is 2^96 or more.
+__global__ void k_group_scales(const uint16_t* scales, int64_t n, int* large) {
+  bool any = false;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+    const int e = (scales[i] >> 7) & 255;
+    any = any || (e >= 127 + 96 && e < 255);
+  }
+  if (__any_sync(0xffffffffu, any) && (threadIdx.x & 31) == 0) *large = 1;
+}
+
 // ---------------------------------------------------------------- matrix-vector product
 //
 // HBM bound: in * out / 2 bytes of codes and 2 (Uint4: 3) bytes per group of scales are read once,
@@ -128,7 +142,7 @@ struct GArgs {
   const uint8_t* w;
   Layout l;
   const double* bias;
-  int rows, cols, act, bias_len, scale_type;
+  int rows, cols, act, bias_len;
   const float* x;
   int64_t x_ld;
   float* pre;
@@ -226,7 +240,7 @@ __device__ __forceinline__ void ld_words(const uint8_t* p, uint32_t* w) {
 }
 
 // kNT n8 tiles of tokens (1: up to 4 tokens, 2: up to 8). kSub: inputs of a scale set (32, 64, 128
-// or 256). kScale: the scales' type.
+// or 256). kScale: the scales' kind (kScaleF16, kScaleBF16 or kScaleLarge).
 template <int kCode, int kNT, int kSub, int kScale>
 __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_constant__ GArgs a) {
   using Record = GRecord<kCode, kSub>;
@@ -413,8 +427,19 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
       const uint8_t* xp[kNT];
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) xp[nt] = xcol[nt] + c * xstep[nt];
-      float sum[kNT][4];  // the record's, in units of the thread's token's 2^-e
+      float sum[kNT][4];  // the record's, in units of the thread's token's xs
       float part[kNT][4];
+      // The power of two that x was multiplied by is undone after the scales, which carry no sum (below
+      // 2^31) past the largest float while they are below 2^96. With larger ones (kScaleLarge) as much
+      // of a small x's power as keeps sums below 1 is undone before them, or a result that is finite
+      // would pass through an infinity. (Done for all BFloat16 scales, 8 tokens take a tenth longer.)
+      constexpr float kLeast = 0x1p-32f;
+      auto undo = [&](int nt) { return 4 * nt + t < a.n ? sxs[(4 * nt + t) * a.slab_chunks + c] : 0.0f; };
+      float xa[kNT];
+      if constexpr (kScale == kScaleLarge) {
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) xa[nt] = fminf(fmaxf(undo(nt), kLeast), 1.0f);
+      }
 #pragma unroll
       for (int u = 0; u < kChunk / kUnit; ++u) {
         uint4 xb[kNT][2];
@@ -455,13 +480,17 @@ __global__ void __launch_bounds__(kGThreads, 1) k_group_gemv(const __grid_consta
 #pragma unroll
             for (int nt = 0; nt < kNT; ++nt)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) sum[nt][e] = (set == 0 ? 0.0f : sum[nt][e]) + part[nt][e] * (e < 2 ? s0 : s1);
+              for (int e = 0; e < 4; ++e) {
+                if constexpr (kScale == kScaleLarge) part[nt][e] *= xa[nt];
+                sum[nt][e] = (set == 0 ? 0.0f : sum[nt][e]) + part[nt][e] * (e < 2 ? s0 : s1);
+              }
           }
         }
       }
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
-        const float xs = 4 * nt + t < a.n ? sxs[(4 * nt + t) * a.slab_chunks + c] : 0.0f;
+        float xs = undo(nt);
+        if constexpr (kScale == kScaleLarge) xs = xs > 1.0f ? xs : (xs < kLeast ? xs * (1.0f / kLeast) : 1.0f);
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[nt][e] += sum[nt][e] * xs;
       }
@@ -673,6 +702,7 @@ GKernel kernel_of(int sg, int code, int n) {
 }
 
 GKernel kernel_of(const GroupDense& g, const Layout& l, int n) {
+  if (g.scale_type == kScaleLarge) return kernel_of<32, kScaleLarge>(g.code, n);
   return g.scale_type == kScaleF16 ? kernel_of<kScaleF16>(l.sg, g.code, n) : kernel_of<kScaleBF16>(l.sg, g.code, n);
 }
 
@@ -725,7 +755,16 @@ Status gdense_fill(GroupDense* g, const GroupDenseSrc& src) {
   b.group = g->group;
   b.groups = g->groups;
   b.code = g->code;
-  b.l = layout_of(g->rows, g->cols, g->group, g->code);
+  if (g->scale_type == kScaleBF16) {
+    Staged large;
+    int any = 0;
+    WB_TRY(large.put(&any, sizeof any));
+    k_group_scales<<<static_cast<unsigned>(std::min<size_t>((n_groups + 255) / 256, 4 * g->sms)), 256>>>(b.scales, n_groups, static_cast<int*>(large.p));
+    WB_CUDA(cudaGetLastError());
+    WB_CUDA(cudaMemcpy(&any, large.p, sizeof any, cudaMemcpyDeviceToHost));
+    if (any) g->scale_type = kScaleLarge;
+  }
+  b.l = layout_of(g->rows, g->cols, g->group, g->code, g->scale_type);
   WB_CUDA(cudaMalloc(&g->w, b.l.group_bytes * b.l.row_groups));
   b.out = g->w;
   k_group_build<<<static_cast<unsigned>(static_cast<int64_t>(b.l.row_groups) * b.l.chunks), 128>>>(b);
@@ -780,13 +819,12 @@ Status gdense_forward(GroupDense* g, int n, const float* x, int64_t x_ld, float*
   WB_CUDA(cudaSetDevice(g->device));
   GArgs a;
   a.w = g->w;
-  a.l = layout_of(g->rows, g->cols, g->group, g->code);
+  a.l = layout_of(g->rows, g->cols, g->group, g->code, g->scale_type);
   a.bias = g->bias;
   a.rows = g->rows;
   a.cols = g->cols;
   a.act = g->act;
   a.bias_len = g->bias_len;
-  a.scale_type = g->scale_type;
   a.x_ld = x_ld;
   a.part = g->part;
   a.tickets = g->tickets;

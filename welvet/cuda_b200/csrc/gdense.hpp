@@ -17,7 +17,8 @@ struct GroupDense {
   int device = 0;
   int rows = 0, cols = 0;  // outputs, inputs
   int group = 0, groups = 0;
-  int code = 0, scale_type = 0, act = -1;
+  int code = 0, act = -1;
+  int scale_type = 0;  // kScaleF16, kScaleBF16, or the kernel's own kind of very large BFloat16 scales
   uint8_t* w = nullptr;  // codes, scales and zero points in the kernel's records (gdense.cu)
   double* bias = nullptr;
   int bias_len = 0;
