@@ -338,6 +338,14 @@ WELVET_API welvet_status welvet_b200_gdense_mount(int32_t in, int32_t out, int32
  * the outputs must not overlap x. Made for 1..8 rows; more rows run in passes of 8 over the weights. */
 WELVET_API welvet_status welvet_b200_gdense_execute_device(welvet_b200_gdense* g, int32_t rows, const float* x_dev,
                                                            int64_t x_ld, float* pre_dev, float* post_dev, void* stream);
+/* The launch plan of execute_device for `rows` rows (1..8) of such a layer on a GPU of `sms`
+ * multiprocessors, as the library plans it: slabs of the inputs, chunks (256 inputs) of a slab, blocks of
+ * a slab, whether runs of records are the warps' (1) or the blocks' (0), whether runs are whole row
+ * groups (16 outputs), shared memory in bytes, row groups, chunks, runs of a slab, row groups that are
+ * cut by runs. Writes the first n values, returns their number (10), -1 for arguments that mount
+ * refuses. Host arithmetic only. */
+WELVET_API int32_t welvet_b200_gdense_plan(int32_t in, int32_t out, int32_t group, int32_t code, int32_t sms, int32_t rows,
+                                           int64_t* values, int32_t n);
 WELVET_API void welvet_b200_gdense_release(welvet_b200_gdense* g);
 
 /* ---------------------------------------------------------------- multi-GPU (one box)

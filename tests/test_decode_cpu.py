@@ -84,3 +84,29 @@ def test_group_sizes_past_the_index_range(in_, out):
 
 def test_nil_handles_of_a_step_with_flags():
     assert W.lib().welvet_b200_mha_decode_active_device(None, None, FAKE, None, FAKE, 0, FAKE, None).code == 1
+
+
+SHAPES = [(1, 1), (16, 64), (100, 130), (1024, 4096), (4096, 4096), (14336, 4096), (4096, 14336), (14331, 4090), (40, 16385), (256, 4609),
+          (256, 17400), (38100, 600), (19024, 4609), (65536, 16384), (37888, 256), (3000, 100000), (500000, 64)]
+
+
+@pytest.mark.parametrize("rows", range(1, 9))
+@pytest.mark.parametrize("out,in_", SHAPES)
+def test_group_plans(out, in_, rows):
+    """What the kernel relies on: every slab has a chunk, every warp of a block a record, x and the sums
+    that wait fit shared memory, runs that are whole row groups are no more than there are."""
+    for code in (14, 15, 16):
+        p = D.gdense_plan(in_, out, 64, code, rows)
+        assert p["row_groups"] == -(-out // 16) and p["chunks"] == -(-in_ // 256)
+        assert 0 < p["slabs"] * p["slab_chunks"] - p["chunks"] + 1 <= p["slab_chunks"]  # the last slab has a chunk
+        assert p["slabs"] * p["slab_blocks"] <= 148 or p["slabs"] > 148
+        last = p["chunks"] - (p["slabs"] - 1) * p["slab_chunks"]
+        assert p["runs"] == p["slab_blocks"] * (16 if p["solo"] else 1)
+        if p["whole"]:
+            assert not p["solo"] and p["runs"] <= p["row_groups"] and p["cut"] == 0
+        elif p["slab_blocks"] > 1:
+            assert p["row_groups"] * last >= 16 * p["slab_blocks"]
+        assert p["cut"] <= p["slabs"] * (p["runs"] - 1) and p["smem"] <= 227 * 1024
+    for bad in (dict(rows=0), dict(rows=9), dict(sms=0), dict(group=48), dict(code=9), dict(out=0)):
+        with pytest.raises(ValueError):
+            D.gdense_plan(**{**dict(in_features=in_, out=out, group=64, code=14, rows=rows), **bad})

@@ -324,3 +324,75 @@ def test_scales_at_the_ends_of_their_range(D, code, n, scale, size):
     y = torch.full((n, rows), float("nan"), device="cuda")
     g.forward(torch.from_numpy(x).cuda(), y)
     check(y.cpu().numpy(), x, W, (scale, size))
+
+
+def big_layer(D, rows, cols, group, code, scale_dtype, seed):
+    """(layer, W's rows of a block in 64 bits on the GPU) of random codes, made on the GPU."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    half, groups = (cols + 1) // 2, -(-cols // group)
+    codes = torch.randint(0, 256, (rows, half), dtype=torch.uint8, device="cuda", generator=g)
+    if cols % 2:
+        codes[:, -1] &= 15
+    s = (torch.rand((rows, groups), device="cuda", generator=g) * 0.018 + 0.002).to(scale_dtype)
+    z = torch.randint(0, 16, (rows, groups), dtype=torch.uint8, device="cuda", generator=g) if code == "uint4" else None
+    layer = D.GroupDense.from_codes(codes, s, cols, group, D.CODES[code], zeros=z)
+    which = torch.arange(cols, device="cuda") // group
+    values = torch.tensor(FP4 if code == "fp4" else [i - 16 * (i > 7) for i in range(16)] if code == "int4" else list(range(16)),
+                          dtype=torch.float64, device="cuda")
+
+    def block(at, n):
+        c = torch.stack([codes[at: at + n] & 15, codes[at: at + n] >> 4], -1).reshape(-1, 2 * half)[:, :cols].long()
+        w = values[c]
+        if z is not None:
+            w = w - z[at: at + n].double()[:, which]
+        return w * s[at: at + n].double()[:, which]
+
+    return layer, block
+
+
+# rows, cols, x's rows, and the form of the launch that the shape is here for
+FORMS = [
+    (256, 4609, 8, dict(slabs=2, solo=0, whole=1)),           # slabs of 10 and 9 chunks, the last of one input
+    (40, 16385, 3, dict(slabs=2, solo=0, whole=0, cut=6)),    # slabs, and blocks' runs that cut row groups
+    (40, 16385, 1, dict(slabs=1, solo=0, whole=0, cut=3)),
+    (250, 17400, 8, dict(slabs=4, solo=0, whole=0, cut=64)),
+    (38100, 600, 1, dict(slabs=1, solo=1, cut=1578)),         # warps' runs that cut row groups
+    (38100, 600, 5, dict(slabs=1, solo=1, cut=1578)),
+    (38100, 600, 8, dict(slabs=1, solo=1, cut=1578)),
+    (19020, 4609, 8, dict(slabs=2, solo=1, cut=2117)),        # the same in slabs
+    (4096, 14336, 8, dict(slabs=4, solo=0, whole=1)),
+    (3000, 50000, 7, dict(slabs=11, solo=0)),
+]
+
+
+@pytest.mark.parametrize("code,group,scale", [("int4", 128, "f16"), ("uint4", 64, "bf16"), ("fp4", 32, "f16")])
+@pytest.mark.parametrize("rows,cols,n,form", FORMS)
+def test_forms_of_the_launch(D, rows, cols, n, form, code, group, scale):
+    """Slabs of the inputs, runs of the warps and of the blocks, and row groups that runs cut: against 64
+    bits, and the same bits in calls that follow one another with other numbers of rows between them
+    (tickets and partial sums are the handle's)."""
+    import torch
+    plan = D.gdense_plan(cols, rows, group, D.CODES[code], n, torch.cuda.get_device_properties(0).multi_processor_count)
+    assert {k: plan[k] for k in form} == form
+    layer, block = big_layer(D, rows, cols, group, code, torch.float16 if scale == "f16" else torch.bfloat16, rows + n)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn((17, cols), device="cuda", generator=g)
+    out = {m: torch.full((m, rows), float("nan"), device="cuda") for m in {n, 1, 4, 17}}
+    layer.forward(x[:n], out[n])
+    first = out[n].clone()
+    for at in range(0, rows, 4096):
+        W = block(at, min(4096, rows - at))
+        want = x[:n].double() @ W.T
+        bound = 2.0 ** -18 * (x[:n].double().abs() @ W.abs().T) + 2.0 ** -22 * want.abs()
+        assert bool(((first[:, at: at + 4096] - want).abs() <= bound).all())
+    for m in (1, n, 17, n, 4, n, n):
+        out[m].fill_(float("nan"))
+        layer.forward(x[:m], out[m])
+        if m == n:
+            assert torch.equal(out[n], first)
+        if m == 17 and n == 8:  # passes of eight
+            assert torch.equal(out[17][:8], first)
+    again = out[17].clone()
+    layer.forward(x, out[17])
+    assert torch.equal(again, out[17]) and bool(torch.isfinite(again).all())

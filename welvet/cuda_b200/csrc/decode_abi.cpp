@@ -285,6 +285,18 @@ welvet_status welvet_b200_gdense_execute_device(welvet_b200_gdense* g, int32_t r
   });
 }
 
+int32_t welvet_b200_gdense_plan(int32_t in, int32_t out, int32_t group, int32_t code, int32_t sms, int32_t rows,
+                                int64_t* values, int32_t n) {
+  int32_t count = -1;
+  const welvet_status st = guarded([&] {
+    WB_TRY(group_shape(in, out, group, code, wb::kScaleF16));
+    if (sms <= 0 || rows < 1 || rows > 8 || (n > 0 && !values)) return wb::Status::Invalid("group dense: plan");
+    count = wb::gdense_plan_values(out, in, group, code, sms, rows, values, n < 0 ? 0 : n);
+    return wb::Status::Ok();
+  });
+  return st.code == 0 ? count : -1;
+}
+
 void welvet_b200_gdense_release(welvet_b200_gdense* g) {
   if (!g) return;
   delete g->g;

@@ -659,7 +659,7 @@ struct GPlan {
   int slabs, slab_chunks, slab_blocks, solo, aligned, smem;
 };
 
-GPlan plan_of(const GroupDense& g, const Layout& l, int n) {
+GPlan plan_of(int sms, const Layout& l, int n) {
   GPlan p;
   const int fit = (kXBytes - 2 * n * 64) / (n * (2 * kChunk * 2 + 4));  // chunks of x in shared memory
   p.slabs = (l.chunks + fit - 1) / fit;
@@ -668,7 +668,7 @@ GPlan plan_of(const GroupDense& g, const Layout& l, int n) {
   // every warp of a block has a record or more
   const int64_t last = l.chunks - (p.slabs - 1) * p.slab_chunks;
   const int64_t most = std::max<int64_t>(1, l.row_groups * last / kGWarps);
-  p.slab_blocks = static_cast<int>(std::min<int64_t>(std::max(1, g.sms / p.slabs), most));
+  p.slab_blocks = static_cast<int>(std::min<int64_t>(std::max(1, sms / p.slabs), most));
   p.solo = l.row_groups >= p.slab_blocks * kGWarps;
   p.aligned = 0;
   p.smem = 2 * n * (p.slab_chunks * kChunk * 2 + 64) + (n * p.slab_chunks + 3) / 4 * 16;
@@ -777,7 +777,7 @@ Status gdense_fill(GroupDense* g, const GroupDenseSrc& src) {
   // workspaces for every number of tokens
   size_t part = 0, tickets = 0, slabs = 0;
   for (int n = 1; n <= kMaxTokens; ++n) {
-    const GPlan p = plan_of(*g, b.l, n);
+    const GPlan p = plan_of(g->sms, b.l, n);
     part = std::max<size_t>(part, static_cast<size_t>(p.slabs) * p.slab_blocks * (p.solo ? kGWarps : 1) * 2 * 16 * kMaxTokens * 4);
     tickets = std::max<size_t>(tickets, static_cast<size_t>(p.slabs) * b.l.row_groups * 4);
     if (p.slabs > 1) slabs = std::max<size_t>(slabs, static_cast<size_t>(p.slabs) * n * g->rows * 4);
@@ -834,7 +834,7 @@ Status gdense_forward(GroupDense* g, int n, const float* x, int64_t x_ld, float*
     a.x = x + b * x_ld;
     a.pre = pre ? pre + static_cast<int64_t>(b) * g->rows : nullptr;
     a.post = post + static_cast<int64_t>(b) * g->rows;
-    const GPlan p = plan_of(*g, a.l, a.n);
+    const GPlan p = plan_of(g->sms, a.l, a.n);
     a.slabs = p.slabs;
     a.slab_chunks = p.slab_chunks;
     a.slab_blocks = p.slab_blocks;
@@ -844,6 +844,29 @@ Status gdense_forward(GroupDense* g, int n, const float* x, int64_t x_ld, float*
     if (p.slabs > 1) WB_TRY(g_launch(k_group_slabs, dim3((g->rows + 255) / 256, a.n), 256, 0, st, a));
   }
   return Status::Ok();
+}
+
+int gdense_plan_values(int rows, int cols, int group, int code, int sms, int n, int64_t* out, int count) {
+  const Layout l = layout_of(rows, cols, group, code, kScaleF16);
+  const GPlan p = plan_of(sms, l, n);
+  const int64_t runs = static_cast<int64_t>(p.slab_blocks) * (p.solo ? kGWarps : 1);
+  // row groups that a run's end cuts, over all slabs
+  int64_t cut = 0;
+  for (int s = 0; s < p.slabs && !p.aligned; ++s) {
+    const int64_t chunks = std::min(p.slab_chunks, l.chunks - s * p.slab_chunks), total = l.row_groups * chunks;
+    int64_t last = -1;
+    for (int64_t i = 1; i < runs; ++i) {
+      const int64_t at = i * total / runs;
+      if (at % chunks != 0 && at / chunks != last) {
+        last = at / chunks;
+        ++cut;
+      }
+    }
+  }
+  const int64_t values[] = {p.slabs, p.slab_chunks, p.slab_blocks, p.solo, p.aligned, p.smem, l.row_groups, l.chunks, runs, cut};
+  constexpr int kValues = sizeof(values) / sizeof(values[0]);
+  for (int i = 0; i < std::min(count, kValues); ++i) out[i] = values[i];
+  return kValues;
 }
 
 Status group_quantize(int rows, int cols, int group, int code, int scale_type, const float* W, uint8_t* codes, void* scales,

@@ -44,6 +44,11 @@ Status gdense_mount(int device, int rows, int cols, int group, int code, int sca
 // x [n][cols] (rows x_ld apart), pre (may be null) and post [n][rows].
 Status gdense_forward(GroupDense* g, int n, const float* x, int64_t x_ld, float* pre, float* post, cudaStream_t st);
 
+// The launch plan of a call of n tokens (1..8) on a GPU of `sms` multiprocessors, host arithmetic only:
+// slabs, chunks of a slab, blocks of a slab, runs are the warps', runs are whole row groups, bytes of
+// shared memory, row groups, chunks, runs of a slab, row groups that runs cut. Returns their number.
+int gdense_plan_values(int rows, int cols, int group, int code, int sms, int n, int64_t* out, int count);
+
 // W [rows][cols] float32 -> codes, scales, zeros (Uint4) in the layout gdense_mount takes.
 Status group_quantize(int rows, int cols, int group, int code, int scale_type, const float* W, uint8_t* codes, void* scales,
                       uint8_t* zeros, cudaStream_t st);

@@ -50,6 +50,7 @@ _sig("welvet_b200_group_quantize", _ST, c_int32, c_int32, c_int32, c_int32, c_in
 _sig("welvet_b200_gdense_mount", _ST, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p,
      c_int32, c_void_p, c_size_t, POINTER(c_void_p))
 _sig("welvet_b200_gdense_execute_device", _ST, c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p)
+_sig("welvet_b200_gdense_plan", c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, POINTER(c_int64), c_int32)
 _sig("welvet_b200_gdense_release", None, c_void_p)
 
 _sig("welvet_b200_mha_decode_device", _ST, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_void_p)
@@ -242,6 +243,17 @@ def group_quantize(W, group: int, code: int, scale_dtype=torch.bfloat16, stream=
     check(_L.welvet_b200_group_quantize(in_, out, group, code, _SCALES[scale_dtype], W.data_ptr(), codes.data_ptr(),
                                         scales.data_ptr(), None if zeros is None else zeros.data_ptr(), _stream(stream, W)))
     return codes, scales, zeros
+
+
+_PLAN = ("slabs", "slab_chunks", "slab_blocks", "solo", "whole", "smem", "row_groups", "chunks", "runs", "cut")
+
+
+def gdense_plan(in_features: int, out: int, group: int, code: int, rows: int, sms: int = 148) -> dict:
+    """How a call of `rows` rows (1..8) on such a layer is launched (welvet_b200_gdense_plan)."""
+    v = (c_int64 * len(_PLAN))()
+    if _L.welvet_b200_gdense_plan(in_features, out, group, code, sms, rows, v, len(_PLAN)) != len(_PLAN):
+        raise ValueError("gdense_plan: no such layer or number of rows")
+    return dict(zip(_PLAN, v))
 
 
 class GroupDense:
