@@ -910,3 +910,32 @@ def test_append_divides_by_the_scale(D, dtype, dim, ks, vs):
         want = (x / torch.tensor(scale, dtype=torch.float32, device="cuda")).float()
         want = (want.clamp(-448, 448) if dtype == "f8" else want).to(types()[dtype])
         assert torch.equal(pool.reshape(per * page, kv, dim)[:n].float(), want.float())
+
+
+@pytest.mark.parametrize("dtype,H,kv,dim,lens", [
+    ("f32", 4, 1, 96, [1500, 40]), ("f32", 16, 4, 256, [900]), ("f32", 4, 2, 64, [333, 4000]), ("bf16", 8, 8, 192, [1200, 333]),
+    ("bf16", 32, 8, 128, [700, 701, 64]), ("bf16", 3, 1, 256, [5000]), ("f16", 10, 2, 128, [2222]), ("f16", 8, 1, 256, [100, 3100]),
+    ("f8", 4, 4, 96, [640, 64]), ("f8", 16, 2, 256, [1800])])
+def test_attend_is_as_exact_as_fp32(D, dtype, H, kv, dim, lens):
+    """Against 64 bits, the result is no further off than the formula in fp32 with one running sum a score:
+    sums are held in 32 bits, and what parts of 22 bits and more lose is less than a chain of `dim`
+    rounded additions does."""
+    import torch
+    rng = np.random.default_rng(7 * dim + H)
+    n, page = len(lens), 16
+    per = -(-max(lens) // page)
+    kp, vp, table = make_cache(rng, dtype, n, per, page, kv, dim)
+    q = torch.from_numpy((rng.standard_normal((n, H, dim)) * 1.5).astype(np.float32)).cuda()
+    out = torch.empty_like(q)
+    D.PagedKV(kp, vp, table, i32(lens), num_heads=H).attend(q, out)
+    got = plain = 0.0
+    for b, L in enumerate(lens):
+        used = table[b].long()
+        k, v = (p.float()[used].reshape(-1, kv, dim)[:L].repeat_interleave(H // kv, 1) for p in (kp, vp))
+        zs = [torch.einsum("hd,shd->hs", q[b].double(), k.double()), torch.zeros((H, L), device="cuda")]
+        for d in range(dim):
+            zs[1] += q[b, :, d: d + 1] * k[:, :, d].T
+        want, fp32 = (torch.einsum("hs,shd->hd", torch.softmax(z / math.sqrt(dim), -1), v.to(z.dtype)).double() for z in zs)
+        got += float((out[b].double() - want).square().sum())
+        plain += float((fp32 - want).square().sum())
+    assert got <= plain, (got ** 0.5, plain ** 0.5)
