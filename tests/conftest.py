@@ -16,6 +16,16 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "slow: longer CPU test")
 
 
+@pytest.hookimpl(wrapper=True)
+def pytest_runtest_call(item):
+    """A test that comes to ask for the reference's own build is skipped where that does not exist."""
+    import oracle as O
+    try:
+        return (yield)
+    except O.NotBuilt as e:
+        pytest.skip(str(e))
+
+
 @pytest.fixture(scope="session")
 def oracle():
     import oracle as O

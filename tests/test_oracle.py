@@ -151,3 +151,12 @@ def test_attention_rows_matches_the_loop_restatement(cfg):
     rows = [0, T // 2, T - 1]
     got = attention_rows(q[rows], k, v, rows, *args)
     np.testing.assert_allclose(got, full[rows], rtol=1e-6, atol=1e-7)
+
+
+def test_asking_for_an_absent_reference_build_is_an_error(monkeypatch):
+    import oracle as O
+    monkeypatch.setattr(O, "_ref", None)
+    monkeypatch.setattr(O, "ref_available", lambda: False)
+    with pytest.raises(O.NotBuilt, match="not built"):
+        O.ref()
+    assert issubclass(O.NotBuilt, RuntimeError)
