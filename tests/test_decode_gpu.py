@@ -315,3 +315,58 @@ def test_prompt_into_a_row_that_was_used(D, wb):
     cache.check_error()
     assert cache.lens.tolist() == [0, 12, 0] and cache.seen.tolist() == [0, 12, 0]
     assert torch.equal(k, cache.k_pages) and torch.equal(positions, cache.positions)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f8"])
+@pytest.mark.parametrize("pos,mask,max_seq,heads,kv,dim", [(0, 1, 400, 8, 2, 128), (3, 3, 70, 4, 4, 96), (2, 1, 400, 6, 3, 40), (1, 3, 33, 16, 1, 128)])
+def test_steps_against_64_bits(D, wb, dtype, pos, mask, max_seq, heads, kv, dim):
+    """The cell's wiring (slots, positions, slopes, scale, window, heads' groups) held to the operators' own
+    bound: prompts and single tokens of a Float32 cell, whose projections of up to 2^20 weights are sums in
+    64 bits rounded once. Stored rows are within half a step of the type, attention is compared over what
+    is stored, with the query off by its projection's rounding (2^-24) and its rotation's (three more of
+    the pair): both move a score by no more than 4 * 2^-24 * 2 |q||k| scale."""
+    import torch
+    from test_kv_gpu import EPS, attend64, rotate64, rotation_bound, rows_of, stored64
+    rng = np.random.default_rng(pos * 100 + dim)
+    d_model, n, prompts, total = 256, 2, (150, 9), 160
+    w = [(rng.standard_normal((r, d_model)) * 0.06).astype(np.float32) for r in (heads * dim, kv * dim, kv * dim)]
+    w.append((rng.standard_normal((d_model, heads * dim)) * 0.06).astype(np.float32))
+    cell = wb.MhaCell(*w, d_model, heads, kv, dim, max(max_seq, 150) if mask == 1 else max_seq, mask, pos, wb.FLOAT32)
+    if mask == 3:
+        prompts = (max_seq, 9)  # the cell's own prompt holds max_seq_len positions
+    dt = {"f32": torch.float32, "bf16": torch.bfloat16, "f8": torch.float8_e4m3fn}[dtype]
+    cache = cache_for(D, n, heads, kv, dim, total + 32, dt)
+    xs = rng.standard_normal((n, total, d_model)).astype(np.float32)
+    for s, m in enumerate(prompts):
+        D.mha_prefill(cell, cache, s, torch.from_numpy(xs[s, :m].copy()).cuda(), torch.empty((m, d_model), device="cuda"))
+    at = list(prompts)
+    theta = 10000.0 if pos in (0, 3) else 0.0
+    q64, k64, v64 = ((xs.astype(np.float64) @ m.T.astype(np.float64)) for m in w[:3])
+    for step in range(10):
+        x = np.stack([xs[s, at[s]] for s in range(n)])
+        y, attn = torch.empty((n, d_model), device="cuda"), torch.empty((n, heads * dim), device="cuda")
+        D.mha_decode(cell, cache, torch.from_numpy(x).cuda(), y, attn)
+        at = [a + 1 for a in at]
+    cache.check_error()
+    assert cache.lens.tolist() == at
+    q = np.stack([rotate64(q64[s, at[s] - 1].reshape(1, heads, dim), np.array([at[s] - 1.0]), theta)[0] for s in range(n)])
+    for s in range(n):
+        for pool, x64, turn in ((cache.k_pages, k64, theta), (cache.v_pages, v64, 0.0)):
+            x = x64[s, : at[s]].reshape(at[s], kv, dim)
+            want = rotate64(x, np.arange(at[s], dtype=np.float64), turn)
+            st, half = stored64(want, dtype, 1.0)
+            tol = half + (rotation_bound(x, turn) + EPS * (np.abs(x) + np.abs(np.roll(x, dim // 2, -1)))) * (1 + 2.0 ** -4)
+            for h in range(kv):
+                assert np.all(np.abs(rows_of(pool, cache.page_table, s, at[s], h) - st[:, h]) <= tol[:, h])
+    scale = 1.0 / np.sqrt(dim)
+    want, _, bound = attend64(torch.from_numpy(q).cuda(), cache.k_pages, cache.v_pages, cache.page_table, at, scale,
+                              max_seq if mask == 3 else 0, pos in (2, 3))
+    for s in range(n):
+        for h in range(heads):
+            k, v = (rows_of(p, cache.page_table, s, at[s], h // (heads // kv)) for p in (cache.k_pages, cache.v_pages))
+            dq = 4 * EPS * 2 * scale * np.max(np.linalg.norm(k, axis=1)) * np.linalg.norm(q[s, h])
+            bound[s, h] += 2 * dq * np.max(np.abs(v))
+    got = attn.reshape(n, heads, dim).cpu().numpy().astype(np.float64)
+    assert np.all(np.abs(got - want) <= bound)
+    out = got.reshape(n, -1) @ w[3].T.astype(np.float64)
+    assert np.all(np.abs(y.cpu().numpy() - out) <= 2 * EPS * np.abs(out) + 1e-30)
