@@ -331,9 +331,9 @@ struct Tiled {
   static constexpr int kSub = kRow <= 128 ? 2 : 1;      // 16-key blocks of a warp's tile
   static constexpr int kStages = kRow <= 256 || kRow > 384 ? 3 : 2;
   static constexpr int kThreads = 32 * kWarps;
-  // of an SM: three where a tile is small enough for 168 registers (160-byte rows; 128-byte rows, two
-  // blocks of keys a warp, took 245 us for 157)
-  static constexpr int kBlocks = kRow == 160 ? 3 : (kRow <= 384 && DP <= 128 ? 2 : 1);
+  // of an SM (three, 168 registers a thread, were slower wherever they fit: rows of 160 bytes 125 us for
+  // 105, of 128 bytes 245 for 157)
+  static constexpr int kBlocks = kRow <= 384 && DP <= 128 ? 2 : 1;
   static constexpr int kKeys = 16 * kSub * kWarps;  // keys of a block tile
   static constexpr int kLanes = kRow <= 64 ? 4 : 8;  // lanes that copy a row
   static constexpr int kSets = kBF16 ? 2 : 1;
