@@ -354,9 +354,11 @@ def big_layer(D, rows, cols, group, code, scale_dtype, seed):
 # rows, cols, x's rows, and the form of the launch that the shape is here for
 FORMS = [
     (256, 4609, 8, dict(slabs=2, solo=0, whole=1)),           # slabs of 10 and 9 chunks, the last of one input
-    (40, 16385, 3, dict(slabs=2, solo=0, whole=0, cut=6)),    # slabs, and blocks' runs that cut row groups
-    (40, 16385, 1, dict(slabs=1, solo=0, whole=0, cut=3)),
-    (250, 17400, 8, dict(slabs=4, solo=0, whole=0, cut=64)),
+    (40, 40001, 3, dict(slabs=4, solo=0, whole=0, cut=12)),   # slabs, and blocks' runs that cut row groups
+    (40, 40001, 1, dict(slabs=2, solo=0, whole=0, cut=6)),
+    (40, 30000, 1, dict(slabs=1, solo=0, whole=1)),
+    (2400, 32768, 1, dict(slabs=1, solo=0, whole=0, cut=146)),
+    (250, 17400, 8, dict(slabs=4, solo=0, whole=1)),
     (38100, 600, 1, dict(slabs=1, solo=1, cut=1578)),         # warps' runs that cut row groups
     (38100, 600, 5, dict(slabs=1, solo=1, cut=1578)),
     (38100, 600, 8, dict(slabs=1, solo=1, cut=1578)),

@@ -674,12 +674,17 @@ GPlan plan_of(int sms, const Layout& l, int n) {
   p.smem = 2 * n * (p.slab_chunks * kChunk * 2 + 64) + (n * p.slab_chunks + 3) / 4 * 16;
   if (!p.solo) {
     p.smem += kHold * kGWarps * 16 * (n > 4 ? 8 : 4) * 4;
-    // Whole row groups leave blocks idle for part of the last round; cut ones cost a join of about
-    // 2.5 us at the run's end. At 5 TB/s a microsecond is 5 MB of records.
+    // Whole row groups leave blocks idle for part of the last round, runs that cut them pay a join at
+    // their end. Measured at one token, whole and cut: 19 MB of records missed by idle blocks (4800 x
+    // 16384) 13.6 and 14.7 us, 20 MB (9504 x 16384) 20.0 and 20.9, 25 MB (2400 x 20480) 12.9 and 12.4,
+    // 39 MB (2400 x 32768) 17.8 and 15.9.
     const int per = (l.row_groups + p.slab_blocks - 1) / p.slab_blocks;
     const double idle = static_cast<double>(per) * p.slab_blocks / l.row_groups - 1.0;
-    p.aligned = l.row_groups >= p.slab_blocks && idle * l.group_bytes * l.row_groups < 2.5 * 5e6;
-    if (l.row_groups < p.slab_blocks && l.group_bytes < 2.5 * 50e3) {  // one row group a block, if that is little
+    p.aligned = l.row_groups >= p.slab_blocks && idle * l.group_bytes * l.row_groups < 22e6;
+    // Fewer row groups than blocks: one a block, unless it is long. One a block and cut: 135 KB (1024 x
+    // 16384) 6.8 and 10.0 us, 270 KB (1024 x 32768) 11.5 and 12.9, with half the row groups (512 x 32768)
+    // 11.4 and 11.4.
+    if (l.row_groups < p.slab_blocks && l.group_bytes < 300e3) {
       p.slab_blocks = l.row_groups;
       p.aligned = 1;
     }
