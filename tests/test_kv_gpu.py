@@ -939,3 +939,45 @@ def test_attend_is_as_exact_as_fp32(D, dtype, H, kv, dim, lens):
         got += float((out[b].double() - want).square().sum())
         plain += float((fp32 - want).square().sum())
     assert got <= plain, (got ** 0.5, plain ** 0.5)
+
+
+@pytest.mark.parametrize("dim,long", [(64, False), (64, True), (33, False), (33, True)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_evict_skips_rows_of_bad_pages(D, wb, dim, long, in_place):
+    """A row that cannot move leaves its slot as it was, its weight and position too; the others move, and
+    the error word says so."""
+    import torch
+    rng = np.random.default_rng(dim)
+    kv, page, n, keep = 2, 16, 5000 if long else 160, 2000 if long else 80
+    per = -(-n // page)
+    kp, vp, table = make_cache(rng, "f32", 1, per, page, kv, dim)
+    broken = table.clone()
+    broken[0, 0], broken[0, per - 1] = -1, 1 << 20  # of slots to fill, and of slots to take
+    w = rng.random((1, kv, per * page)).astype(np.float32)
+    pos = np.broadcast_to(np.arange(per * page, dtype=np.int32) * 3, w.shape).copy()
+    k0, v0 = kp.clone(), vp.clone()
+    w_in, p_in = torch.from_numpy(w).cuda(), i32(pos)
+    w_out, p_out = (w_in.clone(), p_in.clone()) if in_place else (torch.full_like(w_in, -1), torch.full_like(p_in, -1))
+    lens = i32([n])
+    c = D.PagedKV(kp, vp, broken, lens, num_heads=kv, seen=i32([3 * n]), weights=w_out, positions=p_out)
+    c.evict(keep, **({} if in_place else dict(weights_in=w_in, positions_in=p_in)))
+    with pytest.raises(wb.WelvetError) as e:
+        c.check_error()
+    assert e.value.code == 1 and "page" in str(e.value) and lens.tolist() == [keep]
+    t, moved, skipped = table.cpu().numpy()[0], 0, 0
+    got_w, got_p = w_out.cpu().numpy(), p_out.cpu().numpy()
+    kb, ka = k0.cpu().numpy(), kp.cpu().numpy()
+    for h in range(kv):
+        order = np.lexsort((np.arange(n), -w[0, h, :n]))
+        stays = np.zeros(n, bool)
+        stays[order[:keep]] = True
+        src = np.arange(keep)
+        fill, take = np.flatnonzero(~stays[:keep]), keep + np.flatnonzero(stays[keep:])
+        ok = (fill >= page) & (take < (per - 1) * page)
+        src[fill[ok]] = take[ok]
+        moved, skipped = moved + int(ok.sum()), skipped + int((~ok).sum())
+        np.testing.assert_array_equal(got_w[0, h, :keep], w[0, h, src])
+        np.testing.assert_array_equal(got_p[0, h, :keep], pos[0, h, src])
+        for j in range(keep):
+            np.testing.assert_array_equal(ka[t[j // page], j % page, h], kb[t[src[j] // page], src[j] % page, h])
+    assert moved and skipped

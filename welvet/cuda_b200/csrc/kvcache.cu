@@ -288,7 +288,7 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kv, c
       }
       Row ahead{};
       if (i + step < n) ahead = fetch(i + step);
-      if (at == 0) {
+      if (ok && at == 0) {
         c.weights[rec + row.to] = weight;
         c.positions[rec + row.to] = pos;
       }
@@ -307,14 +307,14 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kv, c
   } else {
     for (int i = worker; i < n; i += workers) {
       const int to = fill[i], from = take[i];
-      if (lane == 0) {
-        c.weights[rec + to] = p.a.weights_in[rec + from];
-        c.positions[rec + to] = p.a.positions_in[rec + from];
-      }
       int64_t kt, vt, kf, vf;
       if (!(row_of(to, &kt, &vt) && row_of(from, &kf, &vf))) {
         if (lane == 0) atomicCAS(c.err, 0, kKvErrPage);
         continue;
+      }
+      if (lane == 0) {
+        c.weights[rec + to] = p.a.weights_in[rec + from];
+        c.positions[rec + to] = p.a.positions_in[rec + from];
       }
       for (int o = lane; o < bytes; o += 32) {
         c.k.base[kt + o] = c.k.base[kf + o];
