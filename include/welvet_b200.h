@@ -293,7 +293,7 @@ WELVET_API void welvet_b200_kv_release(welvet_b200_kv* kv);
 /* An MHA cell's step over a cache of its head counts and width. decode: one new token per sequence,
  * x_dev [num_seqs][d_model] -> attn_dev [num_seqs][q_dim] (may be NULL), y_dev [num_seqs][d_model]:
  * projections, rotary and append, attention with the cell's mask, position kind and scale (mask 3's
- * window is max_seq_len), output projection; accumulate as in kv_attend. decode_active: a sequence with
+ * window is the cell's, max_seq_len where it has none), output projection; accumulate as in kv_attend. decode_active: a sequence with
  * active_dev[s] = 0 ([num_seqs], NULL: none) is left out, as one that has ended or not begun: nothing of
  * its slots, weights or page-table row is read or written, its rows of attn and y are zeros (with its length
  * at 0 kv_evict leaves it alone too). prefill: `tokens` rows of a prompt from position 0, attended among

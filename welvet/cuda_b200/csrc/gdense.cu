@@ -117,11 +117,12 @@ __global__ void k_group_scales(const uint16_t* scales, int64_t n, int* large) {
 // token. Products are exact; a scale set's sum (fp32, at most 256 products) is multiplied by its
 // scale and added to the row's fp32 sum. (Records copied to rings of shared memory by the bulk
 // engine, 8 warps a block, were slower on layers below 100 MB: the ring leaves half the warps.)
-// Measured at one token: FP4, 16384 -> 65536, groups of 32 (0.6 GB), 106 us, 5.7 TB/s (87 % of a
-// copy); Int4, 4096 -> 4096, groups of 128 (8.7 MB), 5.3 us, of which 1.3 are the bytes and the
-// rest launch, prologue, one pass of loads and the blocks' join (8.4 at eight tokens: each block makes
-// its own f16 parts of x); Int4, 16384 -> 65536, groups of 128: 97, 103 and 134 us at 1, 4 and 8 tokens
-// (the second tile of tokens doubles the MMAs).
+// Measured at one token: FP4, 16384 -> 65536, groups of 32 (0.6 GB), 107 to 112 us by the GPU and its
+// power cap, 5.4 to 5.7 TB/s (82 to 86 % of a copy); Int4, 4096 -> 4096, groups of 128 (8.7 MB), 5.2 us,
+// of which 1.3 are the bytes and the rest launch, prologue, one pass of loads and the blocks' join (8.2
+// at eight tokens: each block makes its own f16 parts of x); Int4, 16384 -> 65536, groups of 128: 102 to
+// 109, 112 to 118 and 146 to 157 us at 1, 4 and 8 tokens (the second tile of tokens doubles the MMAs);
+// Uint4, groups of 64, 114 to 120 us at one.
 // tcgen05 needs N >= 8 and M = 128 rows of dequantised weights in shared or tensor memory; at 1..8
 // tokens the conversion is the work, and the register path takes its result without a store.
 //
@@ -181,7 +182,9 @@ __device__ __forceinline__ void g_mma0(float (&d)[4], const uint32_t (&a)[4], ui
 
 // A fragment of one block: E2M1 bytes through the converter; integer codes n as the f16 1024 + n
 // (or 1024 + 16 n, where the nibble stands four bits higher), minus 1024 + zero (or times 1/16,
-// minus 64 + zero), both exact.
+// minus 64 + zero), both exact. That f16 numbers of exponent 10 hold an integer in their last bits, so
+// that an OR converts it, is the published way (Kim, Henry, Fahim, Hassan Awadalla, "Who Says Elephants
+// Can't Run", 2022); the constants follow from the format.
 template <int kCode>
 __device__ __forceinline__ void g_decode(uint32_t w, __half2 z0, __half2 z1, uint32_t (&a)[4]) {
   if constexpr (kCode == kCodeFp4) {
@@ -588,10 +591,12 @@ __global__ void __launch_bounds__(256) k_group_slabs(const __grid_constant__ GAr
   g_write(a, o, b, v);
 }
 
-// The quantiser, run once per matrix and bound by its 4 bytes read per weight. One warp per (row,
-// group): the group's range gives its scale, rounded to the scale's type before the codes are
-// chosen, so that decoding multiplies by what the codes were divided by. A group that holds an
-// infinity or NaN gets a NaN scale: its row says so, where codes would hide it.
+// The quantiser, run once per matrix: 16384 x 16384 in groups of 64 (1.07 GB read) take 1.03 ms (Int4),
+// 1.14 (Uint4) and 1.59 (FP4), a sixth of a copy's rate, bound by a division per weight and the few
+// loads that a warp has in flight. One warp per (row, group): the group's range gives its scale, rounded
+// to the scale's type before the codes are chosen, so that decoding multiplies by what the codes were
+// divided by. A group that holds an infinity or NaN gets a NaN scale: its row says so, where codes would
+// hide it.
 template <int kCode>
 __global__ void __launch_bounds__(256)
     k_group_quantize(const float* __restrict__ W, int rows, int cols, int group, int groups, int scale_type, uint8_t* codes,

@@ -4,10 +4,11 @@
 // keys with a running maximum and sum; all scores are held in units of log2, so that a weight is
 // one exp2. HBM bound: a key and a value row are read once for all the query heads that share
 // them, 2 sizeof(T) head_dim bytes against 4 head_dim flops per query head. Measured, 8 key-value
-// heads of 128, 4 query heads each: bf16, 64 sequences of 8191 slots (2.15 GB), 337 us, 6.4 TB/s
-// (97 % of a copy) in runs of calls short of the power cap, 385 us in seconds of them (1.64 GHz);
-// E4M3, 30k..131k slots (0.87 GB), 157 and 181 us, 5.5 and 4.8 TB/s: half the bytes for the same
-// products, so instruction issue and its latency at 8 warps an SM bound it before the copies do.
+// heads of 128, 4 query heads each: 64 sequences of 8191 slots (2.15 GB), bf16 351 to 372 us by the GPU
+// and its power cap, 5.8 to 6.1 TB/s (88 to 93 % of a copy), f16 340 us, 6.3 TB/s; f32, 16 sequences of
+// 8191 (1.07 GB), 240 to 247 us, 4.4 TB/s: four MMAs and eight conversions of parts a step bound it;
+// E4M3, 30k..131k slots (0.87 GB), 177 to 182 us, 4.9 TB/s: half the bytes of bf16 for the same products,
+// so instruction issue and its latency at 8 warps an SM bound it before the copies do.
 #include "kvcache.cuh"
 #include "kvcache.hpp"
 #include "pipeline.cuh"
@@ -219,8 +220,11 @@ __global__ void k_attend_weights(const __grid_constant__ AttendParams p) {
 //                             the weights scaled by 2^15 (f16's subnormals then lie below 2^-39)
 //   bf16                      three bf16 parts, 24 bits: the third in a second MMA
 //   f32                       two tf32 parts of both operands, 22 bits
-// The register-path MMA is used, not tcgen05: with 8 query rows an M = 128 tile would be 94 %
-// padding, and at HBM speed the warp MMAs of a 16-key tile take about a third of its time.
+// The register-path MMA is used, not tcgen05: at HBM speed the warp MMAs of a 16-key tile take about a
+// third of its time, and their results are where the softmax needs them. The price of eight query
+// heads as the rows of a tile is the second reading of the rows by a head group's next block: 16 query
+// heads a key-value head (32 x 4096 slots, bf16) 172 to 177 us, 47 % of a copy, for 100 to 107 at
+// eight. Keys as the rows, with heads' parts as the columns, would serve more heads from one reading.
 //
 // Work is cut into tiles of 16 or 32 keys per warp; the tiles of all (sequence, key-value head) units
 // are cut into equal runs, so that ragged lengths balance. A block takes a run; where a key-value
@@ -343,10 +347,11 @@ struct Tiled {
   static constexpr int kSmem = kRing + kSets * kSteps * 512;  // and the query's fragments
 };
 
-// Beginning and finishing a unit costs a block about as much as kOver tiles (the ragged batch of 64
-// took 57.6, 53.9, 57.8 and 64.6 us with 1, 2, 4 and 7): the list that the
+// Beginning and finishing a unit costs a block about as much as kOver tiles: the list that the
 // blocks divide has kOver places before each unit's tiles, so that runs of short units (one tile
-// each) get fewer of them.
+// each) get fewer of them. With 1, 2 and 4, us: 64 sequences of 1..8191 slots 54.7, 54.1, 58.4; 16 of
+// 100..30000 44.7, 43.1, 43.3; 12 of 500..60000 in E4M3 74.0, 71.6, 72.5; 256 of 1..700 51.0, 54.0,
+// 62.2; 40 of 10..4000 with heads of 64 21.3, 21.9, 24.0.
 constexpr int kOver = 2;
 
 // A tile's place in that list: `at`, of sequence b, unit u, tile of the unit's nt.
@@ -515,7 +520,9 @@ __global__ void __launch_bounds__(Tiled<T, DP, kFull>::kThreads, Tiled<T, DP, kF
     }
     total += chunk;
     // A unit cut into P runs costs about P / 50 tiles of joining: runs are at least as long as
-    // balances that, and never empty.
+    // balances that, and never empty. It shows where few units are long: one key-value head of 50000
+    // slots with weights 21.0 us, with the shortest runs 25.8; 30000 slots 13.4 and 13.2. With 1 / 25 and
+    // 1 / 200 the batches above take the same times.
     const float tiles = static_cast<float>(total) / static_cast<float>(c.num_seqs * c.num_kv);
     const int shortest = max(1, static_cast<int>(sqrtf(tiles * (1.0f / 50.0f))));
     n_runs = max(1, min(static_cast<int>(gridDim.x) / p.head_groups, total / shortest));
@@ -1272,8 +1279,8 @@ Status attend_plan(KvCache* c) {
     c->attend_blocks = static_cast<int>(std::min<int64_t>(std::max(1, per_sm * sms / hg), most)) * hg;
     c->part_bytes = static_cast<size_t>(c->attend_blocks) * 2 * 8 * (v.head_dim + 4) * 4;
     // Clusters where all of them are resident together and a block's tiles are so few that ragged
-    // lengths cannot cost more than the second launch (one sequence of 500 slots, 16 heads: 6.0 us
-    // against 7.9; with 16 tiles a block they are the slower form, 19 us against 17).
+    // lengths cannot cost more than the second launch (one sequence of 500 slots, 16 heads: 6.1 us
+    // against 7.3; with 16 tiles a block they are the slower form, 19 us against 17).
     const int64_t tiles = (v.max_slots + G::kKeys - 1) / G::kKeys;
     int size = kMaxCluster;
     while (size > 1 && (units * hg * size > static_cast<int64_t>(per_sm) * sms || size > tiles)) size /= 2;

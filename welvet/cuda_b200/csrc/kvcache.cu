@@ -42,8 +42,8 @@ __device__ __forceinline__ void rotate(float& a, float& b, float cs, float sn) {
 // One block per new token: the token's angles once into shared memory, then its key, value and
 // query heads, pair (d, d + half) by pair. HBM bound: 4 B read per element, the page's type
 // written (and 4 B for q). kVec: four consecutive pairs a thread (16-byte accesses).
-// kDim: the width, 0 where it is not a constant (13k prompt tokens of 48 heads of 128: 74 us, 90 without).
-// kDiv: the scales are not both powers of two.
+// kDim: the width, 0 where it is not a constant (13k prompt tokens of 48 heads of 128: 81 us, 95 without).
+// kDiv: the scales are not both powers of two (the same tokens: 100 us).
 template <typename T, bool kVec, int kDim, bool kDiv>
 __global__ void __launch_bounds__(kAppendThreads, 4) k_append(const __grid_constant__ AppendParams p) {
   __shared__ float s_cos[kMaxPairs], s_sin[kMaxPairs];
@@ -329,9 +329,9 @@ __device__ __forceinline__ void move_rows(const EvictParams& p, int b, int kv, c
 // memory), then, in slot order, the slots below keep that go (to fill) and those above it that stay
 // (to take). Both lists are equally long and no slot is in both, so the rows can move in any order.
 // A cluster of one block moves them itself; larger ones leave the lists to k_evict_move.
-// Latency bound: 8 bytes a slot are read, the rest is a dozen barriers. About 24 us of the 56
+// Latency bound: 8 bytes a slot are read, the rest is a dozen barriers. About 24 us of the 58
 // at 24 heads of 40k..65k slots (10 MB read, eight blocks a head); 32 sequences x 8 heads of 1025..1056
-// slots cut to 1024 take 9 us with their rows, in one launch.
+// slots cut to 1024 take 10.4 us with their rows, in one launch.
 template <int kSize, bool kVec>
 __global__ void __launch_bounds__(kEvictThreads, 2) k_evict_select(const __grid_constant__ EvictParams p) {
   namespace cg = cooperative_groups;
