@@ -299,9 +299,10 @@ WELVET_API void welvet_b200_kv_release(welvet_b200_kv* kv);
  * at 0 kv_evict leaves it alone too). prefill: `tokens` rows of a prompt from position 0, attended among
  * themselves as in mha_execute_device (tokens <= the cell's max_seq_len) and appended to a sequence whose
  * length is 0, whatever its seen; its seen becomes `tokens`. One that holds slots keeps them, and
- * kv_check_error says so. A call of more rows than any before allocates the
- * cell's work buffers, so it runs once before it is captured; buffers that a captured call of the cell
- * (these two, mha_execute_device) works on stay where they are until the cell is released. */
+ * kv_check_error says so. The first step for a number
+ * of sequences and a prompt longer than any before allocate the cell's work buffers, so a call runs once
+ * before it is captured; those of steps, and all that a captured call of the cell (mha_execute_device
+ * too) works on, stay where they are until the cell is released. */
 WELVET_API welvet_status welvet_b200_mha_decode_device(welvet_b200_mha* s, welvet_b200_kv* kv, const float* x_dev,
                                                        float* attn_dev, float* y_dev, int32_t accumulate, void* stream);
 WELVET_API welvet_status welvet_b200_mha_decode_active_device(welvet_b200_mha* s, welvet_b200_kv* kv, const float* x_dev,

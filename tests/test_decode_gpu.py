@@ -370,3 +370,46 @@ def test_steps_against_64_bits(D, wb, dtype, pos, mask, max_seq, heads, kv, dim)
     assert np.all(np.abs(got - want) <= bound)
     out = got.reshape(n, -1) @ w[3].T.astype(np.float64)
     assert np.all(np.abs(y.cpu().numpy() - out) <= 2 * EPS * np.abs(out) + 1e-30)
+
+
+def test_steps_are_the_same_launches_after_a_longer_prompt(D, wb, monkeypatch):
+    """The projections' prepared form of few rows stays available to a step whatever prompts came before it,
+    and a step that is captured right after a prompt needs no allocation."""
+    import ctypes
+
+    import torch
+    monkeypatch.setenv("WELVET_B200_GEMV_PREP", "1")  # the form that layers of 8192 rows take
+    g = torch.Generator(device="cuda").manual_seed(61)
+    d_model, heads, kv, dim, n = 1024, 9, 9, 128, 3
+    w = [torch.randn((r, d_model), generator=g, device="cuda") * 0.03 for r in (heads * dim, kv * dim, kv * dim)]
+    w.append(torch.randn((d_model, heads * dim), generator=g, device="cuda") * 0.03)
+    x, long = (torch.randn((t, d_model), generator=g, device="cuda") for t in (n, 70))
+    seen = []
+    for before in (False, True):
+        cell = wb.MhaCell(*w, d_model, heads, kv, dim, 400, 1, 0, wb.FP8E4M3)
+        cache, other = (cache_for(D, s, heads, kv, dim, 400, torch.bfloat16) for s in (n, 1))
+        y = torch.empty((n, d_model), device="cuda")
+        if before:
+            D.mha_prefill(cell, other, 0, long, torch.empty_like(long))
+        D.mha_decode(cell, cache, x, y)
+        graph = torch.cuda.CUDAGraph(keep_graph=True)
+        with torch.cuda.graph(graph):
+            D.mha_decode(cell, cache, x, y)
+        nodes = ctypes.c_size_t()
+        assert ctypes.CDLL("libcudart.so.12").cudaGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(nodes)) == 0
+        graph.instantiate()
+        graph.replay()
+        seen.append((nodes.value, y))
+    assert seen[0][0] == seen[1][0] and torch.equal(seen[0][1], seen[1][1])
+    cell = wb.MhaCell(*w, d_model, heads, kv, dim, 400, 1, 0, wb.FP8E4M3)
+    cache, other = (cache_for(D, s, heads, kv, dim, 400, torch.bfloat16) for s in (n, 1))
+    D.mha_prefill(cell, other, 0, long, torch.empty_like(long))
+    graph, y = torch.cuda.CUDAGraph(), torch.empty((n, d_model), device="cuda")
+    with torch.cuda.graph(graph):
+        D.mha_decode(cell, cache, x, y)
+    other.lens.zero_()
+    more = torch.cat([long] * 4)
+    D.mha_prefill(cell, other, 0, more, torch.empty_like(more))
+    for _ in range(2):
+        graph.replay()
+    assert torch.equal(y, seen[0][1]) and cache.lens.tolist() == [2] * n

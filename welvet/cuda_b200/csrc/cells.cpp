@@ -332,6 +332,7 @@ MhaCell::~MhaCell() {
   cudaSetDevice(device);
   release_work();
   for (MhaWork& w : outgrown) w.release_work();
+  for (auto& w : steps) w->release_work();
 }
 
 Status mha_mount(int device, const MhaConfig& cfg_in, DType dt, const float* Q, const float* K, const float* V,
@@ -359,10 +360,30 @@ Status mha_mount_src(int device, const MhaConfig& cfg_in, DType dt, const Weight
   return Status::Ok();
 }
 
-Status mha_reserve(MhaCell* c, int bs, cudaStream_t st) {
+static bool is_capturing(cudaStream_t st) {
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
   if (cudaStreamIsCapturing(st, &capture) != cudaSuccess) cudaGetLastError();  // the legacy stream beside a capture
-  const bool capturing = capture == cudaStreamCaptureStatusActive;
+  return capture == cudaStreamCaptureStatusActive;
+}
+
+// What the projections of `bs` rows write and work in.
+static Status alloc_projections(const MhaCell& c, int bs, MhaWork* w, cudaStream_t st) {
+  const MhaConfig& g = c.cfg;
+  const size_t qd = static_cast<size_t>(g.num_heads) * g.head_dim, kvd = static_cast<size_t>(g.num_kv_heads) * g.head_dim;
+  const size_t n = static_cast<size_t>(bs);
+  WB_CUDA(cudaMalloc(&w->qb, n * qd * 4));
+  WB_CUDA(cudaMalloc(&w->kb, n * kvd * 4));
+  WB_CUDA(cudaMalloc(&w->vb, n * kvd * 4));
+  WB_CUDA(cudaMalloc(&w->attn, n * qd * 4));
+  WB_TRY(alloc_io(c.q, bs, &w->io_q, st));
+  WB_TRY(alloc_io(c.k, bs, &w->io_k, st));
+  WB_TRY(alloc_io(c.v, bs, &w->io_v, st));
+  w->io_o.max_tb = xsplit_policy() >= 2 ? 128 : 0;  // attention output: fp32, two x planes
+  return alloc_io(c.o, bs, &w->io_o, st);
+}
+
+Status mha_reserve(MhaCell* c, int bs, cudaStream_t st) {
+  const bool capturing = is_capturing(st);
   if (c->bs >= bs) {
     c->captured |= capturing;
     return Status::Ok();
@@ -379,20 +400,12 @@ Status mha_reserve(MhaCell* c, int bs, cudaStream_t st) {
   const size_t n = static_cast<size_t>(bs);
   WB_CUDA(cudaMalloc(&c->x_pad, n * c->q.x_stride * 4));
   WB_CUDA(cudaMemsetAsync(c->x_pad, 0, n * c->q.x_stride * 4, st));
-  WB_CUDA(cudaMalloc(&c->qb, n * qd * 4));
-  WB_CUDA(cudaMalloc(&c->kb, n * kvd * 4));
-  WB_CUDA(cudaMalloc(&c->vb, n * kvd * 4));
-  WB_CUDA(cudaMalloc(&c->attn, n * qd * 4));
   WB_CUDA(cudaMalloc(&c->attn_pad, n * c->o.x_stride * 4));
   WB_CUDA(cudaMemsetAsync(c->attn_pad, 0, n * c->o.x_stride * 4, st));
   WB_CUDA(cudaMalloc(&c->Qr, n * qd * 8));
   WB_CUDA(cudaMalloc(&c->Kr, n * kvd * 8));
   WB_CUDA(cudaMalloc(&c->Vd, n * kvd * 8));
-  WB_TRY(alloc_io(c->q, bs, &c->io_q, st));
-  WB_TRY(alloc_io(c->k, bs, &c->io_k, st));
-  WB_TRY(alloc_io(c->v, bs, &c->io_v, st));
-  c->io_o.max_tb = xsplit_policy() >= 2 ? 128 : 0;  // attention output: fp32, two x planes
-  WB_TRY(alloc_io(c->o, bs, &c->io_o, st));
+  WB_TRY(alloc_projections(*c, bs, c, st));
   c->bs = bs;
   c->captured = capturing;
   return Status::Ok();
@@ -434,31 +447,57 @@ static Status mha_cache_fits(const MhaCell& c, const KvCache& kv) {
 
 static double mha_theta(const MhaConfig& g) { return g.pos == 0 || g.pos == 3 ? g.rope_theta : 0.0; }
 
+// The buffers of a step of `rows` sequences, made by the first one. A first one that is captured, which
+// must not allocate, works on a prompt's where they are large enough.
+static Status mha_step_work(MhaCell* c, int rows, MhaWork** out, cudaStream_t st) {
+  for (auto& w : c->steps)
+    if (w->bs == rows) {
+      *out = w.get();
+      return Status::Ok();
+    }
+  if (c->bs >= rows && is_capturing(st)) {
+    *out = c;
+    return mha_reserve(c, rows, st);
+  }
+  auto w = std::make_unique<MhaWork>();
+  const Status made = alloc_projections(*c, rows, w.get(), st);
+  if (!made.ok()) {
+    cudaGetLastError();  // a failed allocation must not be taken for a later launch's error
+    w->release_work();
+    return made;
+  }
+  w->bs = rows;
+  c->steps.push_back(std::move(w));
+  *out = c->steps.back().get();
+  return Status::Ok();
+}
+
 Status mha_decode_device(MhaCell* c, KvCache* kv, const float* x, float* attn, float* y, bool accumulate,
                          const int32_t* active, cudaStream_t st) {
   WB_TRY(mha_cache_fits(*c, *kv));
   const MhaConfig& g = c->cfg;
   const int rows = kv->view.num_seqs, qd = g.num_heads * g.head_dim, kvd = g.num_kv_heads * g.head_dim;
   if (accumulate && !kv->view.weights) return Status::Invalid("mha: the cache has no weights to accumulate");
-  WB_TRY(mha_reserve(c, rows, st));
-  WB_TRY(forward_device(c->q, rows, x, g.d_model, c->qb, c->qb, &c->io_q, st, false));
-  WB_TRY(forward_device(c->k, rows, x, g.d_model, c->kb, c->kb, &c->io_k, st, false));
-  WB_TRY(forward_device(c->v, rows, x, g.d_model, c->vb, c->vb, &c->io_v, st, false));
+  MhaWork* w = nullptr;
+  WB_TRY(mha_step_work(c, rows, &w, st));
+  WB_TRY(forward_device(c->q, rows, x, g.d_model, w->qb, w->qb, &w->io_q, st, false));
+  WB_TRY(forward_device(c->k, rows, x, g.d_model, w->kb, w->kb, &w->io_k, st, false));
+  WB_TRY(forward_device(c->v, rows, x, g.d_model, w->vb, w->vb, &w->io_v, st, false));
   KvAppendArgs ap;
   ap.rows = rows;
-  ap.k = c->kb;
-  ap.v = c->vb;
-  ap.q = c->qb;
-  ap.q_out = c->qb;
+  ap.k = w->kb;
+  ap.v = w->vb;
+  ap.q = w->qb;
+  ap.q_out = w->qb;
   ap.k_ld = ap.v_ld = kvd;
   ap.q_ld = ap.q_out_ld = qd;
   ap.theta = mha_theta(g);
   ap.active = active;
   ap.step_lens = kv->step_lens;
   WB_TRY(kv_append(kv, ap, st));
-  float* attn_out = attn ? attn : c->attn;
+  float* attn_out = attn ? attn : w->attn;
   KvAttendArgs at;
-  at.q = c->qb;
+  at.q = w->qb;
   at.out = attn_out;
   at.q_ld = at.out_ld = qd;
   at.scale = static_cast<float>(g.scale_override);
@@ -468,7 +507,7 @@ Status mha_decode_device(MhaCell* c, KvCache* kv, const float* x, float* attn, f
   at.accumulate = accumulate;
   at.lens = active ? kv->step_lens : nullptr;
   WB_TRY(kv_attend(kv, at, st));
-  return forward_device(c->o, rows, attn_out, qd, y, y, &c->io_o, st, false);
+  return forward_device(c->o, rows, attn_out, qd, y, y, &w->io_o, st, false);
 }
 
 Status mha_prefill_device(MhaCell* c, KvCache* kv, int sequence, int tokens, const float* x, float* attn, float* y,

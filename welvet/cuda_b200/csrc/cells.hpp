@@ -10,6 +10,7 @@
 #include "dense.hpp"
 #include "kvcache.hpp"
 
+#include <memory>
 #include <vector>
 
 namespace wb {
@@ -87,6 +88,9 @@ struct MhaCell : MhaWork {
   WeightStore sq, sk, sv, so;
   DeviceDense q, k, v, o;
   std::vector<MhaWork> outgrown;  // buffers that a graph still replays on, kept as long as the cell
+  // Of decode steps, one for each number of sequences, kept as long as the cell: the projections' scratch
+  // goes by the rows that it is made for, and a step is not slower after a longer prompt.
+  std::vector<std::unique_ptr<MhaWork>> steps;
   ~MhaCell();
 };
 

@@ -6,9 +6,10 @@ runs three operators over it: `append` (new tokens, rotated and cast, into the p
 attention weight). `GroupDense` is a Dense layer of 4-bit codes with one scale per group of
 inputs, for one to eight rows at a time. `mha_decode` and `mha_prefill` run an MHA cell over such a
 cache. All calls are asynchronous on the current stream (or `stream`) and can be captured in a CUDA
-graph. The calls of a cache and of a layer allocate nothing; a cell's allocate its work buffers when
-a call has more rows than any before, so a step runs once before it is captured. Buffers that were
-captured stay until the cell is released: a longer prompt may follow, and the graph replays on.
+graph. The calls of a cache and of a layer allocate nothing; a cell's allocate its work buffers
+at the first step for a number of sequences and at a prompt longer than any before, so a step runs
+once before it is captured. Buffers of steps, and those that were captured, stay until the cell is
+released: a longer prompt may follow, and the graph replays on.
 """
 from __future__ import annotations
 
