@@ -253,8 +253,8 @@ WELVET_API welvet_status welvet_b200_kv_create(const welvet_b200_kv_desc* desc, 
  * sequence (rows = num_seqs). Row i of a sequence takes slot start[s] + i and position
  * start_seen[s] + i; afterwards lens = start + n and seen = start_seen + n (start, start_seen NULL:
  * lens and seen themselves, advanced in place). theta > 0 rotates k, and q [rows][num_heads *
- * head_dim] into q_out (may be q), as the MHA cell does (pairs d, d + head_dim/2); values are stored
- * as they are. A slot past max_slots or a page id outside the pool is skipped and recorded; so is
+ * head_dim] into q_out (may be q), as the MHA cell does (pairs d, d + head_dim/2); values are not
+ * rotated. Pages hold k / k_scale and v / v_scale, rounded. A slot past max_slots or a page id outside the pool is skipped and recorded; so is
  * what cu_tokens gives a sequence beyond `rows`, and a cu_tokens that decreases: lengths advance by the
  * rows that there are. */
 WELVET_API welvet_status welvet_b200_kv_append(welvet_b200_kv* kv, int32_t rows, const float* k, int64_t k_ld,
@@ -343,7 +343,8 @@ WELVET_API welvet_status welvet_b200_gdense_execute_device(welvet_b200_gdense* g
  * multiprocessors, as the library plans it: slabs of the inputs, chunks (256 inputs) of a slab, blocks of
  * a slab, whether runs of records are the warps' (1) or the blocks' (0), whether runs are whole row
  * groups (16 outputs), shared memory in bytes, row groups, chunks, runs of a slab, row groups that are
- * cut by runs. Writes the first n values, returns their number (10), -1 for arguments that mount
+ * cut by runs. (Layers with BFloat16 scales of 2^96 and more, whose rows are longer, may be planned as
+ * a slightly wider layer.) Writes the first n values, returns their number (10), -1 for arguments that mount
  * refuses. Host arithmetic only. */
 WELVET_API int32_t welvet_b200_gdense_plan(int32_t in, int32_t out, int32_t group, int32_t code, int32_t sms, int32_t rows,
                                            int64_t* values, int32_t n);
