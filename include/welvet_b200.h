@@ -254,9 +254,9 @@ WELVET_API welvet_status welvet_b200_kv_create(const welvet_b200_kv_desc* desc, 
  * start_seen[s] + i; afterwards lens = start + n and seen = start_seen + n (start, start_seen NULL:
  * lens and seen themselves, advanced in place). theta > 0 rotates k, and q [rows][num_heads *
  * head_dim] into q_out (may be q), as the MHA cell does (pairs d, d + head_dim/2); values are not
- * rotated. Pages hold k / k_scale and v / v_scale, rounded. A slot past max_slots or a page id outside the pool is skipped and recorded; so is
- * what cu_tokens gives a sequence beyond `rows`, and a cu_tokens that decreases: lengths advance by the
- * rows that there are. */
+ * rotated. Pages hold k / k_scale and v / v_scale, rounded. A slot past max_slots or a page id outside
+ * the pool is skipped and recorded; so is what cu_tokens gives a sequence beyond `rows`, and a cu_tokens
+ * that decreases: lengths advance by the rows that there are. */
 WELVET_API welvet_status welvet_b200_kv_append(welvet_b200_kv* kv, int32_t rows, const float* k, int64_t k_ld,
                                                const float* v, int64_t v_ld, const float* q, int64_t q_ld,
                                                float* q_out, int64_t q_out_ld, const int32_t* cu_tokens, double theta,
@@ -290,19 +290,19 @@ WELVET_API welvet_status welvet_b200_kv_evict(welvet_b200_kv* kv, int32_t keep, 
 WELVET_API welvet_status welvet_b200_kv_check_error(welvet_b200_kv* kv, void* stream);
 WELVET_API void welvet_b200_kv_release(welvet_b200_kv* kv);
 
-/* An MHA cell's step over a cache of its head counts and width. decode: one new token per sequence,
- * x_dev [num_seqs][d_model] -> attn_dev [num_seqs][q_dim] (may be NULL), y_dev [num_seqs][d_model]:
- * projections, rotary and append, attention with the cell's mask, position kind and scale (mask 3's
- * window is the cell's, max_seq_len where it has none), output projection; accumulate as in kv_attend. decode_active: a sequence with
- * active_dev[s] = 0 ([num_seqs], NULL: none) is left out, as one that has ended or not begun: nothing of
- * its slots, weights or page-table row is read or written, its rows of attn and y are zeros (with its length
- * at 0 kv_evict leaves it alone too). prefill: `tokens` rows of a prompt from position 0, attended among
- * themselves as in mha_execute_device (tokens <= the cell's max_seq_len) and appended to a sequence whose
- * length is 0, whatever its seen; its seen becomes `tokens`. One that holds slots keeps them, and
- * kv_check_error says so. The first step for a number
- * of sequences and a prompt longer than any before allocate the cell's work buffers, so a call runs once
- * before it is captured; those of steps, and all that a captured call of the cell (mha_execute_device
- * too) works on, stay where they are until the cell is released. */
+/* An MHA cell's step over a cache of its head counts and width. decode: one new token per sequence, x_dev
+ * [num_seqs][d_model] -> attn_dev [num_seqs][q_dim] (may be NULL), y_dev [num_seqs][d_model]: projections,
+ * rotary and append, attention with the cell's mask, position kind and scale (mask 3's window is the
+ * cell's, max_seq_len where it has none), output projection; accumulate as in kv_attend. decode_active: a
+ * sequence with active_dev[s] = 0 ([num_seqs], NULL: none) is left out, as one that has ended or not
+ * begun: nothing of its slots, weights or page-table row is read or written, its rows of attn and y are
+ * zeros (with its length at 0 kv_evict leaves it alone too). prefill: `tokens` rows of a prompt from
+ * position 0, attended among themselves as in mha_execute_device (tokens <= the cell's max_seq_len) and
+ * appended to a sequence whose length is 0, whatever its seen; its seen becomes `tokens`. One that holds
+ * slots keeps them, and kv_check_error says so. The first step for a number of sequences and a prompt
+ * longer than any before allocate the cell's work buffers, so a call runs once before it is captured;
+ * those of steps, and all that a captured call of the cell (mha_execute_device too) works on, stay where
+ * they are until the cell is released. */
 WELVET_API welvet_status welvet_b200_mha_decode_device(welvet_b200_mha* s, welvet_b200_kv* kv, const float* x_dev,
                                                        float* attn_dev, float* y_dev, int32_t accumulate, void* stream);
 WELVET_API welvet_status welvet_b200_mha_decode_active_device(welvet_b200_mha* s, welvet_b200_kv* kv, const float* x_dev,
